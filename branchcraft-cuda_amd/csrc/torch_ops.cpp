@@ -9,13 +9,16 @@
 // Workspaces for split launches come from PyTorch's caching allocator, which
 // keeps the ops safe under HIP graph capture.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdint>
+#include <tuple>
 #include <vector>
 
 #include "branchcraft.h"
@@ -420,6 +423,206 @@ at::Tensor int_tensor_hip(const at::Tensor& like, at::IntArrayRef values) {
   return out;
 }
 
+// Block table, row offsets, slot map and positions of a step (see
+// bc_build_tables); `tokens` rows, those behind the last request -1.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_tables_hip(
+    const at::Tensor& page_ids, const at::Tensor& lengths, const at::Tensor& counts,
+    int64_t max_pages, int64_t tokens) {
+  check_dev_contig(page_ids, "page_ids", at::kInt);
+  check_dev_contig(lengths, "lengths", at::kInt);
+  check_dev_contig(counts, "counts", at::kInt);
+  TORCH_CHECK(page_ids.dim() == 1 && lengths.dim() == 1 && counts.sizes() == lengths.sizes(),
+              "build_tables shape mismatch");
+  TORCH_CHECK(lengths.size(0) > 0, "build_tables: no requests");
+  TORCH_CHECK(max_pages >= 1 && max_pages < (1 << 27) && tokens >= 0 && tokens < (1 << 27) &&
+                  page_ids.numel() <= INT32_MAX && lengths.numel() < INT32_MAX,
+              "build_tables: max_pages must be at least 1, tokens at least 0, both below 2**27");
+  TORCH_CHECK(page_ids.device() == lengths.device() && page_ids.device() == counts.device(),
+              "all tensors must share a device");
+  const c10::DeviceGuard guard(lengths.device());
+  const int64_t b = lengths.size(0);
+  auto pages = at::empty({b, max_pages}, lengths.options());
+  auto starts = at::empty({b + 1}, lengths.options());
+  auto slots = at::empty({tokens}, lengths.options());
+  auto positions = at::empty({tokens}, lengths.options());
+  check_launch(bc_build_tables(page_ids.data_ptr<int>(), int(page_ids.numel()),
+                               lengths.data_ptr<int>(), counts.data_ptr<int>(), int(b),
+                               int(max_pages), int(tokens), pages.data_ptr<int>(),
+                               starts.data_ptr<int>(), slots.data_ptr<int>(),
+                               positions.data_ptr<int>(), current_stream()),
+               "build_tables");
+  return {pages, starts, slots, positions};
+}
+
+// Strides of a [P, 16, Hkv, D] pool in any order of its outer dimensions (a
+// dimension of one entry has none).
+bc_pool_strides pool_strides(const at::Tensor& t) {
+  auto at = [&](int i) { return (long long)(t.size(i) > 1 ? t.stride(i) : 0); };
+  return {at(0), at(1), at(2)};
+}
+
+bc_row_strides row_strides(const at::Tensor& t) {
+  auto at = [&](int i) { return (long long)(t.size(i) > 1 ? t.stride(i) : 0); };
+  return {at(0), at(1)};
+}
+
+void check_rows(const at::Tensor& t, const char* name, int64_t rank) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
+  TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, name,
+              " must be FP16 or BF16");
+  TORCH_CHECK(t.dim() == rank, name, " must have ", rank, " dimensions");
+  TORCH_CHECK(t.size(-1) == 64 || t.size(-1) == 128, name, ": head dimension must be 64 or 128");
+  TORCH_CHECK(t.stride(-1) == 1, name, ": head dimension must be contiguous");
+}
+
+const bc_half* raw(const at::Tensor& t) { return static_cast<const bc_half*>(t.data_ptr()); }
+
+// New tokens' K and V rows into the slots of a slot map (see bc_append_kv).
+void append_kv_hip(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k,
+                   const at::Tensor& v, const at::Tensor& slots) {
+  check_rows(cache_k, "cache_k", 4);
+  check_rows(cache_v, "cache_v", 4);
+  check_rows(k, "k", 3);
+  check_rows(v, "v", 3);
+  check_dev_contig(slots, "slots", at::kInt);
+  TORCH_CHECK(cache_k.scalar_type() == cache_v.scalar_type() &&
+                  cache_k.scalar_type() == k.scalar_type() &&
+                  cache_k.scalar_type() == v.scalar_type(),
+              "append_kv_: pools and rows must share a dtype");
+  TORCH_CHECK(cache_k.size(0) > 0 && cache_k.size(1) == BC_PAGE_SIZE &&
+                  cache_v.sizes() == cache_k.sizes() && v.sizes() == k.sizes() &&
+                  k.size(1) > 0 && k.size(1) == cache_k.size(2) &&
+                  k.size(2) == cache_k.size(3) && slots.dim() == 1 &&
+                  slots.size(0) == k.size(0),
+              "append_kv_ shape mismatch");
+  TORCH_CHECK(cache_k.device() == cache_v.device() && cache_k.device() == k.device() &&
+                  cache_k.device() == v.device() && cache_k.device() == slots.device(),
+              "all tensors must share a device");
+  TORCH_CHECK(k.size(0) <= INT32_MAX && cache_k.size(0) <= INT32_MAX,
+              "append_kv_: too many tokens or pages");
+  at::assert_no_internal_overlap(cache_k);
+  at::assert_no_internal_overlap(cache_v);
+  at::assert_no_overlap(cache_k, cache_v);
+  for (const at::Tensor* rows : {&k, &v}) {
+    at::assert_no_overlap(cache_k, *rows);
+    at::assert_no_overlap(cache_v, *rows);
+  }
+  if (k.size(0) == 0) return;
+  const c10::DeviceGuard guard(cache_k.device());
+  bc_shape shape{1, int(k.size(1)), int(k.size(1)), int(k.size(2)), 1, int(cache_k.size(0))};
+  check_launch(bc_append_kv(shape, raw(k), raw(v), row_strides(k), row_strides(v),
+                            static_cast<bc_half*>(cache_k.data_ptr()),
+                            static_cast<bc_half*>(cache_v.data_ptr()), pool_strides(cache_k),
+                            pool_strides(cache_v), slots.data_ptr<int>(), int(k.size(0)),
+                            current_stream()),
+               "append_kv_");
+}
+
+// Above the kernel: it has no derivative, so tensors that autograd tracks or
+// that carry a tangent are refused, and the pools' version counters move, so
+// that a backward that saved a pool before the rows entered it raises.
+void append_kv_autograd(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k,
+                        const at::Tensor& v, const at::Tensor& slots) {
+  for (const at::Tensor* x :
+       std::initializer_list<const at::Tensor*>{&cache_k, &cache_v, &k, &v})
+    TORCH_CHECK(!(x->requires_grad() && at::GradMode::is_enabled()) &&
+                    !x->_fw_grad(0).defined(),
+                "append_kv_ is not differentiable: detach its tensors or call it under no_grad");
+  static const auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("branchcraft::append_kv_", "")
+          .typed<void(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&,
+                      const at::Tensor&)>();
+  cache_k.unsafeGetTensorImpl()->bump_version();
+  cache_v.unsafeGetTensorImpl()->bump_version();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  op.call(cache_k, cache_v, k, v, slots);
+}
+
+// Attention of each request's new tokens over its pages (see
+// bc_chunk_attention).  The workspace comes from the caching allocator on the
+// current stream and its size from shapes alone, so that the op never reads
+// lengths back and can be captured.
+at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& pages, const at::Tensor& lengths,
+                               const at::Tensor& starts, std::optional<double> scale,
+                               bool causal, int64_t window, double cap,
+                               const std::optional<at::Tensor>& slopes,
+                               const std::optional<at::Tensor>& prefix,
+                               const std::optional<at::Tensor>& first) {
+  check_rows(q, "q", 3);
+  check_rows(k, "k", 4);
+  check_rows(v, "v", 4);
+  check_dev_contig(pages, "pages", at::kInt);
+  check_dev_contig(lengths, "lengths", at::kInt);
+  check_dev_contig(starts, "starts", at::kInt);
+  TORCH_CHECK(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(),
+              "q, k and v must share a dtype");
+  TORCH_CHECK(pages.dim() == 2 && lengths.dim() == 1 && starts.dim() == 1,
+              "invalid chunk attention tensor rank");
+  const int64_t t = q.size(0), hq = q.size(1), d = q.size(2);
+  const int64_t b = lengths.size(0), hkv = k.size(2);
+  TORCH_CHECK(b > 0 && hq > 0 && hkv > 0 && hq % hkv == 0, "unsupported chunk attention shape");
+  TORCH_CHECK(k.size(0) > 0 && k.size(1) == BC_PAGE_SIZE && k.size(3) == d &&
+                  v.sizes() == k.sizes(),
+              "K/V cache shape mismatch");
+  TORCH_CHECK(pages.size(0) == b && pages.size(1) >= 1 && starts.size(0) == b + 1,
+              "chunk attention metadata mismatch");
+  TORCH_CHECK(t <= INT32_MAX && k.size(0) <= INT32_MAX && pages.size(1) <= INT32_MAX &&
+                  b < INT32_MAX && hq <= BC_MAX_CHUNK_HEADS,
+              "chunk attention: too many rows, heads, pages or requests");
+  const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(double(d));
+  TORCH_CHECK(s > 0 && std::isfinite(float(s)) && float(s) > 0,
+              "scale must be positive and finite");
+  TORCH_CHECK(window >= 0, "window must not be negative");
+  TORCH_CHECK(cap >= 0 && std::isfinite(float(cap)) && (cap == 0 || float(cap) > 0),
+              "cap must be finite and not negative");
+  TORCH_CHECK(q.device() == k.device() && q.device() == v.device() &&
+                  q.device() == pages.device() && q.device() == lengths.device() &&
+                  q.device() == starts.device(),
+              "all tensors must share a device");
+  auto option = [&](const std::optional<at::Tensor>& x, const char* name, at::ScalarType type,
+                    int64_t n) -> const void* {
+    if (!x.has_value() || !x->defined()) return nullptr;
+    check_dev_contig(*x, name, type);
+    TORCH_CHECK(x->dim() == 1 && x->size(0) == n, name, " must have ", n, " entries");
+    TORCH_CHECK(x->device() == q.device(), "all tensors must share a device");
+    return x->data_ptr();
+  };
+  bc_chunk_inputs in{};
+  in.slopes = static_cast<const float*>(option(slopes, "slopes", at::kFloat, hq));
+  in.prefix = static_cast<const int32_t*>(option(prefix, "prefix", at::kInt, b));
+  in.first = static_cast<const int32_t*>(option(first, "first", at::kInt, t));
+  TORCH_CHECK(causal || !in.prefix, "prefix needs causal attention");
+  const c10::DeviceGuard guard(q.device());
+  auto output = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  if (t == 0) return output;
+  in.q = raw(q);
+  in.k = raw(k);
+  in.v = raw(v);
+  in.pages = pages.data_ptr<int>();
+  in.lengths = lengths.data_ptr<int>();
+  in.starts = starts.data_ptr<int>();
+  in.output = static_cast<bc_half*>(output.data_ptr());
+  in.q_strides = row_strides(q);
+  in.k_strides = pool_strides(k);
+  in.v_strides = pool_strides(v);
+  in.tokens = int(t);
+  in.dtype = q.scalar_type() == at::kHalf ? BC_FLOAT16 : BC_BFLOAT16;
+  in.causal = causal;
+  in.window = int(std::min<int64_t>(window, INT32_MAX));
+  in.scale = float(s);
+  in.cap = float(cap);
+  bc_shape shape{int(b), int(hq), int(hkv), int(d), int(pages.size(1)), int(k.size(0))};
+  const size_t ws_bytes = bc_chunk_attention_workspace_size(shape, int(t));
+  at::Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({int64_t(ws_bytes)}, q.options().dtype(at::kByte));
+  check_launch(bc_chunk_attention(shape, in, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
+                                  current_stream()),
+               "chunk_attention");
+  return output;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(branchcraft, m) {
@@ -431,6 +634,9 @@ TORCH_LIBRARY(branchcraft, m) {
   m.def("write_prefix_(Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor k, Tensor v, int[] pages) -> ()");
   m.def("int_tensor(Tensor like, int[] values) -> Tensor");
   m.def("paged_decode(Tensor q, Tensor k, Tensor v, Tensor pages, Tensor lengths, int splits=0) -> Tensor");
+  m.def("build_tables(Tensor page_ids, Tensor lengths, Tensor counts, int max_pages, int tokens) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("append_kv_(Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor k, Tensor v, Tensor slots) -> ()");
+  m.def("chunk_attention(Tensor q, Tensor k, Tensor v, Tensor pages, Tensor lengths, Tensor starts, float? scale=None, bool causal=True, int window=0, float cap=0., Tensor? slopes=None, Tensor? prefix=None, Tensor? first=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(branchcraft, CUDA, m) {
@@ -442,8 +648,12 @@ TORCH_LIBRARY_IMPL(branchcraft, CUDA, m) {
   m.impl("write_prefix_", write_prefix_hip);
   m.impl("int_tensor", int_tensor_hip);
   m.impl("paged_decode", paged_decode_hip);
+  m.impl("build_tables", build_tables_hip);
+  m.impl("append_kv_", append_kv_hip);
+  m.impl("chunk_attention", chunk_attention_hip);
 }
 
 TORCH_LIBRARY_IMPL(branchcraft, Autograd, m) {
   m.impl("write_prefix_", write_prefix_autograd);
+  m.impl("append_kv_", append_kv_autograd);
 }

@@ -25,6 +25,8 @@ BC_SCRATCH_SLOT_BYTES = 18 << 20
 BC_PAGE_SIZE = 16
 BC_MAX_SPLITS = 256
 BC_MAX_TREE_NODES = 256
+BC_FLOAT16 = 0
+BC_BFLOAT16 = 1
 
 # Every entry point include/branchcraft.h declares.
 EXPORTED = (
@@ -32,6 +34,8 @@ EXPORTED = (
     "bc_tree_verify_workspace_size", "bc_tree_verify_ws", "bc_commit_path", "bc_commit_paths", "bc_copy_pages",
     "bc_write_prefix", "bc_write_ints", "bc_packed_decode", "bc_packed_decode_workspace_size",
     "bc_packed_decode_ws", "bc_packed_decode_noalloc", "bc_version",
+    "bc_build_tables", "bc_append_kv", "bc_chunk_attention",
+    "bc_chunk_attention_workspace_size",
 )
 
 
@@ -52,6 +56,23 @@ class Scratch(Structure):
 class TreeInputs(Structure):
     _fields_ = [("prefix", Inputs), ("draft_q", c_void_p), ("draft_k", c_void_p),
                 ("draft_v", c_void_p), ("parent", c_void_p), ("output", c_void_p)]
+
+
+class RowStrides(Structure):
+    _fields_ = [("token", c_longlong), ("head", c_longlong)]
+
+
+class PoolStrides(Structure):
+    _fields_ = [("page", c_longlong), ("slot", c_longlong), ("head", c_longlong)]
+
+
+class ChunkInputs(Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("pages", c_void_p),
+                ("lengths", c_void_p), ("starts", c_void_p), ("slopes", c_void_p),
+                ("prefix", c_void_p), ("first", c_void_p), ("output", c_void_p),
+                ("q_strides", RowStrides), ("k_strides", PoolStrides),
+                ("v_strides", PoolStrides), ("tokens", c_int), ("dtype", c_int),
+                ("causal", c_int), ("window", c_int), ("scale", c_float), ("cap", c_float)]
 
 
 _lib = None
@@ -108,6 +129,16 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
                                              c_void_p, c_longlong, c_longlong, c_longlong,
                                              c_longlong, c_float, c_void_p]
     lib.bc_packed_decode_noalloc.restype = c_int
+    lib.bc_build_tables.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.bc_build_tables.restype = c_int
+    lib.bc_append_kv.argtypes = [Shape, c_void_p, c_void_p, RowStrides, RowStrides, c_void_p,
+                                 c_void_p, PoolStrides, PoolStrides, c_void_p, c_int, c_void_p]
+    lib.bc_append_kv.restype = c_int
+    lib.bc_chunk_attention.argtypes = [Shape, ChunkInputs, c_void_p, c_size_t, c_void_p]
+    lib.bc_chunk_attention.restype = c_int
+    lib.bc_chunk_attention_workspace_size.argtypes = [Shape, c_int]
+    lib.bc_chunk_attention_workspace_size.restype = c_size_t
     lib.bc_version.argtypes = []
     lib.bc_version.restype = c_char_p
     if path is None:
@@ -122,5 +153,6 @@ def shape(batch, query_heads, kv_heads, dim, max_pages, physical_pages) -> Shape
 __all__ = ["BC_SUCCESS", "BC_ERROR_INVALID_VALUE", "BC_ERROR_OUT_OF_MEMORY",
            "BC_STATIC_SCRATCH_BYTES", "BC_PAGE_SIZE", "BC_MAX_SPLITS",
            "BC_MAX_TREE_NODES", "EXPORTED", "Shape", "Inputs", "Scratch",
-           "TreeInputs", "load", "shape", "LIB_PATH", "POINTER", "c_int32",
+           "TreeInputs", "RowStrides", "PoolStrides", "ChunkInputs", "BC_FLOAT16",
+           "BC_BFLOAT16", "load", "shape", "LIB_PATH", "POINTER", "c_int32",
            "c_uint16"]

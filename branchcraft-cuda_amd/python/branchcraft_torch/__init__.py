@@ -4,7 +4,8 @@ Importing this module loads ``_C.so`` (built in-tree by
 ``branchcraft-cuda_amd/build.py``) which registers ``torch.ops.branchcraft``
 with the reference's schemas (bindings/torch_ops.cpp:144-148 of
 Haaziq386/branchcraft-cuda) plus ``paged_decode`` (the reference's C++
-``branchcraft::decode``), ``copy_pages_`` and ``commit_paths_``.  There is
+``branchcraft::decode``), ``copy_pages_``, ``commit_paths_`` and the chunk ops
+(``build_tables``, ``append_kv_``, ``chunk_attention``).  There is
 no CPU or Python fallback: a missing extension raises ImportError, and the
 ops have only a GPU implementation.
 
@@ -66,6 +67,24 @@ def _fake_int_tensor(like, values):
     return like.new_empty((len(values),), dtype=torch.int32)
 
 
+@torch.library.register_fake("branchcraft::build_tables")
+def _fake_build_tables(page_ids, lengths, counts, max_pages, tokens):
+    batch = lengths.shape[0]
+    return tuple(lengths.new_empty(shape)
+                 for shape in ((batch, max_pages), (batch + 1,), (tokens,), (tokens,)))
+
+
+@torch.library.register_fake("branchcraft::append_kv_")
+def _fake_append_kv(cache_k, cache_v, k, v, slots):
+    return None
+
+
+@torch.library.register_fake("branchcraft::chunk_attention")
+def _fake_chunk_attention(q, k, v, pages, lengths, starts, scale=None, causal=True, window=0,
+                          cap=0.0, slopes=None, prefix=None, first=None):
+    return q.new_empty(q.shape)
+
+
 def tree_verify(q, prefix_k, prefix_v, pages, lengths, draft_k, draft_v, parent):
     """FP32 [batch, node, query head, dim] outputs; every node attends to its
     request's paged prefix and its own ancestor chain (itself included)."""
@@ -124,6 +143,41 @@ def int_tensor(like, values):
     return torch.ops.branchcraft.int_tensor(like, values)
 
 
+def build_tables(page_ids, lengths, counts, max_pages, tokens):
+    """Block table, row offsets, slot map and positions of a step, on the GPU:
+    ``(pages [batch, max_pages], starts [batch + 1], slots [tokens], positions
+    [tokens])``, all int32.  Request b has ``lengths[b]`` tokens, the last
+    ``counts[b]`` of them new, and its ceil(length / 16) page ids follow those of
+    the request before it in ``page_ids``.  -1 stands behind a request's pages,
+    in rows behind the last request, and for rows without a slot."""
+    return torch.ops.branchcraft.build_tables(page_ids, lengths, counts, max_pages, tokens)
+
+
+def append_kv_(cache_k, cache_v, k, v, slots):
+    """Write new tokens' K and V rows ([tokens, KV heads, dim], FP16 or BF16, any
+    strides with a contiguous last dim) to the slots of ``build_tables``; -1 and
+    slots outside the pool are skipped.  The pools may be strided views, such
+    as the two halves of a packed cache."""
+    return torch.ops.branchcraft.append_kv_(cache_k, cache_v, k, v, slots)
+
+
+def chunk_attention(q, k, v, pages, lengths, starts, *, scale=None, causal=True, window=0,
+                    cap=0.0, slopes=None, prefix=None, first=None):
+    """Attention of every request's new tokens over its pages: [tokens, query
+    heads, dim] in the inputs' type (FP16 or BF16).
+
+    Request b's rows of ``q`` are ``starts[b] .. starts[b+1] - 1``, the last of
+    its ``lengths[b]`` tokens, whose K and V the pages already hold.  The row at
+    place p sees the tokens up to p (all with ``causal=False``; at least the
+    first ``prefix[b]`` with a prefix), from ``p - window + 1`` with a window,
+    from ``first[row]`` with documents.  Scores are ``scale * q.k`` (default
+    1/sqrt(dim)), then ``cap * tanh(score / cap)``, then minus ``slopes[head] *
+    |p - token|``.  Rows that see nothing, and rows of no request, are zero."""
+    return torch.ops.branchcraft.chunk_attention(
+        q, k, v, pages, lengths, starts, scale, causal, window, cap, slopes, prefix, first)
+
+
 __all__ = ["tree_verify", "packed_decode_out", "paged_decode",
            "commit_path_", "copy_pages_", "commit_paths_", "write_prefix_", "int_tensor",
+           "build_tables", "append_kv_", "chunk_attention",
            "LIBRARY_PATH"]

@@ -10,15 +10,17 @@ a shared partial page and the accepted-path copy -- runs as the
 ``copy_pages_`` and ``commit_path_`` HIP ops on the current stream.
 ``commit_many`` commits several requests with two launches (every clone, then
 every accepted node) and one for their index lists, and leaves the same pages and page tables
-as committing them one by one in the same order.
+as committing them one by one in the same order.  ``extend`` appends ordinary new
+tokens to several requests and attends to them: a chunk of a prompt, a turn, a
+decode step.
 """
 
 from __future__ import annotations
 
 import torch
 
-from . import (commit_path_, commit_paths_, copy_pages_, int_tensor, tree_verify,
-               write_prefix_)
+from . import (append_kv_, build_tables, chunk_attention, commit_path_, commit_paths_,
+               copy_pages_, int_tensor, tree_verify, write_prefix_)
 from .pages import CommitPlan, PageOwner, Snapshot
 
 __all__ = ["PagedTreeCache", "Snapshot", "CommitPlan"]
@@ -172,6 +174,74 @@ class PagedTreeCache:
         if error is not None:
             raise error
         return plans
+
+    def extend(self, requests: list[int], counts: list[int], q: torch.Tensor,
+               k: torch.Tensor, v: torch.Tensor, **options) -> torch.Tensor:
+        """Append ``counts[i]`` new tokens to request ``requests[i]`` and attend.
+
+        ``k`` and ``v`` [tokens, KV heads, dim] hold the new tokens' rows,
+        request after request, and ``q`` [tokens, query heads, dim] their
+        queries; the result is ``chunk_attention`` of them over the requests'
+        pages, the new tokens included (``options`` are its keywords).  Pages
+        are planned as consecutive commits would take them: shared partial
+        pages are cloned first.  A pool without room for all of it raises
+        before anything changes.  A count may be zero."""
+        if len(requests) != len(counts) or len(set(requests)) != len(requests) or not requests:
+            raise ValueError("requests must be distinct and match counts")
+        if any(n < 0 for n in counts):
+            raise ValueError("counts must not be negative")
+        total = sum(counts)
+        shape = (total, *self.k.shape[2:])
+        if tuple(k.shape) != shape or tuple(v.shape) != shape:
+            raise ValueError("k and v must have one row of the cache's heads per new token")
+        if (q.ndim != 3 or q.shape[0] != total or q.shape[2] != shape[2] or q.shape[1] < 1
+                or q.shape[1] % shape[1]):
+            raise ValueError("q must have one row of query heads per new token")
+        if any(x.dtype != self.k.dtype or x.device != self.k.device for x in (q, k, v)):
+            raise ValueError("q, k and v must have the cache's type and device")
+        if not self.k.is_cuda:
+            raise ValueError("extend needs a cache on the GPU")
+        if torch.is_grad_enabled() and any(x.requires_grad for x in (self.k, self.v, k, v)):
+            raise ValueError("extend is not differentiable: detach k and v, or use no_grad")
+        q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
+        if options:  # refused here, before any page is taken
+            first = options.get("first")
+            if first is not None and tuple(first.shape) != (total,):
+                raise ValueError("first must have one entry per new token")
+            none = self._upload([-1] * len(requests), [0] * len(requests), [0] * (len(requests) + 1))
+            chunk_attention(q[:0], self.k, self.v, none[0].unsqueeze(1), *none[1:],
+                            **(options if first is None else options | {"first": first[:0]}))
+        owner = self.owner
+        # Requests that share a partial last page: all but the last to write
+        # it take a clone.
+        holders: dict[int, int] = {}
+        needed = 0
+        for request, n in zip(requests, counts):
+            length, pages = owner.lengths[request], owner.pages[request]
+            if not n:
+                continue
+            needed += -(-(length + n) // 16) - len(pages)
+            if length % 16:
+                last = pages[-1]
+                left = holders.setdefault(last, owner.refcount[last])
+                if left > 1:
+                    needed += 1
+                    holders[last] = left - 1
+        if needed > len(owner.free):
+            raise RuntimeError("KV page pool exhausted")
+        plans = [owner.plan_commit(request, n) for request, n in zip(requests, counts) if n]
+        clones = [plan.cow for plan in plans if plan.cow is not None]
+        lists = [owner.pages[request] for request in requests]
+        lengths = [owner.lengths[request] for request in requests]
+        old, fresh, ids, length, count = self._upload(
+            [old for old, _ in clones], [fresh for _, fresh in clones],
+            [page for pages in lists for page in pages], lengths, counts)
+        if clones:
+            copy_pages_(self.k, self.v, old, fresh)
+        width = max(1, *(len(pages) for pages in lists))
+        table, starts, slots, _ = build_tables(ids, length, count, width, total)
+        append_kv_(self.k, self.v, k, v, slots)
+        return chunk_attention(q, self.k, self.v, table, length, starts, **options)
 
     def _run_plans(self, plans, paths, draft_k, draft_v) -> None:
         if not plans:

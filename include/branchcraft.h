@@ -321,6 +321,119 @@ int bc_packed_decode_noalloc(bc_shape shape, const bc_half* q, const bc_half* pa
                              long long head_stride, long long slot_stride,
                              long long kv_stride, float scale, bc_stream_t stream);
 
+/* ---- chunks of new tokens ---- */
+
+/* Element types of bc_chunk_attention's q, k, v and output. */
+enum {
+  BC_FLOAT16 = 0,
+  BC_BFLOAT16 = 1,
+};
+/* Most query heads bc_chunk_attention takes. */
+#define BC_MAX_CHUNK_HEADS 4096
+
+/* Strides in elements; the head dimension is contiguous.  Rows of new tokens
+ * [tokens, heads, D], and pools [P, 16, Hkv, D] in any order of pages, slots
+ * and heads (a contiguous pool: page 16*Hkv*D, slot Hkv*D, head D). */
+typedef struct bc_row_strides {
+  long long token;
+  long long head;
+} bc_row_strides;
+
+typedef struct bc_pool_strides {
+  long long page;
+  long long slot;
+  long long head;
+} bc_pool_strides;
+
+/* Block table, row offsets and slot map of a step from the requests' lengths,
+ * all of them on the device.  Request b has lengths[b] tokens, the last
+ * counts[b] of them new, and its ceil(lengths[b] / 16) page ids follow those
+ * of the request before it in page_ids [held].  Writes
+ *   pages [batch, max_pages]: the request's ids, -1 behind them;
+ *   starts [batch + 1]: the offset of each request's new tokens in the rows
+ *     of a step (and the end of the last one's), at most `tokens`;
+ *   positions [tokens]: each row's place in its request;
+ *   slots [tokens]: 16 * page + place in the page, as bc_append_kv takes it.
+ * Rows behind the last request have -1 for both, and so have the slots of
+ * rows whose place lies before the request, past its row of the table or past
+ * page_ids, or in a page with a negative id or one of 2^27 or more; a
+ * position before the request is -1.  Negative lengths and counts count as
+ * 0.  Rejects: batch or max_pages < 1, held or tokens < 0, null pointers
+ * (those of empty arrays aside), tables or maps of 2^27 entries a request or more. */
+int bc_build_tables(const int32_t* page_ids, int held, const int32_t* lengths,
+                    const int32_t* counts, int batch, int max_pages, int tokens,
+                    int32_t* pages, int32_t* starts, int32_t* slots,
+                    int32_t* positions, bc_stream_t stream);
+
+/* New tokens' K and V rows into the pool, bit for bit: row t of k and v
+ * ([tokens, Hkv, D], 16-bit elements of any type) goes to slot slots[t] % 16
+ * of page slots[t] / 16.  Negative slots and slots of pages outside
+ * [0, physical_pages) are skipped; two rows of one slot leave either row or
+ * a mixture.  Rows and pools must not overlap.  Any 2-byte aligned pointers
+ * and any non-negative strides work (16-byte copies where all of them allow
+ * it).  Uses shape.kv_heads, shape.dim and shape.physical_pages; rejects
+ * values below 1, dim not 64/128, tokens < 0, null pointers, negative
+ * strides. */
+int bc_append_kv(bc_shape shape, const bc_half* k, const bc_half* v,
+                 bc_row_strides k_strides, bc_row_strides v_strides,
+                 bc_half* cache_k, bc_half* cache_v,
+                 bc_pool_strides cache_k_strides, bc_pool_strides cache_v_strides,
+                 const int32_t* slots, int tokens, bc_stream_t stream);
+
+/* Inputs of bc_chunk_attention.  q [tokens, Hq, D]; k, v [P, 16, Hkv, D];
+ * output [tokens, Hq, D] contiguous, of the inputs' type.  pages [B,
+ * max_pages], lengths [B] (each request's tokens in the cache, its new ones
+ * included) and starts [B + 1] (request b's rows are starts[b] ..
+ * starts[b+1] - 1: its last tokens, in order).  Null where they do not apply:
+ * slopes [Hq], prefix [B], first [tokens]. */
+typedef struct bc_chunk_inputs {
+  const bc_half* q;
+  const bc_half* k;
+  const bc_half* v;
+  const int32_t* pages;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const float* slopes;
+  const int32_t* prefix;
+  const int32_t* first;
+  bc_half* output;
+  bc_row_strides q_strides;
+  bc_pool_strides k_strides;
+  bc_pool_strides v_strides;
+  int tokens;
+  int dtype;  /* BC_FLOAT16 or BC_BFLOAT16 */
+  int causal;
+  int window; /* 0: none */
+  float scale;
+  float cap;  /* 0: none */
+} bc_chunk_inputs;
+
+/* Attention of each request's new tokens over its tokens in the paged cache,
+ * theirs included (write them first, with bc_append_kv).  Row i of request b's n
+ * stands at place p = lengths[b] - n + i and sees the tokens lo .. hi:
+ *   hi = lengths[b] - 1 without causal, else p, or prefix[b] - 1 where that
+ *        is more (a prefix that all rows see);
+ *   lo = 0, p - window + 1 with a window, first[row] where that is more (the
+ *        row's document).
+ * score = scale * q.k, then cap * tanh(score / cap) with a cap, then minus
+ * slopes[head] * |p - token| with slopes; the output is the softmax-weighted
+ * sum of V, and zeros for a row that sees nothing and for rows of no request.
+ * Tokens whose page id lies outside [0, physical_pages) are not seen, and
+ * lengths past the table's row end there (places stay counted from
+ * lengths[b]).  What a row does not see never reaches its output, NaN and
+ * infinity included.  Scores, sums and the output's accumulation are 32-bit;
+ * the weights are rounded to the inputs' type for the product with V.
+ * Rejects: batch/Hq/Hkv < 1, Hq % Hkv != 0, Hq over BC_MAX_CHUNK_HEADS,
+ * dim not 64/128, max_pages or physical_pages < 1, tokens or window < 0, scale not positive and finite,
+ * cap negative or not finite, negative strides, null pointers. */
+int bc_chunk_attention(bc_shape shape, bc_chunk_inputs in, void* workspace,
+                       size_t workspace_bytes, bc_stream_t stream);
+
+/* Bytes of workspace with which bc_chunk_attention may split long requests
+ * over several workgroups.  A null workspace, a smaller one or one that is
+ * not aligned to 16 bytes is ignored: nothing is split then. */
+size_t bc_chunk_attention_workspace_size(bc_shape shape, int tokens);
+
 /* Library version string, for logs. */
 const char* bc_version(void);
 
