@@ -1,5 +1,5 @@
 // Device helpers shared by the Branchcraft gfx950 kernels: exp2, DPP and
-// cross-row reductions over wave64 lanes, and 16-byte loads.
+// cross-row reductions over wave64 lanes, 16-byte loads, and token tiles in LDS.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -141,6 +141,43 @@ __device__ __forceinline__ void store4f(float* p, float a, float b, float c, flo
     p[2] = c;
     p[3] = d;
   }
+}
+
+// 16-byte chunk c of token row `row` sits at chunk c ^ swz<D>(row) of the
+// row's place in LDS: rows need no padding (a load straight into LDS fills
+// consecutive lanes' chunks), and both the K reads (16 rows, one chunk each)
+// and the V transpose reads (four rows, four chunks each) touch every bank
+// once.
+template <int D>
+__device__ __forceinline__ int swz(int row) {
+  return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+}
+
+// 16 bytes per lane straight into LDS, lane i's at dst + 16 i (dst
+// wave-uniform).  No register waits for it: the caller waits with
+// wait_loads() before the barrier that publishes the data.
+__device__ __forceinline__ void load_to_lds(const void* src, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(src), "s"(dst)
+               : "memory");
+}
+
+__device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base), "s"(dst)
+               : "memory");
+}
+
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Wave-local LDS handoff: this wave's LDS writes are visible to its own
+// later reads (and its reads done before its later writes).
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 }  // namespace bcd

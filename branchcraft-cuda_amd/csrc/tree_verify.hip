@@ -614,14 +614,6 @@ __device__ __forceinline__ void tile_pv(const _Float16* vtr, const f16x8 (&pb)[2
       acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[dt][st], pl[st], acc[dt], 0, 0, 0);
 }
 
-// Wave-local LDS handoff: this wave's LDS writes are visible to its own
-// later reads (and its reads done before its later writes).
-__device__ __forceinline__ void wave_lds_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // Split tree verification.  Unit = (request, KV head, row tile); its work is
 // one tile space: the draft tiles [0, ntd) followed by the prefix tiles (32
 // tokens each, up to the request's length).  Workgroup `part` of a unit
@@ -1257,35 +1249,6 @@ __device__ __forceinline__ void row_weights(const f32x16& sc, int half, float sc
   pb = __builtin_bit_cast(f16x8, u32x4{wh[0], wh[1], wh[2], wh[3]});
   pl = __builtin_bit_cast(f16x8, u32x4{wl[0], wl[1], wl[2], wl[3]});
 }
-
-// 16-byte chunk c of token row `row` sits at chunk c ^ swz<D>(row) of the
-// row's place in LDS: rows need no padding (a load straight into LDS fills
-// consecutive lanes' chunks), and both the K reads (16 rows, one chunk each)
-// and the V transpose reads (four rows, four chunks each) touch every bank
-// once.
-template <int D>
-__device__ __forceinline__ int swz(int row) {
-  return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-}
-
-// 16 bytes per lane straight into LDS, lane i's at dst + 16 i (dst
-// wave-uniform).  No register waits for it: the caller waits with
-// wait_loads() before the barrier that publishes the data.
-__device__ __forceinline__ void load_to_lds(const void* src, unsigned dst) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-               :
-               : "v"(src), "s"(dst)
-               : "memory");
-}
-
-__device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-               :
-               : "v"(off), "s"(base), "s"(dst)
-               : "memory");
-}
-
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Tiles of one (KV head, row tile) of a request of length len: its draft
 // tiles, then its prefix tiles.
