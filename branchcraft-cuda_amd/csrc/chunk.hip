@@ -7,6 +7,8 @@
 // (src/paged_gqa.cu) or a tree of draft tokens outside the cache
 // (src/tree_attention.cu), and fills pages on the host
 // (python/branchcraft_torch/transaction.py:64-81).
+#include <type_traits>
+
 #include "bc_device.h"
 #include "bc_host.h"
 
@@ -277,6 +279,10 @@ struct Num<_Float16> {
   // running maximum may lag by 2^kRescaleSlack, which leaves the largest at
   // most 2^15, and the smallest normal FP16 weight at 2^-21.
   static constexpr float kLift = 7.f;
+  static __device__ __forceinline__ float add2(uint32_t w, float sum) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, w), v2{(_Float16)1.f, (_Float16)1.f}, sum,
+                                  false);
+  }
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a),
                                                   __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -288,6 +294,10 @@ struct Num<__bf16> {
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kCarry = 0x00800080;
   static constexpr float kLift = 0.f;
+  static __device__ __forceinline__ float add2(uint32_t w, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, w),
+                                           v2{(__bf16)1.f, (__bf16)1.f}, sum, false);
+  }
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a),
                                                    __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -530,7 +540,7 @@ __device__ __forceinline__ void finish_scores(const ChunkParams& C, f32x16 (&sc)
 // Online softmax and O^T += V^T P^T over NT staged tiles.  The maximum moves
 // only when it would grow by more than kRescaleSlack.  Weights are rounded to
 // T, to nearest, for the product (half a step of T each, as the output's own
-// rounding); their sum is taken before the rounding, in 32 bits.
+// rounding); their sum is of the rounded weights, in 32 bits.
 template <typename T, int D, bool PLAIN, int NT>
 __device__ __forceinline__ void weigh(f32x16 (&sc)[NT], Rows<D>& r, const uint16_t* vt,
                                       const Offsets<D>& o, float scale_log2) {
@@ -561,9 +571,8 @@ __device__ __forceinline__ void weigh(f32x16 (&sc)[NT], Rows<D>& r, const uint16
       const float s0 = sc[grp / 2][8 * (grp % 2) + 2 * x], s1 = sc[grp / 2][8 * (grp % 2) + 2 * x + 1];
       const float p0 = fast_exp2(PLAIN ? __builtin_fmaf(s0, scale_log2, -base) : s0 - base);
       const float p1 = fast_exp2(PLAIN ? __builtin_fmaf(s1, scale_log2, -base) : s1 - base);
-      r.l += p0;
-      r.l += p1;
       w[x] = pack2<T>(p0, p1);
+      r.l = N::add2(w[x], r.l);
     }
     pb[grp % 2] = w;
   };
@@ -727,23 +736,41 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
   const uint16_t* const vb = C.v + kvh * C.vh;
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(
       (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)s_kv + wave * 1024);
+  // The pages of 16 steps, one per lane: their addresses, so that a step reads
+  // them out instead of multiplying, and which lie in the pool (others are
+  // loaded from page 0 and masked).
   const int32_t* const table = C.pages + (size_t)it.b * C.max_pages;
-  auto load_ids = [&](int t) { return table[min(max(t * 4 + lane, 0), C.max_pages - 1)]; };
-  auto issue_chunk = [&](int x, const int (&id)[4], int buf) {
-    int p = CPR == 16 ? id[x] : wave < 2 ? id[2 * x % 4] : id[(2 * x + 1) % 4];
-    p = (unsigned)p < (unsigned)C.phys_pages ? p : 0;
+  auto load_ids = [&](int t) { return table[min(t * 4 + lane, C.max_pages - 1)]; };
+  unsigned long long k_at = 0, v_at = 0, pool = 0;
+  auto take_ids = [&](int ids) {
+    const bool in = (unsigned)ids < (unsigned)C.phys_pages;
+    pool = __builtin_amdgcn_ballot_w64(in);
+    const long long id = in ? ids : 0;
+    k_at = (unsigned long long)(kb + id * C.kp);
+    v_at = (unsigned long long)(vb + id * C.vp);
+  };
+  auto lane_of = [&](unsigned long long x, int from) {
+    return (const void*)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), from) << 32 |
+                         (unsigned)__builtin_amdgcn_readlane((int)x, from));
+  };
+  auto issue_chunk = [&](int x, int at, int buf) {
+    const int from = 4 * at + (CPR == 16 ? x : 2 * x + (wave >> 1));
     const unsigned dst = lds0 + buf * (4 * HALF) + x * 4096;
-    load_to_lds(kb + p * C.kp, koff, dst);
-    load_to_lds(vb + p * C.vp, voff, dst + 2 * HALF);
+    load_to_lds(lane_of(k_at, from), koff, dst);
+    load_to_lds(lane_of(v_at, from), voff, dst + 2 * HALF);
   };
-  auto take_ids = [&](int v, int at, int (&id)[4]) {
+  // The tokens of step t that are any: in pages of the pool, below the length.
+  auto tokens_of = [&](int t, int pages) {
+    const int left = it.len - t * kStep;
+    unsigned long long ok = left >= 64 ? ~0ull : left > 0 ? (1ull << left) - 1 : 0ull;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) id[q] = __builtin_amdgcn_readlane(v, 4 * at + q);
+    for (int q = 0; q < 4; ++q)
+      if (!((pages >> q) & 1)) ok &= ~(0xffffull << (16 * q));
+    return ok;
   };
-  // A step that every row of the workgroup sees whole, of valid tokens.
-  auto whole = [&](int t, unsigned long long ok) {
-    return ok == ~0ull && t * kStep >= wg.all_lo && t * kStep + kStep - 1 <= wg.all_hi;
-  };
+  // Steps whole_lo .. whole_hi - 1 are seen whole by every row, given their pages.
+  const int whole_lo = wg.all_lo / kStep + (wg.all_lo % kStep != 0);
+  const int whole_hi = min(wg.all_hi == 0x7fffffff ? 0 : wg.all_hi + 1, it.len) / kStep;
   // Each thread tidies the chunks that its own loads, already waited for,
   // have filled.
   auto inspect = [&](unsigned long long ok, uint16_t* v) {
@@ -753,78 +780,75 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
       u32x4* const at = reinterpret_cast<u32x4*>(v + (tid + 256 * x) * 8);
       bad |= tidy<T>(at, (ok >> (lrow + 256 / CPR * x)) & 1u);
     }
-    return bad;
+    return __builtin_amdgcn_readfirstlane(__syncthreads_or(bad)) != 0;
   };
 
   const Offsets<D> o = read_offsets<D>(lane);
   const float scale_log2 = C.scale * kLog2e;
   bool is_whole = true, bad = false;
-  unsigned long long ok = 0;
-  int ids = 0, ids_next = 0, id[4];
+  int pages = 15;  // of the step at hand, a bit each: in the pool
+  int ids_next = 0;
   if (t0 < tend) {
-    ids = load_ids(t0);
+    take_ids(load_ids(t0));
     ids_next = load_ids(t0 + 16);
-    take_ids(ids, 0, id);
 #pragma unroll
-    for (int x = 0; x < NX; ++x) issue_chunk(x, id, 0);
-    ok = valid_tokens(C, id, it.len - t0 * kStep);
-    is_whole = whole(t0, ok);
+    for (int x = 0; x < NX; ++x) issue_chunk(x, 0, 0);
+    pages = (int)pool & 15;
+    is_whole = pages == 15 && t0 >= whole_lo && t0 < whole_hi;
     // The wait for Q belongs here, not inside the loop over steps.
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qB[s]));
     wait_loads();
-    if (!is_whole) bad = inspect(ok, s_kv + HALF);
-    bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));
+    if (!is_whole)
+      bad = inspect(tokens_of(t0, pages), s_kv + HALF);
+    else
+      __syncthreads();
   }
-  int k = 0;
-  for (int t = t0; t < tend; ++t) {
-    bool whole_n = true;
-    unsigned long long ok_n = 0;
+  // One step, its K and V in buffer `buf`; the next one's loads go out between
+  // the score products.
+  auto step = [&](auto which, int t) {
+    constexpr int buf = decltype(which)::value;
+    const uint16_t* const kt = s_kv + buf * (2 * HALF);
     const bool next = t + 1 < tend;
-    if (next) {
-      const int at = (t + 1 - t0) % 16;
-      if (at == 0) {
-        ids = ids_next;
-        ids_next = load_ids(t + 17);
-      }
-      take_ids(ids, at, id);
-      ok_n = valid_tokens(C, id, it.len - (t + 1) * kStep);
-      whole_n = whole(t + 1, ok_n);
+    const int at = (t + 1 - t0) % 16;
+    if (at == 0 && next) {
+      take_ids(ids_next);
+      ids_next = load_ids(t + 17);
     }
-    const uint16_t* const kt = s_kv + k * (2 * HALF);
+    const int pages_n = (int)(pool >> (4 * at)) & 15;
+    const bool whole_n = !next || (pages_n == 15 && t + 1 >= whole_lo && t + 1 < whole_hi);
     f32x16 sc[2];
     u32x4 kf[2][KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int i = 0; i < 2; ++i) kf[i][s] = lds16(kt + i * 32 * D + o.k[s]);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) sc[i][j] = 0.f;
+    const f32x16 zero = {};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sc[i] = Num<T>::mfma(kf[i][s], qB[s], sc[i]);
+      for (int i = 0; i < 2; ++i) sc[i] = Num<T>::mfma(kf[i][s], qB[s], s == 0 ? zero : sc[i]);
       if (s % 2 == 1 && s / 2 < NX) {
-        if (next) issue_chunk(s / 2, id, k ^ 1);
+        if (next) issue_chunk(s / 2, at, buf ^ 1);
       }
     }
-    const bool edge = !is_whole && (ok != ~0ull || t * kStep < mine.all_lo ||
-                                    t * kStep + kStep - 1 > mine.all_hi);
-    finish_scores<T, D, PLAIN, 2>(C, sc, R, t * kStep, g, edge, ok);
+    const bool edge = !is_whole && (pages != 15 || it.len - t * kStep < kStep ||
+                                    t * kStep < mine.all_lo || t * kStep + kStep - 1 > mine.all_hi);
+    finish_scores<T, D, PLAIN, 2>(C, sc, R, t * kStep, g, edge, edge ? tokens_of(t, pages) : 0);
     weigh<T, D, PLAIN, 2>(sc, R, kt + HALF, o, scale_log2);
     if (bad) add_untidy<T, D>(C, it, kvh, R, t * kStep, kStep, g);
     wait_loads();
     bad = false;
     if (!whole_n)
-      bad = __builtin_amdgcn_readfirstlane(
-          __syncthreads_or(inspect(ok_n, s_kv + (k ^ 1) * (2 * HALF) + HALF)));
+      bad = inspect(tokens_of(t + 1, pages_n), s_kv + (buf ^ 1) * (2 * HALF) + HALF);
     else
       __syncthreads();
-    k ^= 1;
     is_whole = whole_n;
-    ok = ok_n;
+    pages = pages_n;
+  };
+  for (int t = t0; t < tend; t += 2) {
+    step(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < tend) step(std::integral_constant<int, 1>{}, t + 1);
   }
 
   R.l += shfl_xor_f(R.l, 32);
