@@ -187,7 +187,7 @@ __device__ __forceinline__ int clamp_len(const ChunkParams& P, int b) {
 __device__ __forceinline__ int2 row_range(const ChunkParams& P, int b, int t, int pos, int len) {
   int lo = 0, hi = len - 1;
   if (P.causal) hi = min(hi, P.prefix ? max(pos, max(P.prefix[b], 0) - 1) : pos);
-  if (P.window > 0) lo = max(lo, pos - P.window + 1);
+  if (P.window > 0) lo = max(lo, max(pos, 0) - P.window + 1);
   if (P.first) lo = max(lo, P.first[t]);
   return pos < 0 ? make_int2(1, 0) : make_int2(lo, hi);
 }
@@ -313,48 +313,68 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 constexpr int kStep = 64;       // tokens per step of a tile of rows
 constexpr int kFewRows = 32;    // rows of a request that take the narrow form
 constexpr int kManyRows = 128;  // rows per workgroup of the wide form
-constexpr int kLeastSteps = 4;  // fewest steps per part of a split tile
+constexpr int kLeastSteps = 4;  // fewest steps per part of a split tile of rows
+constexpr int kLeastRun = 4;    // fewest 32-token tiles per wave of the narrow form
 
 struct TileParams {
   ChunkParams c;
-  float* part_acc;  // [parts][Hkv][part_rows][D]; null: nothing is split
-  float* part_ml;   // [parts][Hkv][part_rows][2]: maximum and sum
-  int* records;     // count, then four ints per split tile
-  int part_rows;    // rows of a partial
+  float* part_acc;  // [partial row][Hkv][D]; null: nothing is split
+  float* part_ml;   // [partial row][Hkv][2]: maximum and sum
+  int4* records;    // two counts, then two int4 per split tile and narrow request
   int target;       // workgroups that a batch's work is cut for
-  int most_parts;   // partials per KV head that the workspace holds
+  int waves;        // ranges of the narrow requests' tiles, at most, per KV head
+  int most_parts;   // parts of split tiles, at most, per KV head
+  int part_rows;    // rows of such a part
+  int narrow_rows;  // partial rows of the narrow requests; the others' follow
 };
 
-// What a workgroup does: part `part` of `parts` of row tile `tile` of request
-// b, whose rows (new tokens times group) are `rows`, at tokens start .. of the
+// The rows of one request (new tokens times group), at rows start .. of the
 // step, the first of them at place pos0 of the request.
-struct Item {
-  int b, start, n, len, pos0, rows, tile, part, parts, slot;
-  int record;          // of a split tile
-  long long items;     // where no item has the index: how many there are
-  int records;         // likewise
-  bool found;
+struct Request {
+  int b, start, len, pos0, rows;
 };
+
+template <typename F>
+__device__ __forceinline__ int wave_join_i(int x, F f) {
+  x = f(x, dpp_i<kDppRowMirror>(x));
+  x = f(x, dpp_i<kDppRowHalfMirror>(x));
+  x = f(x, dpp_i<kDppQuadXor2>(x));
+  x = f(x, dpp_i<kDppQuadXor1>(x));
+  x = f(x, __shfl_xor(x, 16, 64));
+  return __builtin_amdgcn_readfirstlane(f(x, __shfl_xor(x, 32, 64)));
+}
 
 __device__ __forceinline__ int wave_min_i(int x) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) x = min(x, __shfl_xor(x, s, 64));
-  return x;
+  return wave_join_i(x, [](int a, int b) { return min(a, b); });
 }
 
 __device__ __forceinline__ int wave_max_i(int x) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) x = max(x, __shfl_xor(x, s, 64));
-  return x;
+  return wave_join_i(x, [](int a, int b) { return max(a, b); });
 }
 
 __device__ __forceinline__ int lanes_sum(int x) {
   return __builtin_amdgcn_readfirstlane(wave_sum_i(x));
 }
 
-// One request's share of the plan, a request per lane.
+// Sums up to and including each lane: inside the 16-lane rows, then the rows'
+// last lanes to the rows behind them.
+__device__ __forceinline__ int lanes_upto(int x) {
+  x += dpp_i<0x111>(x);  // row_shr 1, 2, 4, 8
+  x += dpp_i<0x112>(x);
+  x += dpp_i<0x114>(x);
+  x += dpp_i<0x118>(x);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of a row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31
+  return x;
+}
+
+// A request per lane: its rows and its work, as tiles of 128 rows by steps of
+// 64 tokens, or, with few rows, as tiles of 32 tokens (one at least, so that
+// rows which see nothing are written).
 struct Asked {
-  int start, n, len, full, rows, tiles, steps;
+  int start, n, len, full, rows;
+  int tiles, steps;        // of the wide form
+  int first_tile, narrow;  // of the narrow form
 };
 
 __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b) {
@@ -365,79 +385,118 @@ __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b) {
     a.full = max(P.lengths[b], 0);
     a.len = (int)min((long long)a.full, (long long)P.max_pages * BC_PAGE_SIZE);
     a.rows = a.n * P.group;
-    a.tiles = a.rows <= kFewRows ? (a.rows > 0) : (a.rows + kManyRows - 1) / kManyRows;
-    int span = a.len;
-    if (P.causal && P.window > 0) span = min(span, min(P.window, 1 << 29) + kManyRows + kStep);
-    a.steps = max(1, (span + kStep - 1) / kStep);
+    if (a.rows > kFewRows) {
+      a.tiles = (a.rows + kManyRows - 1) / kManyRows;
+      int span = a.len;
+      if (P.causal && P.window > 0) span = min(span, min(P.window, 1 << 29) + kManyRows + kStep);
+      a.steps = max(1, (span + kStep - 1) / kStep);
+    } else if (a.rows > 0) {
+      int lo = P.window > 0 ? (int)max(0ll, (long long)a.full - a.n - P.window + 1) : 0;
+      if (P.first) {
+        int least = 0x7fffffff;
+        for (int i = 0; i < a.n; ++i) least = min(least, P.first[a.start + i]);
+        lo = max(lo, least);
+      }
+      a.first_tile = min(lo, max(a.len - 1, 0)) / 32;
+      a.narrow = max(1, (a.len + 31) / 32 - a.first_tile);
+    }
   }
   return a;
 }
 
-// Item `idx` of the batch, found by every wave for itself from starts and
-// lengths.  A tile of rows whose steps are more than the batch's work over
-// `target` workgroups is cut into equal parts; as no part is shorter than
-// that share, half of it at least, the split tiles have at most 2 * target /
-// Hkv parts per KV head.  A request's last tiles, which see most, come first.
-// `all`: go to the end and count.
-__device__ __forceinline__ Item plan_item(const TileParams& P, long long idx, int lane, bool all) {
+// How a batch is cut: a tile of rows into parts of at most `share` steps, the
+// narrow requests' tiles, one after another, into ranges of `run`, one per
+// wave.  A step of the wide form takes its four waves about as long as half a
+// tile of the narrow one takes its wave.  No part is shorter than half a
+// share, so there are at most 2 * target / Hkv of them, and at most `waves`
+// ranges.
+struct Cutting {
+  int share, run, narrow;
+  int groups;  // workgroups of the narrow requests: four (range, KV head) each
+};
+
+__device__ __forceinline__ Cutting cut_batch(const TileParams& P, const Asked& head, int lane) {
   const ChunkParams& C = P.c;
-  Asked a = asked_of(C, lane);
-  int share = 0x7fffffff;
-  if (P.part_acc) {
-    long long work = (long long)a.tiles * a.steps;
-    for (int b = 64 + lane; b - lane < C.batch; b += 64) {
-      const Asked x = asked_of(C, b);
-      work += (long long)x.tiles * x.steps;
-    }
-    work = wave_sum_ll(work);
-    const double cut = (double)work * C.hkv / P.target;
-    share = max(kLeastSteps, cut < 1e9 ? (int)cut + 1 : 1000000000);
+  float work = (float)head.tiles * (float)head.steps;
+  int narrow = head.narrow;
+  for (int b = 64 + lane; b - lane < C.batch; b += 64) {
+    const Asked x = asked_of(C, b);
+    work += (float)x.tiles * (float)x.steps;
+    narrow += x.narrow;
   }
+  Cutting c;
+  work = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, wave_sum(work))));
+  c.narrow = lanes_sum(narrow);
+  const float share = (work + 0.5f * (float)c.narrow) * (float)C.hkv / (float)P.target;
+  const float run = ((float)c.narrow + 2.f * work) / (float)P.waves;
+  c.share = max(kLeastSteps, (int)__builtin_fminf(share, 1e9f) + 1);
+  c.run = max(min((int)__builtin_fminf(run, 1e9f) + 1, c.narrow), (c.narrow + P.waves - 1) / P.waves);
+  c.run = max(c.run, kLeastRun);
+  c.groups = ((c.narrow + c.run - 1) / c.run * C.hkv + 3) / 4;
+  return c;
+}
+
+// What a workgroup does of the wide form, or, without a workspace, of either:
+// part `part` of `parts` of row tile `tile` of a request.
+struct Item {
+  Request r;
+  int tile, part, parts;
+  int slot;    // of the first part
+  int record;  // of a split tile
+  long long items;             // where no item has the index: how many there are
+  int records, narrow_records; // likewise
+  bool found;
+};
+
+// Item `idx` of the batch, found by every wave for itself from starts and
+// lengths.  A request's last tiles, which see most, come first.  `all`: go to
+// the end and count.
+__device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int share, long long idx,
+                                          int lane, bool all) {
+  const ChunkParams& C = P.c;
+  const bool split = P.part_acc != nullptr;
   Item it{};
   long long before = 0;
-  int slots = 0, records = 0;
+  int slots = 0, records = 0, narrow = 0;
   for (int b0 = 0; b0 < C.batch; b0 += 64) {
     if (b0 > 0) a = asked_of(C, b0 + lane);
-    const int parts = a.steps > share ? (a.steps + share - 1) / share : 1;
-    const int mine = a.tiles * parts;
-    int upto = mine;  // inclusive sum over the lanes
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int x = __shfl_up(upto, s, 64);
-      upto += lane >= s ? x : 0;
-    }
+    const int parts = split && a.steps > share ? (a.steps + share - 1) / share : 1;
+    const int tiles = split ? a.tiles : a.tiles + (a.narrow > 0);
+    const int mine = tiles * parts;
+    const int upto = lanes_upto(mine);
     const int total = __builtin_amdgcn_readlane(upto, 63);
-    const int cut_parts = parts > 1 ? mine : 0, cut_tiles = parts > 1 ? a.tiles : 0;
-    if (!it.found && idx - before < total) {
+    const int cut_parts = parts > 1 ? mine : 0, cut_tiles = parts > 1 ? tiles : 0;
+    if (!it.found && idx >= before && idx - before < total) {
       const int local = (int)(idx - before);
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > local));
       it.found = true;
-      it.b = b0 + at;
-      it.start = __builtin_amdgcn_readlane(a.start, at);
-      it.n = __builtin_amdgcn_readlane(a.n, at);
-      it.len = __builtin_amdgcn_readlane(a.len, at);
-      it.pos0 = __builtin_amdgcn_readlane(a.full, at) - it.n;
-      it.rows = __builtin_amdgcn_readlane(a.rows, at);
+      it.r.b = b0 + at;
+      it.r.start = __builtin_amdgcn_readlane(a.start, at);
+      it.r.len = __builtin_amdgcn_readlane(a.len, at);
+      it.r.pos0 = __builtin_amdgcn_readlane(a.full - a.n, at);
+      it.r.rows = __builtin_amdgcn_readlane(a.rows, at);
       it.parts = __builtin_amdgcn_readlane(parts, at);
       const int in = local - __builtin_amdgcn_readlane(upto - mine, at);
       const int nth = in / it.parts;
       it.part = in - nth * it.parts;
-      it.tile = __builtin_amdgcn_readlane(a.tiles, at) - 1 - nth;
+      it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - nth;
       if (it.parts > 1) {
-        it.slot = slots + lanes_sum(lane < at ? cut_parts : 0) + in;
+        it.slot = slots + lanes_sum(lane < at ? cut_parts : 0) + in - it.part;
         it.record = records + lanes_sum(lane < at ? cut_tiles : 0) + nth;
-        if (it.slot - it.part + it.parts > P.most_parts) it.parts = 1;  // cannot be: see above
+        if (it.slot + it.parts > P.most_parts) it.parts = 1;  // cannot be: see Cutting
       }
       if (!all) return it;
     }
     before += total;
-    if (P.part_acc) {
+    if (split) {
       slots += lanes_sum(cut_parts);
       records += lanes_sum(cut_tiles);
+      narrow += __builtin_popcountll(__builtin_amdgcn_ballot_w64(a.narrow > 0));
     }
   }
   it.items = before;
-  it.records = records;
+  it.records = min(records, P.most_parts / 2);
+  it.narrow_records = narrow;
   return it;
 }
 
@@ -618,7 +677,7 @@ __device__ __forceinline__ bool tidy(u32x4* at, bool real) {
 // What tidy() took out of the tokens t0 .. t0 + count - 1, added to the rows
 // that see it.  Rare, so token by token and from the cache.
 template <typename T, int D>
-__device__ __forceinline__ void add_untidy(const ChunkParams& C, const Item& it, int kvh, Rows<D>& R,
+__device__ __forceinline__ void add_untidy(const ChunkParams& C, const Request& it, int kvh, Rows<D>& R,
                                            int t0, int count, int g) {
   const int32_t* const table = C.pages + (size_t)it.b * C.max_pages;
 #pragma unroll 1
@@ -642,20 +701,38 @@ __device__ __forceinline__ void add_untidy(const ChunkParams& C, const Item& it,
   }
 }
 
-// Page ids that lie in the pool, and the tokens they and the length allow.
+// The tokens, of 16 per bit of `pages`, that lie in pages of the pool, and
+// below the length, `left` tokens away.
 template <int PAGES>
-__device__ __forceinline__ unsigned long long valid_tokens(const ChunkParams& C, const int (&id)[PAGES],
-                                                           int left) {
-  unsigned long long ok = left >= 64 ? ~0ull : left > 0 ? (1ull << left) - 1 : 0ull;
+__device__ __forceinline__ unsigned long long tokens_of(int left, int pages) {
+  unsigned long long ok = left >= 16 * PAGES ? ~0ull >> (64 - 16 * PAGES) : left > 0 ? (1ull << left) - 1 : 0ull;
 #pragma unroll
   for (int q = 0; q < PAGES; ++q)
-    if ((unsigned)id[q] >= (unsigned)C.phys_pages) ok &= ~(0xffffull << (16 * q));
+    if (!((pages >> q) & 1)) ok &= ~(0xffffull << (16 * q));
   return ok;
 }
 
+// The pages of a wave's next 64, one per lane: their addresses, so that a tile
+// reads them out instead of multiplying, and which lie in the pool (others
+// are loaded from page 0 and masked).
+struct Pages {
+  unsigned long long k, v, in_pool;
+  __device__ __forceinline__ void take(const ChunkParams& C, int kvh, int id) {
+    const bool in = (unsigned)id < (unsigned)C.phys_pages;
+    in_pool = __builtin_amdgcn_ballot_w64(in);
+    const long long page = in ? id : 0;
+    k = (unsigned long long)(C.k + kvh * C.kh + page * C.kp);
+    v = (unsigned long long)(C.v + kvh * C.vh + page * C.vp);
+  }
+  static __device__ __forceinline__ const void* at(unsigned long long x, int lane) {
+    const unsigned hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
+    return (const void*)((unsigned long long)hi << 32 | (unsigned)__builtin_amdgcn_readlane((int)x, lane));
+  }
+};
+
 // This lane's row of the wave's 32: its place, what it sees, and its Q.
 template <typename T, int D, bool PLAIN>
-__device__ __forceinline__ void load_rows(const ChunkParams& C, const Item& it, int r, int kvh,
+__device__ __forceinline__ void load_rows(const ChunkParams& C, const Request& it, int r, int kvh,
                                           int g, Rows<D>& R, u32x4 (&qB)[D / 16]) {
   const bool real = r < it.rows;
   const int i = real ? r / C.group : 0, h = kvh * C.group + (real ? r - i * C.group : 0);
@@ -684,14 +761,25 @@ struct Seen {
 template <int D>
 __device__ __forceinline__ Seen wave_seen(const Rows<D>& R, bool real) {
   const bool some = real && R.lo <= R.hi;
-  const int any_lo = wave_min_i(some ? R.lo : 0x7fffffff), any_hi = wave_max_i(some ? R.hi : -1);
-  const int all_lo = wave_max_i(real ? (some ? R.lo : 0x7fffffff) : 0);
-  const int all_hi = wave_min_i(real ? R.hi : 0x7fffffff);
-  return {__builtin_amdgcn_readfirstlane(any_lo), __builtin_amdgcn_readfirstlane(any_hi),
-          __builtin_amdgcn_readfirstlane(all_lo), __builtin_amdgcn_readfirstlane(all_hi)};
+  return {wave_min_i(some ? R.lo : 0x7fffffff), wave_max_i(some ? R.hi : -1),
+          wave_max_i(real ? (some ? R.lo : 0x7fffffff) : 0), wave_min_i(real ? R.hi : 0x7fffffff)};
 }
 
 __device__ __forceinline__ float one_over(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }
+
+// Where a partial row of a KV head lies, in rows.
+__device__ __forceinline__ size_t partial_row(const TileParams& P, int row, int kvh) {
+  return (size_t)row * P.c.hkv + kvh;
+}
+
+// What the join needs of a split tile of rows: rows row0 .. row0 + rows - 1 of
+// the request whose new tokens start at `start`; part p's are the partial
+// rows first + p * stride ...
+__device__ __forceinline__ void put_record(const TileParams& P, int i, int start, int row0, int rows,
+                                           int parts, int first, int stride) {
+  P.records[1 + 2 * i] = make_int4(start, row0, rows, parts);
+  P.records[2 + 2 * i] = make_int4(first, stride, 0, 0);
+}
 
 // The wide form: 128 rows per workgroup, 32 per wave, each step's K and V
 // shared through LDS.
@@ -699,6 +787,7 @@ template <typename T, int D, bool PLAIN>
 __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, int kvh,
                                           uint16_t* s_kv, Seen* s_seen) {
   const ChunkParams& C = P.c;
+  const Request& rq = it.r;
   constexpr int KS = D / 16, CPR = D / 8;
   constexpr int NX = kStep * CPR / 256;  // chunks per thread and step, of K and of V each
   constexpr int HALF = kStep * D;        // halves of a step's K, then as many of V
@@ -708,8 +797,8 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
   const int row0 = it.tile * kManyRows + wave * 32;
   Rows<D> R;
   u32x4 qB[KS];
-  load_rows<T, D, PLAIN>(C, it, row0 + lr, kvh, g, R, qB);
-  const Seen mine = wave_seen(R, row0 + lr < it.rows);
+  load_rows<T, D, PLAIN>(C, rq, row0 + lr, kvh, g, R, qB);
+  const Seen mine = wave_seen(R, row0 + lr < rq.rows);
   if (lane == 0) s_seen[wave] = mine;
   __syncthreads();
   Seen wg = s_seen[0];
@@ -732,45 +821,20 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
   const int lrow = tid / CPR, lcol = 8 * (tid % CPR ^ swz<D>(lrow));
   const unsigned koff = (unsigned)(((lrow % BC_PAGE_SIZE) * C.ks + lcol) * 2);
   const unsigned voff = (unsigned)(((lrow % BC_PAGE_SIZE) * C.vs + lcol) * 2);
-  const uint16_t* const kb = C.k + kvh * C.kh;
-  const uint16_t* const vb = C.v + kvh * C.vh;
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(
       (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)s_kv + wave * 1024);
-  // The pages of 16 steps, one per lane: their addresses, so that a step reads
-  // them out instead of multiplying, and which lie in the pool (others are
-  // loaded from page 0 and masked).
-  const int32_t* const table = C.pages + (size_t)it.b * C.max_pages;
+  const int32_t* const table = C.pages + (size_t)rq.b * C.max_pages;
   auto load_ids = [&](int t) { return table[min(t * 4 + lane, C.max_pages - 1)]; };
-  unsigned long long k_at = 0, v_at = 0, pool = 0;
-  auto take_ids = [&](int ids) {
-    const bool in = (unsigned)ids < (unsigned)C.phys_pages;
-    pool = __builtin_amdgcn_ballot_w64(in);
-    const long long id = in ? ids : 0;
-    k_at = (unsigned long long)(kb + id * C.kp);
-    v_at = (unsigned long long)(vb + id * C.vp);
-  };
-  auto lane_of = [&](unsigned long long x, int from) {
-    return (const void*)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), from) << 32 |
-                         (unsigned)__builtin_amdgcn_readlane((int)x, from));
-  };
+  Pages pg;
   auto issue_chunk = [&](int x, int at, int buf) {
     const int from = 4 * at + (CPR == 16 ? x : 2 * x + (wave >> 1));
     const unsigned dst = lds0 + buf * (4 * HALF) + x * 4096;
-    load_to_lds(lane_of(k_at, from), koff, dst);
-    load_to_lds(lane_of(v_at, from), voff, dst + 2 * HALF);
-  };
-  // The tokens of step t that are any: in pages of the pool, below the length.
-  auto tokens_of = [&](int t, int pages) {
-    const int left = it.len - t * kStep;
-    unsigned long long ok = left >= 64 ? ~0ull : left > 0 ? (1ull << left) - 1 : 0ull;
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (!((pages >> q) & 1)) ok &= ~(0xffffull << (16 * q));
-    return ok;
+    load_to_lds(Pages::at(pg.k, from), koff, dst);
+    load_to_lds(Pages::at(pg.v, from), voff, dst + 2 * HALF);
   };
   // Steps whole_lo .. whole_hi - 1 are seen whole by every row, given their pages.
   const int whole_lo = wg.all_lo / kStep + (wg.all_lo % kStep != 0);
-  const int whole_hi = min(wg.all_hi == 0x7fffffff ? 0 : wg.all_hi + 1, it.len) / kStep;
+  const int whole_hi = min(wg.all_hi == 0x7fffffff ? 0 : wg.all_hi + 1, rq.len) / kStep;
   // Each thread tidies the chunks that its own loads, already waited for,
   // have filled.
   auto inspect = [&](unsigned long long ok, uint16_t* v) {
@@ -789,18 +853,18 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
   int pages = 15;  // of the step at hand, a bit each: in the pool
   int ids_next = 0;
   if (t0 < tend) {
-    take_ids(load_ids(t0));
+    pg.take(C, kvh, load_ids(t0));
     ids_next = load_ids(t0 + 16);
 #pragma unroll
     for (int x = 0; x < NX; ++x) issue_chunk(x, 0, 0);
-    pages = (int)pool & 15;
+    pages = (int)pg.in_pool & 15;
     is_whole = pages == 15 && t0 >= whole_lo && t0 < whole_hi;
     // The wait for Q belongs here, not inside the loop over steps.
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qB[s]));
     wait_loads();
     if (!is_whole)
-      bad = inspect(tokens_of(t0, pages), s_kv + HALF);
+      bad = inspect(tokens_of<4>(rq.len - t0 * kStep, pages), s_kv + HALF);
     else
       __syncthreads();
   }
@@ -812,10 +876,10 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
     const bool next = t + 1 < tend;
     const int at = (t + 1 - t0) % 16;
     if (at == 0 && next) {
-      take_ids(ids_next);
+      pg.take(C, kvh, ids_next);
       ids_next = load_ids(t + 17);
     }
-    const int pages_n = (int)(pool >> (4 * at)) & 15;
+    const int pages_n = (int)(pg.in_pool >> (4 * at)) & 15;
     const bool whole_n = !next || (pages_n == 15 && t + 1 >= whole_lo && t + 1 < whole_hi);
     f32x16 sc[2];
     u32x4 kf[2][KS];
@@ -832,15 +896,15 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
         if (next) issue_chunk(s / 2, at, buf ^ 1);
       }
     }
-    const bool edge = !is_whole && (pages != 15 || it.len - t * kStep < kStep ||
+    const bool edge = !is_whole && (pages != 15 || rq.len - t * kStep < kStep ||
                                     t * kStep < mine.all_lo || t * kStep + kStep - 1 > mine.all_hi);
-    finish_scores<T, D, PLAIN, 2>(C, sc, R, t * kStep, g, edge, edge ? tokens_of(t, pages) : 0);
+    finish_scores<T, D, PLAIN, 2>(C, sc, R, t * kStep, g, edge, edge ? tokens_of<4>(rq.len - t * kStep, pages) : 0);
     weigh<T, D, PLAIN, 2>(sc, R, kt + HALF, o, scale_log2);
-    if (bad) add_untidy<T, D>(C, it, kvh, R, t * kStep, kStep, g);
+    if (bad) add_untidy<T, D>(C, rq, kvh, R, t * kStep, kStep, g);
     wait_loads();
     bad = false;
     if (!whole_n)
-      bad = inspect(tokens_of(t + 1, pages_n), s_kv + (buf ^ 1) * (2 * HALF) + HALF);
+      bad = inspect(tokens_of<4>(rq.len - (t + 1) * kStep, pages_n), s_kv + (buf ^ 1) * (2 * HALF) + HALF);
     else
       __syncthreads();
     is_whole = whole_n;
@@ -854,8 +918,8 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
   R.l += shfl_xor_f(R.l, 32);
   const int r = row0 + lr;
   if (it.parts > 1) {
-    const size_t at = ((size_t)it.slot * C.hkv + kvh) * P.part_rows + wave * 32 + lr;
-    if (r < it.rows) {
+    const size_t at = partial_row(P, P.narrow_rows + (it.slot + it.part) * P.part_rows + wave * 32 + lr, kvh);
+    if (r < rq.rows) {
       if (g == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * at) = make_float2(R.m, R.l);
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
@@ -885,130 +949,287 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
     const int row = i + lane / CPR, c = lane % CPR;
     const u32x4 w = lds16(out + row * D + (c ^ (row % CPR)) * 8);
     const int rr = row0 + row;
-    if (rr < it.rows) {
+    if (rr < rq.rows) {
       const int n = rr / C.group, h = kvh * C.group + rr - n * C.group;
-      *reinterpret_cast<u32x4*>(C.out + ((size_t)(it.start + n) * C.hq + h) * D + 8 * c) = w;
+      *reinterpret_cast<u32x4*>(C.out + ((size_t)(rq.start + n) * C.hq + h) * D + 8 * c) = w;
     }
   }
 }
 
-// The narrow form: the few rows of a request, at most 32, in every wave of
-// the workgroup; each wave streams every fourth tile of 32 tokens through its
-// own part of LDS, K of the next tile behind the scores, V behind the
-// product, without a barrier, and the four states meet at the end.
+// load_to_lds for what a call reads once: the line is marked for early
+// replacement.  64 single tokens over 128-4096 tokens (32/8 heads, D = 128) 122 ->
+// 108 us.
+__device__ __forceinline__ void stream_to_lds(const void* base, unsigned off, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+               :
+               : "v"(off), "s"(base), "s"(dst)
+               : "memory");
+}
+
+// A wave's stream of 32-token tiles through its own part of LDS: K of the next
+// tile goes out behind the scores, V behind the product, and no barrier.
 template <typename T, int D, bool PLAIN>
-__device__ __forceinline__ void narrow_body(const TileParams& P, const Item& it, int kvh,
-                                            uint16_t* s_kv, float2* s_ml) {
+struct Stream {
+  static constexpr int KS = D / 16, CPR = D / 8;
+  static constexpr int RPL = 64 / CPR;         // token rows per load
+  static constexpr int NL = 32 / RPL;          // loads per tile, of K and of V each
+  static constexpr int NV = D == 128 ? 4 : 2;  // lane offsets: the swizzle repeats every 16 rows
+  static constexpr int TILE = 32 * D;
+  static_assert(NL / NV == 2 && NV * RPL == BC_PAGE_SIZE, "a tile is two pages");
+
+  const ChunkParams& C;
+  int kvh, lane;
+  uint16_t* kt;
+  unsigned lds0, koff[NV], voff[NV];
+  Offsets<D> o;
+  Pages pg;
+
+  __device__ __forceinline__ Stream(const ChunkParams& c, int head, uint16_t* area)
+      : C(c), kvh(head), lane(threadIdx.x & 63), kt(area), o(read_offsets<D>(threadIdx.x & 63)) {
+    lds0 = __builtin_amdgcn_readfirstlane(
+        (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)area);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int row = i * RPL + lane / CPR, col = 8 * (lane % CPR ^ swz<D>(row));
+      koff[i] = (unsigned)((row * C.ks + col) * 2);
+      voff[i] = (unsigned)((row * C.vs + col) * 2);
+    }
+  }
+  // Lane i: page i % 2 of tile t + apart * (i / 2).
+  __device__ __forceinline__ int ids(int b, int t, int apart) const {
+    const int i = 2 * (t + apart * (lane >> 1)) + (lane & 1);
+    return C.pages[(size_t)b * C.max_pages + min(i, C.max_pages - 1)];
+  }
+  __device__ __forceinline__ void issue(unsigned long long x, int at, const unsigned (&off)[NV],
+                                        unsigned dst) const {
+    const void* const page[2] = {Pages::at(x, 2 * at), Pages::at(x, 2 * at + 1)};
+#pragma unroll
+    for (int c = 0; c < NL; ++c) stream_to_lds(page[c / NV], off[c % NV], dst + c * 1024);
+  }
+  __device__ __forceinline__ void issue_k(int at) const { issue(pg.k, at, koff, lds0); }
+  __device__ __forceinline__ void issue_v(int at) const { issue(pg.v, at, voff, lds0 + 2 * TILE); }
+  __device__ __forceinline__ int in_pool(int at) const { return (int)(pg.in_pool >> (2 * at)) & 3; }
+
+  // The staged tile's scores; K has been read when this returns.
+  __device__ __forceinline__ void scores(f32x16 (&sc)[1], const u32x4 (&qB)[KS]) const {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // K is there, V may be not
+    const f32x16 zero = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) sc[0] = Num<T>::mfma(lds16(kt + o.k[s]), qB[s], s == 0 ? zero : sc[0]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  // Their softmax and product with V, behind which `next` K loads may be on
+  // their way; V has been read when this returns.
+  __device__ __forceinline__ void product(f32x16 (&sc)[1], const Request& rq, Rows<D>& R, const Seen& mine,
+                                          int t, int pages, bool next) const {
+    const int g = lane >> 5, left = rq.len - t * 32;
+    uint16_t* const vt = kt + TILE;
+    const bool edge = pages != 3 || left < 32 || t * 32 < mine.all_lo || t * 32 + 31 > mine.all_hi;
+    const unsigned long long ok = edge ? tokens_of<2>(left, pages) : 0;
+    finish_scores<T, D, PLAIN, 1>(C, sc, R, t * 32, g, edge, ok);
+    if (next)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // V is there
+    else
+      wait_loads();
+    bool bad = false;
+    if (edge) {
+#pragma unroll
+      for (int c = 0; c < NL; ++c)
+        bad |= tidy<T>(reinterpret_cast<u32x4*>(vt + c * 512 + lane * 8), (ok >> (c * RPL + lane / CPR)) & 1u);
+      bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+      wave_lds_sync();
+    }
+    weigh<T, D, PLAIN, 1>(sc, R, vt, o, C.scale * kLog2e);
+    if (bad) add_untidy<T, D>(C, rq, kvh, R, t * 32, 32, g);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ uint16_t* out_row(const ChunkParams& C, const Request& rq, int r, int kvh) {
+  const int n = r / C.group, h = kvh * C.group + r - n * C.group;
+  return C.out + ((size_t)(rq.start + n) * C.hq + h) * D;
+}
+
+// The narrow form over a batch: the tiles of all requests with few rows, one
+// after another, in ranges of equal length, a range per wave.  A request that
+// a range holds whole leaves as output rows, of others each range leaves a
+// partial.  Range r's partial of a request whose predecessors have n rows
+// starts at partial row 32 r + n: a range's next request is further by the
+// rows of the last one, a request's next range by 32.
+template <typename T, int D, bool PLAIN>
+__device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cutting& cut,
+                                          uint16_t* s_kv) {
   const ChunkParams& C = P.c;
-  constexpr int KS = D / 16, CPR = D / 8;
-  constexpr int RPL = 64 / CPR;   // token rows per load
-  constexpr int NL = 32 / RPL;    // loads per tile, of K and of V each
-  constexpr int NV = D == 128 ? 4 : 2;  // lane offsets: the swizzle repeats every 16 rows
+  const int lane = threadIdx.x & 63, g = lane >> 5, lr = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned task = 4 * blockIdx.x + wave;
+  const int range = task / (unsigned)C.hkv, kvh = task - (unsigned)range * C.hkv;
+  if ((long long)range * cut.run >= cut.narrow) return;
+  const int lo = range * cut.run, hi = min(lo + cut.run, cut.narrow);
+  // The requests that the range meets, one after another.
+  struct Part {
+    Request rq;
+    int x0, tiles, first_tile, nth, row;
+  };
+  int b0 = 0, before = 0, rows_before = 0, nth = 0;
+  int upto, rows, rows_upto;
+  unsigned long long some, left;
+  auto look = [&] {  // at the 64 requests from b0 on
+    upto = lanes_upto(a.narrow);
+    rows = a.narrow > 0 ? a.rows : 0;
+    rows_upto = lanes_upto(rows);
+    some = __builtin_amdgcn_ballot_w64(a.narrow > 0);
+    left = some & __builtin_amdgcn_ballot_w64(before + upto > lo && before + upto - a.narrow < hi);
+  };
+  look();
+  auto next_part = [&](Part& p) {
+    while (!left) {
+      before += __builtin_amdgcn_readlane(upto, 63);
+      rows_before += __builtin_amdgcn_readlane(rows_upto, 63);
+      nth += __builtin_popcountll(some);
+      b0 += 64;
+      if (b0 >= C.batch || before >= hi) return false;
+      a = asked_of(C, b0 + lane);
+      look();
+    }
+    const int at = __builtin_ctzll(left);
+    left &= left - 1;
+    p.rq = Request{b0 + at, __builtin_amdgcn_readlane(a.start, at), __builtin_amdgcn_readlane(a.len, at),
+                   __builtin_amdgcn_readlane(a.full - a.n, at), __builtin_amdgcn_readlane(a.rows, at)};
+    p.tiles = __builtin_amdgcn_readlane(a.narrow, at);
+    p.x0 = before + __builtin_amdgcn_readlane(upto, at) - p.tiles;
+    p.first_tile = __builtin_amdgcn_readlane(a.first_tile, at);
+    p.nth = nth + __builtin_popcountll(some & ((1ull << at) - 1));
+    p.row = rows_before + __builtin_amdgcn_readlane(rows_upto - rows, at);
+    return true;
+  };
+  auto first_of = [&](const Part& p) { return p.first_tile + max(lo, p.x0) - p.x0; };
+
+  Part p;
+  if (!next_part(p)) return;
+  Stream<T, D, PLAIN> st(C, kvh, s_kv + wave * (64 * D));
+  int t = first_of(p), at = 0;
+  st.pg.take(C, kvh, st.ids(p.rq.b, t, 1));
+  int ids_next = st.ids(p.rq.b, t + 32, 1);
+  int pages = st.in_pool(0);
+  st.issue_k(0);
+  st.issue_v(0);
+  for (;;) {  // over the requests
+    Rows<D> R;
+    u32x4 qB[D / 16];
+    load_rows<T, D, PLAIN>(C, p.rq, lr, kvh, g, R, qB);
+    const Seen mine = wave_seen(R, lr < p.rq.rows);
+    const int tend = p.first_tile + min(hi, p.x0 + p.tiles) - p.x0;
+    // The next request's first pages, so that its first tile follows this
+    // one's last as any tile follows another.
+    Part n;
+    const bool more = next_part(n);
+    const int ids_more = more ? st.ids(n.rq.b, first_of(n), 1) : 0;
+    for (;; ++t) {
+      f32x16 sc[1];
+      st.scores(sc, qB);
+      const bool same = t + 1 < tend, next = same || more;
+      int pages_n = 3;
+      if (next) {
+        at = same ? (at + 1) % 32 : 0;
+        if (at == 0) {
+          st.pg.take(C, kvh, same ? ids_next : ids_more);
+          ids_next = same ? st.ids(p.rq.b, t + 33, 1) : st.ids(n.rq.b, first_of(n) + 32, 1);
+        }
+        pages_n = st.in_pool(at);
+        st.issue_k(at);
+      }
+      st.product(sc, p.rq, R, mine, t, pages, next);
+      if (next) st.issue_v(at);
+      pages = pages_n;
+      if (!same) break;
+    }
+    R.l += shfl_xor_f(R.l, 32);
+    const int from = p.x0 / cut.run, parts = (p.x0 + p.tiles - 1) / cut.run - from + 1;
+    const int first = p.row + 32 * from;
+    if (p.x0 >= lo && kvh == 0 && lane == 0)
+      put_record(P, P.most_parts / 2 + p.nth, p.rq.start, 0, p.rq.rows, parts, first, 32);
+    if (parts == 1) {
+      const float inv = one_over(R.l);
+      if (lr < p.rq.rows) {
+        uint16_t* const out = out_row<T, D>(C, p.rq, lr, kvh) + 4 * g;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int jq = 0; jq < 4; ++jq)
+            *reinterpret_cast<uint2*>(out + 32 * dt + 8 * jq) =
+                make_uint2(pack2<T>(R.acc[dt][4 * jq] * inv, R.acc[dt][4 * jq + 1] * inv),
+                           pack2<T>(R.acc[dt][4 * jq + 2] * inv, R.acc[dt][4 * jq + 3] * inv));
+      }
+    } else {
+      const int row = first + 32 * (range - from) + lr;
+      if (lr < p.rq.rows && row < P.narrow_rows) {
+        const size_t to_row = partial_row(P, row, kvh);
+        if (g == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * to_row) = make_float2(R.m, R.l);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int jq = 0; jq < 4; ++jq)
+            *reinterpret_cast<float4*>(P.part_acc + to_row * D + 32 * dt + 8 * jq + 4 * g) =
+                make_float4(R.acc[dt][4 * jq], R.acc[dt][4 * jq + 1], R.acc[dt][4 * jq + 2],
+                            R.acc[dt][4 * jq + 3]);
+      }
+    }
+    if (!more) return;
+    p = n;
+    t = first_of(p);
+  }
+}
+
+// The narrow form without a workspace: a workgroup per request and KV head,
+// its waves every fourth tile each; the four states meet at the end.
+template <typename T, int D, bool PLAIN>
+__device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request& rq, int kvh,
+                                            uint16_t* s_kv, float2* s_ml) {
   constexpr int TILE = 32 * D;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, lr = lane & 31;
   Rows<D> R;
-  u32x4 qB[KS];
-  load_rows<T, D, PLAIN>(C, it, lr, kvh, g, R, qB);
-  const Seen mine = wave_seen(R, lr < it.rows);
-  const int lo = mine.any_lo, hi = mine.any_hi;
-  const int first = lo / kStep;
-  const int steps = hi >= lo ? hi / kStep - first + 1 : 0;
-  const int t0 = 2 * (first + (int)((long long)steps * it.part / it.parts)) + wave;
-  const int tend = min(2 * (first + (int)((long long)steps * (it.part + 1) / it.parts)), hi / 32 + 1);
-
-  unsigned koff[NV], voff[NV];
+  u32x4 qB[D / 16];
+  load_rows<T, D, PLAIN>(C, rq, lr, kvh, g, R, qB);
+  const Seen mine = wave_seen(R, lr < rq.rows);
 #pragma unroll
-  for (int c = 0; c < NV; ++c) {
-    const int row = c * RPL + lane / CPR, col = 8 * (lane % CPR ^ swz<D>(row));
-    koff[c] = (unsigned)((row * C.ks + col) * 2);
-    voff[c] = (unsigned)((row * C.vs + col) * 2);
-  }
-  const uint16_t* const kb = C.k + kvh * C.kh;
-  const uint16_t* const vb = C.v + kvh * C.vh;
-  uint16_t* const kt = s_kv + wave * (2 * TILE);
-  uint16_t* const vt = kt + TILE;
-  const unsigned lds0 = __builtin_amdgcn_readfirstlane(
-      (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)kt);
-  const int32_t* const table = C.pages + (size_t)it.b * C.max_pages;
-  // Lane i: page i % 2 of this wave's tile i / 2 from tile t on.
-  auto load_ids = [&](int t) {
-    return table[min(2 * (t + 4 * (lane >> 1)) + (lane & 1), C.max_pages - 1)];
-  };
-  auto in_pool = [&](int p) { return (unsigned)p < (unsigned)C.phys_pages ? p : 0; };
-  auto issue_k = [&](const int (&id)[2]) {
-#pragma unroll
-    for (int c = 0; c < NL; ++c)
-      load_to_lds(kb + in_pool(id[c / NV]) * C.kp, koff[c % NV], lds0 + c * 1024);
-  };
-  auto issue_v = [&](const int (&id)[2]) {
-#pragma unroll
-    for (int c = 0; c < NL; ++c)
-      load_to_lds(vb + in_pool(id[c / NV]) * C.vp, voff[c % NV], lds0 + 2 * TILE + c * 1024);
-  };
-  static_assert(NL / NV == 2 && NV * RPL == BC_PAGE_SIZE, "a tile is two pages");
-  const Offsets<D> o = read_offsets<D>(lane);
-  const float scale_log2 = C.scale * kLog2e;
-  if (t0 < tend) {
-    int ids = load_ids(t0), ids_next = load_ids(t0 + 128);
-    int id[2] = {__builtin_amdgcn_readlane(ids, 0), __builtin_amdgcn_readlane(ids, 1)};
-#pragma unroll
-    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qB[s]));
-    issue_k(id);
-    issue_v(id);
-    int i = 0;
-    for (int t = t0; t < tend; t += 4) {
-      const bool next = t + 4 < tend;
-      const unsigned long long ok = valid_tokens(C, id, it.len - t * 32) & 0xffffffffull;
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // K is there, V may be not
+  for (int s = 0; s < D / 16; ++s) asm volatile("" : "+v"(qB[s]));
+  Stream<T, D, PLAIN> st(C, kvh, s_kv + wave * (2 * TILE));
+  int t = mine.any_hi < mine.any_lo ? 1 : mine.any_lo / 32 + wave;
+  const int tend = mine.any_hi < mine.any_lo ? 0 : mine.any_hi / 32 + 1;
+  if (t < tend) {
+    st.pg.take(C, kvh, st.ids(rq.b, t, 4));
+    int ids_next = st.ids(rq.b, t + 128, 4), at = 0, pages = st.in_pool(0);
+    st.issue_k(0);
+    st.issue_v(0);
+    for (; t < tend; t += 4) {
       f32x16 sc[1];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) sc[0][j] = 0.f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) sc[0] = Num<T>::mfma(lds16(kt + o.k[s]), qB[s], sc[0]);
-      int id_n[2] = {id[0], id[1]};
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
+      st.scores(sc, qB);
+      const bool next = t + 4 < tend;
+      int pages_n = 3;
       if (next) {
-        i = (i + 1) % 32;
-        if (i == 0) {
-          ids = ids_next;
-          ids_next = load_ids(t + 4 + 128);
+        at = (at + 1) % 32;
+        if (at == 0) {
+          st.pg.take(C, kvh, ids_next);
+          ids_next = st.ids(rq.b, t + 132, 4);
         }
-        id_n[0] = __builtin_amdgcn_readlane(ids, 2 * i);
-        id_n[1] = __builtin_amdgcn_readlane(ids, 2 * i + 1);
-        issue_k(id_n);
+        pages_n = st.in_pool(at);
+        st.issue_k(at);
       }
-      const bool edge = ok != 0xffffffffull || t * 32 < mine.all_lo || t * 32 + 31 > mine.all_hi;
-      finish_scores<T, D, PLAIN, 1>(C, sc, R, t * 32, g, edge, ok);
-      if (next)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // V is there
-      else
-        wait_loads();
-      bool bad = false;
-      if (edge) {
-#pragma unroll
-        for (int c = 0; c < NL; ++c) {
-          u32x4* const at = reinterpret_cast<u32x4*>(vt + c * 512 + lane * 8);
-          bad |= tidy<T>(at, (ok >> (c * RPL + lane / CPR)) & 1u);
-        }
-        bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-        wave_lds_sync();
-      }
-      weigh<T, D, PLAIN, 1>(sc, R, vt, o, scale_log2);
-      if (bad) add_untidy<T, D>(C, it, kvh, R, t * 32, 32, g);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
-      if (next) issue_v(id_n);
-      id[0] = id_n[0];
-      id[1] = id_n[1];
+      st.product(sc, rq, R, mine, t, pages, next);
+      if (next) st.issue_v(at);
+      pages = pages_n;
     }
   }
 
   // The four states through LDS: four-float chunk c of row r at c ^ (r % (D / 4)).
   R.l += shfl_xor_f(R.l, 32);
-  float* const acc = reinterpret_cast<float*>(kt);
+  float* const acc = reinterpret_cast<float*>(st.kt);
   wave_lds_sync();
-  if (lr < it.rows) {
+  if (lr < rq.rows) {
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -1019,7 +1240,7 @@ __device__ __forceinline__ void narrow_body(const TileParams& P, const Item& it,
     if (g == 0) s_ml[wave * 32 + lr] = make_float2(R.m, R.l);
   }
   __syncthreads();
-  for (int x = tid; x < it.rows * (D / 4); x += 256) {
+  for (int x = tid; x < rq.rows * (D / 4); x += 256) {
     const int r = x / (D / 4), c = x % (D / 4);
     float m = kNegInf, l = 0.f;
 #pragma unroll
@@ -1037,16 +1258,9 @@ __device__ __forceinline__ void narrow_body(const TileParams& P, const Item& it,
       sum.z += v.z * a;
       sum.w += v.w * a;
     }
-    if (it.parts > 1) {
-      const size_t at = ((size_t)it.slot * C.hkv + kvh) * P.part_rows + r;
-      if (c == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * at) = make_float2(m, l);
-      *reinterpret_cast<float4*>(P.part_acc + at * D + 4 * c) = sum;
-    } else {
-      const float inv = one_over(l);
-      const int n = r / C.group, h = kvh * C.group + r - n * C.group;
-      *reinterpret_cast<uint2*>(C.out + ((size_t)(it.start + n) * C.hq + h) * D + 4 * c) =
-          make_uint2(pack2<T>(sum.x * inv, sum.y * inv), pack2<T>(sum.z * inv, sum.w * inv));
-    }
+    const float inv = one_over(l);
+    *reinterpret_cast<uint2*>(out_row<T, D>(C, rq, r, kvh) + 4 * c) =
+        make_uint2(pack2<T>(sum.x * inv, sum.y * inv), pack2<T>(sum.z * inv, sum.w * inv));
   }
 }
 
@@ -1068,83 +1282,98 @@ __global__ __launch_bounds__(256, 2) void chunk_tile_kernel(TileParams P) {
   __shared__ float2 s_ml[4 * 32];
   __shared__ Seen s_seen[4];
   const int lane = threadIdx.x & 63;
-  const long long idx = blockIdx.x / (unsigned)P.c.hkv;
-  const int kvh = blockIdx.x - (unsigned)idx * P.c.hkv;
+  // KV heads in the low bits: with eight of them, each XCD serves one.
+  const Asked head = asked_of(P.c, lane);
+  Cutting cut{};
+  if (P.part_acc) cut = cut_batch(P, head, lane);
   const bool counts = blockIdx.x == 0 && P.part_acc;
-  const Item it = plan_item(P, idx, lane, counts);
-  if (counts && threadIdx.x == 0) P.records[0] = it.records;
+  // The narrow requests first: theirs is memory's time, the others' the
+  // matrix units', so they run beside each other.
+  const bool flat = (int)blockIdx.x < cut.groups;
+  // KV heads in the low bits: with eight of them, each XCD serves one.
+  const unsigned in = blockIdx.x - cut.groups, at = in / (unsigned)P.c.hkv;
+  const int kvh = in - at * P.c.hkv;
+  Item it{};
+  if (!flat || counts) it = plan_item(P, head, cut.share, flat ? -1ll : (long long)at, lane, counts);
+  if (counts && threadIdx.x == 0) P.records[0] = make_int4(it.records, it.narrow_records, 0, 0);
+  if (flat) {
+    flat_body<T, D, PLAIN>(P, head, cut, s_kv);
+    return;
+  }
   if (!it.found) {
-    const long long items = it.items * P.c.hkv;
+    const long long items = it.items * P.c.hkv + cut.groups;
     clear_rows<D>(P.c, blockIdx.x - items, gridDim.x - items);
     return;
   }
-  if (it.parts > 1 && it.part == 0 && kvh == 0 && threadIdx.x == 0) {
-    int* const rec = P.records + 4 + 4 * it.record;
-    rec[0] = it.start;
-    rec[1] = it.tile * kManyRows;  // a narrow request has one tile, 0
-    rec[2] = it.rows;
-    rec[3] = it.slot << 12 | it.parts;
-  }
-  if (it.rows <= kFewRows)
-    narrow_body<T, D, PLAIN>(P, it, kvh, s_kv, s_ml);
+  if (it.parts > 1 && it.part == 0 && kvh == 0 && threadIdx.x == 0)
+    put_record(P, it.record, it.r.start, it.tile * kManyRows,
+               min(it.r.rows - it.tile * kManyRows, kManyRows), it.parts,
+               P.narrow_rows + it.slot * P.part_rows, P.part_rows);
+  if (it.r.rows <= kFewRows)
+    narrow_body<T, D, PLAIN>(P.c, it.r, kvh, s_kv, s_ml);
   else
     wide_body<T, D, PLAIN>(P, it, kvh, s_kv, s_seen);
 }
 
-// Joins the parts of the split tiles: grid (split tile, KV head, rows apart),
-// a workgroup takes every gridDim.z'th row of the tile, its waves the parts
-// of a row in turn.
+constexpr int kJoinRows = 8;  // rows of a record that have a workgroup each
+
+// Joins the partials: a workgroup takes every kJoinRows'th row of a record and
+// KV head, its groups of D / 4 lanes the parts of a row in turn.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void chunk_merge_kernel(TileParams P) {
-  constexpr int R = D / 64;
-  __shared__ float s_acc[4][D];
-  __shared__ float2 s_ml[4];
-  if ((int)blockIdx.x >= P.records[0]) return;
-  const int* const rec = P.records + 4 + 4 * blockIdx.x;
-  const int start = rec[0], row0 = rec[1], rows = min(rec[2] - row0, kManyRows);
-  const int slot = rec[3] >> 12, parts = rec[3] & 4095, kvh = blockIdx.y;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (int r = blockIdx.z; r < rows; r += gridDim.z) {
-    float m = kNegInf, l = 0.f, acc[R] = {};
+__global__ __launch_bounds__(256) void chunk_join_kernel(TileParams P) {
+  constexpr int LPR = D / 4, G = 256 / LPR;  // lanes per row, groups
+  __shared__ float4 s_acc[G][LPR];
+  __shared__ float2 s_ml[G];
+  const int4 counts = P.records[0];
+  const int tid = threadIdx.x, grp = tid / LPR, c = tid % LPR;
+  const int total = (counts.x + counts.y) * P.c.hkv * kJoinRows;
+  for (int x = blockIdx.x; x < total; x += gridDim.x) {
+    const int i = x / kJoinRows / P.c.hkv, kvh = x / kJoinRows - i * P.c.hkv;
+    const int at = i < counts.x ? i : P.most_parts / 2 + i - counts.x;
+    const int4 rec = P.records[1 + 2 * at], part = P.records[2 + 2 * at];
+    const int parts = rec.w;
+    if (parts < 2) continue;
+    for (int r = x % kJoinRows; r < rec.z; r += kJoinRows) {
+      float m = kNegInf, l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int p = wave; p < parts; p += 4) {
-      const size_t at = ((size_t)(slot + p) * P.c.hkv + kvh) * P.part_rows + r;
-      const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * at);
-      float v[R];
-#pragma unroll
-      for (int i = 0; i < R; ++i) v[i] = P.part_acc[at * D + R * lane + i];
-      const float mn = __builtin_fmaxf(m, ml.x), base = safe_max(mn);
-      const float a = fast_exp2(m - base), b = fast_exp2(ml.x - base);
-      l = l * a + ml.y * b;
-#pragma unroll
-      for (int i = 0; i < R; ++i) acc[i] = acc[i] * a + v[i] * b;
-      m = mn;
-    }
-    if (lane == 0) s_ml[wave] = make_float2(m, l);
-#pragma unroll
-    for (int i = 0; i < R; ++i) s_acc[wave][R * lane + i] = acc[i];
-    __syncthreads();
-    if (threadIdx.x < D) {
-      float top = kNegInf, sum = 0.f, out = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) top = __builtin_fmaxf(top, s_ml[w].x);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float a = fast_exp2(s_ml[w].x - safe_max(top));
-        sum += s_ml[w].y * a;
-        out += s_acc[w][threadIdx.x] * a;
+      for (int p = grp; p < parts; p += G) {
+        const size_t row = partial_row(P, part.x + p * part.y + r, kvh);
+        const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * row);
+        const float4 v = *reinterpret_cast<const float4*>(P.part_acc + row * D + 4 * c);
+        const float mn = __builtin_fmaxf(m, ml.x), base = safe_max(mn);
+        const float a = fast_exp2(m - base), b = fast_exp2(ml.x - base);
+        l = l * a + ml.y * b;
+        acc.x = acc.x * a + v.x * b;
+        acc.y = acc.y * a + v.y * b;
+        acc.z = acc.z * a + v.z * b;
+        acc.w = acc.w * a + v.w * b;
+        m = mn;
       }
-      const int n = (row0 + r) / P.c.group, h = kvh * P.c.group + row0 + r - n * P.c.group;
-      P.c.out[((size_t)(start + n) * P.c.hq + h) * D + threadIdx.x] = round_to<T>(out * one_over(sum));
+      s_acc[grp][c] = acc;
+      if (c == 0) s_ml[grp] = make_float2(m, l);
+      __syncthreads();
+      if (tid < D) {
+        float top = kNegInf, sum = 0.f, out = 0.f;
+#pragma unroll
+        for (int w = 0; w < G; ++w) top = __builtin_fmaxf(top, s_ml[w].x);
+#pragma unroll
+        for (int w = 0; w < G; ++w) {
+          const float a = fast_exp2(s_ml[w].x - safe_max(top));
+          sum += s_ml[w].y * a;
+          out += reinterpret_cast<const float*>(s_acc[w])[tid] * a;
+        }
+        const Request rq{0, rec.x, 0, 0, 0};
+        out_row<T, D>(P.c, rq, rec.y + r, kvh)[tid] = round_to<T>(out * one_over(sum));
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
-// How a call with a workspace cuts its tiles; most_parts 0: it does not.
+// How a call with a workspace cuts its work; bytes 0: it does not.
 struct Cut {
-  int target, most_parts, part_rows;
+  int target, waves, most_parts, part_rows, narrow_rows;
   size_t acc_bytes, ml_bytes, bytes;
 };
 
@@ -1152,15 +1381,23 @@ Cut cut_of(const bc_shape& s, int tokens) {
   Cut c{};
   const long long steps = ((long long)s.max_pages * BC_PAGE_SIZE + kStep - 1) / kStep;
   const long long rows = (long long)tokens * (s.query_heads / s.kv_heads);
+  if (steps <= kLeastSteps || rows < 1 || rows > 1 << 30 ||
+      (long long)s.batch * (s.max_pages + 1ll) > 1 << 28 ||
+      (long long)s.batch * s.query_heads > 1 << 26)
+    return c;
   c.target = 2 * bch::device_cus();
-  const int most = 2 * c.target / s.kv_heads;
-  if (steps <= kLeastSteps || most < 2 || rows < 1) return c;
-  c.most_parts = most;
-  c.part_rows = rows < kManyRows ? (int)rows : kManyRows;
-  const size_t slots = (size_t)most * s.kv_heads * c.part_rows;
+  c.waves = 2 * c.target / s.kv_heads > 1 ? 2 * c.target / s.kv_heads : 1;
+  c.narrow_rows = 32 * c.waves + (int)(rows < 32ll * s.batch ? rows : 32ll * s.batch);
+  if (rows > kFewRows) {
+    c.most_parts = 2 * c.target / s.kv_heads;
+    c.part_rows = rows < kManyRows ? (int)rows : kManyRows;
+  }
+  const long long all = c.narrow_rows + (long long)c.most_parts * c.part_rows;
+  if (all > 0x7fffffff) return Cut{};
+  const size_t slots = (size_t)all * s.kv_heads;
   c.acc_bytes = slots * s.dim * sizeof(float);
   c.ml_bytes = (slots * 2 * sizeof(float) + 15) / 16 * 16;
-  c.bytes = c.acc_bytes + c.ml_bytes + (4 + 4 * (size_t)(most / 2)) * sizeof(int);
+  c.bytes = c.acc_bytes + c.ml_bytes + (1 + 2 * ((size_t)c.most_parts / 2 + s.batch)) * sizeof(int4);
   return c;
 }
 
@@ -1174,9 +1411,11 @@ hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned
     char* const at = static_cast<char*>(ws);
     P.part_acc = reinterpret_cast<float*>(at);
     P.part_ml = reinterpret_cast<float*>(at + cut.acc_bytes);
-    P.records = reinterpret_cast<int*>(at + cut.acc_bytes + cut.ml_bytes);
-    P.part_rows = cut.part_rows;
+    P.records = reinterpret_cast<int4*>(at + cut.acc_bytes + cut.ml_bytes);
+    P.waves = cut.waves;
     P.most_parts = cut.most_parts;
+    P.part_rows = cut.part_rows;
+    P.narrow_rows = cut.narrow_rows;
   }
   if (C.cap > 0.f || C.slopes)
     chunk_tile_kernel<T, D, false><<<dim3(grid), 256, 0, st>>>(P);
@@ -1184,8 +1423,9 @@ hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned
     chunk_tile_kernel<T, D, true><<<dim3(grid), 256, 0, st>>>(P);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !ws) return err;
-  const dim3 tiles(cut.most_parts / 2, C.hkv, cut.part_rows < 8 ? cut.part_rows : 8);
-  chunk_merge_kernel<T, D><<<tiles, 256, 0, st>>>(P);
+  const long long most = ((long long)cut.most_parts / 2 + C.batch) * C.hkv * kJoinRows;
+  const long long join = most < 4 * cut.target ? most : 4 * cut.target;
+  chunk_join_kernel<T, D><<<dim3((unsigned)join), 256, 0, st>>>(P);
   return hipGetLastError();
 }
 
@@ -1318,7 +1558,7 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
   const bool use = cut.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= cut.bytes;
   const long long tiles = (in.tokens < s.batch ? in.tokens : s.batch) + rows / kManyRows +
                           (use ? cut.most_parts : 0);
-  const long long grid = tiles * s.kv_heads + 1;
+  const long long grid = tiles * s.kv_heads + (use ? ((long long)cut.waves * s.kv_heads + 3) / 4 : 0) + 1;
   const long long far = 1 << 26;
   const bool tiled = aligned16(in.q) && aligned16(in.k) && aligned16(in.v) && aligned16(in.output) &&
                      bits % 8 == 0 && in.k_strides.slot < far && in.v_strides.slot < far &&
