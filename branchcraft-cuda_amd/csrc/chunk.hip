@@ -146,6 +146,7 @@ struct ChunkParams {
   long long vp, vs, vh;      // V's
   int tokens, batch, hq, hkv, group, max_pages, phys_pages;
   int causal, window;
+  unsigned group_mul;        // ceil(2^32 / group), or 0: see by_group
   float scale, cap;
 };
 
@@ -179,6 +180,12 @@ __device__ __forceinline__ int request_of(const ChunkParams& P, int t, int lane)
   return b < P.batch && P.starts[b] <= t ? b : -1;
 }
 
+// r / group, as a multiply-high where the host has seen that it is exact (r *
+// group below 2^32).
+__device__ __forceinline__ int by_group(const ChunkParams& P, int r) {
+  return P.group == 1 ? r : P.group_mul ? (int)__umulhi((unsigned)r, P.group_mul) : r / P.group;
+}
+
 __device__ __forceinline__ int clamp_len(const ChunkParams& P, int b) {
   return max(0, (int)min((long long)P.lengths[b], (long long)P.max_pages * BC_PAGE_SIZE));
 }
@@ -189,7 +196,7 @@ __device__ __forceinline__ int2 row_range(const ChunkParams& P, int b, int t, in
   if (P.causal) hi = min(hi, P.prefix ? max(pos, max(P.prefix[b], 0) - 1) : pos);
   if (P.window > 0) lo = max(lo, max(pos, 0) - P.window + 1);
   if (P.first) lo = max(lo, P.first[t]);
-  return pos < 0 ? make_int2(1, 0) : make_int2(lo, hi);
+  return pos < 0 ? make_int2(0, -1) : make_int2(lo, hi);
 }
 
 // The plain form of the operator, for tensors whose addresses or strides rule
@@ -332,7 +339,12 @@ struct TileParams {
 // step, the first of them at place pos0 of the request.
 struct Request {
   int b, start, len, pos0, rows;
+  int prefix;  // tokens that all rows see
 };
+
+__device__ __forceinline__ int prefix_of(const ChunkParams& P, int b) {
+  return P.prefix && P.causal ? max(P.prefix[b], 0) : 0;
+}
 
 template <typename F>
 __device__ __forceinline__ int wave_join_i(int x, F f) {
@@ -475,6 +487,7 @@ __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int shar
       it.r.len = __builtin_amdgcn_readlane(a.len, at);
       it.r.pos0 = __builtin_amdgcn_readlane(a.full - a.n, at);
       it.r.rows = __builtin_amdgcn_readlane(a.rows, at);
+      it.r.prefix = prefix_of(C, it.r.b);
       it.parts = __builtin_amdgcn_readlane(parts, at);
       const int in = local - __builtin_amdgcn_readlane(upto - mine, at);
       const int nth = in / it.parts;
@@ -505,7 +518,7 @@ template <int D>
 struct Rows {
   f32x16 acc[D / 32];  // O^T: dimension 32 dt + 8 (j / 4) + 4 g + j % 4
   float m, l;
-  float slope;         // times log2 e
+  float slope;         // in the scores' units
   int pos, lo, hi;
 };
 
@@ -546,52 +559,93 @@ __device__ __forceinline__ u32x4 read_v(const uint16_t* lo, const uint16_t* hi) 
   return u32x4{x.x, x.y, y.x, y.y};
 }
 
-// Scores of NT staged tiles, from token t0 on, to the softmax's exponents:
-// raw products in the plain form (their scale is applied with the maximum),
-// log2 units otherwise.  `edge`: mask to the row's lo .. hi and to `valid`.
-template <typename T, int D, bool PLAIN, int NT>
+// How scores become exponents.  All forms end as exp2(scale2 * s - base), with
+// one maximum and one product per score in the softmax itself:
+//  - Plain: s is the product q.k, scale2 = scale log2 e.
+//  - Bias: the same, and the products start from -slope / scale * |p - token|,
+//    one FMA per score in place of a zero.
+//  - Cap: cap tanh(x) = cap - 2 cap / (e^2x + 1), of which the softmax drops the
+//    constant, so s = -1 / (e^2x + 1) and scale2 = 2 cap log2 e; two more
+//    transcendentals per score.  A bias is added to s in these units.
+enum class Form { kPlain, kBias, kCap };
+
+template <int D>
+__device__ __forceinline__ float scale2_of(const ChunkParams& C, Form form) {
+  return (form == Form::kCap ? 2.f * C.cap : C.scale) * kLog2e;
+}
+
+// What a score of token t0 + 4 g + off starts from in the biased form.  Without
+// a prefix the tokens behind the row's place are masked, so that the distance
+// needs no magnitude.
+template <int D>
+__device__ __forceinline__ float bias_at(const Rows<D>& r, float from, int off) {
+  return -r.slope * __builtin_fabsf(from - (float)off);
+}
+
+template <int D, int NT>
+__device__ __forceinline__ void start_scores(const ChunkParams& C, f32x16 (&sc)[NT], const Rows<D>& r,
+                                             int t0, int g) {
+  const float from = (float)(r.pos - t0 - 4 * g);
+  if (C.causal && !C.prefix) {
+    const float at = -r.slope * from;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        sc[i][j] = __builtin_fmaf(r.slope, (float)(32 * i + 8 * (j >> 2) + (j & 3)), at);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sc[i][j] = bias_at(r, from, 32 * i + 8 * (j >> 2) + (j & 3));
+  }
+}
+
+// The tokens of a step that a row must not take: those before its lo, behind
+// its hi, or in pages that are not in the pool.
+struct Edges {
+  bool lo, hi, pages;
+  unsigned long long valid;
+};
+
+template <int D, Form FORM, int NT>
 __device__ __forceinline__ void finish_scores(const ChunkParams& C, f32x16 (&sc)[NT],
-                                              const Rows<D>& r, int t0, int g, bool edge,
-                                              unsigned long long valid) {
-  if (!PLAIN) {
-    const float from = (float)(r.pos - t0 - 4 * g);
-    if (C.cap > 0.f) {
-      // cap * tanh(x) in log2 units, x = scale * s / cap.
-      const float in = C.scale / C.cap * (2.f * kLog2e), top = C.cap * kLog2e;
+                                              const Rows<D>& r, int t0, int g, const Edges& e) {
+  if (FORM == Form::kCap) {
+    const float in = C.scale / C.cap * (2.f * kLog2e);
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          sc[i][j] = __builtin_fmaf(
-              -2.f * top, __builtin_amdgcn_rcpf(fast_exp2(sc[i][j] * in) + 1.f), top);
-    } else {
-      const float by = C.scale * kLog2e;
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) sc[i][j] *= by;
-    }
+      for (int j = 0; j < 16; ++j)
+        sc[i][j] = __builtin_amdgcn_rcpf(-1.f - fast_exp2(sc[i][j] * in));
     if (C.slopes) {
+      const float from = (float)(r.pos - t0 - 4 * g);
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          sc[i][j] = __builtin_fmaf(
-              -r.slope, __builtin_fabsf(from - (float)(32 * i + 8 * (j >> 2) + (j & 3))),
-              sc[i][j]);
+        for (int j = 0; j < 16; ++j) sc[i][j] += bias_at(r, from, 32 * i + 8 * (j >> 2) + (j & 3));
     }
   }
-  if (edge) {
-    const int a = r.lo - t0 - 4 * g, b = r.hi - t0 - 4 * g;
+  if (e.hi) {
+    const int b = r.hi - t0 - 4 * g;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sc[i][j] = 32 * i + 8 * (j >> 2) + (j & 3) <= b ? sc[i][j] : kNegInf;
+  }
+  if (e.lo) {
+    const int a = r.lo - t0 - 4 * g;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sc[i][j] = 32 * i + 8 * (j >> 2) + (j & 3) >= a ? sc[i][j] : kNegInf;
+  }
+  if (e.pages) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const uint32_t ok = (uint32_t)(valid >> (32 * i)) >> (4 * g);
+      const uint32_t ok = (uint32_t)(e.valid >> (32 * i)) >> (4 * g);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int off = 8 * (j >> 2) + (j & 3);
-        const bool in = 32 * i + off >= a && 32 * i + off <= b && ((ok >> off) & 1u);
-        sc[i][j] = in ? sc[i][j] : kNegInf;
-      }
+      for (int j = 0; j < 16; ++j) sc[i][j] = (ok >> (8 * (j >> 2) + (j & 3))) & 1u ? sc[i][j] : kNegInf;
     }
   }
 }
@@ -600,9 +654,9 @@ __device__ __forceinline__ void finish_scores(const ChunkParams& C, f32x16 (&sc)
 // only when it would grow by more than kRescaleSlack.  Weights are rounded to
 // T, to nearest, for the product (half a step of T each, as the output's own
 // rounding); their sum is of the rounded weights, in 32 bits.
-template <typename T, int D, bool PLAIN, int NT>
+template <typename T, int D, int NT>
 __device__ __forceinline__ void weigh(f32x16 (&sc)[NT], Rows<D>& r, const uint16_t* vt,
-                                      const Offsets<D>& o, float scale_log2) {
+                                      const Offsets<D>& o, float scale2) {
   constexpr int DT = D / 32, NG = 2 * NT;
   typedef Num<T> N;
   float top = kNegInf;
@@ -610,7 +664,7 @@ __device__ __forceinline__ void weigh(f32x16 (&sc)[NT], Rows<D>& r, const uint16
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) top = __builtin_fmaxf(top, sc[i][j]);
-  if (PLAIN) top *= scale_log2;
+  top *= scale2;
   if (__builtin_amdgcn_ballot_w64(top > r.m + kRescaleSlack)) {
     const float mnew = __builtin_fmaxf(r.m, __builtin_fmaxf(top, shfl_xor_f(top, 32)));
     const float alpha = fast_exp2(r.m - safe_max(mnew));
@@ -628,8 +682,8 @@ __device__ __forceinline__ void weigh(f32x16 (&sc)[NT], Rows<D>& r, const uint16
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const float s0 = sc[grp / 2][8 * (grp % 2) + 2 * x], s1 = sc[grp / 2][8 * (grp % 2) + 2 * x + 1];
-      const float p0 = fast_exp2(PLAIN ? __builtin_fmaf(s0, scale_log2, -base) : s0 - base);
-      const float p1 = fast_exp2(PLAIN ? __builtin_fmaf(s1, scale_log2, -base) : s1 - base);
+      const float p0 = fast_exp2(__builtin_fmaf(s0, scale2, -base));
+      const float p1 = fast_exp2(__builtin_fmaf(s1, scale2, -base));
       w[x] = pack2<T>(p0, p1);
       r.l = N::add2(w[x], r.l);
     }
@@ -731,20 +785,24 @@ struct Pages {
 };
 
 // This lane's row of the wave's 32: its place, what it sees, and its Q.
-template <typename T, int D, bool PLAIN>
+template <typename T, int D, Form FORM>
 __device__ __forceinline__ void load_rows(const ChunkParams& C, const Request& it, int r, int kvh,
                                           int g, Rows<D>& R, u32x4 (&qB)[D / 16]) {
   const bool real = r < it.rows;
-  const int i = real ? r / C.group : 0, h = kvh * C.group + (real ? r - i * C.group : 0);
+  const int i = real ? by_group(C, r) : 0, h = kvh * C.group + (real ? r - i * C.group : 0);
   const int t = it.start + i;
   const uint16_t* const q = C.q + t * C.qt + h * C.qh + 8 * g;
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) qB[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
   R.pos = it.pos0 + i;
   const int2 seen = row_range(C, it.b, t, R.pos, it.len);
-  R.lo = real ? seen.x : 1;
-  R.hi = real ? seen.y : 0;
-  R.slope = !PLAIN && C.slopes ? C.slopes[h] * kLog2e : 0.f;
+  R.lo = real ? seen.x : 0;
+  R.hi = real ? seen.y : -1;
+  R.slope = 0.f;
+  if (FORM != Form::kPlain && C.slopes) {
+    const float slope = C.slopes[h];
+    R.slope = FORM == Form::kCap ? slope / (2.f * C.cap) : slope / C.scale;
+  }
   R.m = kNegInf;
   R.l = 0.f;
 #pragma unroll
@@ -753,11 +811,30 @@ __device__ __forceinline__ void load_rows(const ChunkParams& C, const Request& i
     for (int j = 0; j < 16; ++j) R.acc[dt][j] = 0.f;
 }
 
-// The tokens that a wave's real rows see: all of them (whole) or some (any).
+// Bounds on what rows see: any of them the tokens any_lo .. any_hi at most, all
+// of them all_lo .. all_hi.
 struct Seen {
   int any_lo, any_hi, all_lo, all_hi;
 };
 
+// Of rows r0 .. r1 - 1 of a request, from their places alone (no `first`).
+__device__ __forceinline__ Seen rows_seen(const ChunkParams& C, const Request& rq, int r0, int r1) {
+  if (r0 >= r1) return {0x7fffffff, -1, 0, 0x7fffffff};
+  const int pa = rq.pos0 + by_group(C, r0), pb = rq.pos0 + by_group(C, r1 - 1), end = rq.len - 1;
+  Seen s{0, end, 0, end};
+  if (C.causal) {
+    s.any_hi = min(end, max(pb, rq.prefix - 1));
+    s.all_hi = min(end, max(pa, rq.prefix - 1));
+  }
+  if (C.window > 0) {
+    s.any_lo = max(0, max(pa, 0) - C.window + 1);
+    s.all_lo = max(0, max(pb, 0) - C.window + 1);
+  }
+  if (pa < 0) s.all_hi = -1;  // rows before the request see nothing
+  return s;
+}
+
+// Of the wave's rows as they are.
 template <int D>
 __device__ __forceinline__ Seen wave_seen(const Rows<D>& R, bool real) {
   const bool some = real && R.lo <= R.hi;
@@ -766,6 +843,12 @@ __device__ __forceinline__ Seen wave_seen(const Rows<D>& R, bool real) {
 }
 
 __device__ __forceinline__ float one_over(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }
+
+template <typename T, int D>
+__device__ __forceinline__ uint16_t* out_row(const ChunkParams& C, const Request& rq, int r, int kvh) {
+  const int n = by_group(C, r), h = kvh * C.group + r - n * C.group;
+  return C.out + ((size_t)(rq.start + n) * C.hq + h) * D;
+}
 
 // Where a partial row of a KV head lies, in rows.
 __device__ __forceinline__ size_t partial_row(const TileParams& P, int row, int kvh) {
@@ -783,9 +866,9 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
 
 // The wide form: 128 rows per workgroup, 32 per wave, each step's K and V
 // shared through LDS.
-template <typename T, int D, bool PLAIN>
+template <typename T, int D, Form FORM>
 __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, int kvh,
-                                          uint16_t* s_kv, Seen* s_seen) {
+                                          uint16_t* s_kv, Seen* s_seen, int* s_bad) {
   const ChunkParams& C = P.c;
   const Request& rq = it.r;
   constexpr int KS = D / 16, CPR = D / 8;
@@ -794,37 +877,56 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, lr = lane & 31;
-  const int row0 = it.tile * kManyRows + wave * 32;
+  const int tile0 = it.tile * kManyRows, row0 = tile0 + wave * 32;
+  const int32_t* const table = C.pages + (size_t)rq.b * C.max_pages;
+  auto load_ids = [&](int t) { return table[min(t * 4 + lane, C.max_pages - 1)]; };
   Rows<D> R;
   u32x4 qB[KS];
-  load_rows<T, D, PLAIN>(C, rq, row0 + lr, kvh, g, R, qB);
-  const Seen mine = wave_seen(R, row0 + lr < rq.rows);
-  if (lane == 0) s_seen[wave] = mine;
-  __syncthreads();
-  Seen wg = s_seen[0];
+  Seen mine, wg;
+  int t0, tend, ids = 0, ids_next = 0;
+  // This part's steps of those that the workgroup's rows see, and its first
+  // page ids, ahead of Q's loads where they do not depend on the rows.
+  auto range = [&] {
+    const int first = wg.any_lo / kStep;
+    const int steps = wg.any_hi >= wg.any_lo ? wg.any_hi / kStep - first + 1 : 0;
+    t0 = first + (int)((long long)steps * it.part / it.parts);
+    tend = first + (int)((long long)steps * (it.part + 1) / it.parts);
+    if (t0 < tend) {
+      ids = load_ids(t0);
+      ids_next = load_ids(t0 + 16);
+    }
+  };
+  if (tid < 4) s_bad[tid] = 0;
+  if (!C.first) {
+    mine = rows_seen(C, rq, row0, min(row0 + 32, rq.rows));
+    wg = rows_seen(C, rq, tile0, min(tile0 + kManyRows, rq.rows));
+    range();
+    load_rows<T, D, FORM>(C, rq, row0 + lr, kvh, g, R, qB);
+  } else {
+    load_rows<T, D, FORM>(C, rq, row0 + lr, kvh, g, R, qB);
+    mine = wave_seen(R, row0 + lr < rq.rows);
+    if (lane == 0) s_seen[wave] = mine;
+    __syncthreads();
+    wg = s_seen[0];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) {
-    wg.any_lo = min(wg.any_lo, s_seen[w].any_lo);
-    wg.any_hi = max(wg.any_hi, s_seen[w].any_hi);
-    wg.all_lo = max(wg.all_lo, s_seen[w].all_lo);
-    wg.all_hi = min(wg.all_hi, s_seen[w].all_hi);
+    for (int w = 1; w < 4; ++w) {
+      wg.any_lo = min(wg.any_lo, s_seen[w].any_lo);
+      wg.any_hi = max(wg.any_hi, s_seen[w].any_hi);
+      wg.all_lo = max(wg.all_lo, s_seen[w].all_lo);
+      wg.all_hi = min(wg.all_hi, s_seen[w].all_hi);
+    }
+    wg.any_lo = __builtin_amdgcn_readfirstlane(wg.any_lo);
+    wg.any_hi = __builtin_amdgcn_readfirstlane(wg.any_hi);
+    wg.all_lo = __builtin_amdgcn_readfirstlane(wg.all_lo);
+    wg.all_hi = __builtin_amdgcn_readfirstlane(wg.all_hi);
+    range();
   }
-  wg.any_lo = __builtin_amdgcn_readfirstlane(wg.any_lo);
-  wg.any_hi = __builtin_amdgcn_readfirstlane(wg.any_hi);
-  wg.all_lo = __builtin_amdgcn_readfirstlane(wg.all_lo);
-  wg.all_hi = __builtin_amdgcn_readfirstlane(wg.all_hi);
-  const int first = wg.any_lo / kStep;
-  const int steps = wg.any_hi >= wg.any_lo ? wg.any_hi / kStep - first + 1 : 0;
-  const int t0 = first + (int)((long long)steps * it.part / it.parts);
-  const int tend = first + (int)((long long)steps * (it.part + 1) / it.parts);
 
   const int lrow = tid / CPR, lcol = 8 * (tid % CPR ^ swz<D>(lrow));
   const unsigned koff = (unsigned)(((lrow % BC_PAGE_SIZE) * C.ks + lcol) * 2);
   const unsigned voff = (unsigned)(((lrow % BC_PAGE_SIZE) * C.vs + lcol) * 2);
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(
       (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)s_kv + wave * 1024);
-  const int32_t* const table = C.pages + (size_t)rq.b * C.max_pages;
-  auto load_ids = [&](int t) { return table[min(t * 4 + lane, C.max_pages - 1)]; };
   Pages pg;
   auto issue_chunk = [&](int x, int at, int buf) {
     const int from = 4 * at + (CPR == 16 ? x : 2 * x + (wave >> 1));
@@ -834,7 +936,7 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
   };
   // Steps whole_lo .. whole_hi - 1 are seen whole by every row, given their pages.
   const int whole_lo = wg.all_lo / kStep + (wg.all_lo % kStep != 0);
-  const int whole_hi = min(wg.all_hi == 0x7fffffff ? 0 : wg.all_hi + 1, rq.len) / kStep;
+  const int whole_hi = (min(wg.all_hi, rq.len - 1) + 1) / kStep;
   // Each thread tidies the chunks that its own loads, already waited for,
   // have filled.
   auto inspect = [&](unsigned long long ok, uint16_t* v) {
@@ -844,17 +946,15 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
       u32x4* const at = reinterpret_cast<u32x4*>(v + (tid + 256 * x) * 8);
       bad |= tidy<T>(at, (ok >> (lrow + 256 / CPR * x)) & 1u);
     }
-    return __builtin_amdgcn_readfirstlane(__syncthreads_or(bad)) != 0;
+    return bad;
   };
 
   const Offsets<D> o = read_offsets<D>(lane);
-  const float scale_log2 = C.scale * kLog2e;
+  const float scale2 = scale2_of<D>(C, FORM);
   bool is_whole = true, bad = false;
   int pages = 15;  // of the step at hand, a bit each: in the pool
-  int ids_next = 0;
   if (t0 < tend) {
-    pg.take(C, kvh, load_ids(t0));
-    ids_next = load_ids(t0 + 16);
+    pg.take(C, kvh, ids);
 #pragma unroll
     for (int x = 0; x < NX; ++x) issue_chunk(x, 0, 0);
     pages = (int)pg.in_pool & 15;
@@ -863,10 +963,8 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qB[s]));
     wait_loads();
-    if (!is_whole)
-      bad = inspect(tokens_of<4>(rq.len - t0 * kStep, pages), s_kv + HALF);
-    else
-      __syncthreads();
+    if (!is_whole) bad = inspect(tokens_of<4>(rq.len - t0 * kStep, pages), s_kv + HALF);
+    bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));
   }
   // One step, its K and V in buffer `buf`; the next one's loads go out between
   // the score products.
@@ -888,25 +986,32 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
 #pragma unroll
       for (int i = 0; i < 2; ++i) kf[i][s] = lds16(kt + i * 32 * D + o.k[s]);
     const f32x16 zero = {};
+    if (FORM == Form::kBias) start_scores<D, 2>(C, sc, R, t * kStep, g);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sc[i] = Num<T>::mfma(kf[i][s], qB[s], s == 0 ? zero : sc[i]);
+      for (int i = 0; i < 2; ++i)
+        sc[i] = Num<T>::mfma(kf[i][s], qB[s], FORM != Form::kBias && s == 0 ? zero : sc[i]);
       if (s % 2 == 1 && s / 2 < NX) {
         if (next) issue_chunk(s / 2, at, buf ^ 1);
       }
     }
-    const bool edge = !is_whole && (pages != 15 || rq.len - t * kStep < kStep ||
-                                    t * kStep < mine.all_lo || t * kStep + kStep - 1 > mine.all_hi);
-    finish_scores<T, D, PLAIN, 2>(C, sc, R, t * kStep, g, edge, edge ? tokens_of<4>(rq.len - t * kStep, pages) : 0);
-    weigh<T, D, PLAIN, 2>(sc, R, kt + HALF, o, scale_log2);
+    Edges e{t * kStep < mine.all_lo, t * kStep + kStep - 1 > mine.all_hi, pages != 15, 0};
+    if (e.pages) e.valid = tokens_of<4>(rq.len - t * kStep, pages);
+    finish_scores<D, FORM, 2>(C, sc, R, t * kStep, g, e);
+    weigh<T, D, 2>(sc, R, kt + HALF, o, scale2);
     if (bad) add_untidy<T, D>(C, rq, kvh, R, t * kStep, kStep, g);
     wait_loads();
-    bad = false;
-    if (!whole_n)
-      bad = inspect(tokens_of<4>(rq.len - (t + 1) * kStep, pages_n), s_kv + (buf ^ 1) * (2 * HALF) + HALF);
-    else
-      __syncthreads();
+    // Step s of the part sets flag s % 4 before the barrier that ends the step
+    // before it; the flag is read behind that barrier and cleared behind the
+    // next, two barriers before it is set again.
+    const int s = t - t0;
+    if (!whole_n && inspect(tokens_of<4>(rq.len - (t + 1) * kStep, pages_n),
+                            s_kv + (buf ^ 1) * (2 * HALF) + HALF))
+      s_bad[(s + 1) & 3] = 1;
+    __syncthreads();
+    if (bad && tid == 0) s_bad[s & 3] = 0;
+    bad = !whole_n && __builtin_amdgcn_readfirstlane(s_bad[(s + 1) & 3]);
     is_whole = whole_n;
     pages = pages_n;
   };
@@ -950,8 +1055,7 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
     const u32x4 w = lds16(out + row * D + (c ^ (row % CPR)) * 8);
     const int rr = row0 + row;
     if (rr < rq.rows) {
-      const int n = rr / C.group, h = kvh * C.group + rr - n * C.group;
-      *reinterpret_cast<u32x4*>(C.out + ((size_t)(rq.start + n) * C.hq + h) * D + 8 * c) = w;
+      *reinterpret_cast<u32x4*>(out_row<T, D>(C, rq, rr, kvh) + 8 * c) = w;
     }
   }
 }
@@ -968,7 +1072,7 @@ __device__ __forceinline__ void stream_to_lds(const void* base, unsigned off, un
 
 // A wave's stream of 32-token tiles through its own part of LDS: K of the next
 // tile goes out behind the scores, V behind the product, and no barrier.
-template <typename T, int D, bool PLAIN>
+template <typename T, int D, Form FORM>
 struct Stream {
   static constexpr int KS = D / 16, CPR = D / 8;
   static constexpr int RPL = 64 / CPR;         // token rows per load
@@ -1011,11 +1115,14 @@ struct Stream {
   __device__ __forceinline__ int in_pool(int at) const { return (int)(pg.in_pool >> (2 * at)) & 3; }
 
   // The staged tile's scores; K has been read when this returns.
-  __device__ __forceinline__ void scores(f32x16 (&sc)[1], const u32x4 (&qB)[KS]) const {
+  __device__ __forceinline__ void scores(f32x16 (&sc)[1], const u32x4 (&qB)[KS], const Rows<D>& R,
+                                         int t) const {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // K is there, V may be not
     const f32x16 zero = {};
+    if (FORM == Form::kBias) start_scores<D, 1>(C, sc, R, t * 32, lane >> 5);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) sc[0] = Num<T>::mfma(lds16(kt + o.k[s]), qB[s], s == 0 ? zero : sc[0]);
+    for (int s = 0; s < KS; ++s)
+      sc[0] = Num<T>::mfma(lds16(kt + o.k[s]), qB[s], FORM != Form::kBias && s == 0 ? zero : sc[0]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
   // Their softmax and product with V, behind which `next` K loads may be on
@@ -1024,32 +1131,25 @@ struct Stream {
                                           int t, int pages, bool next) const {
     const int g = lane >> 5, left = rq.len - t * 32;
     uint16_t* const vt = kt + TILE;
-    const bool edge = pages != 3 || left < 32 || t * 32 < mine.all_lo || t * 32 + 31 > mine.all_hi;
-    const unsigned long long ok = edge ? tokens_of<2>(left, pages) : 0;
-    finish_scores<T, D, PLAIN, 1>(C, sc, R, t * 32, g, edge, ok);
+    const Edges e{t * 32 < mine.all_lo, t * 32 + 31 > mine.all_hi, pages != 3, tokens_of<2>(left, pages)};
+    finish_scores<D, FORM, 1>(C, sc, R, t * 32, g, e);
     if (next)
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // V is there
     else
       wait_loads();
     bool bad = false;
-    if (edge) {
+    if (e.lo || e.hi || e.pages || left < 32) {
 #pragma unroll
       for (int c = 0; c < NL; ++c)
-        bad |= tidy<T>(reinterpret_cast<u32x4*>(vt + c * 512 + lane * 8), (ok >> (c * RPL + lane / CPR)) & 1u);
+        bad |= tidy<T>(reinterpret_cast<u32x4*>(vt + c * 512 + lane * 8), (e.valid >> (c * RPL + lane / CPR)) & 1u);
       bad = __builtin_amdgcn_ballot_w64(bad) != 0;
       wave_lds_sync();
     }
-    weigh<T, D, PLAIN, 1>(sc, R, vt, o, C.scale * kLog2e);
+    weigh<T, D, 1>(sc, R, vt, o, scale2_of<D>(C, FORM));
     if (bad) add_untidy<T, D>(C, rq, kvh, R, t * 32, 32, g);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 };
-
-template <typename T, int D>
-__device__ __forceinline__ uint16_t* out_row(const ChunkParams& C, const Request& rq, int r, int kvh) {
-  const int n = r / C.group, h = kvh * C.group + r - n * C.group;
-  return C.out + ((size_t)(rq.start + n) * C.hq + h) * D;
-}
 
 // The narrow form over a batch: the tiles of all requests with few rows, one
 // after another, in ranges of equal length, a range per wave.  A request that
@@ -1057,7 +1157,7 @@ __device__ __forceinline__ uint16_t* out_row(const ChunkParams& C, const Request
 // partial.  Range r's partial of a request whose predecessors have n rows
 // starts at partial row 32 r + n: a range's next request is further by the
 // rows of the last one, a request's next range by 32.
-template <typename T, int D, bool PLAIN>
+template <typename T, int D, Form FORM>
 __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cutting& cut,
                                           uint16_t* s_kv) {
   const ChunkParams& C = P.c;
@@ -1096,7 +1196,8 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
     const int at = __builtin_ctzll(left);
     left &= left - 1;
     p.rq = Request{b0 + at, __builtin_amdgcn_readlane(a.start, at), __builtin_amdgcn_readlane(a.len, at),
-                   __builtin_amdgcn_readlane(a.full - a.n, at), __builtin_amdgcn_readlane(a.rows, at)};
+                   __builtin_amdgcn_readlane(a.full - a.n, at), __builtin_amdgcn_readlane(a.rows, at),
+                   prefix_of(C, b0 + at)};
     p.tiles = __builtin_amdgcn_readlane(a.narrow, at);
     p.x0 = before + __builtin_amdgcn_readlane(upto, at) - p.tiles;
     p.first_tile = __builtin_amdgcn_readlane(a.first_tile, at);
@@ -1108,7 +1209,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
 
   Part p;
   if (!next_part(p)) return;
-  Stream<T, D, PLAIN> st(C, kvh, s_kv + wave * (64 * D));
+  Stream<T, D, FORM> st(C, kvh, s_kv + wave * (64 * D));
   int t = first_of(p), at = 0;
   st.pg.take(C, kvh, st.ids(p.rq.b, t, 1));
   int ids_next = st.ids(p.rq.b, t + 32, 1);
@@ -1118,8 +1219,8 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
   for (;;) {  // over the requests
     Rows<D> R;
     u32x4 qB[D / 16];
-    load_rows<T, D, PLAIN>(C, p.rq, lr, kvh, g, R, qB);
-    const Seen mine = wave_seen(R, lr < p.rq.rows);
+    load_rows<T, D, FORM>(C, p.rq, lr, kvh, g, R, qB);
+    const Seen mine = C.first ? wave_seen(R, lr < p.rq.rows) : rows_seen(C, p.rq, 0, p.rq.rows);
     const int tend = p.first_tile + min(hi, p.x0 + p.tiles) - p.x0;
     // The next request's first pages, so that its first tile follows this
     // one's last as any tile follows another.
@@ -1128,7 +1229,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
     const int ids_more = more ? st.ids(n.rq.b, first_of(n), 1) : 0;
     for (;; ++t) {
       f32x16 sc[1];
-      st.scores(sc, qB);
+      st.scores(sc, qB, R, t);
       const bool same = t + 1 < tend, next = same || more;
       int pages_n = 3;
       if (next) {
@@ -1184,7 +1285,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
 
 // The narrow form without a workspace: a workgroup per request and KV head,
 // its waves every fourth tile each; the four states meet at the end.
-template <typename T, int D, bool PLAIN>
+template <typename T, int D, Form FORM>
 __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request& rq, int kvh,
                                             uint16_t* s_kv, float2* s_ml) {
   constexpr int TILE = 32 * D;
@@ -1193,11 +1294,9 @@ __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request&
   const int g = lane >> 5, lr = lane & 31;
   Rows<D> R;
   u32x4 qB[D / 16];
-  load_rows<T, D, PLAIN>(C, rq, lr, kvh, g, R, qB);
-  const Seen mine = wave_seen(R, lr < rq.rows);
-#pragma unroll
-  for (int s = 0; s < D / 16; ++s) asm volatile("" : "+v"(qB[s]));
-  Stream<T, D, PLAIN> st(C, kvh, s_kv + wave * (2 * TILE));
+  load_rows<T, D, FORM>(C, rq, lr, kvh, g, R, qB);
+  const Seen mine = C.first ? wave_seen(R, lr < rq.rows) : rows_seen(C, rq, 0, rq.rows);
+  Stream<T, D, FORM> st(C, kvh, s_kv + wave * (2 * TILE));
   int t = mine.any_hi < mine.any_lo ? 1 : mine.any_lo / 32 + wave;
   const int tend = mine.any_hi < mine.any_lo ? 0 : mine.any_hi / 32 + 1;
   if (t < tend) {
@@ -1207,7 +1306,7 @@ __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request&
     st.issue_v(0);
     for (; t < tend; t += 4) {
       f32x16 sc[1];
-      st.scores(sc, qB);
+      st.scores(sc, qB, R, t);
       const bool next = t + 4 < tend;
       int pages_n = 3;
       if (next) {
@@ -1276,11 +1375,12 @@ __device__ __forceinline__ void clear_rows(const ChunkParams& C, long long at, l
     out[x < head * row ? x : x + gap] = u32x4{0, 0, 0, 0};
 }
 
-template <typename T, int D, bool PLAIN>
+template <typename T, int D, Form FORM>
 __global__ __launch_bounds__(256, 2) void chunk_tile_kernel(TileParams P) {
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[2 * 2 * kStep * D];
   __shared__ float2 s_ml[4 * 32];
   __shared__ Seen s_seen[4];
+  __shared__ int s_bad[4];
   const int lane = threadIdx.x & 63;
   // KV heads in the low bits: with eight of them, each XCD serves one.
   const Asked head = asked_of(P.c, lane);
@@ -1297,7 +1397,7 @@ __global__ __launch_bounds__(256, 2) void chunk_tile_kernel(TileParams P) {
   if (!flat || counts) it = plan_item(P, head, cut.share, flat ? -1ll : (long long)at, lane, counts);
   if (counts && threadIdx.x == 0) P.records[0] = make_int4(it.records, it.narrow_records, 0, 0);
   if (flat) {
-    flat_body<T, D, PLAIN>(P, head, cut, s_kv);
+    flat_body<T, D, FORM>(P, head, cut, s_kv);
     return;
   }
   if (!it.found) {
@@ -1310,46 +1410,72 @@ __global__ __launch_bounds__(256, 2) void chunk_tile_kernel(TileParams P) {
                min(it.r.rows - it.tile * kManyRows, kManyRows), it.parts,
                P.narrow_rows + it.slot * P.part_rows, P.part_rows);
   if (it.r.rows <= kFewRows)
-    narrow_body<T, D, PLAIN>(P.c, it.r, kvh, s_kv, s_ml);
+    narrow_body<T, D, FORM>(P.c, it.r, kvh, s_kv, s_ml);
   else
-    wide_body<T, D, PLAIN>(P, it, kvh, s_kv, s_seen);
+    wide_body<T, D, FORM>(P, it, kvh, s_kv, s_seen, s_bad);
 }
 
-constexpr int kJoinRows = 8;  // rows of a record that have a workgroup each
+// One part's state joined to another's.
+__device__ __forceinline__ void join(float& m, float& l, float4& acc, float m2, float l2, float4 v) {
+  const float top = __builtin_fmaxf(m, m2), base = safe_max(top);
+  const float a = fast_exp2(m - base), b = fast_exp2(m2 - base);
+  m = top;
+  l = l * a + l2 * b;
+  acc.x = acc.x * a + v.x * b;
+  acc.y = acc.y * a + v.y * b;
+  acc.z = acc.z * a + v.z * b;
+  acc.w = acc.w * a + v.w * b;
+}
 
-// Joins the partials: a workgroup takes every kJoinRows'th row of a record and
-// KV head, its groups of D / 4 lanes the parts of a row in turn.
+constexpr int kFewParts = 16;  // parts that one wave joins by itself
+
+// Joins the partials: `apart` workgroups share the rows of a record and KV
+// head.  Few parts: a wave per row, each group of D / 4 lanes taking the parts
+// in turn; many: the whole workgroup per row.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void chunk_join_kernel(TileParams P) {
-  constexpr int LPR = D / 4, G = 256 / LPR;  // lanes per row, groups
+__global__ __launch_bounds__(256) void chunk_join_kernel(TileParams P, int apart) {
+  constexpr int LPR = D / 4, G = 256 / LPR, GW = 64 / LPR;  // lanes per row, groups, groups per wave
   __shared__ float4 s_acc[G][LPR];
   __shared__ float2 s_ml[G];
-  const int4 counts = P.records[0];
   const int tid = threadIdx.x, grp = tid / LPR, c = tid % LPR;
-  const int total = (counts.x + counts.y) * P.c.hkv * kJoinRows;
+  const int4 counts = P.records[0];
+  const int total = (counts.x + counts.y) * P.c.hkv * apart;
   for (int x = blockIdx.x; x < total; x += gridDim.x) {
-    const int i = x / kJoinRows / P.c.hkv, kvh = x / kJoinRows - i * P.c.hkv;
+    const int in = x / apart, sub = x - in * apart, i = in / P.c.hkv, kvh = in - i * P.c.hkv;
     const int at = i < counts.x ? i : P.most_parts / 2 + i - counts.x;
     const int4 rec = P.records[1 + 2 * at], part = P.records[2 + 2 * at];
     const int parts = rec.w;
     if (parts < 2) continue;
-    for (int r = x % kJoinRows; r < rec.z; r += kJoinRows) {
-      float m = kNegInf, l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const Request rq{0, rec.x, 0, 0, 0, 0};
+    auto gather = [&](int r, int from, int step, float& m, float& l, float4& acc) {
 #pragma unroll 4
-      for (int p = grp; p < parts; p += G) {
+      for (int p = from; p < parts; p += step) {
         const size_t row = partial_row(P, part.x + p * part.y + r, kvh);
         const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * row);
-        const float4 v = *reinterpret_cast<const float4*>(P.part_acc + row * D + 4 * c);
-        const float mn = __builtin_fmaxf(m, ml.x), base = safe_max(mn);
-        const float a = fast_exp2(m - base), b = fast_exp2(ml.x - base);
-        l = l * a + ml.y * b;
-        acc.x = acc.x * a + v.x * b;
-        acc.y = acc.y * a + v.y * b;
-        acc.z = acc.z * a + v.z * b;
-        acc.w = acc.w * a + v.w * b;
-        m = mn;
+        join(m, l, acc, ml.x, ml.y, *reinterpret_cast<const float4*>(P.part_acc + row * D + 4 * c));
       }
+    };
+    if (parts <= kFewParts) {
+      for (int r = 4 * sub + (tid >> 6); r < rec.z; r += 4 * apart) {
+        float m = kNegInf, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        gather(r, grp % GW, GW, m, l, acc);
+#pragma unroll
+        for (int s = LPR; s < 64; s <<= 1)
+          join(m, l, acc, shfl_xor_f(m, s), shfl_xor_f(l, s),
+               make_float4(shfl_xor_f(acc.x, s), shfl_xor_f(acc.y, s), shfl_xor_f(acc.z, s),
+                           shfl_xor_f(acc.w, s)));
+        const float inv = one_over(l);
+        if (grp % GW == 0)
+          *reinterpret_cast<uint2*>(out_row<T, D>(P.c, rq, rec.y + r, kvh) + 4 * c) =
+              make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+      }
+      continue;
+    }
+    for (int r = sub; r < rec.z; r += apart) {
+      float m = kNegInf, l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      gather(r, grp, G, m, l, acc);
       s_acc[grp][c] = acc;
       if (c == 0) s_ml[grp] = make_float2(m, l);
       __syncthreads();
@@ -1363,7 +1489,6 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(TileParams P) {
           sum += s_ml[w].y * a;
           out += reinterpret_cast<const float*>(s_acc[w])[tid] * a;
         }
-        const Request rq{0, rec.x, 0, 0, 0};
         out_row<T, D>(P.c, rq, rec.y + r, kvh)[tid] = round_to<T>(out * one_over(sum));
       }
       __syncthreads();
@@ -1381,7 +1506,11 @@ Cut cut_of(const bc_shape& s, int tokens) {
   Cut c{};
   const long long steps = ((long long)s.max_pages * BC_PAGE_SIZE + kStep - 1) / kStep;
   const long long rows = (long long)tokens * (s.query_heads / s.kv_heads);
-  if (steps <= kLeastSteps || rows < 1 || rows > 1 << 30 ||
+  // Short tables are not cut: joining costs a launch (one token over 512: 8.2
+  // us, cut 12.5; 64 over 16-512 18.9, 25.8), unless tiles of rows are few (128
+  // new tokens of 1024: 22.1 cut, 27.4).
+  const bool few = rows <= (long long)kFewRows * s.batch;
+  if (steps <= (few ? 16 : 8) || rows < 1 || rows > 1 << 30 ||
       (long long)s.batch * (s.max_pages + 1ll) > 1 << 28 ||
       (long long)s.batch * s.query_heads > 1 << 26)
     return c;
@@ -1417,15 +1546,23 @@ hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned
     P.part_rows = cut.part_rows;
     P.narrow_rows = cut.narrow_rows;
   }
-  if (C.cap > 0.f || C.slopes)
-    chunk_tile_kernel<T, D, false><<<dim3(grid), 256, 0, st>>>(P);
+  if (C.cap > 0.f)
+    chunk_tile_kernel<T, D, Form::kCap><<<dim3(grid), 256, 0, st>>>(P);
+  else if (C.slopes)
+    chunk_tile_kernel<T, D, Form::kBias><<<dim3(grid), 256, 0, st>>>(P);
   else
-    chunk_tile_kernel<T, D, true><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kPlain><<<dim3(grid), 256, 0, st>>>(P);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !ws) return err;
-  const long long most = ((long long)cut.most_parts / 2 + C.batch) * C.hkv * kJoinRows;
-  const long long join = most < 4 * cut.target ? most : 4 * cut.target;
-  chunk_join_kernel<T, D><<<dim3((unsigned)join), 256, 0, st>>>(P);
+  // Enough workgroups for the rows of a record and KV head, on average, but not
+  // more than a round of them: 1024 in place of 2048 save 2 us.
+  const long long pairs = (long long)C.batch * C.hkv, rows = (long long)C.tokens * C.group / C.batch;
+  long long apart = 2ll * cut.target / pairs;
+  apart = apart < rows ? apart : rows;
+  apart = apart < 2 ? 2 : apart > 32 ? 32 : apart;
+  const long long most = ((long long)cut.most_parts / 2 + C.batch) * C.hkv * apart;
+  const long long grid_join = most < 2 * cut.target ? most : 2 * cut.target;
+  chunk_join_kernel<T, D><<<dim3((unsigned)grid_join), 256, 0, st>>>(P, (int)apart);
   return hipGetLastError();
 }
 
@@ -1521,6 +1658,9 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
   }
   if (in.tokens == 0) return BC_SUCCESS;
   if (!in.q || !in.output) return BC_ERROR_INVALID_VALUE;
+  const int group = s.query_heads / s.kv_heads;
+  const bool exact = (long long)in.tokens * group * group < 1ll << 32;
+  const unsigned group_mul = group > 1 && exact ? (unsigned)(((1ull << 32) + group - 1) / group) : 0;
   const ChunkParams P{in.q,
                       in.k,
                       in.v,
@@ -1543,11 +1683,12 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
                       s.batch,
                       s.query_heads,
                       s.kv_heads,
-                      s.query_heads / s.kv_heads,
+                      group,
                       s.max_pages,
                       s.physical_pages,
                       in.causal != 0,
                       in.window,
+                      group_mul,
                       in.scale,
                       in.cap};
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
