@@ -146,7 +146,8 @@ struct ChunkParams {
   long long vp, vs, vh;      // V's
   int tokens, batch, hq, hkv, group, max_pages, phys_pages;
   int causal, window;
-  unsigned group_mul;        // ceil(2^32 / group), or 0: see by_group
+  unsigned group_mul;        // ceil(2^32 / group), or 0: see divide
+  unsigned hkv_mul;          // the same of hkv
   float scale, cap;
 };
 
@@ -180,10 +181,14 @@ __device__ __forceinline__ int request_of(const ChunkParams& P, int t, int lane)
   return b < P.batch && P.starts[b] <= t ? b : -1;
 }
 
-// r / group, as a multiply-high where the host has seen that it is exact (r *
-// group below 2^32).
+// x / by, as a multiply-high where the host has passed mul = ceil(2^32 / by),
+// having seen that it is exact (x * by below 2^32).
+__device__ __forceinline__ int divide(int x, int by, unsigned mul) {
+  return by == 1 ? x : mul ? (int)__umulhi((unsigned)x, mul) : x / by;
+}
+
 __device__ __forceinline__ int by_group(const ChunkParams& P, int r) {
-  return P.group == 1 ? r : P.group_mul ? (int)__umulhi((unsigned)r, P.group_mul) : r / P.group;
+  return divide(r, P.group, P.group_mul);
 }
 
 __device__ __forceinline__ int clamp_len(const ChunkParams& P, int b) {
@@ -334,6 +339,36 @@ struct TileParams {
   int part_rows;    // rows of such a part
   int narrow_rows;  // partial rows of the narrow requests; the others' follow
 };
+
+// The kernel's arguments, read anew: each phase of the tile kernel loads the
+// fields that it needs in one round at its start, and none lives through
+// another phase.  Read through the argument itself they were loaded in five
+// rounds, most of them spilled to lanes of a vector register.
+typedef const __attribute__((address_space(4))) TileParams* Args;
+
+__device__ __forceinline__ const TileParams& reread(Args args) {
+  unsigned long long at = (unsigned long long)args;
+  asm volatile("" : "+s"(at));
+  return *(const TileParams*)(Args)at;
+}
+
+__device__ __forceinline__ void pin_plan(const TileParams& P) {
+  const ChunkParams& C = P.c;
+  asm volatile("" ::"s"(C.starts), "s"(C.lengths), "s"(C.prefix), "s"(C.first), "s"(C.tokens),
+               "s"(C.batch), "s"(C.group), "s"(C.hkv), "s"(C.hkv_mul), "s"(C.max_pages),
+               "s"(C.causal), "s"(C.window), "s"(P.part_acc), "s"(P.target), "s"(P.waves),
+               "s"(P.most_parts));
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ __forceinline__ void pin_rows(const TileParams& P) {
+  const ChunkParams& C = P.c;
+  asm volatile("" ::"s"(C.q), "s"(C.k), "s"(C.v), "s"(C.pages), "s"(C.slopes), "s"(C.first),
+               "s"(C.qt), "s"(C.qh), "s"(C.kp), "s"(C.ks), "s"(C.kh), "s"(C.vp), "s"(C.vs),
+               "s"(C.vh), "s"(C.group), "s"(C.group_mul), "s"(C.max_pages), "s"(C.phys_pages),
+               "s"(C.causal), "s"(C.window), "s"(C.scale), "s"(C.cap));
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 // The rows of one request (new tokens times group), at rows start .. of the
 // step, the first of them at place pos0 of the request.
@@ -490,7 +525,7 @@ __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int shar
       it.r.prefix = prefix_of(C, it.r.b);
       it.parts = __builtin_amdgcn_readlane(parts, at);
       const int in = local - __builtin_amdgcn_readlane(upto - mine, at);
-      const int nth = in / it.parts;
+      const int nth = it.parts == 1 ? in : in / it.parts;
       it.part = in - nth * it.parts;
       it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - nth;
       if (it.parts > 1) {
@@ -612,6 +647,13 @@ template <int D, Form FORM, int NT>
 __device__ __forceinline__ void finish_scores(const ChunkParams& C, f32x16 (&sc)[NT],
                                               const Rows<D>& r, int t0, int g, const Edges& e) {
   if (FORM == Form::kCap) {
+    // The first products to be read here may be the last instruction before a
+    // branch, over which the compiler counts no wait states: it left one or two
+    // between a matrix instruction and the read of its result, which needs
+    // twelve.  (The other forms come to their first read through the masks.)
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
     const float in = C.scale / C.cap * (2.f * kLog2e);
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -867,9 +909,9 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
 // The wide form: 128 rows per workgroup, 32 per wave, each step's K and V
 // shared through LDS.
 template <typename T, int D, Form FORM>
-__device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, int kvh,
+__device__ __forceinline__ void wide_body(const TileParams& A, Args args, const Item& it, int kvh,
                                           uint16_t* s_kv, Seen* s_seen, int* s_bad) {
-  const ChunkParams& C = P.c;
+  const ChunkParams& C = A.c;
   const Request& rq = it.r;
   constexpr int KS = D / 16, CPR = D / 8;
   constexpr int NX = kStep * CPR / 256;  // chunks per thread and step, of K and of V each
@@ -1020,6 +1062,7 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
     if (t + 1 < tend) step(std::integral_constant<int, 1>{}, t + 1);
   }
 
+  const TileParams& P = reread(args);
   R.l += shfl_xor_f(R.l, 32);
   const int r = row0 + lr;
   if (it.parts > 1) {
@@ -1055,7 +1098,7 @@ __device__ __forceinline__ void wide_body(const TileParams& P, const Item& it, i
     const u32x4 w = lds16(out + row * D + (c ^ (row % CPR)) * 8);
     const int rr = row0 + row;
     if (rr < rq.rows) {
-      *reinterpret_cast<u32x4*>(out_row<T, D>(C, rq, rr, kvh) + 8 * c) = w;
+      *reinterpret_cast<u32x4*>(out_row<T, D>(P.c, rq, rr, kvh) + 8 * c) = w;
     }
   }
 }
@@ -1376,13 +1419,15 @@ __device__ __forceinline__ void clear_rows(const ChunkParams& C, long long at, l
 }
 
 template <typename T, int D, Form FORM>
-__global__ __launch_bounds__(256, 2) void chunk_tile_kernel(TileParams P) {
+__global__ __launch_bounds__(256, 2) void chunk_tile_kernel(TileParams) {
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[2 * 2 * kStep * D];
   __shared__ float2 s_ml[4 * 32];
   __shared__ Seen s_seen[4];
   __shared__ int s_bad[4];
   const int lane = threadIdx.x & 63;
-  // KV heads in the low bits: with eight of them, each XCD serves one.
+  const Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  const TileParams& P = reread(args);
+  pin_plan(P);
   const Asked head = asked_of(P.c, lane);
   Cutting cut{};
   if (P.part_acc) cut = cut_batch(P, head, lane);
@@ -1391,13 +1436,15 @@ __global__ __launch_bounds__(256, 2) void chunk_tile_kernel(TileParams P) {
   // matrix units', so they run beside each other.
   const bool flat = (int)blockIdx.x < cut.groups;
   // KV heads in the low bits: with eight of them, each XCD serves one.
-  const unsigned in = blockIdx.x - cut.groups, at = in / (unsigned)P.c.hkv;
+  const int in = blockIdx.x - cut.groups, at = divide(in, P.c.hkv, P.c.hkv_mul);
   const int kvh = in - at * P.c.hkv;
   Item it{};
   if (!flat || counts) it = plan_item(P, head, cut.share, flat ? -1ll : (long long)at, lane, counts);
   if (counts && threadIdx.x == 0) P.records[0] = make_int4(it.records, it.narrow_records, 0, 0);
   if (flat) {
-    flat_body<T, D, FORM>(P, head, cut, s_kv);
+    const TileParams& A = reread(args);
+    pin_rows(A);
+    flat_body<T, D, FORM>(A, head, cut, s_kv);
     return;
   }
   if (!it.found) {
@@ -1409,10 +1456,12 @@ __global__ __launch_bounds__(256, 2) void chunk_tile_kernel(TileParams P) {
     put_record(P, it.record, it.r.start, it.tile * kManyRows,
                min(it.r.rows - it.tile * kManyRows, kManyRows), it.parts,
                P.narrow_rows + it.slot * P.part_rows, P.part_rows);
+  const TileParams& A = reread(args);
+  pin_rows(A);
   if (it.r.rows <= kFewRows)
-    narrow_body<T, D, FORM>(P.c, it.r, kvh, s_kv, s_ml);
+    narrow_body<T, D, FORM>(A.c, it.r, kvh, s_kv, s_ml);
   else
-    wide_body<T, D, FORM>(P, it, kvh, s_kv, s_seen, s_bad);
+    wide_body<T, D, FORM>(A, args, it, kvh, s_kv, s_seen, s_bad);
 }
 
 // One part's state joined to another's.
@@ -1661,6 +1710,8 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
   const int group = s.query_heads / s.kv_heads;
   const bool exact = (long long)in.tokens * group * group < 1ll << 32;
   const unsigned group_mul = group > 1 && exact ? (unsigned)(((1ull << 32) + group - 1) / group) : 0;
+  const bool few_heads = s.kv_heads > 1 && s.kv_heads <= 64;  // grids below 2^26, see `tiled`
+  const unsigned hkv_mul = few_heads ? (unsigned)(((1ull << 32) + s.kv_heads - 1) / s.kv_heads) : 0;
   const ChunkParams P{in.q,
                       in.k,
                       in.v,
@@ -1689,6 +1740,7 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
                       in.causal != 0,
                       in.window,
                       group_mul,
+                      hkv_mul,
                       in.scale,
                       in.cap};
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -1703,7 +1755,7 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
   const long long far = 1 << 26;
   const bool tiled = aligned16(in.q) && aligned16(in.k) && aligned16(in.v) && aligned16(in.output) &&
                      bits % 8 == 0 && in.k_strides.slot < far && in.v_strides.slot < far &&
-                     rows <= 1 << 30 && grid <= 0x7fffffff;
+                     rows <= 1 << 30 && grid <= 1 << 26;
   void* const ws = use ? workspace : nullptr;
   if (tiled) {
     if (in.dtype == BC_FLOAT16)
