@@ -10,6 +10,7 @@
 // keeps the ops safe under HIP graph capture.
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -441,10 +442,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_tables_hip(
               "all tensors must share a device");
   const c10::DeviceGuard guard(lengths.device());
   const int64_t b = lengths.size(0);
-  auto pages = at::empty({b, max_pages}, lengths.options());
-  auto starts = at::empty({b + 1}, lengths.options());
-  auto slots = at::empty({tokens}, lengths.options());
-  auto positions = at::empty({tokens}, lengths.options());
+  // Straight from the allocator: a dispatched at::empty takes 0.8 us, and the
+  // call's time is the host's.
+  auto ints = [&](at::IntArrayRef size) {
+    return at::Tensor(at::detail::empty_cuda(size, at::kInt, lengths.device(), std::nullopt));
+  };
+  auto pages = ints({b, max_pages}), starts = ints({b + 1});
+  auto slots = ints({tokens}), positions = ints({tokens});
   check_launch(bc_build_tables(page_ids.data_ptr<int>(), int(page_ids.numel()),
                                lengths.data_ptr<int>(), counts.data_ptr<int>(), int(b),
                                int(max_pages), int(tokens), pages.data_ptr<int>(),
@@ -656,4 +660,6 @@ TORCH_LIBRARY_IMPL(branchcraft, CUDA, m) {
 TORCH_LIBRARY_IMPL(branchcraft, Autograd, m) {
   m.impl("write_prefix_", write_prefix_autograd);
   m.impl("append_kv_", append_kv_autograd);
+  // Whole numbers have no gradient: past autograd at once (0.8 of 8.7 us a call).
+  m.impl("build_tables", torch::CppFunction::makeFallthrough());
 }
