@@ -887,6 +887,13 @@ __device__ __forceinline__ Seen wave_seen(const Rows<D>& R, bool real) {
           wave_max_i(real ? (some ? R.lo : 0x7fffffff) : 0), wave_min_i(real ? R.hi : 0x7fffffff)};
 }
 
+// Ends the wait for Q where it stands.
+template <int N>
+__device__ __forceinline__ void wait_rows(u32x4 (&qB)[N]) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) asm volatile("" : "+v"(qB[s]));
+}
+
 __device__ __forceinline__ float one_over(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }
 
 template <typename T, int D>
@@ -1004,13 +1011,14 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     for (int x = 0; x < NX; ++x) issue_chunk(x, 0, 0);
     pages = (int)pg.in_pool & 15;
     is_whole = pages == 15 && t0 >= whole_lo && t0 < whole_hi;
-    // The wait for Q belongs here, not inside the loop over steps.
-#pragma unroll
-    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qB[s]));
     wait_loads();
     if (!is_whole) bad = inspect(tokens_of<4>(rq.len - t0 * kStep, pages), s_kv + HALF);
     bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));
   }
+  // The wait for Q belongs here, on every path into the loop: at its first use
+  // the compiler's wait, inside the loop, also covers the loads that each step
+  // has just issued.
+  wait_rows(qB);
   // One step, its K and V in buffer `buf`; the next one's loads go out between
   // the score products.
   auto step = [&](auto which, int t) {
@@ -1273,6 +1281,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
     Part n;
     const bool more = next_part(n);
     const int ids_more = more ? st.ids(n.rq.b, first_of(n), 1) : 0;
+    wait_rows(qB);
     for (;; ++t) {
       f32x16 sc[1];
       st.scores(sc, qB, R, t);
@@ -1350,6 +1359,7 @@ __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request&
     int ids_next = st.ids(rq.b, t + 128, 4), at = 0, pages = st.in_pool(0);
     st.issue_k(0);
     st.issue_v(0);
+    wait_rows(qB);
     for (; t < tend; t += 4) {
       f32x16 sc[1];
       st.scores(sc, qB, R, t);
