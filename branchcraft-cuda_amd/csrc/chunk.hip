@@ -167,10 +167,15 @@ __device__ __forceinline__ uint16_t round_to(float x) {
   return __builtin_bit_cast(uint16_t, (T)x);  // to nearest, ties to even
 }
 
-// tanh in terms of one exponential: 1 - 2 / (e^2x + 1), whose absolute error
-// is a few 2^-24; exact at both infinities.
-__device__ __forceinline__ float fast_tanh(float x) {
-  return 1.f - 2.f * __builtin_amdgcn_rcpf(fast_exp2(x * (2.f * kLog2e)) + 1.f);
+// tanh in terms of one exponential, 1 - 2 / (e^2x + 1), which is off by a few
+// 2^-24 and so loses small arguments; those take the first terms of the
+// series, whose next one is below 2^-24 of x for |x| < 0.3.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float y = x * x;
+  const float small =
+      x + x * y * (-1.f / 3.f + y * (2.f / 15.f + y * (-17.f / 315.f + y * (62.f / 2835.f))));
+  const float large = 1.f - 2.f * __builtin_amdgcn_rcpf(fast_exp2(x * (2.f * kLog2e)) + 1.f);
+  return __builtin_fabsf(x) < 0.3f ? small : large;
 }
 
 // The request that row t belongs to: the number of ends at or below t, for
@@ -239,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void chunk_rows_kernel(ChunkParams P) {
         float dot = 0.f;
         for (int d = 0; d < D; ++d) dot += load_elem<T>(q + d) * load_elem<T>(k + d);
         s = dot * P.scale;
-        if (P.cap > 0.f) s = P.cap * fast_tanh(s / P.cap);
+        if (P.cap > 0.f) s = P.cap * tanh_of(s / P.cap);
         s = s * kLog2e - slope * fabsf((float)(pos - j));
       }
       const float mn = __builtin_fmaxf(m, wave_max(s));
@@ -534,7 +539,10 @@ __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int shar
       if (it.parts > 1) {
         it.slot = slots + lanes_sum(lane < at ? cut_parts : 0) + in - it.part;
         it.record = records + lanes_sum(lane < at ? cut_tiles : 0) + nth;
-        if (it.slot + it.parts > P.most_parts) it.parts = 1;  // cannot be: see Cutting
+        // Cannot be (see Cutting) unless starts decrease.
+        if (it.slot < 0 || it.slot + it.parts > P.most_parts || it.record < 0 ||
+            it.record >= P.most_parts / 2)
+          it.parts = 1;
       }
       if (!all) return it;
     }
@@ -604,8 +612,10 @@ __device__ __forceinline__ u32x4 read_v(const uint16_t* lo, const uint16_t* hi) 
 //    one FMA per score in place of a zero.
 //  - Cap: cap tanh(x) = cap - 2 cap / (e^2x + 1), of which the softmax drops the
 //    constant, so s = -1 / (e^2x + 1) and scale2 = 2 cap log2 e; two more
-//    transcendentals per score.  A bias is added to s in these units.
+//    transcendentals per score.  That is off by about cap 2^-23, so large caps
+//    take s = tanh(x) / 2 by tanh_of.  A bias is added to s in these units.
 enum class Form { kPlain, kBias, kCap };
+constexpr float kFineCap = 256.f;
 
 template <int D>
 __device__ __forceinline__ float scale2_of(const ChunkParams& C, Form form) {
@@ -657,12 +667,19 @@ __device__ __forceinline__ void finish_scores(const ChunkParams& C, f32x16 (&sc)
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 15");
     __builtin_amdgcn_sched_barrier(0);
-    const float in = C.scale / C.cap * (2.f * kLog2e);
+    const float in = C.scale / C.cap;
+    if (C.cap <= kFineCap) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+      for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        sc[i][j] = __builtin_amdgcn_rcpf(-1.f - fast_exp2(sc[i][j] * in));
+        for (int j = 0; j < 16; ++j)
+          sc[i][j] = __builtin_amdgcn_rcpf(-1.f - fast_exp2(sc[i][j] * (in * (2.f * kLog2e))));
+    } else {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sc[i][j] = 0.5f * tanh_of(sc[i][j] * in);
+    }
     if (C.slopes) {
       const float from = (float)(r.pos - t0 - 4 * g);
 #pragma unroll
@@ -1310,8 +1327,10 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
     R.l += shfl_xor_f(R.l, 32);
     const int from = p.x0 / cut.run, parts = (p.x0 + p.tiles - 1) / cut.run - from + 1;
     const int first = p.row + 32 * from;
+    // Partials past their place cannot be unless starts decrease.
+    const bool fits = first + 32 * (parts - 1) + p.rq.rows <= P.narrow_rows;
     if (p.x0 >= lo && kvh == 0 && lane == 0)
-      put_record(P, P.most_parts / 2 + p.nth, p.rq.start, 0, p.rq.rows, parts, first, 32);
+      put_record(P, P.most_parts / 2 + p.nth, p.rq.start, 0, p.rq.rows, fits ? parts : 0, first, 32);
     if (parts == 1) {
       const float inv = one_over(R.l);
       if (lr < p.rq.rows) {
@@ -1326,7 +1345,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
       }
     } else {
       const int row = first + 32 * (range - from) + lr;
-      if (lr < p.rq.rows && row < P.narrow_rows) {
+      if (lr < p.rq.rows && fits) {
         const size_t to_row = partial_row(P, row, kvh);
         if (g == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * to_row) = make_float2(R.m, R.l);
 #pragma unroll
@@ -1718,9 +1737,9 @@ extern "C" size_t bc_chunk_attention_workspace_size(bc_shape s, int tokens) {
 
 extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspace,
                                   size_t workspace_bytes, bc_stream_t stream) {
-  if (!chunk_shape_ok(s, in.tokens) || in.window < 0 || !(in.scale > 0.f) ||
-      !(in.scale < __builtin_huge_valf()) || !(in.cap >= 0.f) ||
-      !(in.cap < __builtin_huge_valf()) ||
+  if (!chunk_shape_ok(s, in.tokens) || in.window < 0 || !(in.scale >= BC_LEAST_SCALE) ||
+      !(in.scale <= BC_MOST_SCALE) ||
+      !(in.cap == 0.f || (in.cap >= BC_LEAST_SCALE && in.cap <= BC_MOST_SCALE)) ||
       (in.dtype != BC_FLOAT16 && in.dtype != BC_BFLOAT16))
     return BC_ERROR_INVALID_VALUE;
   if (!in.k || !in.v || !in.pages || !in.lengths || !in.starts) return BC_ERROR_INVALID_VALUE;

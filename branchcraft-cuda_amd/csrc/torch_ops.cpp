@@ -576,11 +576,11 @@ at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const a
                   b < INT32_MAX && hq <= BC_MAX_CHUNK_HEADS,
               "chunk attention: too many rows, heads, pages or requests");
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(double(d));
-  TORCH_CHECK(s > 0 && std::isfinite(float(s)) && float(s) > 0,
-              "scale must be positive and finite");
+  TORCH_CHECK(float(s) >= BC_LEAST_SCALE && float(s) <= BC_MOST_SCALE,
+              "scale must be positive, between ", BC_LEAST_SCALE, " and ", BC_MOST_SCALE);
   TORCH_CHECK(window >= 0, "window must not be negative");
-  TORCH_CHECK(cap >= 0 && std::isfinite(float(cap)) && (cap == 0 || float(cap) > 0),
-              "cap must be finite and not negative");
+  TORCH_CHECK(cap == 0 || (float(cap) >= BC_LEAST_SCALE && float(cap) <= BC_MOST_SCALE),
+              "cap must be 0 (none), or between ", BC_LEAST_SCALE, " and ", BC_MOST_SCALE);
   TORCH_CHECK(q.device() == k.device() && q.device() == v.device() &&
                   q.device() == pages.device() && q.device() == lengths.device() &&
                   q.device() == starts.device(),

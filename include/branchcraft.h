@@ -330,6 +330,10 @@ enum {
 };
 /* Most query heads bc_chunk_attention takes. */
 #define BC_MAX_CHUNK_HEADS 4096
+/* Bounds of its scale, and of a cap: quotients of the two, and of a slope and
+ * the scale, stay inside 32 bits. */
+#define BC_LEAST_SCALE 1e-12f
+#define BC_MOST_SCALE 1e12f
 
 /* Strides in elements; the head dimension is contiguous.  Rows of new tokens
  * [tokens, heads, D], and pools [P, 16, Hkv, D] in any order of pages, slots
@@ -384,7 +388,8 @@ int bc_append_kv(bc_shape shape, const bc_half* k, const bc_half* v,
  * output [tokens, Hq, D] contiguous, of the inputs' type.  pages [B,
  * max_pages], lengths [B] (each request's tokens in the cache, its new ones
  * included) and starts [B + 1] (request b's rows are starts[b] ..
- * starts[b+1] - 1: its last tokens, in order).  Null where they do not apply:
+ * starts[b+1] - 1: its last tokens, in order; starts must not decrease, or
+ * some rows' output is not specified).  Null where they do not apply:
  * slopes [Hq], prefix [B], first [tokens]. */
 typedef struct bc_chunk_inputs {
   const bc_half* q;
@@ -424,8 +429,9 @@ typedef struct bc_chunk_inputs {
  * infinity included.  Scores, sums and the output's accumulation are 32-bit;
  * the weights are rounded to the inputs' type for the product with V.
  * Rejects: batch/Hq/Hkv < 1, Hq % Hkv != 0, Hq over BC_MAX_CHUNK_HEADS,
- * dim not 64/128, max_pages or physical_pages < 1, tokens or window < 0, scale not positive and finite,
- * cap negative or not finite, negative strides, null pointers. */
+ * dim not 64/128, max_pages or physical_pages < 1, tokens or window < 0, a
+ * scale, or a cap other than 0, outside [BC_LEAST_SCALE, BC_MOST_SCALE],
+ * negative strides, null pointers. */
 int bc_chunk_attention(bc_shape shape, bc_chunk_inputs in, void* workspace,
                        size_t workspace_bytes, bc_stream_t stream);
 

@@ -29,7 +29,7 @@ BAD_SHAPES = [dict(batch=0), dict(query_heads=0), dict(kv_heads=0), dict(query_h
 BAD_INPUTS = [dict(q=None), dict(k=None), dict(v=None), dict(pages=None), dict(lengths=None),
               dict(starts=None), dict(output=None), dict(tokens=-1), dict(window=-1), dict(dtype=2),
               dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0),
-              dict(cap=math.nan), dict(cap=math.inf), dict(q_strides=capi.RowStrides(-1, 128)),
+              dict(cap=math.nan), dict(cap=math.inf), dict(cap=1e-13), dict(cap=1e13), dict(scale=1e-13), dict(scale=1e13), dict(q_strides=capi.RowStrides(-1, 128)),
               dict(k_strides=capi.PoolStrides(1, -1, 1)), dict(v_strides=capi.PoolStrides(1, 1, -1))]
 
 
@@ -39,7 +39,7 @@ def test_chunk_rejects_shapes(bad):
     assert capi.load().bc_chunk_attention_workspace_size(_shape(**bad), 3) == 0
 
 
-@pytest.mark.parametrize("bad", BAD_INPUTS, ids=lambda bad: next(iter(bad)))
+@pytest.mark.parametrize("bad", BAD_INPUTS, ids=str)
 def test_chunk_rejects_inputs(bad):
     assert capi.load().bc_chunk_attention(_shape(), _chunk(**bad), None, 0, None) == INVALID
 
@@ -111,3 +111,28 @@ def test_cpu_tensors_have_no_implementation():
     ints = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(NotImplementedError):
         bt.build_tables(ints, ints, ints, 1, 1)
+
+
+def test_matrix_results_are_waited_for():
+    """Wait states between a matrix instruction of the tile kernels and the
+    vector instructions that touch its registers, over branches too: the
+    compiler keeps twelve to a read of the result, and ten are the fewest that
+    an accumulator's next writer has passed with."""
+    import shutil
+    import tempfile
+    from pathlib import Path
+
+    import asm_hazards as H
+    if not (shutil.which("hipcc") or Path("/opt/rocm/bin/hipcc").exists()):
+        pytest.skip("hipcc not available")
+    with tempfile.TemporaryDirectory() as tmp:
+        kernels = H.kernels(H.compile_device_asm(H.CSRC / "chunk.hip", Path(tmp)))
+    found = 0
+    for name, lines in kernels.items():
+        insts, labels = H.parse(lines)
+        if not any(op.startswith("v_mfma") for op, _ in insts):
+            continue
+        found += 1
+        best = H.scan(insts, labels, window=12)
+        assert best.get("RAW", 12) >= 12 and best.get("WAW", 10) >= 10 and best.get("WARC", 10) >= 10, (name, best)
+    assert found == 12
