@@ -424,6 +424,12 @@ at::Tensor int_tensor_hip(const at::Tensor& like, at::IntArrayRef values) {
   return out;
 }
 
+// Memory straight from the allocator: a dispatched at::empty takes 0.8 us, and
+// small calls' time is the host's.
+at::Tensor new_tensor(const at::Tensor& like, at::IntArrayRef size, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(size, type, like.device(), std::nullopt));
+}
+
 // Block table, row offsets, slot map and positions of a step (see
 // bc_build_tables); `tokens` rows, those behind the last request -1.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_tables_hip(
@@ -442,11 +448,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_tables_hip(
               "all tensors must share a device");
   const c10::DeviceGuard guard(lengths.device());
   const int64_t b = lengths.size(0);
-  // Straight from the allocator: a dispatched at::empty takes 0.8 us, and the
-  // call's time is the host's.
-  auto ints = [&](at::IntArrayRef size) {
-    return at::Tensor(at::detail::empty_cuda(size, at::kInt, lengths.device(), std::nullopt));
-  };
+  auto ints = [&](at::IntArrayRef size) { return new_tensor(lengths, size, at::kInt); };
   auto pages = ints({b, max_pages}), starts = ints({b + 1});
   auto slots = ints({tokens}), positions = ints({tokens});
   check_launch(bc_build_tables(page_ids.data_ptr<int>(), int(page_ids.numel()),
@@ -522,16 +524,19 @@ void append_kv_hip(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k
                "append_kv_");
 }
 
-// Above the kernel: it has no derivative, so tensors that autograd tracks or
-// that carry a tangent are refused, and the pools' version counters move, so
-// that a backward that saved a pool before the rows entered it raises.
+// Neither has a derivative.
+void refuse_tracked(const char* op, std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* x : tensors)
+    TORCH_CHECK(!(x->requires_grad() && at::GradMode::is_enabled()) && !x->_fw_grad(0).defined(),
+                op, " is not differentiable: detach its tensors or call it under no_grad");
+}
+
+// Above the kernel: tensors that autograd tracks or that carry a tangent are
+// refused, and the pools' version counters move, so that a backward that saved
+// a pool before the rows entered it raises.
 void append_kv_autograd(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k,
                         const at::Tensor& v, const at::Tensor& slots) {
-  for (const at::Tensor* x :
-       std::initializer_list<const at::Tensor*>{&cache_k, &cache_v, &k, &v})
-    TORCH_CHECK(!(x->requires_grad() && at::GradMode::is_enabled()) &&
-                    !x->_fw_grad(0).defined(),
-                "append_kv_ is not differentiable: detach its tensors or call it under no_grad");
+  refuse_tracked("append_kv_", {&cache_k, &cache_v, &k, &v});
   static const auto op =
       c10::Dispatcher::singleton()
           .findSchemaOrThrow("branchcraft::append_kv_", "")
@@ -599,7 +604,7 @@ at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const a
   in.first = static_cast<const int32_t*>(option(first, "first", at::kInt, t));
   TORCH_CHECK(causal || !in.prefix, "prefix needs causal attention");
   const c10::DeviceGuard guard(q.device());
-  auto output = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  auto output = new_tensor(q, q.sizes(), q.scalar_type());
   if (t == 0) return output;
   in.q = raw(q);
   in.k = raw(k);
@@ -620,11 +625,28 @@ at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const a
   bc_shape shape{int(b), int(hq), int(hkv), int(d), int(pages.size(1)), int(k.size(0))};
   const size_t ws_bytes = bc_chunk_attention_workspace_size(shape, int(t));
   at::Tensor ws;
-  if (ws_bytes > 0) ws = at::empty({int64_t(ws_bytes)}, q.options().dtype(at::kByte));
+  if (ws_bytes > 0) ws = new_tensor(q, {int64_t(ws_bytes)}, at::kByte);
   check_launch(bc_chunk_attention(shape, in, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
                                   current_stream()),
                "chunk_attention");
   return output;
+}
+
+at::Tensor chunk_attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                    const at::Tensor& pages, const at::Tensor& lengths,
+                                    const at::Tensor& starts, std::optional<double> scale,
+                                    bool causal, int64_t window, double cap,
+                                    const std::optional<at::Tensor>& slopes,
+                                    const std::optional<at::Tensor>& prefix,
+                                    const std::optional<at::Tensor>& first) {
+  refuse_tracked("chunk_attention", {&q, &k, &v});
+  if (slopes.has_value() && slopes->defined()) refuse_tracked("chunk_attention", {&*slopes});
+  static const auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("branchcraft::chunk_attention", "")
+          .typed<decltype(chunk_attention_hip)>();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, v, pages, lengths, starts, scale, causal, window, cap, slopes, prefix, first);
 }
 
 }  // namespace
@@ -660,6 +682,7 @@ TORCH_LIBRARY_IMPL(branchcraft, CUDA, m) {
 TORCH_LIBRARY_IMPL(branchcraft, Autograd, m) {
   m.impl("write_prefix_", write_prefix_autograd);
   m.impl("append_kv_", append_kv_autograd);
+  m.impl("chunk_attention", chunk_attention_autograd);
   // Whole numbers have no gradient: past autograd at once (0.8 of 8.7 us a call).
   m.impl("build_tables", torch::CppFunction::makeFallthrough());
 }

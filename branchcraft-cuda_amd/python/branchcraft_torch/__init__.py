@@ -85,6 +85,12 @@ def _fake_chunk_attention(q, k, v, pages, lengths, starts, scale=None, causal=Tr
     return q.new_empty(q.shape)
 
 
+# The ops themselves: through the packet a call costs its host 0.4 us more.
+_build_tables = torch.ops.branchcraft.build_tables.default
+_append_kv = torch.ops.branchcraft.append_kv_.default
+_chunk_attention = torch.ops.branchcraft.chunk_attention.default
+
+
 def tree_verify(q, prefix_k, prefix_v, pages, lengths, draft_k, draft_v, parent):
     """FP32 [batch, node, query head, dim] outputs; every node attends to its
     request's paged prefix and its own ancestor chain (itself included)."""
@@ -150,7 +156,7 @@ def build_tables(page_ids, lengths, counts, max_pages, tokens):
     ``counts[b]`` of them new, and its ceil(length / 16) page ids follow those of
     the request before it in ``page_ids``.  -1 stands behind a request's pages,
     in rows behind the last request, and for rows without a slot."""
-    return torch.ops.branchcraft.build_tables(page_ids, lengths, counts, max_pages, tokens)
+    return _build_tables(page_ids, lengths, counts, max_pages, tokens)
 
 
 def append_kv_(cache_k, cache_v, k, v, slots):
@@ -158,7 +164,7 @@ def append_kv_(cache_k, cache_v, k, v, slots):
     strides with a contiguous last dim) to the slots of ``build_tables``; -1 and
     slots outside the pool are skipped.  The pools may be strided views, such
     as the two halves of a packed cache."""
-    return torch.ops.branchcraft.append_kv_(cache_k, cache_v, k, v, slots)
+    return _append_kv(cache_k, cache_v, k, v, slots)
 
 
 def chunk_attention(q, k, v, pages, lengths, starts, *, scale=None, causal=True, window=0,
@@ -172,9 +178,10 @@ def chunk_attention(q, k, v, pages, lengths, starts, *, scale=None, causal=True,
     first ``prefix[b]`` with a prefix), from ``p - window + 1`` with a window,
     from ``first[row]`` with documents.  Scores are ``scale * q.k`` (default
     1/sqrt(dim)), then ``cap * tanh(score / cap)``, then minus ``slopes[head] *
-    |p - token|``.  Rows that see nothing, and rows of no request, are zero."""
-    return torch.ops.branchcraft.chunk_attention(
-        q, k, v, pages, lengths, starts, scale, causal, window, cap, slopes, prefix, first)
+    |p - token|``.  Rows that see nothing, and rows of no request, are zero.
+    Not differentiable: tensors that autograd tracks are refused."""
+    return _chunk_attention(q, k, v, pages, lengths, starts, scale, causal, window, cap, slopes,
+                            prefix, first)
 
 
 __all__ = ["tree_verify", "packed_decode_out", "paged_decode",

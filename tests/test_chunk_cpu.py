@@ -90,7 +90,7 @@ def test_fake_tensors_and_versions():
         assert out.shape == q.shape and out.dtype == q.dtype
 
 
-def test_append_refuses_what_autograd_tracks():
+def test_what_autograd_tracks_is_refused():
     import branchcraft_torch as bt
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
@@ -104,6 +104,16 @@ def test_append_refuses_what_autograd_tracks():
                 bt.append_kv_(*args, slots)
             with torch.no_grad():
                 bt.append_kv_(*args, slots)
+        q = torch.zeros(7, 4, 64, device="cuda", dtype=torch.float16)
+        ints = [torch.zeros(n, device="cuda", dtype=torch.int32) for n in ((1, 4), (1,), (2,))]
+        slopes = torch.zeros(4, device="cuda")
+        for at in range(4):
+            args = [q, *pools, slopes]
+            args[at] = args[at].clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                bt.chunk_attention(*args[:3], *ints, slopes=args[3])
+            with torch.no_grad():
+                assert not bt.chunk_attention(*args[:3], *ints, slopes=args[3]).requires_grad
 
 
 def test_cpu_tensors_have_no_implementation():
