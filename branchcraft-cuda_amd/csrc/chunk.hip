@@ -113,6 +113,8 @@ struct AppendParams {
 };
 
 // Workgroup i copies rows_per_block rows, K then V, in elements of type E.
+// HBM-bound: 8192 rows of 8 heads x 128 out of a fused projection (67 MB) 12.1
+// us, 5.5 TB/s, as a large copy; 64 rows 2.6 us.
 template <typename E>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams P, int rows_per_block) {
   const int t0 = blockIdx.x * rows_per_block;
@@ -933,8 +935,16 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
   P.records[2 + 2 * i] = make_int4(first, stride, 0, 0);
 }
 
-// The wide form: 128 rows per workgroup, 32 per wave, each step's K and V
-// shared through LDS.
+// The wide form: 128 rows per workgroup, 32 per wave, each 64-token step's K
+// and V shared through two LDS buffers, which loads straight into LDS fill one
+// step ahead; one barrier a step, two workgroups per CU (three at D = 64).
+//  - 128 rows: the step's 32 KB from L2 serve 4.2 MFLOP.  32 rows per wave: the
+//    output takes 64 registers, and eight waves fit a CU's register file.
+//  - Bound at D = 128 by the matrix units and the clock that they leave (2048
+//    rows over 32768 tokens, 32/8 heads: 1020 us, 1044 TFLOP/s; a library
+//    product of 8192^3 1246), at D = 64 by the vector units: the same softmax
+//    for half the products (32 heads, 512 over 2048: 177 us, 680 TFLOP/s).
+//  - A workgroup's start and end take 7 us beside its neighbour's steps of 1.9.
 template <typename T, int D, Form FORM>
 __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const Item& it, int kvh,
                                           uint16_t* s_kv, Seen* s_seen, int* s_bad) {
@@ -1229,7 +1239,12 @@ struct Stream {
 };
 
 // The narrow form over a batch: the tiles of all requests with few rows, one
-// after another, in ranges of equal length, a range per wave.  A request that
+// after another, in ranges of equal length, a range per wave.  HBM-bound: 64
+// single tokens over 128-4096 tokens (32/8 heads, D = 128, 585 MB) 96 us, 6.5
+// TB/s in this kernel; with a part of a request per workgroup, the longest
+// parts last, it took 127.  The waves of a workgroup take the KV heads of one
+// range, whose lines lie side by side: 108 -> 99 us with four waves per CU in
+// place of eight.  A request that
 // a range holds whole leaves as output rows, of others each range leaves a
 // partial.  Range r's partial of a request whose predecessors have n rows
 // starts at partial row 32 r + n: a range's next request is further by the
@@ -1516,7 +1531,7 @@ __device__ __forceinline__ void join(float& m, float& l, float4& acc, float m2, 
 
 constexpr int kFewParts = 16;  // parts that one wave joins by itself
 
-// Joins the partials: `apart` workgroups share the rows of a record and KV
+// Joins the partials, latency-bound (4 to 5 us): `apart` workgroups share the rows of a record and KV
 // head.  Few parts: a wave per row, each group of D / 4 lanes taking the parts
 // in turn; many: the whole workgroup per row.
 template <typename T, int D>
