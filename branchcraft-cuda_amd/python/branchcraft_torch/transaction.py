@@ -201,8 +201,8 @@ class PagedTreeCache:
             raise ValueError("q, k and v must have the cache's type and device")
         if not self.k.is_cuda:
             raise ValueError("extend needs a cache on the GPU")
-        if torch.is_grad_enabled() and any(x.requires_grad for x in (self.k, self.v, k, v)):
-            raise ValueError("extend is not differentiable: detach k and v, or use no_grad")
+        if torch.is_grad_enabled() and any(x.requires_grad for x in (self.k, self.v, q, k, v)):
+            raise ValueError("extend is not differentiable: detach q, k and v, or use no_grad")
         q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
         if options:  # refused here, before any page is taken
             first = options.get("first")

@@ -227,6 +227,7 @@ def test_extend_refuses_before_anything_changes():
                 ([a, b], [31, -1], q, k, {}), ([a], [29], q, k, {}), ([a], [30], q[:, :3], k, {}),
                 ([a], [30], q.bfloat16(), k, {}), ([a], [30], q, k.cpu(), {}),
                 ([a], [5], q[:5], k[:5].clone().requires_grad_(), {}),
+                ([a], [5], q[:5].clone().requires_grad_(), k[:5], {}),
                 ([a], [5], q[:5], k[:5], dict(cap=-1.0)), ([a], [5], q[:5], k[:5], dict(windows=1)),
                 ([a], [5], q[:5], k[:5], dict(first=torch.zeros(4, device="cuda", dtype=torch.int32)))]
     for requests, counts, qq, kk, options in refusals:
