@@ -201,8 +201,9 @@ __device__ __forceinline__ int by_group(const ChunkParams& P, int r) {
   return divide(r, P.group, P.group_mul);
 }
 
+// Inside the table's row, and so a few steps below 2^31 (BC_MAX_TABLE_PAGES).
 __device__ __forceinline__ int clamp_len(const ChunkParams& P, int b) {
-  return max(0, (int)min((long long)P.lengths[b], (long long)P.max_pages * BC_PAGE_SIZE));
+  return min(max(P.lengths[b], 0), P.max_pages * BC_PAGE_SIZE);
 }
 
 // The tokens lo .. hi that row t at position pos of request b sees.
@@ -434,13 +435,14 @@ struct Asked {
   int first_tile, narrow;  // of the narrow form
 };
 
-__device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b) {
+// With `tiles` the narrow form's tiles are those that the rows' documents reach.
+__device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b, bool tiles) {
   Asked a{};
   if (b < P.batch) {
     a.start = min(max(P.starts[b], 0), P.tokens);
     a.n = max(min(max(P.starts[b + 1], 0), P.tokens) - a.start, 0);
     a.full = max(P.lengths[b], 0);
-    a.len = (int)min((long long)a.full, (long long)P.max_pages * BC_PAGE_SIZE);
+    a.len = min(a.full, P.max_pages * BC_PAGE_SIZE);
     a.rows = a.n * P.group;
     if (a.rows > kFewRows) {
       a.tiles = (a.rows + kManyRows - 1) / kManyRows;
@@ -449,9 +451,11 @@ __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b) {
       a.steps = max(1, (span + kStep - 1) / kStep);
     } else if (a.rows > 0) {
       int lo = P.window > 0 ? (int)max(0ll, (long long)a.full - a.n - P.window + 1) : 0;
-      if (P.first) {
+      if (P.first && tiles) {
         int least = 0x7fffffff;
-        for (int i = 0; i < a.n; ++i) least = min(least, P.first[a.start + i]);
+        for (int i = 0; i < a.n; i += 4)  // four loads at a time
+#pragma unroll
+          for (int x = 0; x < 4; ++x) least = min(least, P.first[a.start + min(i + x, a.n - 1)]);
         lo = max(lo, least);
       }
       a.first_tile = min(lo, max(a.len - 1, 0)) / 32;
@@ -477,7 +481,7 @@ __device__ __forceinline__ Cutting cut_batch(const TileParams& P, const Asked& h
   float work = (float)head.tiles * (float)head.steps;
   int narrow = head.narrow;
   for (int b = 64 + lane; b - lane < C.batch; b += 64) {
-    const Asked x = asked_of(C, b);
+    const Asked x = asked_of(C, b, true);
     work += (float)x.tiles * (float)x.steps;
     narrow += x.narrow;
   }
@@ -516,7 +520,7 @@ __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int shar
   long long before = 0;
   int slots = 0, records = 0, narrow = 0;
   for (int b0 = 0; b0 < C.batch; b0 += 64) {
-    if (b0 > 0) a = asked_of(C, b0 + lane);
+    if (b0 > 0) a = asked_of(C, b0 + lane, split);
     const int parts = split && a.steps > share ? (a.steps + share - 1) / share : 1;
     const int tiles = split ? a.tiles : a.tiles + (a.narrow > 0);
     const int mine = tiles * parts;
@@ -906,6 +910,12 @@ __device__ __forceinline__ Seen wave_seen(const Rows<D>& R, bool real) {
           wave_max_i(real ? (some ? R.lo : 0x7fffffff) : 0), wave_min_i(real ? R.hi : 0x7fffffff)};
 }
 
+// Waits until at most N of the wave's vector loads are on their way.
+template <int N>
+__device__ __forceinline__ void wait_to() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // Ends the wait for Q where it stands.
 template <int N>
 __device__ __forceinline__ void wait_rows(u32x4 (&qB)[N]) {
@@ -1141,9 +1151,7 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     const int row = i + lane / CPR, c = lane % CPR;
     const u32x4 w = lds16(out + row * D + (c ^ (row % CPR)) * 8);
     const int rr = row0 + row;
-    if (rr < rq.rows) {
-      *reinterpret_cast<u32x4*>(out_row<T, D>(P.c, rq, rr, kvh) + 8 * c) = w;
-    }
+    if (rr < rq.rows) *reinterpret_cast<u32x4*>(out_row<T, D>(P.c, rq, rr, kvh) + 8 * c) = w;
   }
 }
 
@@ -1204,7 +1212,7 @@ struct Stream {
   // The staged tile's scores; K has been read when this returns.
   __device__ __forceinline__ void scores(f32x16 (&sc)[1], const u32x4 (&qB)[KS], const Rows<D>& R,
                                          int t) const {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // K is there, V may be not
+    wait_to<NL>();  // K is there, V may be not
     const f32x16 zero = {};
     if (FORM == Form::kBias) start_scores<D, 1>(C, sc, R, t * 32, lane >> 5);
 #pragma unroll
@@ -1220,10 +1228,8 @@ struct Stream {
     uint16_t* const vt = kt + TILE;
     const Edges e{t * 32 < mine.all_lo, t * 32 + 31 > mine.all_hi, pages != 3, tokens_of<2>(left, pages)};
     finish_scores<D, FORM, 1>(C, sc, R, t * 32, g, e);
-    if (next)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // V is there
-    else
-      wait_loads();
+    if (next) wait_to<NL>();  // V is there
+    else wait_loads();
     bool bad = false;
     if (e.lo || e.hi || e.pages || left < 32) {
 #pragma unroll
@@ -1244,11 +1250,11 @@ struct Stream {
 // TB/s in this kernel; with a part of a request per workgroup, the longest
 // parts last, it took 127.  The waves of a workgroup take the KV heads of one
 // range, whose lines lie side by side: 108 -> 99 us with four waves per CU in
-// place of eight.  A request that
-// a range holds whole leaves as output rows, of others each range leaves a
-// partial.  Range r's partial of a request whose predecessors have n rows
-// starts at partial row 32 r + n: a range's next request is further by the
-// rows of the last one, a request's next range by 32.
+// place of eight.
+// A request that a range holds whole leaves as output rows, of others each
+// range leaves a partial.  Range r's partial of a request whose predecessors
+// have n rows starts at partial row 32 r + n: a range's next request is
+// further by the rows of the last one, a request's next range by 32.
 template <typename T, int D, Form FORM>
 __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cutting& cut,
                                           uint16_t* s_kv) {
@@ -1282,7 +1288,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
       nth += __builtin_popcountll(some);
       b0 += 64;
       if (b0 >= C.batch || before >= hi) return false;
-      a = asked_of(C, b0 + lane);
+      a = asked_of(C, b0 + lane, true);
       look();
     }
     const int at = __builtin_ctzll(left);
@@ -1481,7 +1487,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
   const Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
   const TileParams& P = reread(args);
   pin_plan(P);
-  const Asked head = asked_of(P.c, lane);
+  const Asked head = asked_of(P.c, lane, P.part_acc != nullptr);
   Cutting cut{};
   if (P.part_acc) cut = cut_batch(P, head, lane);
   const bool counts = blockIdx.x == 0 && P.part_acc;
@@ -1685,7 +1691,7 @@ extern "C" int bc_build_tables(const int32_t* page_ids, int held, const int32_t*
     return BC_ERROR_INVALID_VALUE;
   const TableParams P{page_ids, lengths, counts,    pages,     starts, slots, positions,
                       held,     batch,   max_pages, tokens};
-  if (max_pages >= 1 << 27 || tokens >= 1 << 27 || batch == 0x7fffffff) return BC_ERROR_INVALID_VALUE;
+  if (max_pages > BC_MAX_TABLE_PAGES || tokens >= 1 << 27 || batch == 0x7fffffff) return BC_ERROR_INVALID_VALUE;
   const int longest = tokens > max_pages ? tokens : max_pages;
   // At most about four workgroups per CU.
   const int spans = (longest - 1) / kTableSpan + 1, rounds = 4 * bch::device_cus() / (batch + 1);
@@ -1741,7 +1747,8 @@ namespace {
 bool chunk_shape_ok(const bc_shape& s, int tokens) {
   return s.batch >= 1 && s.query_heads >= 1 && s.kv_heads >= 1 &&
          s.query_heads % s.kv_heads == 0 && s.query_heads <= BC_MAX_CHUNK_HEADS &&
-         (s.dim == 64 || s.dim == 128) && s.max_pages >= 1 && s.physical_pages >= 1 && tokens >= 0;
+         (s.dim == 64 || s.dim == 128) && s.max_pages >= 1 && s.max_pages <= BC_MAX_TABLE_PAGES && s.physical_pages >= 1 &&
+         tokens >= 0;
 }
 
 }  // namespace

@@ -441,9 +441,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_tables_hip(
   TORCH_CHECK(page_ids.dim() == 1 && lengths.dim() == 1 && counts.sizes() == lengths.sizes(),
               "build_tables shape mismatch");
   TORCH_CHECK(lengths.size(0) > 0, "build_tables: no requests");
-  TORCH_CHECK(max_pages >= 1 && max_pages < (1 << 27) && tokens >= 0 && tokens < (1 << 27) &&
-                  page_ids.numel() <= INT32_MAX && lengths.numel() < INT32_MAX,
-              "build_tables: max_pages must be at least 1, tokens at least 0, both below 2**27");
+  TORCH_CHECK(max_pages >= 1 && max_pages <= BC_MAX_TABLE_PAGES && tokens >= 0 &&
+                  tokens < (1 << 27) && page_ids.numel() <= INT32_MAX &&
+                  lengths.numel() < INT32_MAX,
+              "build_tables: max_pages must be 1 to ", BC_MAX_TABLE_PAGES,
+              ", tokens at least 0 and below 2**27");
   TORCH_CHECK(page_ids.device() == lengths.device() && page_ids.device() == counts.device(),
               "all tensors must share a device");
   const c10::DeviceGuard guard(lengths.device());
@@ -577,7 +579,7 @@ at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const a
               "K/V cache shape mismatch");
   TORCH_CHECK(pages.size(0) == b && pages.size(1) >= 1 && starts.size(0) == b + 1,
               "chunk attention metadata mismatch");
-  TORCH_CHECK(t <= INT32_MAX && k.size(0) <= INT32_MAX && pages.size(1) <= INT32_MAX &&
+  TORCH_CHECK(t <= INT32_MAX && k.size(0) <= INT32_MAX && pages.size(1) <= BC_MAX_TABLE_PAGES &&
                   b < INT32_MAX && hq <= BC_MAX_CHUNK_HEADS,
               "chunk attention: too many rows, heads, pages or requests");
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(double(d));

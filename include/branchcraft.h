@@ -330,6 +330,9 @@ enum {
 };
 /* Most query heads bc_chunk_attention takes. */
 #define BC_MAX_CHUNK_HEADS 4096
+/* Longest row of a page table for it and bc_build_tables: 256 tokens short of
+ * 2^31. */
+#define BC_MAX_TABLE_PAGES 134217712
 /* Bounds of its scale, and of a cap: quotients of the two, and of a slope and
  * the scale, stay inside 32 bits. */
 #define BC_LEAST_SCALE 1e-12f
@@ -363,7 +366,8 @@ typedef struct bc_pool_strides {
  * page_ids, or in a page with a negative id or one of 2^27 or more; a
  * position before the request is -1.  Negative lengths and counts count as
  * 0.  Rejects: batch or max_pages < 1, held or tokens < 0, null pointers
- * (those of empty arrays aside), tables or maps of 2^27 entries a request or more. */
+ * (those of empty arrays aside), max_pages over BC_MAX_TABLE_PAGES, 2^27
+ * tokens or more. */
 int bc_build_tables(const int32_t* page_ids, int held, const int32_t* lengths,
                     const int32_t* counts, int batch, int max_pages, int tokens,
                     int32_t* pages, int32_t* starts, int32_t* slots,
@@ -429,9 +433,9 @@ typedef struct bc_chunk_inputs {
  * infinity included.  Scores, sums and the output's accumulation are 32-bit;
  * the weights are rounded to the inputs' type for the product with V.
  * Rejects: batch/Hq/Hkv < 1, Hq % Hkv != 0, Hq over BC_MAX_CHUNK_HEADS,
- * dim not 64/128, max_pages or physical_pages < 1, tokens or window < 0, a
- * scale, or a cap other than 0, outside [BC_LEAST_SCALE, BC_MOST_SCALE],
- * negative strides, null pointers. */
+ * dim not 64/128, max_pages < 1 or over BC_MAX_TABLE_PAGES, physical_pages
+ * below 1, tokens or window < 0, a scale, or a cap other than 0, outside
+ * [BC_LEAST_SCALE, BC_MOST_SCALE], negative strides, null pointers. */
 int bc_chunk_attention(bc_shape shape, bc_chunk_inputs in, void* workspace,
                        size_t workspace_bytes, bc_stream_t stream);
 

@@ -25,7 +25,8 @@ def _chunk(**kw):
 
 
 BAD_SHAPES = [dict(batch=0), dict(query_heads=0), dict(kv_heads=0), dict(query_heads=30), dict(dim=96),
-              dict(max_pages=0), dict(physical_pages=0), dict(query_heads=8192, kv_heads=8192)]
+              dict(max_pages=0), dict(physical_pages=0), dict(query_heads=8192, kv_heads=8192),
+              dict(max_pages=(1 << 27) - 15)]
 BAD_INPUTS = [dict(q=None), dict(k=None), dict(v=None), dict(pages=None), dict(lengths=None),
               dict(starts=None), dict(output=None), dict(tokens=-1), dict(window=-1), dict(dtype=2),
               dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0),
@@ -68,7 +69,7 @@ def test_build_tables_rejects():
     lib = capi.load()
     good = [FAKE, 9, FAKE, FAKE, 2, 4, 3, FAKE, FAKE, FAKE, FAKE, None]
     for at, bad in [(0, None), (1, -1), (2, None), (3, None), (4, 0), (5, 0), (6, -1), (7, None), (8, None),
-                    (9, None), (10, None), (5, 2**28), (6, 2**28)]:
+                    (9, None), (10, None), (5, 2**28), (5, 2**27 - 15), (6, 2**28)]:
         args = list(good)
         args[at] = bad
         assert lib.bc_build_tables(*args) == INVALID, (at, bad)
