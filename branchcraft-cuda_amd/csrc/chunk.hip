@@ -1705,7 +1705,7 @@ extern "C" int bc_append_kv(bc_shape s, const bc_half* k, const bc_half* v, bc_r
                             bc_pool_strides cks, bc_pool_strides cvs, const int32_t* slots,
                             int tokens, bc_stream_t stream) {
   if (!k || !v || !cache_k || !cache_v || !slots || tokens < 0 || s.physical_pages < 1 ||
-      s.kv_heads < 1 || (s.dim != 64 && s.dim != 128))
+      s.kv_heads < 1 || s.kv_heads > BC_MAX_CHUNK_HEADS || (s.dim != 64 && s.dim != 128))
     return BC_ERROR_INVALID_VALUE;
   const long long all[] = {ks.token, ks.head, vs.token, vs.head, cks.page,
                            cks.slot, cks.head, cvs.page, cvs.slot, cvs.head};

@@ -506,8 +506,9 @@ void append_kv_hip(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k
   TORCH_CHECK(cache_k.device() == cache_v.device() && cache_k.device() == k.device() &&
                   cache_k.device() == v.device() && cache_k.device() == slots.device(),
               "all tensors must share a device");
-  TORCH_CHECK(k.size(0) <= INT32_MAX && cache_k.size(0) <= INT32_MAX,
-              "append_kv_: too many tokens or pages");
+  TORCH_CHECK(k.size(0) <= INT32_MAX && cache_k.size(0) <= INT32_MAX &&
+                  k.size(1) <= BC_MAX_CHUNK_HEADS,
+              "append_kv_: too many tokens, heads or pages");
   at::assert_no_internal_overlap(cache_k);
   at::assert_no_internal_overlap(cache_v);
   at::assert_no_overlap(cache_k, cache_v);

@@ -18,6 +18,7 @@ decode step.
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import (append_kv_, build_tables, chunk_attention, commit_path_, commit_paths_,
                copy_pages_, int_tensor, tree_verify, write_prefix_)
@@ -188,22 +189,26 @@ class PagedTreeCache:
         before anything changes.  A count may be zero."""
         if len(requests) != len(counts) or len(set(requests)) != len(requests) or not requests:
             raise ValueError("requests must be distinct and match counts")
-        if any(n < 0 for n in counts):
-            raise ValueError("counts must not be negative")
         total = sum(counts)
+        if any(n < 0 for n in counts) or total >= 1 << 27:
+            raise ValueError("counts must not be negative, and below 2**27 in all")
         shape = (total, *self.k.shape[2:])
         if tuple(k.shape) != shape or tuple(v.shape) != shape:
             raise ValueError("k and v must have one row of the cache's heads per new token")
         if (q.ndim != 3 or q.shape[0] != total or q.shape[2] != shape[2] or q.shape[1] < 1
-                or q.shape[1] % shape[1]):
+                or q.shape[1] % shape[1] or q.shape[1] > 4096):
             raise ValueError("q must have one row of query heads per new token")
         if any(x.dtype != self.k.dtype or x.device != self.k.device for x in (q, k, v)):
             raise ValueError("q, k and v must have the cache's type and device")
         if not self.k.is_cuda:
             raise ValueError("extend needs a cache on the GPU")
-        if torch.is_grad_enabled() and any(x.requires_grad for x in (self.k, self.v, q, k, v)):
+        if (torch.is_grad_enabled() and any(x.requires_grad for x in (self.k, self.v, q, k, v))
+                or any(unpack_dual(x).tangent is not None for x in (q, k, v))):
             raise ValueError("extend is not differentiable: detach q, k and v, or use no_grad")
-        q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
+        # Rows that are views of the pool are read before it is written.
+        store = [x.untyped_storage().data_ptr() for x in (self.k, self.v)]
+        q, k, v = (x.contiguous() if x.stride(-1) != 1 else
+                   x.clone() if x.untyped_storage().data_ptr() in store else x for x in (q, k, v))
         if options:  # refused here, before any page is taken
             first = options.get("first")
             if first is not None and tuple(first.shape) != (total,):

@@ -328,7 +328,7 @@ enum {
   BC_FLOAT16 = 0,
   BC_BFLOAT16 = 1,
 };
-/* Most query heads bc_chunk_attention takes. */
+/* Most query heads bc_chunk_attention takes, and KV heads bc_append_kv. */
 #define BC_MAX_CHUNK_HEADS 4096
 /* Longest row of a page table for it and bc_build_tables: 256 tokens short of
  * 2^31. */
@@ -380,8 +380,8 @@ int bc_build_tables(const int32_t* page_ids, int held, const int32_t* lengths,
  * a mixture.  Rows and pools must not overlap.  Any 2-byte aligned pointers
  * and any non-negative strides work (16-byte copies where all of them allow
  * it).  Uses shape.kv_heads, shape.dim and shape.physical_pages; rejects
- * values below 1, dim not 64/128, tokens < 0, null pointers, negative
- * strides. */
+ * values below 1, kv_heads over BC_MAX_CHUNK_HEADS, dim not 64/128, tokens <
+ * 0, null pointers, negative strides. */
 int bc_append_kv(bc_shape shape, const bc_half* k, const bc_half* v,
                  bc_row_strides k_strides, bc_row_strides v_strides,
                  bc_half* cache_k, bc_half* cache_v,

@@ -224,7 +224,8 @@ def test_extend_refuses_before_anything_changes():
     with pytest.raises(RuntimeError, match="exhausted"):
         cache.extend([a, b], [29, 1], q, k, k)  # 20 + 29 tokens: two more pages and a clone; two are free
     refusals = [([a, a], [15, 15], q, k, {}), ([a], [30, 0], q, k, {}), ([], [], q[:0], k[:0], {}),
-                ([a, b], [31, -1], q, k, {}), ([a], [29], q, k, {}), ([a], [30], q[:, :3], k, {}),
+                ([a, b], [31, -1], q, k, {}),
+                ([a], [5], q[:5, :1].expand(5, 4098, 64), k[:5], {}), ([a], [29], q, k, {}), ([a], [30], q[:, :3], k, {}),
                 ([a], [30], q.bfloat16(), k, {}), ([a], [30], q, k.cpu(), {}),
                 ([a], [5], q[:5], k[:5].clone().requires_grad_(), {}),
                 ([a], [5], q[:5].clone().requires_grad_(), k[:5], {}),
@@ -235,3 +236,34 @@ def test_extend_refuses_before_anything_changes():
             cache.extend(requests, counts, qq, kk, kk.detach(), **options)
         assert state() == before
     assert cache.extend([a, b], [12, 3], q[:15], k[:15], k[:15]).shape == (15, 4, 64)
+
+
+def test_extend_refuses_a_tangent_before_anything_changes():
+    from torch.autograd import forward_ad
+    from branchcraft_torch.transaction import PagedTreeCache
+    g = torch.Generator("cuda").manual_seed(6)
+    cache = PagedTreeCache(4, 2, 64)
+    a = cache.new(random_rows(g, 20, 2, 64), random_rows(g, 20, 2, 64))
+    rows = random_rows(g, 5, 2, 64)
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="differentiable"):
+            cache.extend([a], [5], rows, rows, forward_ad.make_dual(rows, rows))
+    assert cache.lengths[a] == 20 and len(cache.pages[a]) == 2
+
+
+def test_extend_with_rows_of_the_pool_itself():
+    """Another request's tokens once more, as views of its pages."""
+    from branchcraft_torch.transaction import PagedTreeCache
+    g = torch.Generator("cuda").manual_seed(5)
+    caches = [PagedTreeCache(8, 2, 64) for _ in range(2)]
+    k, v, q = random_rows(g, 40, 2, 64), random_rows(g, 40, 2, 64), random_rows(g, 12, 4, 64)
+    outs = []
+    for cache in caches:
+        a, b = cache.new(k, v), cache.new(k[:5], v[:5])
+        page = cache.pages[a][1]
+        rows = [pool[page, 2:14] for pool in (cache.k, cache.v)]
+        if cache is caches[1]:
+            rows = [x.clone() for x in rows]
+        outs.append(cache.extend([b, a], [5, 7], q, *rows))
+    assert torch.equal(bits(outs[0]), bits(outs[1]))
+    assert torch.equal(bits(caches[0].k), bits(caches[1].k)) and torch.equal(bits(caches[0].v), bits(caches[1].v))

@@ -30,7 +30,8 @@ BAD_SHAPES = [dict(batch=0), dict(query_heads=0), dict(kv_heads=0), dict(query_h
 BAD_INPUTS = [dict(q=None), dict(k=None), dict(v=None), dict(pages=None), dict(lengths=None),
               dict(starts=None), dict(output=None), dict(tokens=-1), dict(window=-1), dict(dtype=2),
               dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0),
-              dict(cap=math.nan), dict(cap=math.inf), dict(cap=1e-13), dict(cap=1e13), dict(scale=1e-13), dict(scale=1e13), dict(q_strides=capi.RowStrides(-1, 128)),
+              dict(cap=math.nan), dict(cap=math.inf), dict(cap=1e-13), dict(cap=1e13), dict(scale=1e-13), dict(scale=1e13),
+              dict(q_strides=capi.RowStrides(-1, 128)),
               dict(k_strides=capi.PoolStrides(1, -1, 1)), dict(v_strides=capi.PoolStrides(1, 1, -1))]
 
 
@@ -56,7 +57,8 @@ def test_append_rejects():
     lib = capi.load()
     row, pool = capi.RowStrides(1024, 128), capi.PoolStrides(16384, 1024, 128)
     good = [_shape(), FAKE, FAKE, row, row, FAKE, FAKE, pool, pool, FAKE, 3, None]
-    for at, bad in [(0, _shape(dim=80)), (0, _shape(kv_heads=0)), (0, _shape(physical_pages=0)), (1, None),
+    for at, bad in [(0, _shape(dim=80)), (0, _shape(kv_heads=0)), (0, _shape(kv_heads=4097)),
+                    (0, _shape(physical_pages=0)), (1, None),
                     (2, None), (5, None), (6, None), (9, None), (10, -1), (3, capi.RowStrides(-8, 1)),
                     (4, capi.RowStrides(8, -1)), (7, capi.PoolStrides(-1, 1, 1)),
                     (8, capi.PoolStrides(1, 1, -1))]:
