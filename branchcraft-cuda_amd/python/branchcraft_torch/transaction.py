@@ -205,10 +205,11 @@ class PagedTreeCache:
         if (torch.is_grad_enabled() and any(x.requires_grad for x in (self.k, self.v, q, k, v))
                 or any(unpack_dual(x).tangent is not None for x in (q, k, v))):
             raise ValueError("extend is not differentiable: detach q, k and v, or use no_grad")
+        q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
         # Rows that are views of the pool are read before it is written.
-        store = [x.untyped_storage().data_ptr() for x in (self.k, self.v)]
-        q, k, v = (x.contiguous() if x.stride(-1) != 1 else
-                   x.clone() if x.untyped_storage().data_ptr() in store else x for x in (q, k, v))
+        if {*map(type, (self.k, q, k, v))} <= {torch.Tensor, torch.nn.Parameter}:
+            store = [x.untyped_storage().data_ptr() for x in (self.k, self.v)]
+            q, k, v = (x.clone() if x.untyped_storage().data_ptr() in store else x for x in (q, k, v))
         if options:  # refused here, before any page is taken
             first = options.get("first")
             if first is not None and tuple(first.shape) != (total,):

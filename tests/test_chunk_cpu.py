@@ -119,6 +119,22 @@ def test_what_autograd_tracks_is_refused():
                 assert not bt.chunk_attention(*args[:3], *ints, slopes=args[3]).requires_grad
 
 
+def test_extend_on_fake_tensors():
+    """Page tables and shapes without a GPU; no warning about an address."""
+    import warnings
+    from branchcraft_torch.transaction import PagedTreeCache
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(), warnings.catch_warnings():
+        warnings.simplefilter("error")
+        cache = PagedTreeCache(8, 2, 64)
+        rows = torch.zeros(20, 2, 64, device="cuda", dtype=torch.float16)
+        q = torch.zeros(6, 4, 64, device="cuda", dtype=torch.float16)
+        a = cache.new(rows, rows)
+        b = cache.fork(a)
+        assert cache.extend([a, b], [3, 3], q, rows[:6], rows[:6], cap=3.0).shape == (6, 4, 64)
+        assert cache.lengths == {a: 23, b: 23} and cache.pages[a][1] != cache.pages[b][1]
+
+
 def test_cpu_tensors_have_no_implementation():
     import branchcraft_torch as bt
     ints = torch.zeros(2, dtype=torch.int32)
