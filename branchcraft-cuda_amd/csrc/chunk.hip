@@ -511,14 +511,18 @@ struct Item {
 
 // Item `idx` of the batch, found by every wave for itself from starts and
 // lengths.  A request's last tiles, which see most, come first.  `all`: go to
-// the end and count.
+// the end and count.  Where starts decrease, requests overlap and the grid,
+// which is sized for the rows of a step, may end before the items: the records
+// counted are those whose writer, the first part's workgroup, is among the
+// first `launched` items and has place for its parts.  Both bounds rise from
+// one record to the next, so these are the first ones.
 __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int share, long long idx,
-                                          int lane, bool all) {
+                                          int lane, bool all, int launched) {
   const ChunkParams& C = P.c;
   const bool split = P.part_acc != nullptr;
   Item it{};
   long long before = 0;
-  int slots = 0, records = 0, narrow = 0;
+  int slots = 0, cut = 0, records = 0, narrow = 0;
   for (int b0 = 0; b0 < C.batch; b0 += 64) {
     if (b0 > 0) a = asked_of(C, b0 + lane, split);
     const int parts = split && a.steps > share ? (a.steps + share - 1) / share : 1;
@@ -544,18 +548,24 @@ __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int shar
       it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - nth;
       if (it.parts > 1) {
         it.slot = slots + lanes_sum(lane < at ? cut_parts : 0) + in - it.part;
-        it.record = records + lanes_sum(lane < at ? cut_tiles : 0) + nth;
-        // Cannot be (see Cutting) unless starts decrease.
+        it.record = cut + lanes_sum(lane < at ? cut_tiles : 0) + nth;
+        // Cannot be, see Cutting.
         if (it.slot < 0 || it.slot + it.parts > P.most_parts || it.record < 0 ||
             it.record >= P.most_parts / 2)
           it.parts = 1;
       }
       if (!all) return it;
     }
+    if (all && split) {
+      const int ahead = (int)max(0ll, min((long long)launched - before, 0x3fffffffll)) - (upto - mine);
+      const int places = P.most_parts - slots - (lanes_upto(cut_parts) - cut_parts);
+      const int in_grid = ahead > 0 ? (ahead - 1) / parts + 1 : 0;
+      records += lanes_sum(min(cut_tiles, min(in_grid, max(places, 0) / parts)));
+    }
     before += total;
     if (split) {
       slots += lanes_sum(cut_parts);
-      records += lanes_sum(cut_tiles);
+      cut += lanes_sum(cut_tiles);
       narrow += __builtin_popcountll(__builtin_amdgcn_ballot_w64(a.narrow > 0));
     }
   }
@@ -1498,7 +1508,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
   const int in = blockIdx.x - cut.groups, at = divide(in, P.c.hkv, P.c.hkv_mul);
   const int kvh = in - at * P.c.hkv;
   Item it{};
-  if (!flat || counts) it = plan_item(P, head, cut.share, flat ? -1ll : (long long)at, lane, counts);
+  if (!flat || counts) {
+    const int launched = counts ? (int)(gridDim.x - cut.groups + P.c.hkv - 1) / P.c.hkv : 0;
+    it = plan_item(P, head, cut.share, flat ? -1ll : (long long)at, lane, counts, launched);
+  }
   if (counts && threadIdx.x == 0) P.records[0] = make_int4(it.records, it.narrow_records, 0, 0);
   if (flat) {
     const TileParams& A = reread(args);
