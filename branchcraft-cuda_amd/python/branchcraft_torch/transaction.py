@@ -211,12 +211,15 @@ class PagedTreeCache:
             store = [x.untyped_storage().data_ptr() for x in (self.k, self.v)]
             q, k, v = (x.clone() if x.untyped_storage().data_ptr() in store else x for x in (q, k, v))
         if options:  # refused here, before any page is taken
-            first = options.get("first")
-            if first is not None and tuple(first.shape) != (total,):
-                raise ValueError("first must have one entry per new token")
+            empty, first = options, options.get("first")
+            if first is not None:
+                if tuple(first.shape) != (total,):
+                    raise ValueError("first must have one entry per new token")
+                # The tensor of the call below; its empty slice is contiguous in any case.
+                options["first"] = first = first.contiguous()
+                empty = options | {"first": first[:0]}
             none = self._upload([-1] * len(requests), [0] * len(requests), [0] * (len(requests) + 1))
-            chunk_attention(q[:0], self.k, self.v, none[0].unsqueeze(1), *none[1:],
-                            **(options if first is None else options | {"first": first[:0]}))
+            chunk_attention(q[:0], self.k, self.v, none[0].unsqueeze(1), *none[1:], **empty)
         owner = self.owner
         # Requests that share a partial last page: all but the last to write
         # it take a clone.

@@ -1,0 +1,39 @@
+"""PagedTreeCache.extend: what it refuses leaves pages, lengths and rows as they
+were, and what it takes need not be laid out one way."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(g, n, heads, d=64):
+    return torch.randn((n, heads, d), generator=g, device="cuda", dtype=torch.float16)
+
+
+def caches(n, *, pages=8, tokens=20, seed=1):
+    from branchcraft_torch.transaction import PagedTreeCache
+    out = []
+    for _ in range(n):
+        g = torch.Generator("cuda").manual_seed(seed)
+        cache = PagedTreeCache(pages, 2, 64)
+        a = cache.new(rows(g, tokens, 2), rows(g, tokens, 2))
+        out.append((cache, a, cache.fork(a)))
+    return out, g
+
+
+def state(cache):
+    return ({x: list(p) for x, p in cache.pages.items()}, dict(cache.lengths), list(cache.free),
+            list(cache.refcount))
+
+
+def test_a_strided_first_is_taken():
+    """Every second entry of a list of document starts."""
+    both, g = caches(2)
+    q, k, v = rows(g, 7, 4), rows(g, 7, 2), rows(g, 7, 2)
+    first = torch.tensor([0, 9, 3, 9, 20, 9, 21, 9, 1, 9, 20, 9, 4, 9], device="cuda", dtype=torch.int32)[::2]
+    assert not first.is_contiguous()
+    outs = [cache.extend([a, b], [4, 3], q, k, v, first=f)
+            for (cache, a, b), f in zip(both, (first, first.contiguous()))]
+    assert torch.equal(*outs)
+    assert state(both[0][0]) == state(both[1][0])
