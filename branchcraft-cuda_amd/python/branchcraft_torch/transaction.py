@@ -202,8 +202,8 @@ class PagedTreeCache:
             raise ValueError("q, k and v must have the cache's type and device")
         if not self.k.is_cuda:
             raise ValueError("extend needs a cache on the GPU")
-        if (torch.is_grad_enabled() and any(x.requires_grad for x in (self.k, self.v, q, k, v))
-                or any(unpack_dual(x).tangent is not None for x in (q, k, v))):
+        if any(x.requires_grad and torch.is_grad_enabled() or unpack_dual(x).tangent is not None
+               for x in (self.k, self.v, q, k, v)):
             raise ValueError("extend is not differentiable: detach q, k and v, or use no_grad")
         q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
         # Rows that are views of the pool are read before it is written.

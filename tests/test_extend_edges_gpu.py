@@ -37,3 +37,18 @@ def test_a_strided_first_is_taken():
             for (cache, a, b), f in zip(both, (first, first.contiguous()))]
     assert torch.equal(*outs)
     assert state(both[0][0]) == state(both[1][0])
+
+
+def test_a_tangent_on_the_pool_is_refused_before_anything_changes():
+    from torch.autograd import forward_ad
+    ((cache, a, b),), g = caches(1)
+    q, k, v = rows(g, 7, 4), rows(g, 7, 2), rows(g, 7, 2)
+    before = state(cache)
+    for name in ("k", "v"):
+        with forward_ad.dual_level():
+            plain = getattr(cache, name)
+            setattr(cache, name, forward_ad.make_dual(plain, torch.ones_like(plain)))
+            with pytest.raises(ValueError, match="differentiable"):
+                cache.extend([a, b], [4, 3], q, k, v)
+            setattr(cache, name, plain)
+        assert state(cache) == before
