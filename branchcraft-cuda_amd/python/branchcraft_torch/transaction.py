@@ -206,10 +206,16 @@ class PagedTreeCache:
                for x in (self.k, self.v, q, k, v)):
             raise ValueError("extend is not differentiable: detach q, k and v, or use no_grad")
         q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
-        # Rows that are views of the pool are read before it is written.
-        if {*map(type, (self.k, q, k, v))} <= {torch.Tensor, torch.nn.Parameter}:
-            store = [x.untyped_storage().data_ptr() for x in (self.k, self.v)]
-            q, k, v = (x.clone() if x.untyped_storage().data_ptr() in store else x for x in (q, k, v))
+        # Rows that are views of the pool are read before it is written: of one
+        # storage with it, or, where all are plain tensors and have an address, of
+        # another one of the same memory.
+        plain = {*map(type, (self.k, self.v, q, k, v))} <= {torch.Tensor, torch.nn.Parameter}
+
+        def store(x: torch.Tensor) -> int:
+            return x.untyped_storage().data_ptr() if plain else x.untyped_storage()._cdata
+
+        pools = store(self.k), store(self.v)
+        q, k, v = (x.clone() if store(x) in pools else x for x in (q, k, v))
         if options:  # refused here, before any page is taken
             empty, first = options, options.get("first")
             if first is not None:

@@ -52,3 +52,20 @@ def test_a_tangent_on_the_pool_is_refused_before_anything_changes():
                 cache.extend([a, b], [4, 3], q, k, v)
             setattr(cache, name, plain)
         assert state(cache) == before
+
+
+def test_rows_that_are_views_of_a_subclass_pool():
+    """As with a plain pool: they are read before the pool is written."""
+    class Pool(torch.Tensor):
+        pass
+
+    both, g = caches(2)
+    q, outs = rows(g, 7, 4), []
+    for turn, (cache, a, b) in enumerate(both):
+        if turn:
+            cache.k, cache.v = cache.k.as_subclass(Pool), cache.v.as_subclass(Pool)
+        page = cache.pages[a][0]
+        outs.append(cache.extend([a, b], [4, 3], q, cache.k[page, 2:9], cache.v[page, 2:9]).as_subclass(torch.Tensor))
+    assert torch.equal(*outs)
+    assert all(torch.equal(getattr(both[0][0], x), getattr(both[1][0], x).as_subclass(torch.Tensor)) for x in "kv")
+    assert state(both[0][0]) == state(both[1][0])
