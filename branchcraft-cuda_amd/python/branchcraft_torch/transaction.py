@@ -186,7 +186,8 @@ class PagedTreeCache:
         pages, the new tokens included (``options`` are its keywords).  Pages
         are planned as consecutive commits would take them: shared partial
         pages are cloned first.  A pool without room for all of it raises
-        before anything changes.  A count may be zero."""
+        before anything changes, and so does a stream under capture.  A count may
+        be zero."""
         if len(requests) != len(counts) or len(set(requests)) != len(requests) or not requests:
             raise ValueError("requests must be distinct and match counts")
         total = sum(counts)
@@ -205,11 +206,14 @@ class PagedTreeCache:
         if any(x.requires_grad and torch.is_grad_enabled() or unpack_dual(x).tangent is not None
                for x in (self.k, self.v, q, k, v)):
             raise ValueError("extend is not differentiable: detach q, k and v, or use no_grad")
+        plain = {*map(type, (self.k, self.v, q, k, v))} <= {torch.Tensor, torch.nn.Parameter}
+        if plain and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("extend cannot be captured: its pages are planned on the host, "
+                               "once per call; capture build_tables, append_kv_ and chunk_attention")
         q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
         # Rows that are views of the pool are read before it is written: of one
         # storage with it, or, where all are plain tensors and have an address, of
         # another one of the same memory.
-        plain = {*map(type, (self.k, self.v, q, k, v))} <= {torch.Tensor, torch.nn.Parameter}
 
         def store(x: torch.Tensor) -> int:
             return x.untyped_storage().data_ptr() if plain else x.untyped_storage()._cdata

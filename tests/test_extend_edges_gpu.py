@@ -69,3 +69,17 @@ def test_rows_that_are_views_of_a_subclass_pool():
     assert torch.equal(*outs)
     assert all(torch.equal(getattr(both[0][0], x), getattr(both[1][0], x).as_subclass(torch.Tensor)) for x in "kv")
     assert state(both[0][0]) == state(both[1][0])
+
+
+def test_a_capture_is_refused_before_anything_changes():
+    """Pages are planned on the host, once; a graph would replay that plan."""
+    ((cache, a, b),), g = caches(1)
+    q, k, v = rows(g, 7, 4), rows(g, 7, 2), rows(g, 7, 2)
+    before = state(cache)
+    out = torch.zeros(1, device="cuda")
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        out += 1
+        with pytest.raises(RuntimeError, match="captured"):
+            cache.extend([a, b], [4, 3], q, k, v)
+    assert state(cache) == before
+    assert cache.extend([a, b], [4, 3], q, k, v).shape == q.shape
