@@ -174,6 +174,20 @@ class PageOwner:
         self.lengths[request] = plan.new_length
         return plan
 
+    def undo_commit(self, plan: CommitPlan) -> None:
+        """Take back the newest plan: tables, lengths, refcounts and the order
+        of the free list are as before it."""
+        pages = self.pages[plan.request]
+        length = plan.new_length - len(plan.dest_pages)
+        while len(pages) > (length + PAGE_SIZE - 1) // PAGE_SIZE:
+            self.release(pages.pop())
+        if plan.cow is not None:
+            old, fresh = plan.cow
+            self.refcount[old] += 1
+            pages[-1] = old
+            self.release(fresh)
+        self.lengths[plan.request] = length
+
     def check_invariants(self) -> None:
         """Refcounts equal live references; the free list holds exactly the
         unreferenced pages, once each."""

@@ -186,8 +186,8 @@ class PagedTreeCache:
         pages, the new tokens included (``options`` are its keywords).  Pages
         are planned as consecutive commits would take them: shared partial
         pages are cloned first.  A pool without room for all of it raises
-        before anything changes, and so does a stream under capture.  A count may
-        be zero."""
+        before anything changes, and so does a stream under capture; a call that
+        fails later leaves pages and lengths as before it.  A count may be zero."""
         if len(requests) != len(counts) or len(set(requests)) != len(requests) or not requests:
             raise ValueError("requests must be distinct and match counts")
         total = sum(counts)
@@ -249,18 +249,25 @@ class PagedTreeCache:
         if needed > len(owner.free):
             raise RuntimeError("KV page pool exhausted")
         plans = [owner.plan_commit(request, n) for request, n in zip(requests, counts) if n]
-        clones = [plan.cow for plan in plans if plan.cow is not None]
-        lists = [owner.pages[request] for request in requests]
-        lengths = [owner.lengths[request] for request in requests]
-        old, fresh, ids, length, count = self._upload(
-            [old for old, _ in clones], [fresh for _, fresh in clones],
-            [page for pages in lists for page in pages], lengths, counts)
-        if clones:
-            copy_pages_(self.k, self.v, old, fresh)
-        width = max(1, *(len(pages) for pages in lists))
-        table, starts, slots, _ = build_tables(ids, length, count, width, total)
-        append_kv_(self.k, self.v, k, v, slots)
-        return chunk_attention(q, self.k, self.v, table, length, starts, **options)
+        try:
+            clones = [plan.cow for plan in plans if plan.cow is not None]
+            lists = [owner.pages[request] for request in requests]
+            lengths = [owner.lengths[request] for request in requests]
+            old, fresh, ids, length, count = self._upload(
+                [old for old, _ in clones], [fresh for _, fresh in clones],
+                [page for pages in lists for page in pages], lengths, counts)
+            if clones:
+                copy_pages_(self.k, self.v, old, fresh)
+            width = max(1, *(len(pages) for pages in lists))
+            table, starts, slots, _ = build_tables(ids, length, count, width, total)
+            append_kv_(self.k, self.v, k, v, slots)
+            return chunk_attention(q, self.k, self.v, table, length, starts, **options)
+        except BaseException:
+            # An allocation that failed, say.  Rows written so far lie behind
+            # every holder's length, or in pages that are free again.
+            for plan in reversed(plans):
+                owner.undo_commit(plan)
+            raise
 
     def _run_plans(self, plans, paths, draft_k, draft_v) -> None:
         if not plans:
