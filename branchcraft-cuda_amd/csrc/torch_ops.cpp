@@ -374,10 +374,25 @@ void write_prefix_hip(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor
                "write_prefix_");
 }
 
-// Above the kernel: pools or rows that autograd tracks, or that carry a tangent,
-// are copied page by page with ops that have derivatives (and refuse a leaf
-// pool).  Otherwise the pools' version counters move, so that a backward that
-// saved a pool before a prompt entered it raises, as after those copies.
+// Above the kernel, with or without autograd above it (inference mode leaves it
+// out for tensors that were made outside): the pools' version counters move.
+void write_prefix_versions(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k,
+                           const at::Tensor& v, at::IntArrayRef pages) {
+  static const auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("branchcraft::write_prefix_", "")
+          .typed<void(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&,
+                      at::IntArrayRef)>();
+  cache_k.unsafeGetTensorImpl()->bump_version();
+  cache_v.unsafeGetTensorImpl()->bump_version();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  op.call(cache_k, cache_v, k, v, pages);
+}
+
+// Pools or rows that autograd tracks, or that carry a tangent, are copied page
+// by page with ops that have derivatives (and refuse a leaf pool).  Otherwise
+// the pools' version counters move, so that a backward that saved a pool before
+// a prompt entered it raises, as after those copies.
 void write_prefix_autograd(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k,
                            const at::Tensor& v, at::IntArrayRef pages) {
   auto tracked = [](const at::Tensor& x) {
@@ -393,15 +408,7 @@ void write_prefix_autograd(at::Tensor& cache_k, at::Tensor& cache_v, const at::T
     }
     return;
   }
-  static const auto op =
-      c10::Dispatcher::singleton()
-          .findSchemaOrThrow("branchcraft::write_prefix_", "")
-          .typed<void(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&,
-                      at::IntArrayRef)>();
-  cache_k.unsafeGetTensorImpl()->bump_version();
-  cache_v.unsafeGetTensorImpl()->bump_version();
-  const at::AutoDispatchBelowADInplaceOrView below;
-  op.call(cache_k, cache_v, k, v, pages);
+  write_prefix_versions(cache_k, cache_v, k, v, pages);
 }
 
 // A host list as an int32 tensor on `like`'s device, written in stream order
@@ -534,12 +541,11 @@ void refuse_tracked(const char* op, std::initializer_list<const at::Tensor*> ten
                 op, " is not differentiable: detach its tensors or call it under no_grad");
 }
 
-// Above the kernel: tensors that autograd tracks or that carry a tangent are
-// refused, and the pools' version counters move, so that a backward that saved
-// a pool before the rows entered it raises.
-void append_kv_autograd(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k,
+// Above the kernel, with or without autograd above it (inference mode leaves it
+// out for tensors that were made outside): the pools' version counters move, so
+// that a backward that saved a pool before the rows entered it raises.
+void append_kv_versions(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k,
                         const at::Tensor& v, const at::Tensor& slots) {
-  refuse_tracked("append_kv_", {&cache_k, &cache_v, &k, &v});
   static const auto op =
       c10::Dispatcher::singleton()
           .findSchemaOrThrow("branchcraft::append_kv_", "")
@@ -549,6 +555,13 @@ void append_kv_autograd(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tens
   cache_v.unsafeGetTensorImpl()->bump_version();
   const at::AutoDispatchBelowADInplaceOrView below;
   op.call(cache_k, cache_v, k, v, slots);
+}
+
+// Tensors that autograd tracks or that carry a tangent are refused.
+void append_kv_autograd(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tensor& k,
+                        const at::Tensor& v, const at::Tensor& slots) {
+  refuse_tracked("append_kv_", {&cache_k, &cache_v, &k, &v});
+  append_kv_versions(cache_k, cache_v, k, v, slots);
 }
 
 // Attention of each request's new tokens over its pages (see
@@ -680,6 +693,11 @@ TORCH_LIBRARY_IMPL(branchcraft, CUDA, m) {
   m.impl("build_tables", build_tables_hip);
   m.impl("append_kv_", append_kv_hip);
   m.impl("chunk_attention", chunk_attention_hip);
+}
+
+TORCH_LIBRARY_IMPL(branchcraft, ADInplaceOrView, m) {
+  m.impl("write_prefix_", write_prefix_versions);
+  m.impl("append_kv_", append_kv_versions);
 }
 
 TORCH_LIBRARY_IMPL(branchcraft, Autograd, m) {

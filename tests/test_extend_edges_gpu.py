@@ -83,3 +83,16 @@ def test_a_capture_is_refused_before_anything_changes():
             cache.extend([a, b], [4, 3], q, k, v)
     assert state(cache) == before
     assert cache.extend([a, b], [4, 3], q, k, v).shape == q.shape
+
+
+def test_inference_mode_moves_the_pools_counters():
+    """A pool made outside and rows made inside, the whole step."""
+    both, g = caches(2)
+    (cache, a, b), (other, _, _) = both
+    q, k, v = rows(g, 7, 4), rows(g, 7, 2), rows(g, 7, 2)
+    want = other.extend([a, b], [4, 3], q, k, v, cap=9.0)
+    versions = cache.k._version, cache.v._version
+    with torch.inference_mode():
+        got = cache.extend([a, b], [4, 3], q.clone(), k.clone(), v.clone(), cap=9.0)
+    assert torch.equal(got, want) and torch.equal(cache.k, other.k) and torch.equal(cache.v, other.v)
+    assert cache.k._version > versions[0] and cache.v._version > versions[1]
