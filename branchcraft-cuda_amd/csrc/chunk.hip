@@ -17,6 +17,9 @@ using namespace bcd;
 namespace {
 
 constexpr int kThreads = 256;
+// Most workgroups of a launch's first dimension: HIP takes fewer than 2^32
+// threads.  Kernels whose work may need more go over it in turns.
+constexpr int kMostGroups = (1 << 24) - 1;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -112,23 +115,26 @@ struct AppendParams {
   int tokens, phys_pages, row_vec, head_vec;
 };
 
-// Workgroup i copies rows_per_block rows, K then V, in elements of type E.
+// A workgroup copies rows_per_block rows at a time, K then V, in elements of
+// type E.
 // HBM-bound: 8192 rows of 8 heads x 128 out of a fused projection (67 MB) 12.1
 // us, 5.5 TB/s, as a large copy; 64 rows 2.6 us.
 template <typename E>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams P, int rows_per_block) {
-  const int t0 = blockIdx.x * rows_per_block;
-  const int n = min(rows_per_block, P.tokens - t0) * P.row_vec;
-  for (int x = threadIdx.x; x < n; x += kThreads) {
-    const int i = x / P.row_vec, c = x - i * P.row_vec;
-    const int h = c / P.head_vec, e = c - h * P.head_vec;
-    const int slot = P.slots[t0 + i];
-    if (slot < 0 || (slot >> 4) >= P.phys_pages) continue;
-    const long long t = t0 + i, page = slot >> 4, in = slot & 15;
-    static_cast<E*>(P.cache_k)[page * P.cp[0] + in * P.cs[0] + h * P.ch[0] + e] =
-        static_cast<const E*>(P.k)[t * P.ts[0] + h * P.hs[0] + e];
-    static_cast<E*>(P.cache_v)[page * P.cp[1] + in * P.cs[1] + h * P.ch[1] + e] =
-        static_cast<const E*>(P.v)[t * P.ts[1] + h * P.hs[1] + e];
+  for (long long t0 = (long long)blockIdx.x * rows_per_block; t0 < P.tokens;
+       t0 += (long long)gridDim.x * rows_per_block) {
+    const int n = (int)min((long long)rows_per_block, P.tokens - t0) * P.row_vec;
+    for (int x = threadIdx.x; x < n; x += kThreads) {
+      const int i = x / P.row_vec, c = x - i * P.row_vec;
+      const int h = c / P.head_vec, e = c - h * P.head_vec;
+      const int slot = P.slots[t0 + i];
+      if (slot < 0 || (slot >> 4) >= P.phys_pages) continue;
+      const long long t = t0 + i, page = slot >> 4, in = slot & 15;
+      static_cast<E*>(P.cache_k)[page * P.cp[0] + in * P.cs[0] + h * P.ch[0] + e] =
+          static_cast<const E*>(P.k)[t * P.ts[0] + h * P.hs[0] + e];
+      static_cast<E*>(P.cache_v)[page * P.cp[1] + in * P.cs[1] + h * P.ch[1] + e] =
+          static_cast<const E*>(P.v)[t * P.ts[1] + h * P.hs[1] + e];
+    }
   }
 }
 
@@ -221,12 +227,8 @@ __device__ __forceinline__ int2 row_range(const ChunkParams& P, int b, int t, in
 // keeps D / 64 dimensions of the output.  Tokens that the row does not see
 // are never multiplied, whatever their K and V hold.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void chunk_rows_kernel(ChunkParams P) {
+__device__ __forceinline__ void attend_row(const ChunkParams& P, int t, int h, int lane) {
   constexpr int R = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = blockIdx.x, h = blockIdx.y * (kThreads / 64) + wave;
-  if (h >= P.hq) return;
   const int b = request_of(P, t, lane);
   float acc[R] = {}, m = kNegInf, l = 0.f;
   if (b >= 0) {
@@ -275,8 +277,19 @@ __global__ __launch_bounds__(kThreads) void chunk_rows_kernel(ChunkParams P) {
 }
 
 template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void chunk_rows_kernel(ChunkParams P) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.y * (kThreads / 64) + wave;
+  if (h >= P.hq) return;
+  for (unsigned row = blockIdx.x; row < (unsigned)P.tokens; row += gridDim.x)
+    attend_row<T, D>(P, (int)row, h, lane);
+}
+
+template <typename T, int D>
 void launch_rows(const ChunkParams& P, hipStream_t st) {
-  const dim3 grid(P.tokens, (P.hq + kThreads / 64 - 1) / (kThreads / 64));
+  const dim3 grid(P.tokens < kMostGroups ? P.tokens : kMostGroups,
+                  (P.hq + kThreads / 64 - 1) / (kThreads / 64));
   chunk_rows_kernel<T, D><<<grid, kThreads, 0, st>>>(P);
 }
 
@@ -1704,7 +1717,9 @@ extern "C" int bc_build_tables(const int32_t* page_ids, int held, const int32_t*
     return BC_ERROR_INVALID_VALUE;
   const TableParams P{page_ids, lengths, counts,    pages,     starts, slots, positions,
                       held,     batch,   max_pages, tokens};
-  if (max_pages > BC_MAX_TABLE_PAGES || tokens >= 1 << 27 || batch == 0x7fffffff) return BC_ERROR_INVALID_VALUE;
+  static_assert(BC_MAX_TABLE_REQUESTS + 1 <= kMostGroups, "a workgroup row per request and one");
+  if (max_pages > BC_MAX_TABLE_PAGES || tokens >= 1 << 27 || batch > BC_MAX_TABLE_REQUESTS)
+    return BC_ERROR_INVALID_VALUE;
   const int longest = tokens > max_pages ? tokens : max_pages;
   // At most about four workgroups per CU.
   const int spans = (longest - 1) / kTableSpan + 1, rounds = 4 * bch::device_cus() / (batch + 1);
@@ -1746,7 +1761,8 @@ extern "C" int bc_append_kv(bc_shape s, const bc_half* k, const bc_half* v, bc_r
                        s.kv_heads * s.dim / e,
                        s.dim / e};
   const int rows = P.row_vec >= kThreads ? 1 : kThreads / P.row_vec;
-  const dim3 grid((tokens - 1) / rows + 1);
+  const int groups = (tokens - 1) / rows + 1;
+  const dim3 grid(groups < kMostGroups ? groups : kMostGroups);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (vec)
     append_kernel<uint4><<<grid, kThreads, 0, st>>>(P, rows);
@@ -1791,7 +1807,7 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
   const int group = s.query_heads / s.kv_heads;
   const bool exact = (long long)in.tokens * group * group < 1ll << 32;
   const unsigned group_mul = group > 1 && exact ? (unsigned)(((1ull << 32) + group - 1) / group) : 0;
-  const bool few_heads = s.kv_heads > 1 && s.kv_heads <= 64;  // grids below 2^26, see `tiled`
+  const bool few_heads = s.kv_heads > 1 && s.kv_heads <= 64;  // grids below 2^24, see `tiled`
   const unsigned hkv_mul = few_heads ? (unsigned)(((1ull << 32) + s.kv_heads - 1) / s.kv_heads) : 0;
   const ChunkParams P{in.q,
                       in.k,
@@ -1836,7 +1852,7 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
   const long long far = 1 << 26;
   const bool tiled = aligned16(in.q) && aligned16(in.k) && aligned16(in.v) && aligned16(in.output) &&
                      bits % 8 == 0 && in.k_strides.slot < far && in.v_strides.slot < far &&
-                     rows <= 1 << 30 && grid <= 1 << 26;
+                     rows <= 1 << 30 && grid <= kMostGroups;
   void* const ws = use ? workspace : nullptr;
   if (tiled) {
     if (in.dtype == BC_FLOAT16)

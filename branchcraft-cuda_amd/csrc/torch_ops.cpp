@@ -450,9 +450,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_tables_hip(
   TORCH_CHECK(lengths.size(0) > 0, "build_tables: no requests");
   TORCH_CHECK(max_pages >= 1 && max_pages <= BC_MAX_TABLE_PAGES && tokens >= 0 &&
                   tokens < (1 << 27) && page_ids.numel() <= INT32_MAX &&
-                  lengths.numel() < INT32_MAX,
+                  lengths.numel() <= BC_MAX_TABLE_REQUESTS,
               "build_tables: max_pages must be 1 to ", BC_MAX_TABLE_PAGES,
-              ", tokens at least 0 and below 2**27");
+              ", tokens at least 0 and below 2**27, requests at most ", BC_MAX_TABLE_REQUESTS);
   TORCH_CHECK(page_ids.device() == lengths.device() && page_ids.device() == counts.device(),
               "all tensors must share a device");
   const c10::DeviceGuard guard(lengths.device());

@@ -333,6 +333,8 @@ enum {
 /* Longest row of a page table for it and bc_build_tables: 256 tokens short of
  * 2^31. */
 #define BC_MAX_TABLE_PAGES 134217712
+/* Most requests of a bc_build_tables call: a launch has fewer than 2^32 threads. */
+#define BC_MAX_TABLE_REQUESTS 16777214
 /* Bounds of its scale, and of a cap: quotients of the two, and of a slope and
  * the scale, stay inside 32 bits. */
 #define BC_LEAST_SCALE 1e-12f
@@ -366,8 +368,8 @@ typedef struct bc_pool_strides {
  * page_ids, or in a page with a negative id or one of 2^27 or more; a
  * position before the request is -1.  Negative lengths and counts count as
  * 0.  Rejects: batch or max_pages < 1, held or tokens < 0, null pointers
- * (those of empty arrays aside), max_pages over BC_MAX_TABLE_PAGES, 2^27
- * tokens or more. */
+ * (those of empty arrays aside), batch over BC_MAX_TABLE_REQUESTS, max_pages
+ * over BC_MAX_TABLE_PAGES, 2^27 tokens or more. */
 int bc_build_tables(const int32_t* page_ids, int held, const int32_t* lengths,
                     const int32_t* counts, int batch, int max_pages, int tokens,
                     int32_t* pages, int32_t* starts, int32_t* slots,

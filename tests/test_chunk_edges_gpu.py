@@ -45,3 +45,59 @@ def test_starts_that_decrease_leave_only_written_records():
     for start, row0, rows, parts in records[1:1 + 2 * split:2].tolist():
         assert parts >= 2 and 0 <= start and 0 < rows <= 128 and start + -(-(row0 + rows) // (hq // hkv)) <= t
     assert bool((whole[:64] == 7).all()) and bool((whole[64 + t:] == 7).all())
+
+
+FAR = (1 << 24) + 100  # rows that as many workgroups of 256 threads would take past 2^32 threads
+
+
+def one_off(*shape, dtype=F16, seed=2):
+    """Random values one element off the allocator's alignment."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    n = 1
+    for x in shape:
+        n *= x
+    return torch.randn(n + 1, generator=g, device="cuda").to(dtype)[1:].view(shape)
+
+
+def test_append_of_more_rows_than_a_launch_has_workgroups():
+    import branchcraft_torch as bt
+    k, v = one_off(1, 4, 64), one_off(1, 4, 64, seed=3)
+    pools = [torch.zeros((3, 16, 4, 64), device="cuda", dtype=F16) for _ in range(2)]
+    slots = torch.full((FAR,), -1, device="cuda", dtype=torch.int32)
+    rows = [0, 5, (1 << 24) - 2, (1 << 24) - 1, 1 << 24, FAR - 2, FAR - 1]
+    slots[torch.tensor(rows, device="cuda")] = torch.arange(20, 20 + len(rows), device="cuda", dtype=torch.int32)
+    bt.append_kv_(*pools, k.expand(FAR, 4, 64), v.expand(FAR, 4, 64), slots)
+    for pool, x in zip(pools, (k, v)):
+        flat = pool.view(-1, 4, 64)
+        assert torch.equal(flat[20:20 + len(rows)], x.expand(len(rows), 4, 64))
+        assert not flat[:20].any() and not flat[20 + len(rows):].any()
+
+
+def test_rows_of_more_rows_than_a_launch_has_workgroups():
+    """The form without 16-byte loads; the request is the last three rows."""
+    import branchcraft_torch as bt
+    q, k, v = one_off(1, 1, 64), one_off(4, 16, 1, 64, seed=4), one_off(4, 16, 1, 64, seed=5)
+    meta = [torch.tensor(x, device="cuda", dtype=torch.int32) for x in ([[2, 0, 3]], [40], [FAR - 3, FAR])]
+    got = bt.chunk_attention(q.expand(FAR, 1, 64), k, v, *meta)
+    want, tol = C.reference(q.expand(3, 1, 64).cpu(), k.cpu(), v.cpu(), meta[0].cpu(), meta[1].cpu(),
+                            torch.tensor([0, 3]))
+    C.check(got[-3:], want, tol)
+    assert not got[:-3].any()
+
+
+def test_tiles_of_more_heads_and_requests_than_a_launch_has_workgroups():
+    """4096 requests of one token for each of 4096 KV heads: row by row."""
+    import branchcraft_torch as bt
+    heads = batch = 4096
+    g = torch.Generator("cuda").manual_seed(6)
+    q = torch.randn((1, heads, 64), generator=g, device="cuda").to(BF16)
+    k, v = (torch.randn((2, 16, heads, 64), generator=g, device="cuda").to(BF16) for _ in range(2))
+    lengths = 1 + torch.arange(batch, device="cuda", dtype=torch.int32) % 16
+    pages = (torch.arange(batch, device="cuda", dtype=torch.int32) % 2)[:, None].contiguous()
+    starts = torch.arange(batch + 1, device="cuda", dtype=torch.int32)
+    got = bt.chunk_attention(q.expand(batch, heads, 64), k, v, pages, lengths, starts)
+    some = [0, 1, 6, 4095]
+    for h in (slice(0, 2), slice(4094, 4096)):
+        want, tol = C.reference(q[:, h].expand(4, 2, 64).cpu(), k[:, :, h].cpu(), v[:, :, h].cpu(),
+                                pages[some].cpu(), lengths[some].cpu(), torch.arange(5))
+        C.check(got[some][:, h], want, tol)
