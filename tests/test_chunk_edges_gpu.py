@@ -101,3 +101,47 @@ def test_tiles_of_more_heads_and_requests_than_a_launch_has_workgroups():
         want, tol = C.reference(q[:, h].expand(4, 2, 64).cpu(), k[:, :, h].cpu(), v[:, :, h].cpu(),
                                 pages[some].cpu(), lengths[some].cpu(), torch.arange(5))
         C.check(got[some][:, h], want, tol)
+
+
+def both(fix, **options):
+    import branchcraft_torch as bt
+    dev = C.on_gpu(fix)
+    want, tol = C.reference(**fix, **options)
+    C.check(bt.chunk_attention(*(dev[n] for n in ("q", "k", "v", "pages", "lengths", "starts")), **options),
+            want, tol)
+
+
+@pytest.mark.parametrize("shape", [([40, 3], [35, 1]), ([1100, 70], [34, 2])], ids=["short", "split"])
+def test_more_than_64_kv_heads(shape):
+    both(C.batch(*shape, 73, 73, 64, F16, seed=30))
+    both(C.batch(*shape, 146, 73, 64, BF16, seed=31), window=30)
+
+
+@pytest.mark.parametrize("lengths", [[1, 40, 300], [2100, 5, 900]], ids=["short", "split"])
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(33, 1, 128, F16), (80, 2, 64, BF16), (129, 1, 64, F16)])
+def test_groups_of_more_rows_than_the_narrow_form_takes(hq, hkv, d, dtype, lengths):
+    """Single tokens whose query heads alone fill a tile."""
+    both(C.batch(lengths, [1, 1, 1], hq, hkv, d, dtype, seed=32))
+
+
+def test_groups_whose_products_pass_32_bits():
+    """256 new tokens of 4096 query heads over one KV head."""
+    import branchcraft_torch as bt
+    fix = C.on_gpu(C.batch([300], [256], 4096, 1, 64, BF16, seed=33))
+    meta = [fix[n] for n in ("pages", "lengths", "starts")]
+    got = bt.chunk_attention(fix["q"], fix["k"], fix["v"], *meta)
+    for heads in ([0, 1], [2047, 4095]):
+        want, tol = C.reference(fix["q"][:, heads].cpu(), fix["k"].cpu(), fix["v"].cpu(),
+                                *(x.cpu() for x in meta))
+        C.check(got[:, heads], want, tol)
+
+
+def test_inference_mode():
+    import branchcraft_torch as bt
+    fix = C.on_gpu(C.batch([90, 40], [33, 2], 4, 2, 64, F16, seed=34))
+    args = [fix[n] for n in ("q", "k", "v", "pages", "lengths", "starts")]
+    want = bt.chunk_attention(*args, cap=4.0)
+    q = args[0].clone().requires_grad_()
+    with torch.inference_mode():
+        assert torch.equal(bt.chunk_attention(*args, cap=4.0), want)
+        assert torch.equal(bt.chunk_attention(q, *args[1:], cap=4.0), want)
