@@ -155,7 +155,10 @@ def build_tables(page_ids, lengths, counts, max_pages, tokens):
     [tokens])``, all int32.  Request b has ``lengths[b]`` tokens, the last
     ``counts[b]`` of them new, and its ceil(length / 16) page ids follow those of
     the request before it in ``page_ids``.  -1 stands behind a request's pages,
-    in rows behind the last request, and for rows without a slot."""
+    in rows behind the last request, and for rows without a slot.  ``tokens``
+    should hold every new token: of a request that is cut, the first rows are
+    placed, and ``chunk_attention``, which takes a request's rows as its last
+    tokens, must not be used for it."""
     return _build_tables(page_ids, lengths, counts, max_pages, tokens)
 
 
@@ -179,6 +182,8 @@ def chunk_attention(q, k, v, pages, lengths, starts, *, scale=None, causal=True,
     from ``first[row]`` with documents.  Scores are ``scale * q.k`` (default
     1/sqrt(dim)), then ``cap * tanh(score / cap)``, then minus ``slopes[head] *
     |p - token|``.  Rows that see nothing, and rows of no request, are zero.
+    The softmax weights are rounded to the inputs' type for the product with V
+    (32-bit for tensors not aligned to 16 bytes, which are much slower).
     Not differentiable: tensors that autograd tracks are refused."""
     return _chunk_attention(q, k, v, pages, lengths, starts, scale, causal, window, cap, slopes,
                             prefix, first)

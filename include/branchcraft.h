@@ -367,7 +367,11 @@ typedef struct bc_pool_strides {
  * rows whose place lies before the request, past its row of the table or past
  * page_ids, or in a page with a negative id or one of 2^27 or more; a
  * position before the request is -1.  Negative lengths and counts count as
- * 0.  Rejects: batch or max_pages < 1, held or tokens < 0, null pointers
+ * 0.  Where `tokens` is less than the sum of counts, the rows that fit are the
+ * first ones: of the request that is cut, its first new tokens.  Such a
+ * request must not be attended to (bc_chunk_attention takes its rows as its
+ * last tokens, and the others are not in the cache); requests that fit whole
+ * are not affected.  Rejects: batch or max_pages < 1, held or tokens < 0, null pointers
  * (those of empty arrays aside), batch over BC_MAX_TABLE_REQUESTS, max_pages
  * over BC_MAX_TABLE_PAGES, 2^27 tokens or more. */
 int bc_build_tables(const int32_t* page_ids, int held, const int32_t* lengths,
@@ -433,7 +437,10 @@ typedef struct bc_chunk_inputs {
  * lengths past the table's row end there (places stay counted from
  * lengths[b]).  What a row does not see never reaches its output, NaN and
  * infinity included.  Scores, sums and the output's accumulation are 32-bit;
- * the weights are rounded to the inputs' type for the product with V.
+ * the weights are rounded to the inputs' type for the product with V (by half
+ * a step each, to nearest), except where q, k, v or the output are not aligned
+ * to 16 bytes, a stride is not a multiple of 8, or a launch would take 2^24
+ * workgroups: these go row by row, with 32-bit weights, and much slower.
  * Rejects: batch/Hq/Hkv < 1, Hq % Hkv != 0, Hq over BC_MAX_CHUNK_HEADS,
  * dim not 64/128, max_pages < 1 or over BC_MAX_TABLE_PAGES, physical_pages
  * below 1, tokens or window < 0, a scale, or a cap other than 0, outside
@@ -442,7 +449,12 @@ int bc_chunk_attention(bc_shape shape, bc_chunk_inputs in, void* workspace,
                        size_t workspace_bytes, bc_stream_t stream);
 
 /* Bytes of workspace with which bc_chunk_attention may split long requests
- * over several workgroups.  A null workspace, a smaller one or one that is
+ * over several workgroups, from the shape alone, whatever the lengths: 0 for
+ * tables of up to 512 tokens (1024 where the rows, tokens * Hq / Hkv, are at
+ * most 32 * batch) and for one request whose rows fill the card; else, on 256
+ * CUs and with up to 128 requests, 85 to 105 MB at D = 128, 50 to 65 MB at D =
+ * 64, and 17 MB with at most 32 rows.
+ * A null workspace, a smaller one or one that is
  * not aligned to 16 bytes is ignored: nothing is split then. */
 size_t bc_chunk_attention_workspace_size(bc_shape shape, int tokens);
 

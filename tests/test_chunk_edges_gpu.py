@@ -145,3 +145,19 @@ def test_inference_mode():
     with torch.inference_mode():
         assert torch.equal(bt.chunk_attention(*args, cap=4.0), want)
         assert torch.equal(bt.chunk_attention(q, *args[1:], cap=4.0), want)
+
+
+def test_a_step_of_too_few_rows():
+    """Capacity for four rows of six: tables and slots are those of the tokens
+    that fit, and so is the attention of every request that fits whole."""
+    import branchcraft_torch as bt
+    fix = C.batch([20, 37, 9], [2, 3, 1], 4, 2, 64, F16, seed=35)
+    dev = C.on_gpu(fix)
+    ids = fix["pages"][fix["pages"] >= 0].cuda()
+    counts = torch.tensor([2, 3, 1], dtype=torch.int32, device="cuda")
+    pages, starts, slots, positions = bt.build_tables(ids, dev["lengths"], counts, fix["pages"].shape[1], 4)
+    assert torch.equal(pages, dev["pages"])
+    assert starts.tolist() == [0, 2, 4, 4] and positions.tolist() == [18, 19, 34, 35]
+    want, tol = C.reference(**fix)
+    got = bt.chunk_attention(dev["q"][:4], dev["k"], dev["v"], pages, dev["lengths"], starts)
+    C.check(got[:2], want[:2], tol[:2])
