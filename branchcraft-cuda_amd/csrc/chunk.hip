@@ -646,7 +646,6 @@ __device__ __forceinline__ u32x4 read_v(const uint16_t* lo, const uint16_t* hi) 
 enum class Form { kPlain, kBias, kCap };
 constexpr float kFineCap = 256.f;
 
-template <int D>
 __device__ __forceinline__ float scale2_of(const ChunkParams& C, Form form) {
   return (form == Form::kCap ? 2.f * C.cap : C.scale) * kLog2e;
 }
@@ -1062,17 +1061,17 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   };
 
   const Offsets<D> o = read_offsets<D>(lane);
-  const float scale2 = scale2_of<D>(C, FORM);
-  bool is_whole = true, bad = false;
+  const float scale2 = scale2_of(C, FORM);
+  bool bad = false;
   int pages = 15;  // of the step at hand, a bit each: in the pool
   if (t0 < tend) {
     pg.take(C, kvh, ids);
 #pragma unroll
     for (int x = 0; x < NX; ++x) issue_chunk(x, 0, 0);
     pages = (int)pg.in_pool & 15;
-    is_whole = pages == 15 && t0 >= whole_lo && t0 < whole_hi;
+    const bool whole = pages == 15 && t0 >= whole_lo && t0 < whole_hi;
     wait_loads();
-    if (!is_whole) bad = inspect(tokens_of<4>(rq.len - t0 * kStep, pages), s_kv + HALF);
+    if (!whole) bad = inspect(tokens_of<4>(rq.len - t0 * kStep, pages), s_kv + HALF);
     bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));
   }
   // The wait for Q belongs here, on every path into the loop: at its first use
@@ -1131,7 +1130,6 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     __syncthreads();
     if (bad && tid == 0) s_bad[s & 3] = 0;
     bad = !whole_n && __builtin_amdgcn_readfirstlane(s_bad[(s + 1) & 3]);
-    is_whole = whole_n;
     pages = pages_n;
   };
   for (int t = t0; t < tend; t += 2) {
@@ -1261,7 +1259,7 @@ struct Stream {
       bad = __builtin_amdgcn_ballot_w64(bad) != 0;
       wave_lds_sync();
     }
-    weigh<T, D, 1>(sc, R, vt, o, scale2_of<D>(C, FORM));
+    weigh<T, D, 1>(sc, R, vt, o, scale2_of(C, FORM));
     if (bad) add_untidy<T, D>(C, rq, kvh, R, t * 32, 32, g);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
