@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kThreads = 256;
 // Most workgroups of a launch's first dimension: HIP takes fewer than 2^32
-// threads.  Kernels whose work may need more go over it in turns.
+// threads.  Work that may need more is gone over in turns.
 constexpr int kMostGroups = (1 << 24) - 1;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -115,26 +115,23 @@ struct AppendParams {
   int tokens, phys_pages, row_vec, head_vec;
 };
 
-// A workgroup copies rows_per_block rows at a time, K then V, in elements of
-// type E.
+// Workgroup i copies rows_per_block rows, K then V, in elements of type E.
 // HBM-bound: 8192 rows of 8 heads x 128 out of a fused projection (67 MB) 12.1
 // us, 5.5 TB/s, as a large copy; 64 rows 2.6 us.
 template <typename E>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams P, int rows_per_block) {
-  for (long long t0 = (long long)blockIdx.x * rows_per_block; t0 < P.tokens;
-       t0 += (long long)gridDim.x * rows_per_block) {
-    const int n = (int)min((long long)rows_per_block, P.tokens - t0) * P.row_vec;
-    for (int x = threadIdx.x; x < n; x += kThreads) {
-      const int i = x / P.row_vec, c = x - i * P.row_vec;
-      const int h = c / P.head_vec, e = c - h * P.head_vec;
-      const int slot = P.slots[t0 + i];
-      if (slot < 0 || (slot >> 4) >= P.phys_pages) continue;
-      const long long t = t0 + i, page = slot >> 4, in = slot & 15;
-      static_cast<E*>(P.cache_k)[page * P.cp[0] + in * P.cs[0] + h * P.ch[0] + e] =
-          static_cast<const E*>(P.k)[t * P.ts[0] + h * P.hs[0] + e];
-      static_cast<E*>(P.cache_v)[page * P.cp[1] + in * P.cs[1] + h * P.ch[1] + e] =
-          static_cast<const E*>(P.v)[t * P.ts[1] + h * P.hs[1] + e];
-    }
+  const int t0 = blockIdx.x * rows_per_block;
+  const int n = min(rows_per_block, P.tokens - t0) * P.row_vec;
+  for (int x = threadIdx.x; x < n; x += kThreads) {
+    const int i = x / P.row_vec, c = x - i * P.row_vec;
+    const int h = c / P.head_vec, e = c - h * P.head_vec;
+    const int slot = P.slots[t0 + i];
+    if (slot < 0 || (slot >> 4) >= P.phys_pages) continue;
+    const long long t = t0 + i, page = slot >> 4, in = slot & 15;
+    static_cast<E*>(P.cache_k)[page * P.cp[0] + in * P.cs[0] + h * P.ch[0] + e] =
+        static_cast<const E*>(P.k)[t * P.ts[0] + h * P.hs[0] + e];
+    static_cast<E*>(P.cache_v)[page * P.cp[1] + in * P.cs[1] + h * P.ch[1] + e] =
+        static_cast<const E*>(P.v)[t * P.ts[1] + h * P.hs[1] + e];
   }
 }
 
@@ -1744,29 +1741,39 @@ extern "C" int bc_append_kv(bc_shape s, const bc_half* k, const bc_half* v, bc_r
   const bool vec = aligned16(k) && aligned16(v) && aligned16(cache_k) && aligned16(cache_v) &&
                    bits % 8 == 0;
   const int e = vec ? 8 : 1;
-  const AppendParams P{k,
-                       v,
-                       cache_k,
-                       cache_v,
-                       slots,
-                       {ks.token / e, vs.token / e},
-                       {ks.head / e, vs.head / e},
-                       {cks.page / e, cvs.page / e},
-                       {cks.slot / e, cvs.slot / e},
-                       {cks.head / e, cvs.head / e},
-                       tokens,
-                       s.physical_pages,
-                       s.kv_heads * s.dim / e,
-                       s.dim / e};
+  AppendParams P{k,
+                 v,
+                 cache_k,
+                 cache_v,
+                 slots,
+                 {ks.token / e, vs.token / e},
+                 {ks.head / e, vs.head / e},
+                 {cks.page / e, cvs.page / e},
+                 {cks.slot / e, cvs.slot / e},
+                 {cks.head / e, cvs.head / e},
+                 0,
+                 s.physical_pages,
+                 s.kv_heads * s.dim / e,
+                 s.dim / e};
   const int rows = P.row_vec >= kThreads ? 1 : kThreads / P.row_vec;
-  const int groups = (tokens - 1) / rows + 1;
-  const dim3 grid(groups < kMostGroups ? groups : kMostGroups);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (vec)
-    append_kernel<uint4><<<grid, kThreads, 0, st>>>(P, rows);
-  else
-    append_kernel<uint16_t><<<grid, kThreads, 0, st>>>(P, rows);
-  return hipGetLastError();
+  // One launch, or several for rows past kMostGroups workgroups (a loop in the
+  // kernel costs every call 1 %).
+  const long long most = (long long)kMostGroups * rows;
+  for (long long t0 = 0; t0 < tokens; t0 += most) {
+    P.k = k + t0 * ks.token;
+    P.v = v + t0 * vs.token;
+    P.slots = slots + t0;
+    P.tokens = (int)(tokens - t0 < most ? tokens - t0 : most);
+    const dim3 grid((P.tokens - 1) / rows + 1);
+    if (vec)
+      append_kernel<uint4><<<grid, kThreads, 0, st>>>(P, rows);
+    else
+      append_kernel<uint16_t><<<grid, kThreads, 0, st>>>(P, rows);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return BC_SUCCESS;
 }
 
 namespace {
