@@ -50,7 +50,7 @@ __device__ __forceinline__ long long wave_sum_ll(long long x) {
 // writes every slices'th span of b's table row and of its rows of the slot
 // map; workgroup row `batch` writes what lies behind the last request.
 // Latency-bound, four rounds of loads and stores: 64 single tokens over tables
-// of 256 pages 3.4 us, 64 new prompts of 128-4096 tokens (1.2 MB) 4.2 (8.0 with
+// of 256 pages 3.3 us, 64 new prompts of 128-4096 tokens (1.2 MB) 4.2 (8.0 with
 // as many slices as the longest possible request has).  A call costs its host 7.
 __global__ __launch_bounds__(kThreads) void build_tables_kernel(TableParams P) {
   const int b = blockIdx.x, tid = threadIdx.x, step = gridDim.y * kTableSpan;
@@ -116,8 +116,10 @@ struct AppendParams {
 };
 
 // Workgroup i copies rows_per_block rows, K then V, in elements of type E.
-// HBM-bound: 8192 rows of 8 heads x 128 out of a fused projection (67 MB) 12.1
-// us, 5.5 TB/s, as a large copy; 64 rows 2.6 us.
+// Memory-bound: 8192 rows of 8 heads x 128 out of a fused projection (67 MB moved)
+// 12.1 us, 5.5 TB/s; torch's copy moves as much, contiguous, in 10.1 (6.6 TB/s,
+// some of it out of the last-level cache), half a GB and more at 5.2-5.4; 64
+// rows 2.6 us.
 template <typename E>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams P, int rows_per_block) {
   const int t0 = blockIdx.x * rows_per_block;
@@ -970,10 +972,12 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
 //  - 128 rows: the step's 32 KB from L2 serve 4.2 MFLOP.  32 rows per wave: the
 //    output takes 64 registers, and eight waves fit a CU's register file.
 //  - Bound at D = 128 by the matrix units and the clock that they leave (2048
-//    rows over 32768 tokens, 32/8 heads: 1020 us, 1044 TFLOP/s; a library
-//    product of 8192^3 1246), at D = 64 by the vector units: the same softmax
-//    for half the products (32 heads, 512 over 2048: 177 us, 680 TFLOP/s).
-//  - A workgroup's start and end take 7 us beside its neighbour's steps of 1.9.
+//    new tokens over 32768, 32/8 heads: 988 to 1045 us with the clock, 1020 to
+//    1080 TFLOP/s; a library product of 8192^3 1246), at D = 64 by the vector
+//    units: the same softmax for half the products (32 heads, 512 new tokens
+//    over 2048, sixteen of them: 180 us, 670 TFLOP/s).
+//  - A full round of workgroups takes 8.6 us, launch included, and 2.1 per step
+//    (2048 new tokens over 2048 to 32768, none masked: 75.8 to 1082 us).
 template <typename T, int D, Form FORM>
 __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const Item& it, int kvh,
                                           uint16_t* s_kv, Seen* s_seen, int* s_bad) {
@@ -1109,8 +1113,9 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     if (e.pages) e.valid = tokens_of<4>(rq.len - t * kStep, pages);
     finish_scores<D, FORM, 2>(C, sc, R, t * kStep, g, e);
     // The softmax and its product ahead of other waves' score products, so that
-    // the two of a SIMD do not fall into step: 4096 of 4096 tokens (D = 128) 160
-    // -> 151 us; at D = 64 and with a cap it takes 2 to 4 % more.
+    // the two of a SIMD do not fall into step: 4096 of 4096 tokens (D = 128) 167
+    // -> 156 us, 2048 of 32768 1070 -> 1034; at D = 64 and with a cap it takes 2
+    // to 4 % more.
     constexpr bool kAhead = D == 128 && FORM != Form::kCap;
     if (kAhead) __builtin_amdgcn_s_setprio(2);
     weigh<T, D, 2>(sc, R, kt + HALF, o, scale2);
@@ -1267,8 +1272,7 @@ struct Stream {
 // single tokens over 128-4096 tokens (32/8 heads, D = 128, 585 MB) 96 us, 6.5
 // TB/s in this kernel; with a part of a request per workgroup, the longest
 // parts last, it took 127.  The waves of a workgroup take the KV heads of one
-// range, whose lines lie side by side: 108 -> 99 us with four waves per CU in
-// place of eight.
+// range, whose lines lie side by side; four waves per CU 96 us, eight 99.
 // A request that a range holds whole leaves as output rows, of others each
 // range leaves a partial.  Range r's partial of a request whose predecessors
 // have n rows starts at partial row 32 r + n: a range's next request is
@@ -1644,11 +1648,11 @@ Cut cut_of(const bc_shape& s, int tokens) {
       (long long)s.batch * s.query_heads > 1 << 26)
     return c;
   c.target = 2 * bch::device_cus();
-  // One request's rows that fill the card as whole tiles need no join (3 us).
+  // One request's rows that fill the card as whole tiles need no join (5 us).
   if (s.batch == 1 && rows / kManyRows * s.kv_heads >= c.target) return Cut{};
   // Four ranges per CU, eight at dim 64, where a tile is half the bytes (64
-  // single tokens over 128-4096: 52.4 us, 54.4 with four; at dim 128 96 us with
-  // four, 102 with eight).
+  // single tokens over 128-4096: 52.5 us, 54.4 with four; at dim 128 96 us with
+  // four, 99 with eight).
   const int per = s.dim == 64 ? 4 : 2;
   c.waves = per * c.target / s.kv_heads > 1 ? per * c.target / s.kv_heads : 1;
   c.narrow_rows = 32 * c.waves + (int)(rows < 32ll * s.batch ? rows : 32ll * s.batch);
