@@ -163,10 +163,16 @@ __device__ __forceinline__ void load_to_lds(const void* src, unsigned dst) {
                : "memory");
 }
 
-__device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+// Two of them from wave-uniform bases.  A vector instruction that writes a base's
+// registers (v_readlane, for one, also where the compiler reloads a spilled one)
+// must lie five wait states back, which the compiler does not count into inline
+// assembly: they stand in it, once for both.
+__device__ __forceinline__ void load2_to_lds(const void* base0, const void* base1, unsigned off0,
+                                             unsigned off1, unsigned dst0, unsigned dst1) {
+  asm volatile("s_mov_b32 m0, %4\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %2\n\t"
+               "s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3"
                :
-               : "v"(off), "s"(base), "s"(dst)
+               : "v"(off0), "v"(off1), "s"(base0), "s"(base1), "s"(dst0), "s"(dst1)
                : "memory");
 }
 

@@ -1043,8 +1043,7 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   auto issue_chunk = [&](int x, int at, int buf) {
     const int from = 4 * at + (CPR == 16 ? x : 2 * x + (wave >> 1));
     const unsigned dst = lds0 + buf * (4 * HALF) + x * 4096;
-    load_to_lds(Pages::at(pg.k, from), koff, dst);
-    load_to_lds(Pages::at(pg.v, from), voff, dst + 2 * HALF);
+    load2_to_lds(Pages::at(pg.k, from), Pages::at(pg.v, from), koff, voff, dst, dst + 2 * HALF);
   };
   // Steps whole_lo .. whole_hi - 1 are seen whole by every row, given their pages.
   const int whole_lo = wg.all_lo / kStep + (wg.all_lo % kStep != 0);
@@ -1178,14 +1177,31 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   }
 }
 
-// load_to_lds for what a call reads once: the line is marked for early
-// replacement.  64 single tokens over 128-4096 tokens (32/8 heads, D = 128) 122 ->
-// 108 us.
-__device__ __forceinline__ void stream_to_lds(const void* base, unsigned off, unsigned dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
-               :
-               : "v"(off), "s"(base), "s"(dst)
-               : "memory");
+// A tile's two pages, N loads of 1 KB each, one after another in LDS, of what a
+// call reads once: the lines are marked for early replacement.  64 single tokens
+// over 128-4096 tokens (32/8 heads, D = 128) 122 -> 108 us.  The bases' five wait
+// states (see load2_to_lds) stand before the first.
+template <int N>
+__device__ __forceinline__ void stream_to_lds(const void* base0, const void* base1,
+                                              const unsigned (&off)[N], unsigned dst) {
+  static_assert(N == 2 || N == 4, "loads per page");
+#define BC_LOAD(OFF, BASE) "global_load_lds_dwordx4 %" #OFF ", %" #BASE " nt\n\t"
+#define BC_NEXT "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\t"
+  if constexpr (N == 2)
+    asm volatile("s_mov_b32 m0, %4\n\ts_nop 3\n\t"
+                 BC_LOAD(0, 2) BC_NEXT BC_LOAD(1, 2) BC_NEXT BC_LOAD(0, 3) BC_NEXT BC_LOAD(1, 3)
+                 :
+                 : "v"(off[0]), "v"(off[1]), "s"(base0), "s"(base1), "s"(dst)
+                 : "memory", "scc");
+  else
+    asm volatile("s_mov_b32 m0, %6\n\ts_nop 3\n\t"
+                 BC_LOAD(0, 4) BC_NEXT BC_LOAD(1, 4) BC_NEXT BC_LOAD(2, 4) BC_NEXT BC_LOAD(3, 4) BC_NEXT
+                 BC_LOAD(0, 5) BC_NEXT BC_LOAD(1, 5) BC_NEXT BC_LOAD(2, 5) BC_NEXT BC_LOAD(3, 5)
+                 :
+                 : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base0), "s"(base1), "s"(dst)
+                 : "memory", "scc");
+#undef BC_LOAD
+#undef BC_NEXT
 }
 
 // A wave's stream of 32-token tiles through its own part of LDS: K of the next
@@ -1224,9 +1240,7 @@ struct Stream {
   }
   __device__ __forceinline__ void issue(unsigned long long x, int at, const unsigned (&off)[NV],
                                         unsigned dst) const {
-    const void* const page[2] = {Pages::at(x, 2 * at), Pages::at(x, 2 * at + 1)};
-#pragma unroll
-    for (int c = 0; c < NL; ++c) stream_to_lds(page[c / NV], off[c % NV], dst + c * 1024);
+    stream_to_lds<NV>(Pages::at(x, 2 * at), Pages::at(x, 2 * at + 1), off, dst);
   }
   __device__ __forceinline__ void issue_k(int at) const { issue(pg.k, at, koff, lds0); }
   __device__ __forceinline__ void issue_v(int at) const { issue(pg.v, at, voff, lds0 + 2 * TILE); }

@@ -1518,8 +1518,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void tree_wide_kernel(TreePar
     const int i = x / CPT, c = x % CPT;
     const unsigned id = CPT == 2 ? ph[2 * i + c] : wave < 2 ? ph[2 * i] : ph[2 * i + 1];
     const unsigned long long off = (unsigned long long)id * page_bytes;
-    load_to_lds(kb + off, loff, lds_of(buf, i, c));
-    load_to_lds(vb + off, loff, lds_of(buf, i, c) + HALF * 2);
+    load2_to_lds(kb + off, vb + off, loff, loff, lds_of(buf, i, c), lds_of(buf, i, c) + HALF * 2);
   };
   // Any step.  Pages outside the pool read page 0, rows past the length
   // their page's rows and draft rows past the node count the last node's: all
