@@ -436,8 +436,10 @@ typedef struct bc_chunk_inputs {
  * Tokens whose page id lies outside [0, physical_pages) are not seen, and
  * lengths past the table's row end there (places stay counted from
  * lengths[b]).  What a row does not see never reaches its output, NaN and
- * infinity included.  Scores, sums and the output's accumulation are 32-bit;
- * the weights are rounded to the inputs' type for the product with V (by half
+ * infinity included.  Scores, sums and the output's accumulation are 32-bit.
+ * Every workgroup walks the batch's lengths to its own work, so that calls of
+ * some hundred requests each are faster than one of thousands.
+ * The weights are rounded to the inputs' type for the product with V (by half
  * a step each, to nearest), except where q, k, v or the output are not aligned
  * to 16 bytes, a stride is not a multiple of 8, or a launch would take 2^24
  * workgroups: these go row by row, with 32-bit weights, and much slower.
