@@ -972,7 +972,7 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
 //  - 128 rows: the step's 32 KB from L2 serve 4.2 MFLOP.  32 rows per wave: the
 //    output takes 64 registers, and eight waves fit a CU's register file.
 //  - Bound at D = 128 by the matrix units and the clock that they leave (2048
-//    new tokens over 32768, 32/8 heads: 988 to 1045 us with the clock, 1020 to
+//    new tokens over 32768, 32/8 heads: 988 to 1050 us with the clock, 1010 to
 //    1080 TFLOP/s; a library product of 8192^3 1246), at D = 64 by the vector
 //    units: the same softmax for half the products (32 heads, 512 new tokens
 //    over 2048, sixteen of them: 180 us, 670 TFLOP/s).
