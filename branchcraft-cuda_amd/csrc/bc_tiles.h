@@ -41,6 +41,8 @@ struct ChunkParams {
   unsigned group_mul;        // ceil(2^32 / group), or 0: see divide
   unsigned hkv_mul;          // the same of hkv
   float scale, cap;
+  const uint8_t* k_scale;    // of an 8-bit cache, whose k, v and their strides are in bytes
+  const uint8_t* v_scale;
 };
 
 __device__ __forceinline__ float to_float(_Float16 x) { return (float)x; }
@@ -54,6 +56,29 @@ __device__ __forceinline__ float load_elem(const uint16_t* p) {
 template <typename T>
 __device__ __forceinline__ uint16_t round_to(float x) {
   return __builtin_bit_cast(uint16_t, (T)x);  // to nearest, ties to even
+}
+
+// Two e4m3 codes of a word (its low half, or its high one) times a power of two
+// of which `scale` has the exponent, as two values of T in one instruction.
+template <typename T, bool HIGH>
+__device__ __forceinline__ uint32_t values2(uint32_t codes, float scale) {
+  if constexpr (std::is_same<T, _Float16>::value)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, HIGH));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HIGH));
+}
+
+// The power of two whose biased exponent a byte of an 8-bit cache's scales is.
+__device__ __forceinline__ float power_of(uint32_t byte) {
+  return __builtin_bit_cast(float, byte << 23);
+}
+
+constexpr int kFp8Block = BC_FP8_BLOCK;
+
+// Where the scales of a slot and head start, [P][Hkv][16][D / 32].
+template <int D>
+__device__ __forceinline__ size_t scale_at(const ChunkParams& P, int page, int kvh, int slot) {
+  return (((size_t)page * P.hkv + kvh) * BC_PAGE_SIZE + slot) * (D / kFp8Block);
 }
 
 // tanh in terms of one exponential, 1 - 2 / (e^2x + 1), which is off by a few
@@ -107,7 +132,7 @@ __device__ __forceinline__ int2 row_range(const ChunkParams& P, int b, int t, in
 // of 64, the online softmax's maximum and sum stay in the wave, and each lane
 // keeps D / 64 dimensions of the output.  Tokens that the row does not see
 // are never multiplied, whatever their K and V hold.
-template <typename T, int D>
+template <typename T, int D, bool FP8>
 __device__ __forceinline__ void attend_row(const ChunkParams& P, int t, int h, int lane) {
   constexpr int R = D / 64;
   const int b = request_of(P, t, lane);
@@ -120,15 +145,25 @@ __device__ __forceinline__ void attend_row(const ChunkParams& P, int t, int h, i
     const uint16_t* const q = P.q + t * P.qt + h * P.qh;
     const int32_t* const row = P.pages + (size_t)b * P.max_pages;
     const float slope = P.slopes ? P.slopes[h] * kLog2e : 0.f;
+    // Value e of slot `slot` of a page of K or V.
+    auto value = [&](const uint16_t* pool, const uint8_t* scales, long long at, int page, int slot, int e) {
+      if constexpr (FP8) {
+        const uint8_t code = reinterpret_cast<const uint8_t*>(pool)[at + e];
+        const uint8_t power = scales[scale_at<D>(P, page, kvh, slot) + e / kFp8Block];
+        return to_float(__builtin_bit_cast(T, (uint16_t)values2<T, false>(code, power_of(power))));
+      } else {
+        return load_elem<T>(pool + at + e);
+      }
+    };
     for (int j0 = seen.x & ~63; j0 <= seen.y; j0 += 64) {
       const int j = j0 + lane;
       const int id = j >= seen.x && j <= seen.y ? row[j >> 4] : -1;
       const bool ok = (unsigned)id < (unsigned)P.phys_pages;
       float s = kNegInf;
       if (ok) {
-        const uint16_t* const k = P.k + id * P.kp + (j & 15) * P.ks + kvh * P.kh;
+        const long long k = id * P.kp + (j & 15) * P.ks + kvh * P.kh;
         float dot = 0.f;
-        for (int d = 0; d < D; ++d) dot += load_elem<T>(q + d) * load_elem<T>(k + d);
+        for (int d = 0; d < D; ++d) dot += load_elem<T>(q + d) * value(P.k, P.k_scale, k, id, j & 15, d);
         s = dot * P.scale;
         if (P.cap > 0.f) s = P.cap * tanh_of(s / P.cap);
         s = s * kLog2e - slope * fabsf((float)(pos - j));
@@ -142,12 +177,11 @@ __device__ __forceinline__ void attend_row(const ChunkParams& P, int t, int h, i
 #pragma unroll
       for (int r = 0; r < R; ++r) acc[r] *= alpha;
       for (unsigned long long left = __builtin_amdgcn_ballot_w64(ok); left; left &= left - 1) {
-        const int from = __builtin_ctzll(left);
+        const int from = __builtin_ctzll(left), page = __shfl(id, from, 64), slot = (j0 + from) & 15;
         const float w = __shfl(p, from, 64);
-        const uint16_t* const v =
-            P.v + __shfl(id, from, 64) * P.vp + ((j0 + from) & 15) * P.vs + kvh * P.vh;
+        const long long v = page * P.vp + slot * P.vs + kvh * P.vh;
 #pragma unroll
-        for (int r = 0; r < R; ++r) acc[r] += w * load_elem<T>(v + 64 * r + lane);
+        for (int r = 0; r < R; ++r) acc[r] += w * value(P.v, P.v_scale, v, page, slot, 64 * r + lane);
       }
     }
   }
@@ -157,21 +191,32 @@ __device__ __forceinline__ void attend_row(const ChunkParams& P, int t, int h, i
     out[64 * r + lane] = round_to<T>(l > 0.f || l != l ? acc[r] / l : 0.f);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool FP8>
 __global__ __launch_bounds__(kThreads) void chunk_rows_kernel(ChunkParams P) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.y * (kThreads / 64) + wave;
   if (h >= P.hq) return;
   for (unsigned row = blockIdx.x; row < (unsigned)P.tokens; row += gridDim.x)
-    attend_row<T, D>(P, (int)row, h, lane);
+    attend_row<T, D, FP8>(P, (int)row, h, lane);
 }
 
-template <typename T, int D>
-void launch_rows(const ChunkParams& P, hipStream_t st) {
+template <bool FP8>
+hipError_t launch_rows(const ChunkParams& P, int dim, int dtype, hipStream_t st) {
   const dim3 grid(P.tokens < kMostGroups ? P.tokens : kMostGroups,
                   (P.hq + kThreads / 64 - 1) / (kThreads / 64));
-  chunk_rows_kernel<T, D><<<grid, kThreads, 0, st>>>(P);
+  if (dtype == BC_FLOAT16) {
+    if (dim == 64)
+      chunk_rows_kernel<_Float16, 64, FP8><<<grid, kThreads, 0, st>>>(P);
+    else
+      chunk_rows_kernel<_Float16, 128, FP8><<<grid, kThreads, 0, st>>>(P);
+  } else {
+    if (dim == 64)
+      chunk_rows_kernel<__bf16, 64, FP8><<<grid, kThreads, 0, st>>>(P);
+    else
+      chunk_rows_kernel<__bf16, 128, FP8><<<grid, kThreads, 0, st>>>(P);
+  }
+  return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------
@@ -1672,7 +1717,9 @@ inline ChunkParams chunk_params(const bc_shape& s, const bc_chunk_inputs& in) {
                      group_mul,
                      hkv_mul,
                      in.scale,
-                     in.cap};
+                     in.cap,
+                     nullptr,
+                     nullptr};
 }
 
 }  // namespace

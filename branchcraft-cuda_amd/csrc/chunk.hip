@@ -229,9 +229,5 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
     return s.dim == 64 ? launch_tiles<__bf16, 64>(P, cut, ws, (unsigned)grid, st)
                        : launch_tiles<__bf16, 128>(P, cut, ws, (unsigned)grid, st);
   }
-  if (in.dtype == BC_FLOAT16)
-    s.dim == 64 ? launch_rows<_Float16, 64>(P, st) : launch_rows<_Float16, 128>(P, st);
-  else
-    s.dim == 64 ? launch_rows<__bf16, 64>(P, st) : launch_rows<__bf16, 128>(P, st);
-  return hipGetLastError();
+  return launch_rows<false>(P, s.dim, in.dtype, st);
 }

@@ -564,24 +564,159 @@ void append_kv_autograd(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tens
   append_kv_versions(cache_k, cache_v, k, v, slots);
 }
 
-// Attention of each request's new tokens over its pages (see
-// bc_chunk_attention).  The workspace comes from the caching allocator on the
-// current stream and its size from shapes alone, so that the op never reads
-// lengths back and can be captured.
-at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                               const at::Tensor& pages, const at::Tensor& lengths,
-                               const at::Tensor& starts, std::optional<double> scale,
-                               bool causal, int64_t window, double cap,
-                               const std::optional<at::Tensor>& slopes,
-                               const std::optional<at::Tensor>& prefix,
-                               const std::optional<at::Tensor>& first) {
+// A pool of 8-bit codes, [P, 16, Hkv, D].
+void check_codes(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
+  TORCH_CHECK(t.scalar_type() == at::kFloat8_e4m3fn, name, " must be float8_e4m3fn");
+  TORCH_CHECK(t.dim() == 4, name, " must have 4 dimensions");
+  TORCH_CHECK(t.size(-1) == 64 || t.size(-1) == 128, name, ": head dimension must be 64 or 128");
+  TORCH_CHECK(t.stride(-1) == 1, name, ": head dimension must be contiguous");
+  const bc_pool_strides s = pool_strides(t);
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) | uintptr_t(s.page | s.slot | s.head)) % 16 == 0,
+              name, " must be aligned to 16 bytes, and so must its pages, slots and heads");
+}
+
+// Its scales, [P, Hkv, 16, D / 32].
+void check_scales(const at::Tensor& t, const char* name, const at::Tensor& codes) {
+  check_dev_contig(t, name, at::kFloat8_e8m0fnu);
+  TORCH_CHECK(t.sizes() == at::IntArrayRef({codes.size(0), codes.size(2), BC_PAGE_SIZE,
+                                            codes.size(3) / BC_FP8_BLOCK}),
+              name, " must be [pages, KV heads, 16, dim / 32]");
+  TORCH_CHECK(t.device() == codes.device(), "all tensors must share a device");
+}
+
+uint8_t* bytes_of(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+// The checks of both calls on an 8-bit cache's rows, and the cache.
+bc_fp8_pool fp8_pool(const char* op, const at::Tensor& cache_k, const at::Tensor& scale_k,
+                     const at::Tensor& cache_v, const at::Tensor& scale_v, const at::Tensor& slots) {
+  check_codes(cache_k, "cache_k");
+  check_codes(cache_v, "cache_v");
+  check_scales(scale_k, "scale_k", cache_k);
+  check_scales(scale_v, "scale_v", cache_v);
+  check_dev_contig(slots, "slots", at::kInt);
+  TORCH_CHECK(cache_k.size(0) > 0 && cache_k.size(1) == BC_PAGE_SIZE && cache_k.size(2) > 0 &&
+                  cache_v.sizes() == cache_k.sizes() && slots.dim() == 1,
+              op, " shape mismatch");
+  TORCH_CHECK(cache_k.device() == cache_v.device() && cache_k.device() == slots.device(),
+              "all tensors must share a device");
+  TORCH_CHECK(slots.size(0) <= INT32_MAX && cache_k.size(0) <= INT32_MAX &&
+                  cache_k.size(2) <= BC_MAX_CHUNK_HEADS,
+              op, ": too many tokens, heads or pages");
+  return {bytes_of(cache_k), bytes_of(cache_v), bytes_of(scale_k), bytes_of(scale_v),
+          pool_strides(cache_k), pool_strides(cache_v)};
+}
+
+bc_shape pool_shape(const at::Tensor& cache) {
+  return {1, int(cache.size(2)), int(cache.size(2)), int(cache.size(3)), 1, int(cache.size(0))};
+}
+
+int dtype_of(at::ScalarType type) { return type == at::kHalf ? BC_FLOAT16 : BC_BFLOAT16; }
+
+// New tokens' K and V rows into an 8-bit cache (see bc_append_fp8_kv).
+void append_fp8_kv_hip(at::Tensor& cache_k, at::Tensor& scale_k, at::Tensor& cache_v,
+                       at::Tensor& scale_v, const at::Tensor& k, const at::Tensor& v,
+                       const at::Tensor& slots) {
+  const bc_fp8_pool pool = fp8_pool("append_fp8_kv_", cache_k, scale_k, cache_v, scale_v, slots);
+  check_rows(k, "k", 3);
+  check_rows(v, "v", 3);
+  TORCH_CHECK(k.scalar_type() == v.scalar_type(), "append_fp8_kv_: k and v must share a dtype");
+  TORCH_CHECK(v.sizes() == k.sizes() && k.size(1) == cache_k.size(2) &&
+                  k.size(2) == cache_k.size(3) && slots.size(0) == k.size(0),
+              "append_fp8_kv_ shape mismatch");
+  TORCH_CHECK(cache_k.device() == k.device() && cache_k.device() == v.device(),
+              "all tensors must share a device");
+  const at::Tensor* const written[] = {&cache_k, &scale_k, &cache_v, &scale_v};
+  for (int i = 0; i < 4; ++i) {
+    at::assert_no_internal_overlap(*written[i]);
+    for (int j = 0; j < i; ++j) at::assert_no_overlap(*written[i], *written[j]);
+    at::assert_no_overlap(*written[i], k);
+    at::assert_no_overlap(*written[i], v);
+  }
+  if (k.size(0) == 0) return;
+  const c10::DeviceGuard guard(cache_k.device());
+  check_launch(bc_append_fp8_kv(pool_shape(cache_k), raw(k), raw(v), row_strides(k), row_strides(v),
+                                dtype_of(k.scalar_type()), pool, slots.data_ptr<int>(),
+                                int(k.size(0)), current_stream()),
+               "append_fp8_kv_");
+}
+
+void append_fp8_kv_versions(at::Tensor& cache_k, at::Tensor& scale_k, at::Tensor& cache_v,
+                            at::Tensor& scale_v, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& slots) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("branchcraft::append_fp8_kv_", "")
+                             .typed<decltype(append_fp8_kv_hip)>();
+  for (at::Tensor* x : {&cache_k, &scale_k, &cache_v, &scale_v})
+    x->unsafeGetTensorImpl()->bump_version();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  op.call(cache_k, scale_k, cache_v, scale_v, k, v, slots);
+}
+
+void append_fp8_kv_autograd(at::Tensor& cache_k, at::Tensor& scale_k, at::Tensor& cache_v,
+                            at::Tensor& scale_v, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& slots) {
+  refuse_tracked("append_fp8_kv_", {&cache_k, &scale_k, &cache_v, &scale_v, &k, &v});
+  append_fp8_kv_versions(cache_k, scale_k, cache_v, scale_v, k, v, slots);
+}
+
+// Rows of an 8-bit cache in 16 bits (see bc_read_fp8_kv).
+std::tuple<at::Tensor, at::Tensor> read_fp8_kv_hip(const at::Tensor& cache_k, const at::Tensor& scale_k,
+                                                   const at::Tensor& cache_v, const at::Tensor& scale_v,
+                                                   const at::Tensor& slots, at::ScalarType dtype) {
+  const bc_fp8_pool pool = fp8_pool("read_fp8_kv", cache_k, scale_k, cache_v, scale_v, slots);
+  TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "dtype must be FP16 or BF16");
+  const c10::DeviceGuard guard(cache_k.device());
+  const at::DimVector size{slots.size(0), cache_k.size(2), cache_k.size(3)};
+  auto k = new_tensor(cache_k, size, dtype), v = new_tensor(cache_k, size, dtype);
+  if (slots.size(0) > 0)
+    check_launch(bc_read_fp8_kv(pool_shape(cache_k), pool, slots.data_ptr<int>(), int(slots.size(0)),
+                                dtype_of(dtype), static_cast<bc_half*>(k.data_ptr()),
+                                static_cast<bc_half*>(v.data_ptr()), current_stream()),
+                 "read_fp8_kv");
+  return {k, v};
+}
+
+std::tuple<at::Tensor, at::Tensor> read_fp8_kv_autograd(const at::Tensor& cache_k,
+                                                        const at::Tensor& scale_k,
+                                                        const at::Tensor& cache_v,
+                                                        const at::Tensor& scale_v,
+                                                        const at::Tensor& slots, at::ScalarType dtype) {
+  refuse_tracked("read_fp8_kv", {&cache_k, &scale_k, &cache_v, &scale_v});
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("branchcraft::read_fp8_kv", "")
+                             .typed<decltype(read_fp8_kv_hip)>();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(cache_k, scale_k, cache_v, scale_v, slots, dtype);
+}
+
+// What the chunk attention ops take besides their caches.
+struct ChunkOptions {
+  std::optional<double> scale;
+  bool causal;
+  int64_t window;
+  double cap;
+  const std::optional<at::Tensor>&slopes, &prefix, &first;
+};
+
+// The checks of a chunk attention op over a 16-bit cache or, with scales, one of
+// 8 bits, and `launch` with the call's shape, inputs and output.
+template <typename F>
+at::Tensor chunk_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool fp8,
+                      const at::Tensor& pages, const at::Tensor& lengths, const at::Tensor& starts,
+                      const ChunkOptions& o, F launch) {
   check_rows(q, "q", 3);
-  check_rows(k, "k", 4);
-  check_rows(v, "v", 4);
+  if (fp8) {
+    check_codes(k, "k");
+    check_codes(v, "v");
+  } else {
+    check_rows(k, "k", 4);
+    check_rows(v, "v", 4);
+  }
   check_dev_contig(pages, "pages", at::kInt);
   check_dev_contig(lengths, "lengths", at::kInt);
   check_dev_contig(starts, "starts", at::kInt);
-  TORCH_CHECK(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(),
+  TORCH_CHECK(fp8 || (q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type()),
               "q, k and v must share a dtype");
   TORCH_CHECK(pages.dim() == 2 && lengths.dim() == 1 && starts.dim() == 1,
               "invalid chunk attention tensor rank");
@@ -596,11 +731,11 @@ at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const a
   TORCH_CHECK(t <= INT32_MAX && k.size(0) <= INT32_MAX && pages.size(1) <= BC_MAX_TABLE_PAGES &&
                   b < INT32_MAX && hq <= BC_MAX_CHUNK_HEADS,
               "chunk attention: too many rows, heads, pages or requests");
-  const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(double(d));
+  const double s = o.scale.has_value() ? *o.scale : 1.0 / std::sqrt(double(d));
   TORCH_CHECK(float(s) >= BC_LEAST_SCALE && float(s) <= BC_MOST_SCALE,
               "scale must be positive, between ", BC_LEAST_SCALE, " and ", BC_MOST_SCALE);
-  TORCH_CHECK(window >= 0, "window must not be negative");
-  TORCH_CHECK(cap == 0 || (float(cap) >= BC_LEAST_SCALE && float(cap) <= BC_MOST_SCALE),
+  TORCH_CHECK(o.window >= 0, "window must not be negative");
+  TORCH_CHECK(o.cap == 0 || (float(o.cap) >= BC_LEAST_SCALE && float(o.cap) <= BC_MOST_SCALE),
               "cap must be 0 (none), or between ", BC_LEAST_SCALE, " and ", BC_MOST_SCALE);
   TORCH_CHECK(q.device() == k.device() && q.device() == v.device() &&
                   q.device() == pages.device() && q.device() == lengths.device() &&
@@ -615,10 +750,10 @@ at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const a
     return x->data_ptr();
   };
   bc_chunk_inputs in{};
-  in.slopes = static_cast<const float*>(option(slopes, "slopes", at::kFloat, hq));
-  in.prefix = static_cast<const int32_t*>(option(prefix, "prefix", at::kInt, b));
-  in.first = static_cast<const int32_t*>(option(first, "first", at::kInt, t));
-  TORCH_CHECK(causal || !in.prefix, "prefix needs causal attention");
+  in.slopes = static_cast<const float*>(option(o.slopes, "slopes", at::kFloat, hq));
+  in.prefix = static_cast<const int32_t*>(option(o.prefix, "prefix", at::kInt, b));
+  in.first = static_cast<const int32_t*>(option(o.first, "first", at::kInt, t));
+  TORCH_CHECK(o.causal || !in.prefix, "prefix needs causal attention");
   const c10::DeviceGuard guard(q.device());
   auto output = new_tensor(q, q.sizes(), q.scalar_type());
   if (t == 0) return output;
@@ -633,19 +768,97 @@ at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const a
   in.k_strides = pool_strides(k);
   in.v_strides = pool_strides(v);
   in.tokens = int(t);
-  in.dtype = q.scalar_type() == at::kHalf ? BC_FLOAT16 : BC_BFLOAT16;
-  in.causal = causal;
-  in.window = int(std::min<int64_t>(window, INT32_MAX));
+  in.dtype = dtype_of(q.scalar_type());
+  in.causal = o.causal;
+  in.window = int(std::min<int64_t>(o.window, INT32_MAX));
   in.scale = float(s);
-  in.cap = float(cap);
-  bc_shape shape{int(b), int(hq), int(hkv), int(d), int(pages.size(1)), int(k.size(0))};
-  const size_t ws_bytes = bc_chunk_attention_workspace_size(shape, int(t));
-  at::Tensor ws;
-  if (ws_bytes > 0) ws = new_tensor(q, {int64_t(ws_bytes)}, at::kByte);
-  check_launch(bc_chunk_attention(shape, in, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
-                                  current_stream()),
-               "chunk_attention");
+  in.cap = float(o.cap);
+  launch(bc_shape{int(b), int(hq), int(hkv), int(d), int(pages.size(1)), int(k.size(0))}, in);
   return output;
+}
+
+// The workspace comes from the caching allocator on the current stream and its
+// size from shapes alone, so that the ops never read lengths back and can be
+// captured.
+at::Tensor workspace_of(const at::Tensor& q, size_t bytes) {
+  return bytes > 0 ? new_tensor(q, {int64_t(bytes)}, at::kByte) : at::Tensor();
+}
+
+// Attention of each request's new tokens over its pages (see
+// bc_chunk_attention).
+at::Tensor chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& pages, const at::Tensor& lengths,
+                               const at::Tensor& starts, std::optional<double> scale,
+                               bool causal, int64_t window, double cap,
+                               const std::optional<at::Tensor>& slopes,
+                               const std::optional<at::Tensor>& prefix,
+                               const std::optional<at::Tensor>& first) {
+  return chunk_call(q, k, v, false, pages, lengths, starts,
+                    {scale, causal, window, cap, slopes, prefix, first},
+                    [&](const bc_shape& shape, const bc_chunk_inputs& in) {
+                      const size_t bytes = bc_chunk_attention_workspace_size(shape, in.tokens);
+                      const at::Tensor ws = workspace_of(q, bytes);
+                      check_launch(bc_chunk_attention(shape, in, bytes ? ws.data_ptr() : nullptr,
+                                                      bytes, current_stream()),
+                                   "chunk_attention");
+                    });
+}
+
+// The same over an 8-bit cache (see bc_fp8_chunk_attention).
+at::Tensor fp8_chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const at::Tensor& scale_k,
+                                   const at::Tensor& v, const at::Tensor& scale_v,
+                                   const at::Tensor& pages, const at::Tensor& lengths,
+                                   const at::Tensor& starts, std::optional<double> scale,
+                                   bool causal, int64_t window, double cap,
+                                   const std::optional<at::Tensor>& slopes,
+                                   const std::optional<at::Tensor>& prefix,
+                                   const std::optional<at::Tensor>& first) {
+  check_codes(k, "k");
+  check_codes(v, "v");
+  check_scales(scale_k, "scale_k", k);
+  check_scales(scale_v, "scale_v", v);
+  return chunk_call(q, k, v, true, pages, lengths, starts,
+                    {scale, causal, window, cap, slopes, prefix, first},
+                    [&](const bc_shape& shape, const bc_chunk_inputs& in) {
+                      const size_t bytes = bc_fp8_chunk_attention_workspace_size(shape, in.tokens);
+                      const at::Tensor ws = workspace_of(q, bytes);
+                      check_launch(bc_fp8_chunk_attention(shape, in, bytes_of(scale_k), bytes_of(scale_v),
+                                                          bytes ? ws.data_ptr() : nullptr, bytes,
+                                                          current_stream()),
+                                   "fp8_chunk_attention");
+                    });
+}
+
+// The same for requests that begin with the same pages (see
+// bc_shared_chunk_attention).
+at::Tensor shared_chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                      const at::Tensor& pages, const at::Tensor& lengths,
+                                      const at::Tensor& starts, const at::Tensor& groups,
+                                      const at::Tensor& shared, std::optional<double> scale,
+                                      bool causal, int64_t window, double cap,
+                                      const std::optional<at::Tensor>& slopes,
+                                      const std::optional<at::Tensor>& prefix,
+                                      const std::optional<at::Tensor>& first) {
+  check_dev_contig(groups, "groups", at::kInt);
+  check_dev_contig(shared, "shared", at::kInt);
+  TORCH_CHECK(groups.dim() == 1 && shared.dim() == 1 && groups.size(0) == shared.size(0) + 1 &&
+                  shared.size(0) <= lengths.size(0),
+              "groups must have one entry more than shared, and shared at most one per request");
+  TORCH_CHECK(groups.device() == q.device() && shared.device() == q.device(),
+              "all tensors must share a device");
+  const int count = int(shared.size(0));
+  return chunk_call(q, k, v, false, pages, lengths, starts,
+                    {scale, causal, window, cap, slopes, prefix, first},
+                    [&](const bc_shape& shape, const bc_chunk_inputs& in) {
+                      const size_t bytes =
+                          bc_shared_chunk_attention_workspace_size(shape, in.tokens, count);
+                      const at::Tensor ws = workspace_of(q, bytes);
+                      check_launch(bc_shared_chunk_attention(shape, in, groups.data_ptr<int>(),
+                                                             shared.data_ptr<int>(), count,
+                                                             bytes ? ws.data_ptr() : nullptr, bytes,
+                                                             current_stream()),
+                                   "shared_chunk_attention");
+                    });
 }
 
 at::Tensor chunk_attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -665,6 +878,42 @@ at::Tensor chunk_attention_autograd(const at::Tensor& q, const at::Tensor& k, co
   return op.call(q, k, v, pages, lengths, starts, scale, causal, window, cap, slopes, prefix, first);
 }
 
+at::Tensor fp8_chunk_attention_autograd(const at::Tensor& q, const at::Tensor& k,
+                                        const at::Tensor& scale_k, const at::Tensor& v,
+                                        const at::Tensor& scale_v, const at::Tensor& pages,
+                                        const at::Tensor& lengths, const at::Tensor& starts,
+                                        std::optional<double> scale, bool causal, int64_t window,
+                                        double cap, const std::optional<at::Tensor>& slopes,
+                                        const std::optional<at::Tensor>& prefix,
+                                        const std::optional<at::Tensor>& first) {
+  refuse_tracked("fp8_chunk_attention", {&q, &k, &scale_k, &v, &scale_v});
+  if (slopes.has_value() && slopes->defined()) refuse_tracked("fp8_chunk_attention", {&*slopes});
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("branchcraft::fp8_chunk_attention", "")
+                             .typed<decltype(fp8_chunk_attention_hip)>();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, scale_k, v, scale_v, pages, lengths, starts, scale, causal, window, cap, slopes,
+                 prefix, first);
+}
+
+at::Tensor shared_chunk_attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                           const at::Tensor& pages, const at::Tensor& lengths,
+                                           const at::Tensor& starts, const at::Tensor& groups,
+                                           const at::Tensor& shared, std::optional<double> scale,
+                                           bool causal, int64_t window, double cap,
+                                           const std::optional<at::Tensor>& slopes,
+                                           const std::optional<at::Tensor>& prefix,
+                                           const std::optional<at::Tensor>& first) {
+  refuse_tracked("shared_chunk_attention", {&q, &k, &v});
+  if (slopes.has_value() && slopes->defined()) refuse_tracked("shared_chunk_attention", {&*slopes});
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("branchcraft::shared_chunk_attention", "")
+                             .typed<decltype(shared_chunk_attention_hip)>();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, v, pages, lengths, starts, groups, shared, scale, causal, window, cap, slopes,
+                 prefix, first);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(branchcraft, m) {
@@ -679,6 +928,10 @@ TORCH_LIBRARY(branchcraft, m) {
   m.def("build_tables(Tensor page_ids, Tensor lengths, Tensor counts, int max_pages, int tokens) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("append_kv_(Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor k, Tensor v, Tensor slots) -> ()");
   m.def("chunk_attention(Tensor q, Tensor k, Tensor v, Tensor pages, Tensor lengths, Tensor starts, float? scale=None, bool causal=True, int window=0, float cap=0., Tensor? slopes=None, Tensor? prefix=None, Tensor? first=None) -> Tensor");
+  m.def("append_fp8_kv_(Tensor(a!) cache_k, Tensor(b!) scale_k, Tensor(c!) cache_v, Tensor(d!) scale_v, Tensor k, Tensor v, Tensor slots) -> ()");
+  m.def("read_fp8_kv(Tensor cache_k, Tensor scale_k, Tensor cache_v, Tensor scale_v, Tensor slots, ScalarType dtype) -> (Tensor, Tensor)");
+  m.def("fp8_chunk_attention(Tensor q, Tensor k, Tensor scale_k, Tensor v, Tensor scale_v, Tensor pages, Tensor lengths, Tensor starts, float? scale=None, bool causal=True, int window=0, float cap=0., Tensor? slopes=None, Tensor? prefix=None, Tensor? first=None) -> Tensor");
+  m.def("shared_chunk_attention(Tensor q, Tensor k, Tensor v, Tensor pages, Tensor lengths, Tensor starts, Tensor groups, Tensor shared, float? scale=None, bool causal=True, int window=0, float cap=0., Tensor? slopes=None, Tensor? prefix=None, Tensor? first=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(branchcraft, CUDA, m) {
@@ -693,17 +946,26 @@ TORCH_LIBRARY_IMPL(branchcraft, CUDA, m) {
   m.impl("build_tables", build_tables_hip);
   m.impl("append_kv_", append_kv_hip);
   m.impl("chunk_attention", chunk_attention_hip);
+  m.impl("append_fp8_kv_", append_fp8_kv_hip);
+  m.impl("read_fp8_kv", read_fp8_kv_hip);
+  m.impl("fp8_chunk_attention", fp8_chunk_attention_hip);
+  m.impl("shared_chunk_attention", shared_chunk_attention_hip);
 }
 
 TORCH_LIBRARY_IMPL(branchcraft, ADInplaceOrView, m) {
   m.impl("write_prefix_", write_prefix_versions);
   m.impl("append_kv_", append_kv_versions);
+  m.impl("append_fp8_kv_", append_fp8_kv_versions);
 }
 
 TORCH_LIBRARY_IMPL(branchcraft, Autograd, m) {
   m.impl("write_prefix_", write_prefix_autograd);
   m.impl("append_kv_", append_kv_autograd);
   m.impl("chunk_attention", chunk_attention_autograd);
+  m.impl("append_fp8_kv_", append_fp8_kv_autograd);
+  m.impl("read_fp8_kv", read_fp8_kv_autograd);
+  m.impl("fp8_chunk_attention", fp8_chunk_attention_autograd);
+  m.impl("shared_chunk_attention", shared_chunk_attention_autograd);
   // Whole numbers have no gradient: past autograd at once (0.8 of 8.7 us a call).
   m.impl("build_tables", torch::CppFunction::makeFallthrough());
 }

@@ -36,6 +36,9 @@ EXPORTED = (
     "bc_packed_decode_ws", "bc_packed_decode_noalloc", "bc_version",
     "bc_build_tables", "bc_append_kv", "bc_chunk_attention",
     "bc_chunk_attention_workspace_size",
+    "bc_append_fp8_kv", "bc_read_fp8_kv", "bc_fp8_chunk_attention",
+    "bc_fp8_chunk_attention_workspace_size", "bc_shared_chunk_attention",
+    "bc_shared_chunk_attention_workspace_size",
 )
 
 
@@ -73,6 +76,11 @@ class ChunkInputs(Structure):
                 ("q_strides", RowStrides), ("k_strides", PoolStrides),
                 ("v_strides", PoolStrides), ("tokens", c_int), ("dtype", c_int),
                 ("causal", c_int), ("window", c_int), ("scale", c_float), ("cap", c_float)]
+
+
+class Fp8Pool(Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("k_strides", PoolStrides), ("v_strides", PoolStrides)]
 
 
 _lib = None
@@ -139,6 +147,22 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
     lib.bc_chunk_attention.restype = c_int
     lib.bc_chunk_attention_workspace_size.argtypes = [Shape, c_int]
     lib.bc_chunk_attention_workspace_size.restype = c_size_t
+    lib.bc_append_fp8_kv.argtypes = [Shape, c_void_p, c_void_p, RowStrides, RowStrides, c_int,
+                                     Fp8Pool, c_void_p, c_int, c_void_p]
+    lib.bc_append_fp8_kv.restype = c_int
+    lib.bc_read_fp8_kv.argtypes = [Shape, Fp8Pool, c_void_p, c_int, c_int, c_void_p, c_void_p,
+                                   c_void_p]
+    lib.bc_read_fp8_kv.restype = c_int
+    lib.bc_fp8_chunk_attention.argtypes = [Shape, ChunkInputs, c_void_p, c_void_p, c_void_p,
+                                           c_size_t, c_void_p]
+    lib.bc_fp8_chunk_attention.restype = c_int
+    lib.bc_fp8_chunk_attention_workspace_size.argtypes = [Shape, c_int]
+    lib.bc_fp8_chunk_attention_workspace_size.restype = c_size_t
+    lib.bc_shared_chunk_attention.argtypes = [Shape, ChunkInputs, c_void_p, c_void_p, c_int,
+                                              c_void_p, c_size_t, c_void_p]
+    lib.bc_shared_chunk_attention.restype = c_int
+    lib.bc_shared_chunk_attention_workspace_size.argtypes = [Shape, c_int, c_int]
+    lib.bc_shared_chunk_attention_workspace_size.restype = c_size_t
     lib.bc_version.argtypes = []
     lib.bc_version.restype = c_char_p
     if path is None:
@@ -153,6 +177,6 @@ def shape(batch, query_heads, kv_heads, dim, max_pages, physical_pages) -> Shape
 __all__ = ["BC_SUCCESS", "BC_ERROR_INVALID_VALUE", "BC_ERROR_OUT_OF_MEMORY",
            "BC_STATIC_SCRATCH_BYTES", "BC_PAGE_SIZE", "BC_MAX_SPLITS",
            "BC_MAX_TREE_NODES", "EXPORTED", "Shape", "Inputs", "Scratch",
-           "TreeInputs", "RowStrides", "PoolStrides", "ChunkInputs", "BC_FLOAT16",
+           "TreeInputs", "RowStrides", "PoolStrides", "ChunkInputs", "Fp8Pool", "BC_FLOAT16",
            "BC_BFLOAT16", "load", "shape", "LIB_PATH", "POINTER", "c_int32",
            "c_uint16"]

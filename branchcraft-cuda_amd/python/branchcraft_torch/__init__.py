@@ -5,9 +5,10 @@ Importing this module loads ``_C.so`` (built in-tree by
 with the reference's schemas (bindings/torch_ops.cpp:144-148 of
 Haaziq386/branchcraft-cuda) plus ``paged_decode`` (the reference's C++
 ``branchcraft::decode``), ``copy_pages_``, ``commit_paths_`` and the chunk ops
-(``build_tables``, ``append_kv_``, ``chunk_attention``).  There is
-no CPU or Python fallback: a missing extension raises ImportError, and the
-ops have only a GPU implementation.
+(``build_tables``, ``append_kv_``, ``chunk_attention``), an 8-bit cache
+(``append_fp8_kv_``, ``read_fp8_kv``, ``fp8_chunk_attention``) and attention for
+forks (``shared_chunk_attention``).  There is no CPU or Python fallback: a missing
+extension raises ImportError, and the ops have only a GPU implementation.
 
 FakeTensor implementations follow python/branchcraft_torch/__init__.py:18-31
 of the reference so that ``torch.compile`` can trace the ops.
@@ -85,10 +86,37 @@ def _fake_chunk_attention(q, k, v, pages, lengths, starts, scale=None, causal=Tr
     return q.new_empty(q.shape)
 
 
+@torch.library.register_fake("branchcraft::append_fp8_kv_")
+def _fake_append_fp8_kv(cache_k, scale_k, cache_v, scale_v, k, v, slots):
+    return None
+
+
+@torch.library.register_fake("branchcraft::read_fp8_kv")
+def _fake_read_fp8_kv(cache_k, scale_k, cache_v, scale_v, slots, dtype):
+    size = (slots.shape[0], *cache_k.shape[2:])
+    return tuple(cache_k.new_empty(size, dtype=dtype) for _ in range(2))
+
+
+@torch.library.register_fake("branchcraft::fp8_chunk_attention")
+def _fake_fp8_chunk_attention(q, k, scale_k, v, scale_v, pages, lengths, starts, scale=None,
+                              causal=True, window=0, cap=0.0, slopes=None, prefix=None, first=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("branchcraft::shared_chunk_attention")
+def _fake_shared_chunk_attention(q, k, v, pages, lengths, starts, groups, shared, scale=None,
+                                 causal=True, window=0, cap=0.0, slopes=None, prefix=None, first=None):
+    return q.new_empty(q.shape)
+
+
 # The ops themselves: through the packet a call costs its host 0.4 us more.
 _build_tables = torch.ops.branchcraft.build_tables.default
 _append_kv = torch.ops.branchcraft.append_kv_.default
 _chunk_attention = torch.ops.branchcraft.chunk_attention.default
+_append_fp8_kv = torch.ops.branchcraft.append_fp8_kv_.default
+_read_fp8_kv = torch.ops.branchcraft.read_fp8_kv.default
+_fp8_chunk_attention = torch.ops.branchcraft.fp8_chunk_attention.default
+_shared_chunk_attention = torch.ops.branchcraft.shared_chunk_attention.default
 
 
 def tree_verify(q, prefix_k, prefix_v, pages, lengths, draft_k, draft_v, parent):
@@ -189,7 +217,46 @@ def chunk_attention(q, k, v, pages, lengths, starts, *, scale=None, causal=True,
                             prefix, first)
 
 
+def append_fp8_kv_(cache_k, scale_k, cache_v, scale_v, k, v, slots):
+    """Round new tokens' K and V rows (as ``append_kv_`` takes them) to 8 bits and
+    write them to the slots of an 8-bit cache: codes ``float8_e4m3fn`` [pages, 16,
+    KV heads, dim] (any strides of whole 16 bytes) and, contiguous, scales
+    ``float8_e8m0fnu`` [pages, KV heads, 16, dim / 32].  A value is its code times
+    the scale of its 32, the least power of two with which they stay within 448.
+    Infinities and NaN become NaN."""
+    return _append_fp8_kv(cache_k, scale_k, cache_v, scale_v, k, v, slots)
+
+
+def read_fp8_kv(cache_k, scale_k, cache_v, scale_v, slots, dtype):
+    """Rows of an 8-bit cache in FP16 or BF16, ``(k, v)``, each [len(slots), KV heads,
+    dim]; zeros for slots of -1 and outside the pool.  What was written from a type
+    comes back in it as exactly code times scale."""
+    return _read_fp8_kv(cache_k, scale_k, cache_v, scale_v, slots, dtype)
+
+
+def fp8_chunk_attention(q, k, scale_k, v, scale_v, pages, lengths, starts, *, scale=None, causal=True,
+                        window=0, cap=0.0, slopes=None, prefix=None, first=None):
+    """``chunk_attention`` over an 8-bit cache (see ``append_fp8_kv_``), in q's type,
+    to which the cache's values are rounded (exactly, where they were written from
+    it)."""
+    return _fp8_chunk_attention(q, k, scale_k, v, scale_v, pages, lengths, starts, scale, causal, window,
+                                cap, slopes, prefix, first)
+
+
+def shared_chunk_attention(q, k, v, pages, lengths, starts, groups, shared, *, scale=None, causal=True,
+                           window=0, cap=0.0, slopes=None, prefix=None, first=None):
+    """``chunk_attention`` for requests that begin alike, such as forks: requests
+    ``groups[g] .. groups[g+1] - 1`` have their first ``shared[g]`` tokens in pages
+    of the same contents, which are read once for all of them (those of the first
+    one).  ``groups`` (rising) and ``shared`` are int32 tensors on the GPU; requests
+    outside all groups share nothing.  The results are ``chunk_attention``'s up to
+    rounding."""
+    return _shared_chunk_attention(q, k, v, pages, lengths, starts, groups, shared, scale, causal, window,
+                                   cap, slopes, prefix, first)
+
+
 __all__ = ["tree_verify", "packed_decode_out", "paged_decode",
            "commit_path_", "copy_pages_", "commit_paths_", "write_prefix_", "int_tensor",
-           "build_tables", "append_kv_", "chunk_attention",
+           "build_tables", "append_kv_", "chunk_attention", "append_fp8_kv_", "read_fp8_kv",
+           "fp8_chunk_attention", "shared_chunk_attention",
            "LIBRARY_PATH"]

@@ -460,6 +460,80 @@ int bc_chunk_attention(bc_shape shape, bc_chunk_inputs in, void* workspace,
  * not aligned to 16 bytes is ignored: nothing is split then. */
 size_t bc_chunk_attention_workspace_size(bc_shape shape, int tokens);
 
+/* ---- caches of 8 bits ---- */
+
+/* Values of a head that share a power of two. */
+#define BC_FP8_BLOCK 32
+
+/* K and V of a paged cache in 8 bits.  Codes, e4m3 [P, 16, Hkv, D], in any order
+ * of pages, slots and heads (strides in bytes, multiples of 16; 16-byte aligned);
+ * scales, a byte for every 32 values of a head, contiguous [P, Hkv, 16, D / 32],
+ * so that those of a page and head lie side by side: byte x is 2^(x - 127).  A
+ * value is its code times its block's scale.  A pool of zeros holds zeros.  Scale
+ * bytes of 255 are never written; values read under one are not specified. */
+typedef struct bc_fp8_pool {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  bc_pool_strides k_strides;
+  bc_pool_strides v_strides;
+} bc_fp8_pool;
+
+/* New tokens' K and V rows ([tokens, Hkv, D] of `dtype`, any 2-byte aligned
+ * pointers and non-negative strides) into the slots of bc_build_tables, rounded
+ * to 8 bits: a block's scale is the least power of two, at least 2^-126, with
+ * which its finite values stay within 448, and a code is the e4m3 value nearest
+ * to value / scale, ties to even.  Infinities and NaN become NaN.  Values past
+ * 1.875 * 2^15 in FP16, and 1.875 * 2^127 in BF16, count as that (they would round
+ * to a power of two that the type does not have), so that rows of a type are read
+ * back, in that type, as exactly code * scale.
+ * Negative slots and slots of pages outside [0, physical_pages) are skipped; two
+ * rows of one slot leave either row or a mixture.  Uses shape.kv_heads, dim and
+ * physical_pages; rejects what bc_append_kv rejects, unaligned pools, and strides
+ * of theirs that are not multiples of 16. */
+int bc_append_fp8_kv(bc_shape shape, const bc_half* k, const bc_half* v,
+                     bc_row_strides k_strides, bc_row_strides v_strides, int dtype,
+                     bc_fp8_pool pool, const int32_t* slots, int tokens, bc_stream_t stream);
+
+/* The rows of `slots` back in `dtype`: k and v, contiguous [tokens, Hkv, D],
+ * 16-byte aligned.  Slots outside the pool give zeros.  Values of BF16 rows that
+ * are past FP16 become infinite in FP16, and small ones are rounded. */
+int bc_read_fp8_kv(bc_shape shape, bc_fp8_pool pool, const int32_t* slots, int tokens,
+                   int dtype, bc_half* k, bc_half* v, bc_stream_t stream);
+
+/* bc_chunk_attention over a cache of 8 bits: in.k and in.v are the codes and
+ * in.k_strides and in.v_strides their strides in bytes (see bc_fp8_pool; the same
+ * alignment is asked for), q, the output and the arithmetic are of in.dtype, to
+ * which the values of K and V are rounded (exactly, where they were written from
+ * it).  Everything else as there. */
+int bc_fp8_chunk_attention(bc_shape shape, bc_chunk_inputs in, const uint8_t* k_scale,
+                           const uint8_t* v_scale, void* workspace, size_t workspace_bytes,
+                           bc_stream_t stream);
+
+/* Bytes of workspace for it, as bc_chunk_attention_workspace_size. */
+size_t bc_fp8_chunk_attention_workspace_size(bc_shape shape, int tokens);
+
+/* ---- requests that begin with the same pages ---- */
+
+/* bc_chunk_attention for forks: the requests groups[g] .. groups[g+1] - 1 have
+ * their first shared[g] tokens in common, in pages of the same contents, of which
+ * those in the first one's row of `pages` are read, once for all of them.
+ * groups [group_count + 1] must rise, within [0, batch]; requests outside them
+ * share nothing, and neither does a group of one.  shared [group_count] need not
+ * be whole pages; at most the table's row counts.  Rows see what they see in
+ * bc_chunk_attention, and the results differ from its by rounding alone.  Without
+ * a workspace, and in the cases that go row by row there, every request's own row
+ * of `pages` is read instead.  Also rejects: group_count < 0 or over batch, null
+ * groups, null shared with groups. */
+int bc_shared_chunk_attention(bc_shape shape, bc_chunk_inputs in, const int32_t* groups,
+                              const int32_t* shared, int group_count, void* workspace,
+                              size_t workspace_bytes, bc_stream_t stream);
+
+/* Bytes of workspace with which it reads shared pages once; 0 where it never
+ * does. */
+size_t bc_shared_chunk_attention_workspace_size(bc_shape shape, int tokens, int group_count);
+
 /* Library version string, for logs. */
 const char* bc_version(void);
 
