@@ -311,8 +311,10 @@ __device__ __forceinline__ void pin_plan(const TileParams& P) {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+template <bool FP8>
 __device__ __forceinline__ void pin_rows(const TileParams& P) {
   const ChunkParams& C = P.c;
+  if constexpr (FP8) asm volatile("" ::"s"(C.k_scale), "s"(C.v_scale), "s"(C.hkv));
   asm volatile("" ::"s"(C.q), "s"(C.k), "s"(C.v), "s"(C.pages), "s"(C.slopes), "s"(C.first),
                "s"(C.qt), "s"(C.qh), "s"(C.kp), "s"(C.ks), "s"(C.kh), "s"(C.vp), "s"(C.vs),
                "s"(C.vh), "s"(C.group), "s"(C.group_mul), "s"(C.max_pages), "s"(C.phys_pages),
@@ -744,9 +746,22 @@ __device__ __forceinline__ bool tidy(u32x4* at, bool real) {
   return real;
 }
 
+// The same of 16 bytes on their way into LDS.
+template <typename T>
+__device__ __forceinline__ bool tidy_value(u32x4& w, bool real) {
+  uint32_t all = 0;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const uint32_t odd = ((w[x] & 0x7fff7fffu) + Num<T>::kCarry) & 0x80008000u;
+    all |= odd;
+    w[x] = real ? w[x] & ~((odd >> 15) * 0xffffu) : 0u;
+  }
+  return real && all;
+}
+
 // What tidy() took out of the tokens t0 .. t0 + count - 1, added to the rows
 // that see it.  Rare, so token by token and from the cache.
-template <typename T, int D>
+template <typename T, int D, bool FP8>
 __device__ __forceinline__ void add_untidy(const ChunkParams& C, const Request& it, int kvh, Rows<D>& R,
                                            int t0, int count, int g) {
   const int32_t* const table = C.pages + (size_t)it.b * C.max_pages;
@@ -755,12 +770,22 @@ __device__ __forceinline__ void add_untidy(const ChunkParams& C, const Request& 
     const int p = table[j >> 4];
     if ((unsigned)p >= (unsigned)C.phys_pages) continue;
     const bool seen = j >= R.lo && j <= R.hi;
-    const uint16_t* const v = C.v + p * C.vp + (j & 15) * C.vs + kvh * C.vh + 4 * g;
+    const long long at = p * C.vp + (j & 15) * C.vs + kvh * C.vh + 4 * g;
+    const uint16_t* const v = C.v + (FP8 ? 0 : at);
+    const uint8_t* const codes = reinterpret_cast<const uint8_t*>(C.v) + (FP8 ? at : 0);
+    const uint8_t* const scales = FP8 ? C.v_scale + scale_at<D>(C, p, kvh, j & 15) : nullptr;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
       for (int jq = 0; jq < 4; ++jq) {
-        const uint2 w = *reinterpret_cast<const uint2*>(v + 32 * dt + 8 * jq);
+        uint2 w;
+        if constexpr (FP8) {
+          const uint32_t four = *reinterpret_cast<const uint32_t*>(codes + 32 * dt + 8 * jq);
+          const float power = power_of(scales[dt]);
+          w = make_uint2(values2<T, false>(four, power), values2<T, true>(four, power));
+        } else {
+          w = *reinterpret_cast<const uint2*>(v + 32 * dt + 8 * jq);
+        }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const float f = to_float(__builtin_bit_cast(T, (uint16_t)((x < 2 ? w.x : w.y) >> (16 * (x & 1)))));
@@ -785,20 +810,50 @@ __device__ __forceinline__ unsigned long long tokens_of(int left, int pages) {
 // The pages of a wave's next 64, one per lane: their addresses, so that a tile
 // reads them out instead of multiplying, and which lie in the pool (others
 // are loaded from page 0 and masked).
+template <bool FP8>
 struct Pages {
   unsigned long long k, v, in_pool;
-  __device__ __forceinline__ void take(const ChunkParams& C, int kvh, int id) {
-    const bool in = (unsigned)id < (unsigned)C.phys_pages;
+  int id;
+  __device__ __forceinline__ void take(const ChunkParams& C, int kvh, int page_id) {
+    const bool in = (unsigned)page_id < (unsigned)C.phys_pages;
     in_pool = __builtin_amdgcn_ballot_w64(in);
-    const long long page = in ? id : 0;
-    k = (unsigned long long)(C.k + kvh * C.kh + page * C.kp);
-    v = (unsigned long long)(C.v + kvh * C.vh + page * C.vp);
+    id = in ? page_id : 0;
+    const long long page = id;
+    if constexpr (FP8) {
+      k = (unsigned long long)C.k + kvh * C.kh + page * C.kp;
+      v = (unsigned long long)C.v + kvh * C.vh + page * C.vp;
+    } else {
+      k = (unsigned long long)(C.k + kvh * C.kh + page * C.kp);
+      v = (unsigned long long)(C.v + kvh * C.vh + page * C.vp);
+    }
   }
   static __device__ __forceinline__ const void* at(unsigned long long x, int lane) {
     const unsigned hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
     return (const void*)((unsigned long long)hi << 32 | (unsigned)__builtin_amdgcn_readlane((int)x, lane));
   }
 };
+
+// Sixteen codes of a page, `off` bytes from its wave-uniform address.
+__device__ __forceinline__ u32x4 load_codes(const void* page, unsigned off) {
+  typedef const __attribute__((address_space(1))) char* Bytes;
+  return __builtin_nontemporal_load((const __attribute__((address_space(1))) u32x4*)((Bytes)page + off));
+}
+
+// Sixteen codes of row `row` of a tile into LDS, as the 16-byte chunks 2 c and
+// 2 c + 1 of its values.
+template <typename T, int D>
+__device__ __forceinline__ void put_values(const u32x4& lo, const u32x4& hi, uint16_t* tile, int row, int c) {
+  *reinterpret_cast<u32x4*>(tile + row * D + ((2 * c) ^ swz<D>(row)) * 8) = lo;
+  *reinterpret_cast<u32x4*>(tile + row * D + ((2 * c + 1) ^ swz<D>(row)) * 8) = hi;
+}
+
+template <typename T>
+__device__ __forceinline__ void values16(const u32x4& w, float power, u32x4& lo, u32x4& hi) {
+  lo = u32x4{values2<T, false>(w[0], power), values2<T, true>(w[0], power), values2<T, false>(w[1], power),
+             values2<T, true>(w[1], power)};
+  hi = u32x4{values2<T, false>(w[2], power), values2<T, true>(w[2], power), values2<T, false>(w[3], power),
+             values2<T, true>(w[3], power)};
+}
 
 // This lane's row of the wave's 32: its place, what it sees, and its Q.
 template <typename T, int D, Form FORM>
@@ -905,7 +960,7 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
 //    over 2048, sixteen of them: 180 us, 670 TFLOP/s).
 //  - A full round of workgroups takes 8.6 us, launch included, and 2.1 per step
 //    (2048 new tokens over 2048 to 32768, none masked: 75.8 to 1082 us).
-template <typename T, int D, Form FORM>
+template <typename T, int D, Form FORM, bool FP8>
 __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const Item& it, int kvh,
                                           uint16_t* s_kv, Seen* s_seen, int* s_bad) {
   const ChunkParams& C = A.c;
@@ -966,11 +1021,49 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   const unsigned voff = (unsigned)(((lrow % BC_PAGE_SIZE) * C.vs + lcol) * 2);
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(
       (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)s_kv + wave * 1024);
-  Pages pg;
+  Pages<FP8> pg;
+  // An 8-bit cache's step goes through registers: codes and their powers are
+  // loaded where loads into LDS would be issued, and converted into LDS behind the
+  // step's product.
+  constexpr int CPR8 = D / 16, NX8 = kStep * CPR8 / 256;  // of 16 codes
+  const int crow = tid / CPR8, ccol = tid % CPR8;
+  const unsigned kcode = (unsigned)((crow % BC_PAGE_SIZE) * C.ks + ccol * 16);
+  const unsigned vcode = (unsigned)((crow % BC_PAGE_SIZE) * C.vs + ccol * 16);
+  u32x4 kc[NX8], vc[NX8];
+  uint32_t kx[NX8], vx[NX8];
+  auto fetch = [&](int x, int at) {
+    const int from = 4 * at + (CPR8 == 8 ? 2 * x + (wave >> 1) : wave);
+    kc[x] = load_codes(Pages<FP8>::at(pg.k, from), kcode);
+    vc[x] = load_codes(Pages<FP8>::at(pg.v, from), vcode);
+    const int page = __builtin_amdgcn_readlane(pg.id, from);
+    const size_t scales = scale_at<D>(C, page, kvh, 0);
+    const unsigned off = (crow % BC_PAGE_SIZE) * (D / kFp8Block) + ccol / 2;
+    kx[x] = C.k_scale[scales + off];
+    vx[x] = C.v_scale[scales + off];
+  };
+  // ... and what inspect() does; `whole`: nothing.
+  auto put = [&](int buf, bool whole, unsigned long long ok) {
+    uint16_t* const k = s_kv + buf * (2 * HALF);
+    bool bad = false;
+#pragma unroll
+    for (int x = 0; x < NX8; ++x) {
+      const int row = crow + 256 / CPR8 * x;
+      u32x4 lo, hi;
+      values16<T>(kc[x], power_of(kx[x]), lo, hi);
+      put_values<T, D>(lo, hi, k, row, ccol);
+      values16<T>(vc[x], power_of(vx[x]), lo, hi);
+      if (!whole) {
+        bad |= tidy_value<T>(lo, (ok >> row) & 1u);
+        bad |= tidy_value<T>(hi, (ok >> row) & 1u);
+      }
+      put_values<T, D>(lo, hi, k + HALF, row, ccol);
+    }
+    return bad;
+  };
   auto issue_chunk = [&](int x, int at, int buf) {
     const int from = 4 * at + (CPR == 16 ? x : 2 * x + (wave >> 1));
     const unsigned dst = lds0 + buf * (4 * HALF) + x * 4096;
-    load2_to_lds(Pages::at(pg.k, from), Pages::at(pg.v, from), koff, voff, dst, dst + 2 * HALF);
+    load2_to_lds(Pages<FP8>::at(pg.k, from), Pages<FP8>::at(pg.v, from), koff, voff, dst, dst + 2 * HALF);
   };
   // Steps whole_lo .. whole_hi - 1 are seen whole by every row, given their pages.
   const int whole_lo = wg.all_lo / kStep + (wg.all_lo % kStep != 0);
@@ -994,11 +1087,19 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   if (t0 < tend) {
     pg.take(C, kvh, ids);
 #pragma unroll
-    for (int x = 0; x < NX; ++x) issue_chunk(x, 0, 0);
+    for (int x = 0; x < (FP8 ? NX8 : NX); ++x)
+      if constexpr (FP8)
+        fetch(x, 0);
+      else
+        issue_chunk(x, 0, 0);
     pages = (int)pg.in_pool & 15;
     const bool whole = pages == 15 && t0 >= whole_lo && t0 < whole_hi;
-    wait_loads();
-    if (!whole) bad = inspect(tokens_of<4>(rq.len - t0 * kStep, pages), s_kv + HALF);
+    if constexpr (FP8) {
+      bad = put(0, whole, tokens_of<4>(rq.len - t0 * kStep, pages));
+    } else {
+      wait_loads();
+      if (!whole) bad = inspect(tokens_of<4>(rq.len - t0 * kStep, pages), s_kv + HALF);
+    }
     bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));
   }
   // The wait for Q belongs here, on every path into the loop: at its first use
@@ -1031,8 +1132,12 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         sc[i] = Num<T>::mfma(kf[i][s], qB[s], FORM != Form::kBias && s == 0 ? zero : sc[i]);
-      if (s % 2 == 1 && s / 2 < NX) {
-        if (next) issue_chunk(s / 2, at, buf ^ 1);
+      if (s % 2 == 1 && s / 2 < (FP8 ? NX8 : NX)) {
+        if constexpr (FP8) {
+          if (next) fetch(s / 2, at);
+        } else {
+          if (next) issue_chunk(s / 2, at, buf ^ 1);
+        }
       }
     }
     Edges e{t * kStep < mine.all_lo, t * kStep + kStep - 1 > mine.all_hi, pages != 15, 0};
@@ -1046,15 +1151,19 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     if (kAhead) __builtin_amdgcn_s_setprio(2);
     weigh<T, D, 2>(sc, R, kt + HALF, o, scale2);
     if (kAhead) __builtin_amdgcn_s_setprio(0);
-    if (bad) add_untidy<T, D>(C, rq, kvh, R, t * kStep, kStep, g);
-    wait_loads();
+    if (bad) add_untidy<T, D, FP8>(C, rq, kvh, R, t * kStep, kStep, g);
+    if constexpr (!FP8) wait_loads();
     // Step s of the part sets flag s % 4 before the barrier that ends the step
     // before it; the flag is read behind that barrier and cleared behind the
     // next, two barriers before it is set again.
     const int s = t - t0;
-    if (!whole_n && inspect(tokens_of<4>(rq.len - (t + 1) * kStep, pages_n),
-                            s_kv + (buf ^ 1) * (2 * HALF) + HALF))
+    if constexpr (FP8) {
+      if (next && put(buf ^ 1, whole_n, tokens_of<4>(rq.len - (t + 1) * kStep, pages_n)))
+        s_bad[(s + 1) & 3] = 1;
+    } else if (!whole_n && inspect(tokens_of<4>(rq.len - (t + 1) * kStep, pages_n),
+                                   s_kv + (buf ^ 1) * (2 * HALF) + HALF)) {
       s_bad[(s + 1) & 3] = 1;
+    }
     __syncthreads();
     if (bad && tid == 0) s_bad[s & 3] = 0;
     bad = !whole_n && __builtin_amdgcn_readfirstlane(s_bad[(s + 1) & 3]);
@@ -1147,7 +1256,7 @@ struct Stream {
   uint16_t* kt;
   unsigned lds0, koff[NV], voff[NV];
   Offsets<D> o;
-  Pages pg;
+  Pages<false> pg;
 
   __device__ __forceinline__ Stream(const ChunkParams& c, int head, uint16_t* area)
       : C(c), kvh(head), lane(threadIdx.x & 63), kt(area), o(read_offsets<D>(threadIdx.x & 63)) {
@@ -1167,7 +1276,7 @@ struct Stream {
   }
   __device__ __forceinline__ void issue(unsigned long long x, int at, const unsigned (&off)[NV],
                                         unsigned dst) const {
-    stream_to_lds<NV>(Pages::at(x, 2 * at), Pages::at(x, 2 * at + 1), off, dst);
+    stream_to_lds<NV>(Pages<false>::at(x, 2 * at), Pages<false>::at(x, 2 * at + 1), off, dst);
   }
   __device__ __forceinline__ void issue_k(int at) const { issue(pg.k, at, koff, lds0); }
   __device__ __forceinline__ void issue_v(int at) const { issue(pg.v, at, voff, lds0 + 2 * TILE); }
@@ -1203,10 +1312,111 @@ struct Stream {
       wave_lds_sync();
     }
     weigh<T, D, 1>(sc, R, vt, o, scale2_of(C, FORM));
-    if (bad) add_untidy<T, D>(C, rq, kvh, R, t * 32, 32, g);
+    if (bad) add_untidy<T, D, false>(C, rq, kvh, R, t * 32, 32, g);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 };
+
+// The same over an 8-bit cache.  Codes come into registers, those of K for the
+// next tile behind the scores, of V behind the product, and are converted into LDS
+// ahead of their use, where the rest is as for 16 bits.  A lane's load has 16 codes
+// of a row; the powers of a tile, 32 rows of K and 32 of V, come a row per lane in
+// one load, from where the lanes take their row's.
+template <typename T, int D, Form FORM>
+struct Stream8 {
+  static constexpr int KS = D / 16, CPR = D / 16;
+  static constexpr int RPL = 64 / CPR;  // token rows per load
+  static constexpr int NL = 32 / RPL;   // loads per tile, of K and of V each
+  static constexpr int NP = NL / 2;     // loads per page
+  static constexpr int TILE = 32 * D;
+  static_assert(NP * RPL == BC_PAGE_SIZE, "a tile is two pages");
+  typedef typename std::conditional<D == 128, uint32_t, uint16_t>::type Powers;
+
+  const ChunkParams& C;
+  int kvh, lane;
+  uint16_t* kt;
+  unsigned koff[NP], voff[NP];
+  Offsets<D> o;
+  Pages<true> pg;
+  u32x4 k[NL], v[NL];
+  uint32_t powers, powers_next;  // of the tile at hand, and of the one on its way
+
+  __device__ __forceinline__ Stream8(const ChunkParams& c, int head, uint16_t* area)
+      : C(c), kvh(head), lane(threadIdx.x & 63), kt(area), o(read_offsets<D>(threadIdx.x & 63)) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int row = i * RPL + lane / CPR, col = lane % CPR * 16;
+      koff[i] = (unsigned)(row * C.ks + col);
+      voff[i] = (unsigned)(row * C.vs + col);
+    }
+  }
+  __device__ __forceinline__ int ids(int b, int t, int apart) const {
+    const int i = 2 * (t + apart * (lane >> 1)) + (lane & 1);
+    return C.pages[(size_t)b * C.max_pages + min(i, C.max_pages - 1)];
+  }
+  __device__ __forceinline__ void issue_k(int at) {
+    const int page = __shfl(pg.id, 2 * at + ((lane >> 4) & 1), 64);
+    const uint8_t* const scales = lane < 32 ? C.k_scale : C.v_scale;
+    powers_next = *reinterpret_cast<const Powers*>(scales + scale_at<D>(C, page, kvh, lane & 15));
+#pragma unroll
+    for (int i = 0; i < NL; ++i) k[i] = load_codes(Pages<true>::at(pg.k, 2 * at + i / NP), koff[i % NP]);
+  }
+  __device__ __forceinline__ void issue_v(int at) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) v[i] = load_codes(Pages<true>::at(pg.v, 2 * at + i / NP), voff[i % NP]);
+  }
+  __device__ __forceinline__ int in_pool(int at) const { return (int)(pg.in_pool >> (2 * at)) & 3; }
+
+  __device__ __forceinline__ float power(int row) const {  // of this lane's codes of row `row` (V's from 32)
+    return power_of(((uint32_t)__shfl((int)powers, row, 64) >> (8 * (lane % CPR / 2))) & 255u);
+  }
+
+  __device__ __forceinline__ void scores(f32x16 (&sc)[1], const u32x4 (&qB)[KS], const Rows<D>& R, int t) {
+    powers = powers_next;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = i * RPL + lane / CPR;
+      u32x4 lo, hi;
+      values16<T>(k[i], power(row), lo, hi);
+      put_values<T, D>(lo, hi, kt, row, lane % CPR);
+    }
+    wave_lds_sync();
+    const f32x16 zero = {};
+    if (FORM == Form::kBias) start_scores<D, 1>(C, sc, R, t * 32, lane >> 5);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      sc[0] = Num<T>::mfma(lds16(kt + o.k[s]), qB[s], FORM != Form::kBias && s == 0 ? zero : sc[0]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  __device__ __forceinline__ void product(f32x16 (&sc)[1], const Request& rq, Rows<D>& R, const Seen& mine,
+                                          int t, int pages, bool) {
+    const int g = lane >> 5, left = rq.len - t * 32;
+    uint16_t* const vt = kt + TILE;
+    const Edges e{t * 32 < mine.all_lo, t * 32 + 31 > mine.all_hi, pages != 3, tokens_of<2>(left, pages)};
+    finish_scores<D, FORM, 1>(C, sc, R, t * 32, g, e);
+    const bool edge = e.lo || e.hi || e.pages || left < 32;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = i * RPL + lane / CPR;
+      u32x4 lo, hi;
+      values16<T>(v[i], power(32 + row), lo, hi);
+      if (edge) {
+        bad |= tidy_value<T>(lo, (e.valid >> row) & 1u);
+        bad |= tidy_value<T>(hi, (e.valid >> row) & 1u);
+      }
+      put_values<T, D>(lo, hi, vt, row, lane % CPR);
+    }
+    bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+    wave_lds_sync();
+    weigh<T, D, 1>(sc, R, vt, o, scale2_of(C, FORM));
+    if (bad) add_untidy<T, D, true>(C, rq, kvh, R, t * 32, 32, g);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+};
+
+template <typename T, int D, Form FORM, bool FP8>
+using StreamOf = typename std::conditional<FP8, Stream8<T, D, FORM>, Stream<T, D, FORM>>::type;
 
 // The narrow form over a batch: the tiles of all requests with few rows, one
 // after another, in ranges of equal length, a range per wave.  HBM-bound: 64
@@ -1218,7 +1428,7 @@ struct Stream {
 // range leaves a partial.  Range r's partial of a request whose predecessors
 // have n rows starts at partial row 32 r + n: a range's next request is
 // further by the rows of the last one, a request's next range by 32.
-template <typename T, int D, Form FORM>
+template <typename T, int D, Form FORM, bool FP8>
 __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cutting& cut,
                                           uint16_t* s_kv) {
   const ChunkParams& C = P.c;
@@ -1270,7 +1480,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
 
   Part p;
   if (!next_part(p)) return;
-  Stream<T, D, FORM> st(C, kvh, s_kv + wave * (64 * D));
+  StreamOf<T, D, FORM, FP8> st(C, kvh, s_kv + wave * (64 * D));
   int t = first_of(p), at = 0;
   st.pg.take(C, kvh, st.ids(p.rq.b, t, 1));
   int ids_next = st.ids(p.rq.b, t + 32, 1);
@@ -1349,7 +1559,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
 
 // The narrow form without a workspace: a workgroup per request and KV head,
 // its waves every fourth tile each; the four states meet at the end.
-template <typename T, int D, Form FORM>
+template <typename T, int D, Form FORM, bool FP8>
 __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request& rq, int kvh,
                                             uint16_t* s_kv, float2* s_ml) {
   constexpr int TILE = 32 * D;
@@ -1360,7 +1570,7 @@ __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request&
   u32x4 qB[D / 16];
   load_rows<T, D, FORM>(C, rq, lr, kvh, g, R, qB);
   const Seen mine = C.first ? wave_seen(R, lr < rq.rows) : rows_seen(C, rq, 0, rq.rows);
-  Stream<T, D, FORM> st(C, kvh, s_kv + wave * (2 * TILE));
+  StreamOf<T, D, FORM, FP8> st(C, kvh, s_kv + wave * (2 * TILE));
   int t = mine.any_hi < mine.any_lo ? 1 : mine.any_lo / 32 + wave;
   const int tend = mine.any_hi < mine.any_lo ? 0 : mine.any_hi / 32 + 1;
   if (t < tend) {
@@ -1440,7 +1650,7 @@ __device__ __forceinline__ void clear_rows(const ChunkParams& C, long long at, l
     out[x < head * row ? x : x + gap] = u32x4{0, 0, 0, 0};
 }
 
-template <typename T, int D, Form FORM>
+template <typename T, int D, Form FORM, bool FP8>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TileParams) {
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[2 * 2 * kStep * D];
   __shared__ float2 s_ml[4 * 32];
@@ -1468,8 +1678,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
   if (counts && threadIdx.x == 0) P.records[0] = make_int4(it.records, it.narrow_records, 0, 0);
   if (flat) {
     const TileParams& A = reread(args);
-    pin_rows(A);
-    flat_body<T, D, FORM>(A, head, cut, s_kv);
+    pin_rows<FP8>(A);
+    flat_body<T, D, FORM, FP8>(A, head, cut, s_kv);
     return;
   }
   if (!it.found) {
@@ -1482,11 +1692,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
                min(it.r.rows - it.tile * kManyRows, kManyRows), it.parts,
                P.narrow_rows + it.slot * P.part_rows, P.part_rows);
   const TileParams& A = reread(args);
-  pin_rows(A);
+  pin_rows<FP8>(A);
   if (it.r.rows <= kFewRows)
-    narrow_body<T, D, FORM>(A.c, it.r, kvh, s_kv, s_ml);
+    narrow_body<T, D, FORM, FP8>(A.c, it.r, kvh, s_kv, s_ml);
   else
-    wide_body<T, D, FORM>(A, args, it, kvh, s_kv, s_seen, s_bad);
+    wide_body<T, D, FORM, FP8>(A, args, it, kvh, s_kv, s_seen, s_bad);
 }
 
 // One part's state joined to another's.
@@ -1610,7 +1820,7 @@ inline Cut cut_of(const bc_shape& s, int tokens) {
   return c;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool FP8>
 hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned grid,
                         hipStream_t st) {
   TileParams P{};
@@ -1627,11 +1837,11 @@ hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned
     P.narrow_rows = cut.narrow_rows;
   }
   if (C.cap > 0.f)
-    chunk_tile_kernel<T, D, Form::kCap><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kCap, FP8><<<dim3(grid), 256, 0, st>>>(P);
   else if (C.slopes)
-    chunk_tile_kernel<T, D, Form::kBias><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kBias, FP8><<<dim3(grid), 256, 0, st>>>(P);
   else
-    chunk_tile_kernel<T, D, Form::kPlain><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kPlain, FP8><<<dim3(grid), 256, 0, st>>>(P);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !ws) return err;
   // Enough workgroups for the rows of a record and KV head, on average, but not
@@ -1644,6 +1854,16 @@ hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned
   const long long grid_join = most < 2 * cut.target ? most : 2 * cut.target;
   chunk_join_kernel<T, D><<<dim3((unsigned)grid_join), 256, 0, st>>>(P, (int)apart);
   return hipGetLastError();
+}
+
+template <bool FP8>
+hipError_t launch_tiles(const ChunkParams& P, int dim, int dtype, const Cut& cut, void* ws, long long grid,
+                        hipStream_t st) {
+  if (dtype == BC_FLOAT16)
+    return dim == 64 ? launch_tiles<_Float16, 64, FP8>(P, cut, ws, (unsigned)grid, st)
+                     : launch_tiles<_Float16, 128, FP8>(P, cut, ws, (unsigned)grid, st);
+  return dim == 64 ? launch_tiles<__bf16, 64, FP8>(P, cut, ws, (unsigned)grid, st)
+                   : launch_tiles<__bf16, 128, FP8>(P, cut, ws, (unsigned)grid, st);
 }
 
 // Workgroups of the tile kernel, at most.

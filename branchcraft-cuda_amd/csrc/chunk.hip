@@ -222,12 +222,6 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
                      stride_bits(in) % 8 == 0 && in.k_strides.slot < far && in.v_strides.slot < far &&
                      rows <= 1 << 30 && grid <= kMostGroups;
   void* const ws = use ? workspace : nullptr;
-  if (tiled) {
-    if (in.dtype == BC_FLOAT16)
-      return s.dim == 64 ? launch_tiles<_Float16, 64>(P, cut, ws, (unsigned)grid, st)
-                         : launch_tiles<_Float16, 128>(P, cut, ws, (unsigned)grid, st);
-    return s.dim == 64 ? launch_tiles<__bf16, 64>(P, cut, ws, (unsigned)grid, st)
-                       : launch_tiles<__bf16, 128>(P, cut, ws, (unsigned)grid, st);
-  }
+  if (tiled) return launch_tiles<false>(P, s.dim, in.dtype, cut, ws, grid, st);
   return launch_rows<false>(P, s.dim, in.dtype, st);
 }

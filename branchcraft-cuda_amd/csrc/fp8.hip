@@ -236,7 +236,9 @@ extern "C" int bc_read_fp8_kv(bc_shape s, bc_fp8_pool pool, const int32_t* slots
   return BC_SUCCESS;
 }
 
-extern "C" size_t bc_fp8_chunk_attention_workspace_size(bc_shape, int) { return 0; }
+extern "C" size_t bc_fp8_chunk_attention_workspace_size(bc_shape s, int tokens) {
+  return chunk_shape_ok(s, tokens) ? cut_of(s, tokens).bytes : 0;
+}
 
 extern "C" int bc_fp8_chunk_attention(bc_shape s, bc_chunk_inputs in, const uint8_t* k_scale,
                                       const uint8_t* v_scale, void* workspace,
@@ -245,11 +247,26 @@ extern "C" int bc_fp8_chunk_attention(bc_shape s, bc_chunk_inputs in, const uint
     return BC_ERROR_INVALID_VALUE;
   const long long pool_bits = in.k_strides.page | in.k_strides.slot | in.k_strides.head |
                               in.v_strides.page | in.v_strides.slot | in.v_strides.head;
-  if (!aligned16(in.k) || !aligned16(in.v) || pool_bits % 16 != 0) return BC_ERROR_INVALID_VALUE;
+  // Powers are read four at a time (two at D = 64).
+  const uintptr_t scales = reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale);
+  if (!aligned16(in.k) || !aligned16(in.v) || pool_bits % 16 != 0 || scales % 4 != 0)
+    return BC_ERROR_INVALID_VALUE;
   if (in.tokens == 0) return BC_SUCCESS;
   if (!in.q || !in.output) return BC_ERROR_INVALID_VALUE;
   ChunkParams P = chunk_params(s, in);
   P.k_scale = k_scale;
   P.v_scale = v_scale;
-  return launch_rows<true>(P, s.dim, in.dtype, reinterpret_cast<hipStream_t>(stream));
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  // As in bc_chunk_attention.
+  const Cut cut = cut_of(s, in.tokens);
+  const bool use = cut.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= cut.bytes;
+  const long long grid = tile_grid(s, in.tokens, cut, use);
+  const long long far = 1 << 27;  // bytes: offsets inside a page are 32-bit
+  const bool tiled = aligned16(in.q) && aligned16(in.output) &&
+                     (in.q_strides.token | in.q_strides.head) % 8 == 0 && in.k_strides.slot < far &&
+                     in.v_strides.slot < far && (long long)in.tokens * P.group <= 1 << 30 &&
+                     grid <= kMostGroups;
+  void* const ws = use ? workspace : nullptr;
+  if (tiled) return launch_tiles<true>(P, s.dim, in.dtype, cut, ws, grid, st);
+  return launch_rows<true>(P, s.dim, in.dtype, st);
 }
