@@ -1132,12 +1132,14 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         sc[i] = Num<T>::mfma(kf[i][s], qB[s], FORM != Form::kBias && s == 0 ? zero : sc[i]);
-      if (s % 2 == 1 && s / 2 < (FP8 ? NX8 : NX)) {
-        if constexpr (FP8) {
-          if (next) fetch(s / 2, at);
-        } else {
-          if (next) issue_chunk(s / 2, at, buf ^ 1);
-        }
+      if (!FP8 && s % 2 == 1 && s / 2 < NX) {
+        if (next) issue_chunk(s / 2, at, buf ^ 1);
+      }
+    }
+    if constexpr (FP8) {
+      if (next) {
+#pragma unroll
+        for (int x = 0; x < NX8; ++x) fetch(x, at);
       }
     }
     Edges e{t * kStep < mine.all_lo, t * kStep + kStep - 1 > mine.all_hi, pages != 15, 0};
@@ -1317,9 +1319,9 @@ struct Stream {
   }
 };
 
-// The same over an 8-bit cache.  Codes come into registers, those of K for the
-// next tile behind the scores, of V behind the product, and are converted into LDS
-// ahead of their use, where the rest is as for 16 bits.  A lane's load has 16 codes
+// The same over an 8-bit cache.  Codes come into registers and are converted into
+// LDS ahead of their use, where the rest is as for 16 bits; the next tile's go out
+// as soon as that has freed their registers.  A lane's load has 16 codes
 // of a row; the powers of a tile, 32 rows of K and 32 of V, come a row per lane in
 // one load, from where the lanes take their row's.
 template <typename T, int D, Form FORM>
@@ -1371,7 +1373,9 @@ struct Stream8 {
     return power_of(((uint32_t)__shfl((int)powers, row, 64) >> (8 * (lane % CPR / 2))) & 255u);
   }
 
-  __device__ __forceinline__ void scores(f32x16 (&sc)[1], const u32x4 (&qB)[KS], const Rows<D>& R, int t) {
+  // As in Stream, but for the next tile's loads, which these issue (`next`, at `at`).
+  __device__ __forceinline__ void scores(f32x16 (&sc)[1], const u32x4 (&qB)[KS], const Rows<D>& R, int t,
+                                         bool next, int at) {
     powers = powers_next;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -1380,6 +1384,7 @@ struct Stream8 {
       values16<T>(k[i], power(row), lo, hi);
       put_values<T, D>(lo, hi, kt, row, lane % CPR);
     }
+    if (next) issue_k(at);
     wave_lds_sync();
     const f32x16 zero = {};
     if (FORM == Form::kBias) start_scores<D, 1>(C, sc, R, t * 32, lane >> 5);
@@ -1389,7 +1394,7 @@ struct Stream8 {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
   __device__ __forceinline__ void product(f32x16 (&sc)[1], const Request& rq, Rows<D>& R, const Seen& mine,
-                                          int t, int pages, bool) {
+                                          int t, int pages, bool next, int at) {
     const int g = lane >> 5, left = rq.len - t * 32;
     uint16_t* const vt = kt + TILE;
     const Edges e{t * 32 < mine.all_lo, t * 32 + 31 > mine.all_hi, pages != 3, tokens_of<2>(left, pages)};
@@ -1407,6 +1412,7 @@ struct Stream8 {
       }
       put_values<T, D>(lo, hi, vt, row, lane % CPR);
     }
+    if (next) issue_v(at);
     bad = __builtin_amdgcn_ballot_w64(bad) != 0;
     wave_lds_sync();
     weigh<T, D, 1>(sc, R, vt, o, scale2_of(C, FORM));
@@ -1501,20 +1507,28 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
     wait_rows(qB);
     for (;; ++t) {
       f32x16 sc[1];
-      st.scores(sc, qB, R, t);
       const bool same = t + 1 < tend, next = same || more;
       int pages_n = 3;
-      if (next) {
+      auto go_on = [&] {  // to the next tile's pages
+        if (!next) return;
         at = same ? (at + 1) % 32 : 0;
         if (at == 0) {
           st.pg.take(C, kvh, same ? ids_next : ids_more);
           ids_next = same ? st.ids(p.rq.b, t + 33, 1) : st.ids(n.rq.b, first_of(n) + 32, 1);
         }
         pages_n = st.in_pool(at);
-        st.issue_k(at);
+      };
+      if constexpr (FP8) {
+        go_on();
+        st.scores(sc, qB, R, t, next, at);
+        st.product(sc, p.rq, R, mine, t, pages, next, at);
+      } else {
+        st.scores(sc, qB, R, t);
+        go_on();
+        if (next) st.issue_k(at);
+        st.product(sc, p.rq, R, mine, t, pages, next);
+        if (next) st.issue_v(at);
       }
-      st.product(sc, p.rq, R, mine, t, pages, next);
-      if (next) st.issue_v(at);
       pages = pages_n;
       if (!same) break;
     }
@@ -1581,20 +1595,28 @@ __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request&
     wait_rows(qB);
     for (; t < tend; t += 4) {
       f32x16 sc[1];
-      st.scores(sc, qB, R, t);
       const bool next = t + 4 < tend;
       int pages_n = 3;
-      if (next) {
+      auto go_on = [&] {
+        if (!next) return;
         at = (at + 1) % 32;
         if (at == 0) {
           st.pg.take(C, kvh, ids_next);
           ids_next = st.ids(rq.b, t + 132, 4);
         }
         pages_n = st.in_pool(at);
-        st.issue_k(at);
+      };
+      if constexpr (FP8) {
+        go_on();
+        st.scores(sc, qB, R, t, next, at);
+        st.product(sc, rq, R, mine, t, pages, next, at);
+      } else {
+        st.scores(sc, qB, R, t);
+        go_on();
+        if (next) st.issue_k(at);
+        st.product(sc, rq, R, mine, t, pages, next);
+        if (next) st.issue_v(at);
       }
-      st.product(sc, rq, R, mine, t, pages, next);
-      if (next) st.issue_v(at);
       pages = pages_n;
     }
   }
@@ -1786,7 +1808,7 @@ struct Cut {
   size_t acc_bytes, ml_bytes, bytes;
 };
 
-inline Cut cut_of(const bc_shape& s, int tokens) {
+inline Cut cut_of(const bc_shape& s, int tokens, bool fp8) {
   Cut c{};
   const long long steps = ((long long)s.max_pages * BC_PAGE_SIZE + kStep - 1) / kStep;
   const long long rows = (long long)tokens * (s.query_heads / s.kv_heads);
@@ -1804,7 +1826,7 @@ inline Cut cut_of(const bc_shape& s, int tokens) {
   // Four ranges per CU, eight at dim 64, where a tile is half the bytes (64
   // single tokens over 128-4096: 52.5 us, 54.4 with four; at dim 128 96 us with
   // four, 99 with eight).
-  const int per = s.dim == 64 ? 4 : 2;
+  const int per = s.dim == 64 || fp8 ? 4 : 2;
   c.waves = per * c.target / s.kv_heads > 1 ? per * c.target / s.kv_heads : 1;
   c.narrow_rows = 32 * c.waves + (int)(rows < 32ll * s.batch ? rows : 32ll * s.batch);
   if (rows > kFewRows) {

@@ -201,7 +201,7 @@ extern "C" int bc_append_kv(bc_shape s, const bc_half* k, const bc_half* v, bc_r
 }
 
 extern "C" size_t bc_chunk_attention_workspace_size(bc_shape s, int tokens) {
-  return chunk_shape_ok(s, tokens) ? cut_of(s, tokens).bytes : 0;
+  return chunk_shape_ok(s, tokens) ? cut_of(s, tokens, false).bytes : 0;
 }
 
 extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspace,
@@ -214,7 +214,7 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
   // Tiles of rows take 16-byte loads, 32-bit offsets inside a page and 31 bits
   // of rows and workgroups; anything else goes row by row.
   const long long rows = (long long)in.tokens * P.group;
-  const Cut cut = cut_of(s, in.tokens);
+  const Cut cut = cut_of(s, in.tokens, false);
   const bool use = cut.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= cut.bytes;
   const long long grid = tile_grid(s, in.tokens, cut, use);
   const long long far = 1 << 26;

@@ -25,113 +25,128 @@ struct Fp8Params {
   int tokens, phys_pages, hkv;
 };
 
-// A thread takes 16 values of a head: half a block.
-constexpr int kPiece = 16;
+// A thread takes eight values of a head, of K and of V: a block is four lanes, a
+// head of D values D / 8.
+constexpr int kPiece = 8;
 
-// Which piece of the rows of K (0) or V (1) thread x has, and where its slot is;
-// false where the slot is outside the pool.
+// Which piece of the rows thread x has, and where its slot is; `inside`: the slot
+// is one of the pool's.
 template <int D>
 struct Piece {
-  int kv, t, h, e;
-  int page, in;
+  unsigned t;
+  int h, e, page, in;
   bool inside;
-  __device__ __forceinline__ Piece(const Fp8Params& P, long long x) {
-    const int per_row = P.hkv * (D / kPiece);
-    const long long row = x / per_row;
-    const int c = (int)(x - row * per_row);
-    kv = blockIdx.y;
-    t = (int)row;
-    h = c / (D / kPiece);
-    e = c % (D / kPiece) * kPiece;
+  __device__ __forceinline__ Piece(const Fp8Params& P, unsigned x) {
+    const unsigned piece = x % (D / kPiece), head = x / (D / kPiece);
+    t = head / (unsigned)P.hkv;
+    h = head - t * P.hkv;
+    e = piece * kPiece;
     const int slot = P.slots[t];
     page = slot >> 4;
     in = slot & 15;
     inside = slot >= 0 && page < P.phys_pages;
   }
-  __device__ __forceinline__ size_t code(const Fp8Params& P) const {
+  __device__ __forceinline__ size_t code(const Fp8Params& P, int kv) const {
     return page * P.page[kv] + in * P.slot[kv] + h * P.head[kv] + e;
   }
-  __device__ __forceinline__ size_t power(const Fp8Params& P) const {
-    return (((size_t)page * P.hkv + h) * BC_PAGE_SIZE + in) * (D / kFp8Block) + e / kFp8Block;
+  __device__ __forceinline__ size_t powers(const Fp8Params& P) const {  // the head's first
+    return (((size_t)page * P.hkv + h) * BC_PAGE_SIZE + in) * (D / kFp8Block);
   }
 };
 
-// Sixteen values of T at p; VEC: two 16-byte loads.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_values(const uint16_t* p, float (&x)[kPiece]) {
-#pragma unroll
-  for (int i = 0; i < kPiece; i += 8) {
-    const uint4 w = load8<VEC>(p + i);
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int y = 0; y < 8; ++y)
-      x[i + y] = to_float(__builtin_bit_cast(T, (uint16_t)(words[y / 2] >> (16 * (y & 1)))));
-  }
-}
-
-// grid = (pieces, 2).  The largest magnitude of a block is that of two lanes side
-// by side.  Infinities and NaN become the NaN code and have no part in the
-// block's power.  Values past 1.875 times the type's largest power of two count as
-// that: they would be rounded to the next power, which the type does not have.
-template <typename T, int D, bool VEC>
-__global__ __launch_bounds__(kThreads) void append_fp8_kernel(Fp8Params P) {
-  const long long x = (long long)blockIdx.x * kThreads + threadIdx.x;
-  if (x >= (long long)P.tokens * P.hkv * (D / kPiece)) return;  // pairs of lanes leave together
-  const Piece<D> at(P, x);
+// Eight values of T as codes, and their block's power.
+template <typename T>
+__device__ __forceinline__ uint2 codes_of(const uint4& w, uint32_t& power) {
   constexpr float kMost = std::is_same<T, _Float16>::value ? 0x1.ep15f : 0x1.ep127f;
+  const uint32_t words[4] = {w.x, w.y, w.z, w.w};
   float val[kPiece], top = 0.f;
-  load_values<T, VEC>(P.rows[at.kv] + at.t * P.ts[at.kv] + at.h * P.hs[at.kv] + at.e, val);
 #pragma unroll
   for (int i = 0; i < kPiece; ++i) {
-    const float size = __builtin_fabsf(val[i]);
-    const bool finite = size < -kNegInf;
-    val[i] = __builtin_copysignf(__builtin_fminf(size, kMost), val[i]);
-    top = finite ? __builtin_fmaxf(top, __builtin_fabsf(val[i])) : top;
-    val[i] = finite ? val[i] : __builtin_nanf("");
+    const float x = to_float(__builtin_bit_cast(T, (uint16_t)(words[i / 2] >> (16 * (i & 1)))));
+    const float size = __builtin_fminf(__builtin_fabsf(x), kMost);
+    const bool finite = __builtin_fabsf(x) < -kNegInf;
+    top = finite ? __builtin_fmaxf(top, size) : top;
+    val[i] = finite ? __builtin_copysignf(size, x) : __builtin_nanf("");
   }
   top = __builtin_fmaxf(top, dpp_f<kDppQuadXor1>(top));
+  top = __builtin_fmaxf(top, dpp_f<kDppQuadXor2>(top));
   // Biased: the largest's exponent, one more where its fraction is above that of
   // 448 = 1.75 * 2^8, less 8; and at least 1, so that the power and its inverse
   // are normal numbers.
-  const uint32_t power =
-      (uint32_t)max((int)((__builtin_bit_cast(uint32_t, top) + 0x1fffffu) >> 23) - 8, 1);
+  power = (uint32_t)max((int)((__builtin_bit_cast(uint32_t, top) + 0x1fffffu) >> 23) - 8, 1);
   const float unit = power_of(254 - power);
-  uint32_t w[kPiece / 4];
+  uint32_t code[2];
 #pragma unroll
-  for (int i = 0; i < kPiece / 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     int c = __builtin_amdgcn_cvt_pk_fp8_f32(val[4 * i] * unit, val[4 * i + 1] * unit, 0, false);
     c = __builtin_amdgcn_cvt_pk_fp8_f32(val[4 * i + 2] * unit, val[4 * i + 3] * unit, c, true);
-    w[i] = (uint32_t)c;
+    code[i] = (uint32_t)c;
   }
-  if (!at.inside) return;
-  *reinterpret_cast<uint4*>(P.pool[at.kv] + at.code(P)) = make_uint4(w[0], w[1], w[2], w[3]);
-  if (at.e % kFp8Block == 0) P.scale[at.kv][at.power(P)] = (uint8_t)power;
+  return make_uint2(code[0], code[1]);
 }
 
-// grid = (pieces, 2).  Rows without a slot are zeros.
+// A head's powers from its blocks' lanes, four apart, to its first lane.
+template <int D>
+__device__ __forceinline__ uint32_t gather_powers(uint32_t power) {
+  uint32_t all = power | (uint32_t)dpp_i<0x104>((int)power) << 8;  // row_shl 4
+  if (D == 128)
+    all |= (uint32_t)dpp_i<0x108>((int)power) << 16 | (uint32_t)dpp_i<0x10c>((int)power) << 24;
+  return all;
+}
+
+template <int D>
+using Powers = typename std::conditional<D == 128, uint32_t, uint16_t>::type;
+
+// The largest magnitude of a block is that of four lanes.  Infinities and NaN become
+// the NaN code and have no part in the block's power.  Values past 1.875 times the
+// type's largest power of two count as that: they would be rounded to the next
+// power, which the type does not have.
+template <typename T, int D, bool VEC>
+__global__ __launch_bounds__(kThreads) void append_fp8_kernel(Fp8Params P) {
+  const unsigned x = blockIdx.x * kThreads + threadIdx.x;
+  if (x >= (unsigned)P.tokens * P.hkv * (D / kPiece)) return;  // the lanes of a head together
+  const Piece<D> at(P, x);
+  uint4 w[2];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+    w[kv] = load8<VEC>(P.rows[kv] + at.t * P.ts[kv] + at.h * P.hs[kv] + at.e);
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    uint32_t power;
+    const uint2 codes = codes_of<T>(w[kv], power);
+    const uint32_t all = gather_powers<D>(power);
+    if (!at.inside) continue;
+    *reinterpret_cast<uint2*>(P.pool[kv] + at.code(P, kv)) = codes;
+    if (at.e == 0) *reinterpret_cast<Powers<D>*>(P.scale[kv] + at.powers(P)) = (Powers<D>)all;
+  }
+}
+
+// Rows without a slot are zeros.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void read_fp8_kernel(Fp8Params P) {
-  const long long x = (long long)blockIdx.x * kThreads + threadIdx.x;
-  if (x >= (long long)P.tokens * P.hkv * (D / kPiece)) return;
+  const unsigned x = blockIdx.x * kThreads + threadIdx.x;
+  if (x >= (unsigned)P.tokens * P.hkv * (D / kPiece)) return;
   const Piece<D> at(P, x);
-  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-  if (at.inside) {
-    const uint4 w = *reinterpret_cast<const uint4*>(P.pool[at.kv] + at.code(P));
-    const float power = power_of(P.scale[at.kv][at.power(P)]);
-    lo = make_uint4(values2<T, false>(w.x, power), values2<T, true>(w.x, power),
-                    values2<T, false>(w.y, power), values2<T, true>(w.y, power));
-    hi = make_uint4(values2<T, false>(w.z, power), values2<T, true>(w.z, power),
-                    values2<T, false>(w.w, power), values2<T, true>(w.w, power));
-  }
-  uint4* const out = reinterpret_cast<uint4*>(P.out[at.kv] + x * kPiece);
-  out[0] = lo;
-  out[1] = hi;
+  uint2 codes[2] = {};
+  float power[2] = {};
+  if (at.inside)
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      codes[kv] = *reinterpret_cast<const uint2*>(P.pool[kv] + at.code(P, kv));
+      power[kv] = power_of(P.scale[kv][at.powers(P) + at.e / kFp8Block]);
+    }
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+    *reinterpret_cast<uint4*>(P.out[kv] + (size_t)x * kPiece) =
+        make_uint4(values2<T, false>(codes[kv].x, power[kv]), values2<T, true>(codes[kv].x, power[kv]),
+                   values2<T, false>(codes[kv].y, power[kv]), values2<T, true>(codes[kv].y, power[kv]));
 }
 
-// Codes go by 16 bytes.
+// Codes go by eight and 16 bytes, powers by two and four.
 bool pool_ok(const bc_shape& s, const bc_fp8_pool& p) {
   if (!p.k || !p.v || !p.k_scale || !p.v_scale || s.physical_pages < 1 || s.kv_heads < 1 ||
-      s.kv_heads > BC_MAX_CHUNK_HEADS || (s.dim != 64 && s.dim != 128) || !aligned16(p.k) || !aligned16(p.v))
+      s.kv_heads > BC_MAX_CHUNK_HEADS || (s.dim != 64 && s.dim != 128) || !aligned16(p.k) || !aligned16(p.v) ||
+      (reinterpret_cast<uintptr_t>(p.k_scale) | reinterpret_cast<uintptr_t>(p.v_scale)) % 4 != 0)
     return false;
   const long long bits = p.k_strides.page | p.k_strides.slot | p.k_strides.head | p.v_strides.page |
                          p.v_strides.slot | p.v_strides.head;
@@ -163,7 +178,7 @@ int most_rows(const bc_shape& s) {
 
 dim3 pieces_grid(const bc_shape& s, int tokens) {
   const long long pieces = (long long)tokens * s.kv_heads * (s.dim / kPiece);
-  return dim3((unsigned)((pieces + kThreads - 1) / kThreads), 2);
+  return dim3((unsigned)((pieces + kThreads - 1) / kThreads));
 }
 
 template <typename T, bool VEC>
@@ -237,7 +252,7 @@ extern "C" int bc_read_fp8_kv(bc_shape s, bc_fp8_pool pool, const int32_t* slots
 }
 
 extern "C" size_t bc_fp8_chunk_attention_workspace_size(bc_shape s, int tokens) {
-  return chunk_shape_ok(s, tokens) ? cut_of(s, tokens).bytes : 0;
+  return chunk_shape_ok(s, tokens) ? cut_of(s, tokens, true).bytes : 0;
 }
 
 extern "C" int bc_fp8_chunk_attention(bc_shape s, bc_chunk_inputs in, const uint8_t* k_scale,
@@ -258,7 +273,7 @@ extern "C" int bc_fp8_chunk_attention(bc_shape s, bc_chunk_inputs in, const uint
   P.v_scale = v_scale;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   // As in bc_chunk_attention.
-  const Cut cut = cut_of(s, in.tokens);
+  const Cut cut = cut_of(s, in.tokens, true);
   const bool use = cut.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= cut.bytes;
   const long long grid = tile_grid(s, in.tokens, cut, use);
   const long long far = 1 << 27;  // bytes: offsets inside a page are 32-bit

@@ -467,8 +467,8 @@ size_t bc_chunk_attention_workspace_size(bc_shape shape, int tokens);
 
 /* K and V of a paged cache in 8 bits.  Codes, e4m3 [P, 16, Hkv, D], in any order
  * of pages, slots and heads (strides in bytes, multiples of 16; 16-byte aligned);
- * scales, a byte for every 32 values of a head, contiguous [P, Hkv, 16, D / 32],
- * so that those of a page and head lie side by side: byte x is 2^(x - 127).  A
+ * scales, a byte for every 32 values of a head, contiguous [P, Hkv, 16, D / 32]
+ * and 4-byte aligned, so that those of a page and head lie side by side: byte x is 2^(x - 127).  A
  * value is its code times its block's scale.  A pool of zeros holds zeros.  Scale
  * bytes of 255 are never written; values read under one are not specified. */
 typedef struct bc_fp8_pool {
