@@ -43,6 +43,9 @@ struct ChunkParams {
   float scale, cap;
   const uint8_t* k_scale;    // of an 8-bit cache, whose k, v and their strides are in bytes
   const uint8_t* v_scale;
+  const int32_t* groups;     // of requests that begin with the same pages
+  const int32_t* shared;
+  int group_count;
 };
 
 __device__ __forceinline__ float to_float(_Float16 x) { return (float)x; }
@@ -288,6 +291,12 @@ struct TileParams {
   int most_parts;   // parts of split tiles, at most, per KV head
   int part_rows;    // rows of such a part
   int narrow_rows;  // partial rows of the narrow requests; the others' follow
+  // With groups, see the entries below: records are one int4 each, of every entry's
+  // tiles (the groups' from own_records on), and behind the parts lie the partial
+  // rows of tiles in one piece, first those of the requests, then the groups'.
+  int single_rows;  // where these begin
+  int total_rows;   // all partial rows
+  int own_records;
 };
 
 // The kernel's arguments, read anew: each phase of the tile kernel loads the
@@ -302,8 +311,10 @@ __device__ __forceinline__ const TileParams& reread(Args args) {
   return *(const TileParams*)(Args)at;
 }
 
+template <bool FORKS>
 __device__ __forceinline__ void pin_plan(const TileParams& P) {
   const ChunkParams& C = P.c;
+  if constexpr (FORKS) asm volatile("" ::"s"(C.groups), "s"(C.shared), "s"(C.group_count));
   asm volatile("" ::"s"(C.starts), "s"(C.lengths), "s"(C.prefix), "s"(C.first), "s"(C.tokens),
                "s"(C.batch), "s"(C.group), "s"(C.hkv), "s"(C.hkv_mul), "s"(C.max_pages),
                "s"(C.causal), "s"(C.window), "s"(P.part_acc), "s"(P.target), "s"(P.waves),
@@ -327,7 +338,17 @@ __device__ __forceinline__ void pin_rows(const TileParams& P) {
 struct Request {
   int b, start, len, pos0, rows;
   int prefix;  // tokens that all rows see
+  // With groups: the entry, the tokens that its group's has (a request's own part
+  // starts there), and of a group's entry its members, g1 > g0, whose rows these
+  // are (pos0 and prefix have no meaning then).
+  int entry, floor, g0, g1;
 };
+
+// With groups a batch has an entry per request, for its own tokens, and then one
+// per group, for what its members share: the rows of all of them, over the first
+// one's pages.  Entries of rows that another entry also has leave partials.
+__device__ __forceinline__ bool is_group(const Request& r) { return r.g1 > r.g0; }
+__device__ __forceinline__ bool joined(const Request& r) { return r.floor > 0 || is_group(r); }
 
 __device__ __forceinline__ int prefix_of(const ChunkParams& P, int b) {
   return P.prefix && P.causal ? max(P.prefix[b], 0) : 0;
@@ -367,18 +388,73 @@ __device__ __forceinline__ int lanes_upto(int x) {
   return x;
 }
 
-// A request per lane: its rows and its work, as tiles of 128 rows by steps of
+// Of 64 rising numbers, one per lane, how many are at most `x`.
+__device__ __forceinline__ int count_upto(int number, int x) {
+  int n = 0;
+#pragma unroll
+  for (int step = 32; step; step >>= 1) n += __shfl(number, n + step - 1, 64) <= x ? step : 0;
+  return n + (__shfl(number, n, 64) <= x ? 1 : 0);
+}
+
+// Group g: its members and the tokens they share, none of fewer than two members.
+struct Group {
+  int g0, g1, shared;
+};
+
+__device__ __forceinline__ Group group_at(const ChunkParams& P, int g) {
+  Group x;
+  x.g0 = min(max(P.groups[g], 0), P.batch);
+  x.g1 = min(max(P.groups[g + 1], 0), P.batch);
+  x.shared = x.g1 - x.g0 > 1 ? min(max(P.shared[g], 0), P.max_pages * BC_PAGE_SIZE) : 0;
+  return x;
+}
+
+// The group of request b, a lane's own; all lanes of the wave take part.  `shared`
+// is 0 where it has none.
+__device__ __forceinline__ int group_of(const ChunkParams& P, int b, int lane, int& shared) {
+  int at = -1;
+  shared = 0;
+  for (int i = 0; i < P.group_count; i += 64) {
+    const bool real = i + lane < P.group_count;
+    const Group x = real ? group_at(P, i + lane) : Group{0x7fffffff, 0, 0};
+    const int n = count_upto(x.g0, b) - 1, from = max(n, 0);
+    const int end = __shfl(x.g1, from, 64), tokens = __shfl(x.shared, from, 64);
+    if (n >= 0) {
+      at = i + n;
+      shared = b < end ? tokens : 0;
+    }
+  }
+  return at;
+}
+
+// An entry per lane: its rows and its work, as tiles of 128 rows by steps of
 // 64 tokens, or, with few rows, as tiles of 32 tokens (one at least, so that
 // rows which see nothing are written).
 struct Asked {
   int start, n, len, full, rows;
   int tiles, steps;        // of the wide form
   int first_tile, narrow;  // of the narrow form
+  int floor, g0, g1;       // with groups
 };
 
+__device__ __forceinline__ int wide_steps(const ChunkParams& P, int span) {
+  if (P.causal && P.window > 0) span = min(span, min(P.window, 1 << 29) + kManyRows + kStep);
+  return max(1, (span + kStep - 1) / kStep);
+}
+
+template <bool FORKS>
+__device__ __forceinline__ int entries_of(const ChunkParams& P) {
+  return FORKS ? P.batch + P.group_count : P.batch;
+}
+
 // With `tiles` the narrow form's tiles are those that the rows' documents reach.
+template <bool FORKS>
 __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b, bool tiles) {
   Asked a{};
+  if constexpr (FORKS) {
+    group_of(P, b, threadIdx.x & 63, a.floor);
+    if (b >= P.batch) a.floor = 0;
+  }
   if (b < P.batch) {
     a.start = min(max(P.starts[b], 0), P.tokens);
     a.n = max(min(max(P.starts[b + 1], 0), P.tokens) - a.start, 0);
@@ -387,9 +463,7 @@ __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b, bool tile
     a.rows = a.n * P.group;
     if (a.rows > kFewRows) {
       a.tiles = (a.rows + kManyRows - 1) / kManyRows;
-      int span = a.len;
-      if (P.causal && P.window > 0) span = min(span, min(P.window, 1 << 29) + kManyRows + kStep);
-      a.steps = max(1, (span + kStep - 1) / kStep);
+      a.steps = wide_steps(P, FORKS ? max(a.len - a.floor, 0) : a.len);
     } else if (a.rows > 0) {
       int lo = P.window > 0 ? (int)max(0ll, (long long)a.full - a.n - P.window + 1) : 0;
       if (P.first && tiles) {
@@ -399,8 +473,27 @@ __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b, bool tile
           for (int x = 0; x < 4; ++x) least = min(least, P.first[a.start + min(i + x, a.n - 1)]);
         lo = max(lo, least);
       }
+      if constexpr (FORKS) lo = max(lo, a.floor);
       a.first_tile = min(lo, max(a.len - 1, 0)) / 32;
       a.narrow = max(1, (a.len + 31) / 32 - a.first_tile);
+    }
+  } else if (FORKS && b - P.batch < P.group_count) {
+    const Group x = group_at(P, b - P.batch);
+    if (x.shared > 0) {
+      a.g0 = x.g0;
+      a.g1 = x.g1;
+      a.start = min(max(P.starts[x.g0], 0), P.tokens);
+      a.n = max(min(max(P.starts[x.g1], 0), P.tokens) - a.start, 0);
+      a.len = x.shared;
+      a.rows = a.n * P.group;
+      // What the members' rows see of it under a window, or of documents, takes a
+      // look at each of them: the wide form does.
+      if (a.rows > kFewRows || (a.rows > 0 && (P.window > 0 || P.first))) {
+        a.tiles = (a.rows + kManyRows - 1) / kManyRows;
+        a.steps = wide_steps(P, a.len);
+      } else if (a.rows > 0) {
+        a.narrow = (a.len + 31) / 32;
+      }
     }
   }
   return a;
@@ -417,12 +510,13 @@ struct Cutting {
   int groups;  // workgroups of the narrow requests: four (range, KV head) each
 };
 
+template <bool FORKS>
 __device__ __forceinline__ Cutting cut_batch(const TileParams& P, const Asked& head, int lane) {
   const ChunkParams& C = P.c;
   float work = (float)head.tiles * (float)head.steps;
   int narrow = head.narrow;
-  for (int b = 64 + lane; b - lane < C.batch; b += 64) {
-    const Asked x = asked_of(C, b, true);
+  for (int b = 64 + lane; b - lane < entries_of<FORKS>(C); b += 64) {
+    const Asked x = asked_of<FORKS>(C, b, true);
     work += (float)x.tiles * (float)x.steps;
     narrow += x.narrow;
   }
@@ -450,6 +544,22 @@ struct Item {
   bool found;
 };
 
+// Entry b0 + at of the batch, of which lane `at` holds what is asked.
+template <bool FORKS>
+__device__ __forceinline__ Request request_at(const ChunkParams& C, const Asked& a, int b0, int at) {
+  Request r{b0 + at, __builtin_amdgcn_readlane(a.start, at), __builtin_amdgcn_readlane(a.len, at),
+            __builtin_amdgcn_readlane(a.full - a.n, at), __builtin_amdgcn_readlane(a.rows, at)};
+  if constexpr (FORKS) {
+    r.entry = r.b;
+    r.floor = __builtin_amdgcn_readlane(a.floor, at);
+    r.g0 = __builtin_amdgcn_readlane(a.g0, at);
+    r.g1 = __builtin_amdgcn_readlane(a.g1, at);
+    if (is_group(r)) r.b = r.g0;
+  }
+  r.prefix = prefix_of(C, r.b);
+  return r;
+}
+
 // Item `idx` of the batch, found by every wave for itself from starts and
 // lengths.  A request's last tiles, which see most, come first.  `all`: go to
 // the end and count.  Where starts decrease, requests overlap and the grid,
@@ -457,15 +567,16 @@ struct Item {
 // counted are those whose writer, the first part's workgroup, is among the
 // first `launched` items and has place for its parts.  Both bounds rise from
 // one record to the next, so these are the first ones.
+template <bool FORKS>
 __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int share, long long idx,
                                           int lane, bool all, int launched) {
   const ChunkParams& C = P.c;
-  const bool split = P.part_acc != nullptr;
+  const bool split = FORKS || P.part_acc != nullptr;
   Item it{};
   long long before = 0;
   int slots = 0, cut = 0, records = 0, narrow = 0;
-  for (int b0 = 0; b0 < C.batch; b0 += 64) {
-    if (b0 > 0) a = asked_of(C, b0 + lane, split);
+  for (int b0 = 0; b0 < entries_of<FORKS>(C); b0 += 64) {
+    if (b0 > 0) a = asked_of<FORKS>(C, b0 + lane, split);
     const int parts = split && a.steps > share ? (a.steps + share - 1) / share : 1;
     const int tiles = split ? a.tiles : a.tiles + (a.narrow > 0);
     const int mine = tiles * parts;
@@ -476,12 +587,7 @@ __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int shar
       const int local = (int)(idx - before);
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > local));
       it.found = true;
-      it.r.b = b0 + at;
-      it.r.start = __builtin_amdgcn_readlane(a.start, at);
-      it.r.len = __builtin_amdgcn_readlane(a.len, at);
-      it.r.pos0 = __builtin_amdgcn_readlane(a.full - a.n, at);
-      it.r.rows = __builtin_amdgcn_readlane(a.rows, at);
-      it.r.prefix = prefix_of(C, it.r.b);
+      it.r = request_at<FORKS>(C, a, b0, at);
       it.parts = __builtin_amdgcn_readlane(parts, at);
       const int in = local - __builtin_amdgcn_readlane(upto - mine, at);
       const int nth = it.parts == 1 ? in : in / it.parts;
@@ -855,8 +961,28 @@ __device__ __forceinline__ void values16(const u32x4& w, float power, u32x4& lo,
              values2<T, true>(w[3], power)};
 }
 
+// The member of a group that row t, a lane's own, belongs to, the row's place in
+// it, and its length.  All lanes of the wave take part.
+struct Place {
+  int b, pos, len;
+};
+
+__device__ __forceinline__ Place place_of(const ChunkParams& P, const Request& group, int t) {
+  const int lane = threadIdx.x & 63;
+  int b = group.g0;  // and as many on as have ended at or below t
+  for (int i = group.g0; i < group.g1; i += 64) {
+    const int end = P.starts[min(i + lane, group.g1 - 1) + 1];
+    const int n = min(count_upto(end, t), group.g1 - i);
+    if (b == i) b = i + n;
+    if (!__builtin_amdgcn_ballot_w64(b == i + 64)) break;
+  }
+  b = min(b, group.g1 - 1);
+  const int pos = max(P.lengths[b], 0) - (min(P.starts[b + 1], P.tokens) - t);
+  return Place{b, pos, clamp_len(P, b)};
+}
+
 // This lane's row of the wave's 32: its place, what it sees, and its Q.
-template <typename T, int D, Form FORM>
+template <typename T, int D, Form FORM, bool FORKS>
 __device__ __forceinline__ void load_rows(const ChunkParams& C, const Request& it, int r, int kvh,
                                           int g, Rows<D>& R, u32x4 (&qB)[D / 16]) {
   const bool real = r < it.rows;
@@ -866,7 +992,15 @@ __device__ __forceinline__ void load_rows(const ChunkParams& C, const Request& i
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) qB[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
   R.pos = it.pos0 + i;
-  const int2 seen = row_range(C, it.b, t, R.pos, it.len);
+  int2 seen;
+  if (FORKS && is_group(it)) {
+    const Place at = place_of(C, it, t);
+    R.pos = at.pos;
+    seen = row_range(C, at.b, t, at.pos, min(at.len, it.len));
+  } else {
+    seen = row_range(C, it.b, t, R.pos, it.len);
+    if constexpr (FORKS) seen.x = max(seen.x, it.floor);
+  }
   R.lo = real ? seen.x : 0;
   R.hi = real ? seen.y : -1;
   R.slope = 0.f;
@@ -902,6 +1036,8 @@ __device__ __forceinline__ Seen rows_seen(const ChunkParams& C, const Request& r
     s.all_lo = max(0, max(pb, 0) - C.window + 1);
   }
   if (pa < 0) s.all_hi = -1;  // rows before the request see nothing
+  s.any_lo = max(s.any_lo, rq.floor);
+  s.all_lo = max(s.all_lo, rq.floor);
   return s;
 }
 
@@ -948,6 +1084,26 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
   P.records[2 + 2 * i] = make_int4(first, stride, 0, 0);
 }
 
+// With groups: the record of tile `tile` of an entry whose rows start at `start`.
+// No two entries have one in common, since the rows of the ones before end there.
+__device__ __forceinline__ int record_of(const TileParams& P, int entry, int start, int tile) {
+  const int from = entry < P.c.batch ? entry : P.own_records + entry - P.c.batch;
+  return from + start * P.c.group / kManyRows + tile;
+}
+
+// The partial row of an entry's first row, where a tile is in one piece.
+__device__ __forceinline__ int single_row(const TileParams& P, const Request& rq) {
+  const int rows = P.c.tokens * P.c.group;
+  return P.single_rows + (is_group(rq) ? rows : 0) + rq.start * P.c.group;
+}
+
+// Part p of the tile's rows are the partial rows first + p * stride ...; parts 0:
+// there are none.
+__device__ __forceinline__ void put_fork_record(const TileParams& P, const Request& rq, int tile, int parts,
+                                                int first, int stride) {
+  P.records[record_of(P, rq.entry, rq.start, tile)] = make_int4(parts, first, stride, 0);
+}
+
 // The wide form: 128 rows per workgroup, 32 per wave, each 64-token step's K
 // and V shared through two LDS buffers, which loads straight into LDS fill one
 // step ahead; one barrier a step, two workgroups per CU (three at D = 64).
@@ -960,7 +1116,7 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
 //    over 2048, sixteen of them: 180 us, 670 TFLOP/s).
 //  - A full round of workgroups takes 8.6 us, launch included, and 2.1 per step
 //    (2048 new tokens over 2048 to 32768, none masked: 75.8 to 1082 us).
-template <typename T, int D, Form FORM, bool FP8>
+template <typename T, int D, Form FORM, bool FP8, bool FORKS>
 __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const Item& it, int kvh,
                                           uint16_t* s_kv, Seen* s_seen, int* s_bad) {
   const ChunkParams& C = A.c;
@@ -991,13 +1147,13 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     }
   };
   if (tid < 4) s_bad[tid] = 0;
-  if (!C.first) {
+  if (!C.first && !(FORKS && is_group(rq))) {
     mine = rows_seen(C, rq, row0, min(row0 + 32, rq.rows));
     wg = rows_seen(C, rq, tile0, min(tile0 + kManyRows, rq.rows));
     range();
-    load_rows<T, D, FORM>(C, rq, row0 + lr, kvh, g, R, qB);
+    load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
   } else {
-    load_rows<T, D, FORM>(C, rq, row0 + lr, kvh, g, R, qB);
+    load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
     mine = wave_seen(R, row0 + lr < rq.rows);
     if (lane == 0) s_seen[wave] = mine;
     __syncthreads();
@@ -1179,8 +1335,9 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   const TileParams& P = reread(args);
   R.l += shfl_xor_f(R.l, 32);
   const int r = row0 + lr;
-  if (it.parts > 1) {
-    const size_t at = partial_row(P, P.narrow_rows + (it.slot + it.part) * P.part_rows + wave * 32 + lr, kvh);
+  if (it.parts > 1 || (FORKS && joined(rq))) {
+    const int first = it.parts > 1 ? P.narrow_rows + (it.slot + it.part) * P.part_rows : single_row(P, rq) + tile0;
+    const size_t at = partial_row(P, first + wave * 32 + lr, kvh);
     if (r < rq.rows) {
       if (g == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * at) = make_float2(R.m, R.l);
 #pragma unroll
@@ -1434,7 +1591,7 @@ using StreamOf = typename std::conditional<FP8, Stream8<T, D, FORM>, Stream<T, D
 // range leaves a partial.  Range r's partial of a request whose predecessors
 // have n rows starts at partial row 32 r + n: a range's next request is
 // further by the rows of the last one, a request's next range by 32.
-template <typename T, int D, Form FORM, bool FP8>
+template <typename T, int D, Form FORM, bool FP8, bool FORKS>
 __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cutting& cut,
                                           uint16_t* s_kv) {
   const ChunkParams& C = P.c;
@@ -1466,15 +1623,13 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
       rows_before += __builtin_amdgcn_readlane(rows_upto, 63);
       nth += __builtin_popcountll(some);
       b0 += 64;
-      if (b0 >= C.batch || before >= hi) return false;
-      a = asked_of(C, b0 + lane, true);
+      if (b0 >= entries_of<FORKS>(C) || before >= hi) return false;
+      a = asked_of<FORKS>(C, b0 + lane, true);
       look();
     }
     const int at = __builtin_ctzll(left);
     left &= left - 1;
-    p.rq = Request{b0 + at, __builtin_amdgcn_readlane(a.start, at), __builtin_amdgcn_readlane(a.len, at),
-                   __builtin_amdgcn_readlane(a.full - a.n, at), __builtin_amdgcn_readlane(a.rows, at),
-                   prefix_of(C, b0 + at)};
+    p.rq = request_at<FORKS>(C, a, b0, at);
     p.tiles = __builtin_amdgcn_readlane(a.narrow, at);
     p.x0 = before + __builtin_amdgcn_readlane(upto, at) - p.tiles;
     p.first_tile = __builtin_amdgcn_readlane(a.first_tile, at);
@@ -1496,8 +1651,9 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
   for (;;) {  // over the requests
     Rows<D> R;
     u32x4 qB[D / 16];
-    load_rows<T, D, FORM>(C, p.rq, lr, kvh, g, R, qB);
-    const Seen mine = C.first ? wave_seen(R, lr < p.rq.rows) : rows_seen(C, p.rq, 0, p.rq.rows);
+    load_rows<T, D, FORM, FORKS>(C, p.rq, lr, kvh, g, R, qB);
+    const Seen mine = C.first || (FORKS && is_group(p.rq)) ? wave_seen(R, lr < p.rq.rows)
+                                                           : rows_seen(C, p.rq, 0, p.rq.rows);
     const int tend = p.first_tile + min(hi, p.x0 + p.tiles) - p.x0;
     // The next request's first pages, so that its first tile follows this
     // one's last as any tile follows another.
@@ -1534,12 +1690,17 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
     }
     R.l += shfl_xor_f(R.l, 32);
     const int from = p.x0 / cut.run, parts = (p.x0 + p.tiles - 1) / cut.run - from + 1;
-    const int first = p.row + 32 * from;
+    const bool single = FORKS && parts == 1 && joined(p.rq);
+    const int first = single ? single_row(P, p.rq) : p.row + 32 * from;
     // Partials past their place cannot be unless starts decrease.
-    const bool fits = first + 32 * (parts - 1) + p.rq.rows <= P.narrow_rows;
-    if (p.x0 >= lo && kvh == 0 && lane == 0)
-      put_record(P, P.most_parts / 2 + p.nth, p.rq.start, 0, p.rq.rows, fits ? parts : 0, first, 32);
-    if (parts == 1) {
+    const bool fits = single || first + 32 * (parts - 1) + p.rq.rows <= P.narrow_rows;
+    if (p.x0 >= lo && kvh == 0 && lane == 0) {
+      if constexpr (FORKS)
+        put_fork_record(P, p.rq, 0, fits ? parts : 0, first, 32);
+      else
+        put_record(P, P.most_parts / 2 + p.nth, p.rq.start, 0, p.rq.rows, fits ? parts : 0, first, 32);
+    }
+    if (parts == 1 && !single) {
       const float inv = one_over(R.l);
       if (lr < p.rq.rows) {
         uint16_t* const out = out_row<T, D>(C, p.rq, lr, kvh) + 4 * g;
@@ -1582,7 +1743,7 @@ __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request&
   const int g = lane >> 5, lr = lane & 31;
   Rows<D> R;
   u32x4 qB[D / 16];
-  load_rows<T, D, FORM>(C, rq, lr, kvh, g, R, qB);
+  load_rows<T, D, FORM, false>(C, rq, lr, kvh, g, R, qB);
   const Seen mine = C.first ? wave_seen(R, lr < rq.rows) : rows_seen(C, rq, 0, rq.rows);
   StreamOf<T, D, FORM, FP8> st(C, kvh, s_kv + wave * (2 * TILE));
   int t = mine.any_hi < mine.any_lo ? 1 : mine.any_lo / 32 + wave;
@@ -1672,7 +1833,7 @@ __device__ __forceinline__ void clear_rows(const ChunkParams& C, long long at, l
     out[x < head * row ? x : x + gap] = u32x4{0, 0, 0, 0};
 }
 
-template <typename T, int D, Form FORM, bool FP8>
+template <typename T, int D, Form FORM, bool FP8, bool FORKS>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TileParams) {
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[2 * 2 * kStep * D];
   __shared__ float2 s_ml[4 * 32];
@@ -1681,11 +1842,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
   const int lane = threadIdx.x & 63;
   const Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
   const TileParams& P = reread(args);
-  pin_plan(P);
-  const Asked head = asked_of(P.c, lane, P.part_acc != nullptr);
+  pin_plan<FORKS>(P);
+  const Asked head = asked_of<FORKS>(P.c, lane, FORKS || P.part_acc != nullptr);
   Cutting cut{};
-  if (P.part_acc) cut = cut_batch(P, head, lane);
-  const bool counts = blockIdx.x == 0 && P.part_acc;
+  if (FORKS || P.part_acc) cut = cut_batch<FORKS>(P, head, lane);
+  const bool counts = !FORKS && blockIdx.x == 0 && P.part_acc;
   // The narrow requests first: theirs is memory's time, the others' the
   // matrix units', so they run beside each other.
   const bool flat = (int)blockIdx.x < cut.groups;
@@ -1695,13 +1856,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
   Item it{};
   if (!flat || counts) {
     const int launched = counts ? (int)(gridDim.x - cut.groups + P.c.hkv - 1) / P.c.hkv : 0;
-    it = plan_item(P, head, cut.share, flat ? -1ll : (long long)at, lane, counts, launched);
+    it = plan_item<FORKS>(P, head, cut.share, flat ? -1ll : (long long)at, lane, counts, launched);
   }
   if (counts && threadIdx.x == 0) P.records[0] = make_int4(it.records, it.narrow_records, 0, 0);
   if (flat) {
     const TileParams& A = reread(args);
     pin_rows<FP8>(A);
-    flat_body<T, D, FORM, FP8>(A, head, cut, s_kv);
+    flat_body<T, D, FORM, FP8, FORKS>(A, head, cut, s_kv);
     return;
   }
   if (!it.found) {
@@ -1709,16 +1870,24 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
     clear_rows<D>(P.c, blockIdx.x - items, gridDim.x - items);
     return;
   }
-  if (it.parts > 1 && it.part == 0 && kvh == 0 && threadIdx.x == 0)
-    put_record(P, it.record, it.r.start, it.tile * kManyRows,
-               min(it.r.rows - it.tile * kManyRows, kManyRows), it.parts,
-               P.narrow_rows + it.slot * P.part_rows, P.part_rows);
+  if constexpr (FORKS) {
+    if (it.part == 0 && kvh == 0 && threadIdx.x == 0)
+      put_fork_record(P, it.r, it.tile, it.parts,
+                      it.parts > 1 ? P.narrow_rows + it.slot * P.part_rows
+                                   : single_row(P, it.r) + it.tile * kManyRows,
+                      P.part_rows);
+  } else {
+    if (it.parts > 1 && it.part == 0 && kvh == 0 && threadIdx.x == 0)
+      put_record(P, it.record, it.r.start, it.tile * kManyRows,
+                 min(it.r.rows - it.tile * kManyRows, kManyRows), it.parts,
+                 P.narrow_rows + it.slot * P.part_rows, P.part_rows);
+  }
   const TileParams& A = reread(args);
   pin_rows<FP8>(A);
-  if (it.r.rows <= kFewRows)
+  if (!FORKS && it.r.rows <= kFewRows)
     narrow_body<T, D, FORM, FP8>(A.c, it.r, kvh, s_kv, s_ml);
   else
-    wide_body<T, D, FORM, FP8>(A, args, it, kvh, s_kv, s_seen, s_bad);
+    wide_body<T, D, FORM, FP8, FORKS>(A, args, it, kvh, s_kv, s_seen, s_bad);
 }
 
 // One part's state joined to another's.
@@ -1802,6 +1971,69 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(TileParams P, int apart
   }
 }
 
+// The join with groups: a wave per row and head, its lanes' groups of D / 4 taking
+// the parts of the request's own tokens and then of its group's in turn.  Rows
+// that their entry has written as output are left.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void fork_join_kernel(TileParams P) {
+  constexpr int LPR = D / 4, GW = 64 / LPR;
+  const ChunkParams& C = P.c;
+  const int lane = threadIdx.x & 63, grp = lane / LPR, c = lane % LPR;
+  const long long total = (long long)C.tokens * C.hq;
+  const long long step = 4ll * gridDim.x;
+  for (long long x = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); x < total; x += step) {
+    const int t = (int)(x / C.hq), h = (int)(x - (long long)t * C.hq), kvh = h / C.group, in = h - kvh * C.group;
+    const int b = request_of(C, t, lane);
+    if (b < 0) continue;
+    int shared;
+    const int g = __builtin_amdgcn_readfirstlane(group_of(C, b, lane, shared));
+    shared = __builtin_amdgcn_readfirstlane(shared);
+    // Record and row of the entry whose rows start at `from` and end at `to`.
+    int parts[2] = {}, first[2] = {}, stride[2] = {};
+    auto look = [&](int i, int entry, int from, int to, bool wide) {
+      from = min(max(from, 0), C.tokens);
+      to = min(max(to, 0), C.tokens);
+      if (t < from || t >= to) return;
+      const int row = (t - from) * C.group + in;
+      const int tile = wide || (to - from) * C.group > kFewRows ? row / kManyRows : 0;
+      const int4 rec = P.records[record_of(P, entry, from, tile)];
+      first[i] = rec.y + row - tile * kManyRows;
+      stride[i] = rec.z;
+      // Where starts decrease, a record may be another's or no one's.
+      const long long last = rec.y + (long long)max(rec.x - 1, 0) * rec.z + row - tile * kManyRows;
+      const bool sane = rec.x > 0 && rec.x <= 2 * (P.waves + P.most_parts) && rec.y >= 0 && rec.z > 0 &&
+                        last < P.total_rows;
+      parts[i] = sane ? rec.x : 0;
+    };
+    look(0, b, C.starts[b], C.starts[b + 1], false);
+    if (shared > 0) {
+      const Group x = group_at(C, g);
+      look(1, C.batch + g, C.starts[x.g0], C.starts[x.g1], C.window > 0 || C.first);
+    } else if (parts[0] < 2) {
+      continue;
+    }
+    float m = kNegInf, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = grp; p < parts[0] + parts[1]; p += GW) {
+      const bool own = p < parts[0];
+      const int at = own ? first[0] + p * stride[0] : first[1] + (p - parts[0]) * stride[1];
+      const size_t row = partial_row(P, at, kvh);
+      const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * row);
+      join(m, l, acc, ml.x, ml.y, *reinterpret_cast<const float4*>(P.part_acc + row * D + 4 * c));
+    }
+#pragma unroll
+    for (int s = LPR; s < 64; s <<= 1)
+      join(m, l, acc, shfl_xor_f(m, s), shfl_xor_f(l, s),
+           make_float4(shfl_xor_f(acc.x, s), shfl_xor_f(acc.y, s), shfl_xor_f(acc.z, s),
+                       shfl_xor_f(acc.w, s)));
+    const float inv = one_over(l);
+    if (grp == 0)
+      *reinterpret_cast<uint2*>(C.out + ((size_t)t * C.hq + h) * D + 4 * c) =
+          make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  }
+}
+
 // How a call with a workspace cuts its work; bytes 0: it does not.
 struct Cut {
   int target, waves, most_parts, part_rows, narrow_rows;
@@ -1859,11 +2091,11 @@ hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned
     P.narrow_rows = cut.narrow_rows;
   }
   if (C.cap > 0.f)
-    chunk_tile_kernel<T, D, Form::kCap, FP8><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kCap, FP8, false><<<dim3(grid), 256, 0, st>>>(P);
   else if (C.slopes)
-    chunk_tile_kernel<T, D, Form::kBias, FP8><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kBias, FP8, false><<<dim3(grid), 256, 0, st>>>(P);
   else
-    chunk_tile_kernel<T, D, Form::kPlain, FP8><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kPlain, FP8, false><<<dim3(grid), 256, 0, st>>>(P);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !ws) return err;
   // Enough workgroups for the rows of a record and KV head, on average, but not
@@ -1961,7 +2193,10 @@ inline ChunkParams chunk_params(const bc_shape& s, const bc_chunk_inputs& in) {
                      in.scale,
                      in.cap,
                      nullptr,
-                     nullptr};
+                     nullptr,
+                     nullptr,
+                     nullptr,
+                     0};
 }
 
 }  // namespace
