@@ -1971,66 +1971,69 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(TileParams P, int apart
   }
 }
 
-// The join with groups: a wave per row and head, its lanes' groups of D / 4 taking
-// the parts of the request's own tokens and then of its group's in turn.  Rows
-// that their entry has written as output are left.
+// The join with groups: `apart` waves share the rows of a new token and KV head; of
+// a wave, each group of D / 4 lanes takes the parts of the request's own tokens and
+// then of its group's in turn.  Rows that their entry has written as output are
+// left.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void fork_join_kernel(TileParams P) {
+__global__ __launch_bounds__(256) void fork_join_kernel(TileParams P, int apart) {
   constexpr int LPR = D / 4, GW = 64 / LPR;
   const ChunkParams& C = P.c;
   const int lane = threadIdx.x & 63, grp = lane / LPR, c = lane % LPR;
-  const long long total = (long long)C.tokens * C.hq;
-  const long long step = 4ll * gridDim.x;
+  const long long total = (long long)C.tokens * C.hkv * apart, step = 4ll * gridDim.x;
   for (long long x = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); x < total; x += step) {
-    const int t = (int)(x / C.hq), h = (int)(x - (long long)t * C.hq), kvh = h / C.group, in = h - kvh * C.group;
+    const long long pair = x / apart;
+    const int sub = (int)(x - pair * apart), t = (int)(pair / C.hkv), kvh = (int)(pair - (long long)t * C.hkv);
     const int b = request_of(C, t, lane);
     if (b < 0) continue;
     int shared;
     const int g = __builtin_amdgcn_readfirstlane(group_of(C, b, lane, shared));
     shared = __builtin_amdgcn_readfirstlane(shared);
-    // Record and row of the entry whose rows start at `from` and end at `to`.
-    int parts[2] = {}, first[2] = {}, stride[2] = {};
-    auto look = [&](int i, int entry, int from, int to, bool wide) {
-      from = min(max(from, 0), C.tokens);
-      to = min(max(to, 0), C.tokens);
-      if (t < from || t >= to) return;
-      const int row = (t - from) * C.group + in;
-      const int tile = wide || (to - from) * C.group > kFewRows ? row / kManyRows : 0;
-      const int4 rec = P.records[record_of(P, entry, from, tile)];
-      first[i] = rec.y + row - tile * kManyRows;
-      stride[i] = rec.z;
-      // Where starts decrease, a record may be another's or no one's.
-      const long long last = rec.y + (long long)max(rec.x - 1, 0) * rec.z + row - tile * kManyRows;
-      const bool sane = rec.x > 0 && rec.x <= 2 * (P.waves + P.most_parts) && rec.y >= 0 && rec.z > 0 &&
-                        last < P.total_rows;
-      parts[i] = sane ? rec.x : 0;
-    };
-    look(0, b, C.starts[b], C.starts[b + 1], false);
-    if (shared > 0) {
-      const Group x = group_at(C, g);
-      look(1, C.batch + g, C.starts[x.g0], C.starts[x.g1], C.window > 0 || C.first);
-    } else if (parts[0] < 2) {
-      continue;
-    }
-    float m = kNegInf, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    // Of the entry whose new tokens are `from` .. `to` - 1: the first of this
+    // token's rows in it, and its record there.  The rows of a token may lie in
+    // two tiles.
+    auto start_of = [&](int from) { return min(max(from, 0), C.tokens); };
+    const Group group = shared > 0 ? group_at(C, g) : Group{};
+    const int own0 = start_of(C.starts[b]);
+    const int all0 = shared > 0 ? start_of(C.starts[group.g0]) : 0;
+    for (int r = sub; r < C.group; r += apart) {
+      int parts[2] = {}, first[2] = {}, stride[2] = {};
+      auto look = [&](int i, int entry, int from) {
+        const int row = max(t - from, 0) * C.group + r, tile = row / kManyRows;
+        const int4 rec = P.records[record_of(P, entry, from, tile)];
+        // Where starts decrease, a record may be another's or no one's.
+        const long long last = rec.y + (long long)max(rec.x - 1, 0) * rec.z + row - tile * kManyRows;
+        const bool sane = rec.x > 0 && rec.x <= 2 * (P.waves + P.most_parts) && rec.y >= 0 && rec.z > 0 &&
+                          last < P.total_rows;
+        parts[i] = sane ? rec.x : 0;
+        first[i] = rec.y + row - tile * kManyRows;
+        stride[i] = rec.z;
+      };
+      look(0, b, own0);
+      if (shared > 0)
+        look(1, C.batch + g, all0);
+      else if (parts[0] < 2)
+        continue;
+      float m = kNegInf, l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int p = grp; p < parts[0] + parts[1]; p += GW) {
-      const bool own = p < parts[0];
-      const int at = own ? first[0] + p * stride[0] : first[1] + (p - parts[0]) * stride[1];
-      const size_t row = partial_row(P, at, kvh);
-      const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * row);
-      join(m, l, acc, ml.x, ml.y, *reinterpret_cast<const float4*>(P.part_acc + row * D + 4 * c));
-    }
+      for (int p = grp; p < parts[0] + parts[1]; p += GW) {
+        const bool own = p < parts[0];
+        const int at = own ? first[0] + p * stride[0] : first[1] + (p - parts[0]) * stride[1];
+        const size_t row = partial_row(P, at, kvh);
+        const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * row);
+        join(m, l, acc, ml.x, ml.y, *reinterpret_cast<const float4*>(P.part_acc + row * D + 4 * c));
+      }
 #pragma unroll
-    for (int s = LPR; s < 64; s <<= 1)
-      join(m, l, acc, shfl_xor_f(m, s), shfl_xor_f(l, s),
-           make_float4(shfl_xor_f(acc.x, s), shfl_xor_f(acc.y, s), shfl_xor_f(acc.z, s),
-                       shfl_xor_f(acc.w, s)));
-    const float inv = one_over(l);
-    if (grp == 0)
-      *reinterpret_cast<uint2*>(C.out + ((size_t)t * C.hq + h) * D + 4 * c) =
-          make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+      for (int s = LPR; s < 64; s <<= 1)
+        join(m, l, acc, shfl_xor_f(m, s), shfl_xor_f(l, s),
+             make_float4(shfl_xor_f(acc.x, s), shfl_xor_f(acc.y, s), shfl_xor_f(acc.z, s),
+                         shfl_xor_f(acc.w, s)));
+      const float inv = one_over(l);
+      if (grp == 0)
+        *reinterpret_cast<uint2*>(C.out + ((size_t)t * C.hq + kvh * C.group + r) * D + 4 * c) =
+            make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    }
   }
 }
 
@@ -2118,6 +2121,16 @@ hipError_t launch_tiles(const ChunkParams& P, int dim, int dtype, const Cut& cut
                      : launch_tiles<_Float16, 128, FP8>(P, cut, ws, (unsigned)grid, st);
   return dim == 64 ? launch_tiles<__bf16, 64, FP8>(P, cut, ws, (unsigned)grid, st)
                    : launch_tiles<__bf16, 128, FP8>(P, cut, ws, (unsigned)grid, st);
+}
+
+// Workgroups of the tile kernel with a workspace, at most, of a batch whose entries
+// of more than 32 rows have `rows` rows in all.  Cut by shares, n tiles have less
+// than target / Hkv + n parts.  A workgroup without work still walks the batch to
+// see that, some 2 us, so none is launched beyond these.
+inline long long split_grid(const bc_shape& s, const Cut& cut, long long rows, long long entries) {
+  const long long wide = rows / (kFewRows + 1) < entries ? rows / (kFewRows + 1) : entries;
+  const long long items = wide > 0 ? rows / kManyRows + wide + cut.target / s.kv_heads + 1 : 0;
+  return items * s.kv_heads + ((long long)cut.waves * s.kv_heads + 3) / 4 + 1;
 }
 
 // Workgroups of the tile kernel, at most.

@@ -67,9 +67,13 @@ hipError_t launch_forks(const ChunkParams& C, const ForkCut& cut, void* ws, unsi
     chunk_tile_kernel<T, D, Form::kPlain, false, true><<<dim3(grid), 256, 0, st>>>(P);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  const long long waves = (long long)C.tokens * C.hq, most = 8ll * cut.target;
-  const long long join = (waves + 3) / 4 < most ? (waves + 3) / 4 : most;
-  fork_join_kernel<T, D><<<dim3((unsigned)join), 256, 0, st>>>(P);
+  // A round of waves, eight workgroups per CU, with the rows of a token and KV head
+  // apart where there is room.
+  const long long pairs = (long long)C.tokens * C.hkv, most = 4ll * cut.target;
+  long long apart = 4 * most / pairs;
+  apart = apart < 1 ? 1 : apart < C.group ? apart : C.group;
+  const long long join = (pairs * apart + 3) / 4;
+  fork_join_kernel<T, D><<<dim3((unsigned)(join < most ? join : most)), 256, 0, st>>>(P, (int)apart);
   return hipGetLastError();
 }
 
@@ -89,10 +93,11 @@ extern "C" int bc_shared_chunk_attention(bc_shape s, bc_chunk_inputs in, const i
     return BC_ERROR_INVALID_VALUE;
   const ForkCut cut = fork_cut(s, in.tokens, group_count);
   const bool use = cut.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= cut.bytes;
-  // As in bc_chunk_attention; each group adds its members' tiles of rows once more.
+  // As in bc_chunk_attention.  Rows count twice, as a request's and as a group's;
+  // under a window, or with documents, a group of few rows is of the wide form.
   const long long rows = (long long)in.tokens * (s.query_heads / s.kv_heads);
-  const long long grid =
-      tile_grid(s, in.tokens, cut, use) + (rows / kManyRows + group_count) * s.kv_heads;
+  const long long few = in.window > 0 || in.first ? (long long)(kFewRows + 1) * group_count : 0;
+  const long long grid = split_grid(s, cut, 2 * rows + few, (long long)s.batch + group_count);
   const long long far = 1 << 26;
   if (!use || !aligned16(in.q) || !aligned16(in.k) || !aligned16(in.v) || !aligned16(in.output) ||
       stride_bits(in) % 8 != 0 || in.k_strides.slot >= far || in.v_strides.slot >= far || grid > kMostGroups)
