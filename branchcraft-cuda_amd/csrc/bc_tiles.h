@@ -402,26 +402,39 @@ struct Group {
 };
 
 __device__ __forceinline__ Group group_at(const ChunkParams& P, int g) {
+  const int from = P.groups[g], to = P.groups[g + 1], tokens = P.shared[g];  // in one round
   Group x;
-  x.g0 = min(max(P.groups[g], 0), P.batch);
-  x.g1 = min(max(P.groups[g + 1], 0), P.batch);
-  x.shared = x.g1 - x.g0 > 1 ? min(max(P.shared[g], 0), P.max_pages * BC_PAGE_SIZE) : 0;
+  x.g0 = min(max(from, 0), P.batch);
+  x.g1 = min(max(to, 0), P.batch);
+  x.shared = x.g1 - x.g0 > 1 ? min(max(tokens, 0), P.max_pages * BC_PAGE_SIZE) : 0;
   return x;
 }
 
-// The group of request b, a lane's own; all lanes of the wave take part.  `shared`
-// is 0 where it has none.
-__device__ __forceinline__ int group_of(const ChunkParams& P, int b, int lane, int& shared) {
-  int at = -1;
-  shared = 0;
-  for (int i = 0; i < P.group_count; i += 64) {
-    const bool real = i + lane < P.group_count;
-    const Group x = real ? group_at(P, i + lane) : Group{0x7fffffff, 0, 0};
-    const int n = count_upto(x.g0, b) - 1, from = max(n, 0);
-    const int end = __shfl(x.g1, from, 64), tokens = __shfl(x.shared, from, 64);
+// Of the 64 groups that the lanes hold, that of request b, a lane's own; -1, and 0
+// tokens, where it has none.  All lanes of the wave take part.
+__device__ __forceinline__ int group_in(const Group& x, int b, int& shared) {
+  const int n = count_upto(x.g0, b) - 1, from = max(n, 0);
+  const int end = __shfl(x.g1, from, 64), tokens = __shfl(x.shared, from, 64);
+  shared = n >= 0 && b < end ? tokens : 0;
+  return n;
+}
+
+// The groups i .. i + 63, a lane each; behind the last, groups of no request.
+__device__ __forceinline__ Group groups_from(const ChunkParams& P, int i) {
+  const int lane = threadIdx.x & 63;
+  const Group x = group_at(P, min(i + lane, P.group_count - 1));
+  return i + lane < P.group_count ? x : Group{0x7fffffff, 0, 0};
+}
+
+// The group of request b, a lane's own, of the first 64 (`head`) or those behind.
+__device__ __forceinline__ int group_of(const ChunkParams& P, const Group& head, int b, int& shared) {
+  int at = group_in(head, b, shared);
+  for (int i = 64; i < P.group_count; i += 64) {
+    int tokens;
+    const int n = group_in(groups_from(P, i), b, tokens);
     if (n >= 0) {
       at = i + n;
-      shared = b < end ? tokens : 0;
+      shared = tokens;
     }
   }
   return at;
@@ -451,14 +464,26 @@ __device__ __forceinline__ int entries_of(const ChunkParams& P) {
 template <bool FORKS>
 __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b, bool tiles) {
   Asked a{};
+  int start = 0, end = 0;
+  Group head{};
   if constexpr (FORKS) {
-    group_of(P, b, threadIdx.x & 63, a.floor);
+    // All that does not depend on each other is loaded in one round.
+    const int i = min(b, P.batch - 1);
+    const int s0 = P.starts[i], s1 = P.starts[i + 1], full = P.lengths[i];
+    head = groups_from(P, 0);
+    start = min(max(s0, 0), P.tokens);
+    end = min(max(s1, 0), P.tokens);
+    a.full = max(full, 0);
+    group_of(P, head, b, a.floor);
     if (b >= P.batch) a.floor = 0;
+  } else if (b < P.batch) {
+    start = min(max(P.starts[b], 0), P.tokens);
+    end = min(max(P.starts[b + 1], 0), P.tokens);
+    a.full = max(P.lengths[b], 0);
   }
   if (b < P.batch) {
-    a.start = min(max(P.starts[b], 0), P.tokens);
-    a.n = max(min(max(P.starts[b + 1], 0), P.tokens) - a.start, 0);
-    a.full = max(P.lengths[b], 0);
+    a.start = start;
+    a.n = max(end - start, 0);
     a.len = min(a.full, P.max_pages * BC_PAGE_SIZE);
     a.rows = a.n * P.group;
     if (a.rows > kFewRows) {
@@ -477,13 +502,24 @@ __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b, bool tile
       a.first_tile = min(lo, max(a.len - 1, 0)) / 32;
       a.narrow = max(1, (a.len + 31) / 32 - a.first_tile);
     }
-  } else if (FORKS && b - P.batch < P.group_count) {
-    const Group x = group_at(P, b - P.batch);
-    if (x.shared > 0) {
+  }
+  if constexpr (FORKS) {
+    // A group's entry: its members from the lane that holds it, and, where the lanes
+    // hold all requests, the ends of its rows from theirs.
+    const int g = b - P.batch;
+    Group x{__shfl(head.g0, max(g, 0), 64), __shfl(head.g1, max(g, 0), 64), __shfl(head.shared, max(g, 0), 64)};
+    if (g >= 64 && g < P.group_count) x = group_at(P, g);
+    int from = __shfl(start, x.g0, 64), to = __shfl(end, x.g1 - 1, 64);
+    const bool is = g >= 0 && g < P.group_count && x.shared > 0;
+    if (is && (P.batch > 64 || b >= 64)) {
+      from = min(max(P.starts[x.g0], 0), P.tokens);
+      to = min(max(P.starts[x.g1], 0), P.tokens);
+    }
+    if (is) {
       a.g0 = x.g0;
       a.g1 = x.g1;
-      a.start = min(max(P.starts[x.g0], 0), P.tokens);
-      a.n = max(min(max(P.starts[x.g1], 0), P.tokens) - a.start, 0);
+      a.start = from;
+      a.n = max(to - from, 0);
       a.len = x.shared;
       a.rows = a.n * P.group;
       // What the members' rows see of it under a window, or of documents, takes a
@@ -510,7 +546,9 @@ struct Cutting {
   int groups;  // workgroups of the narrow requests: four (range, KV head) each
 };
 
-template <bool FORKS>
+// `ROUND`: the shares fill what the narrow requests' workgroups leave of a round;
+// else both are cut to the same time, if each had a part of the card to itself.
+template <bool FORKS, bool ROUND>
 __device__ __forceinline__ Cutting cut_batch(const TileParams& P, const Asked& head, int lane) {
   const ChunkParams& C = P.c;
   float work = (float)head.tiles * (float)head.steps;
@@ -529,6 +567,10 @@ __device__ __forceinline__ Cutting cut_batch(const TileParams& P, const Asked& h
   c.run = max(min((int)__builtin_fminf(run, 1e9f) + 1, c.narrow), (c.narrow + P.waves - 1) / P.waves);
   c.run = max(c.run, kLeastRun);
   c.groups = ((c.narrow + c.run - 1) / c.run * C.hkv + 3) / 4;
+  if (ROUND) {
+    const float part = work * (float)C.hkv / (float)max(P.target - c.groups, P.target / 4);
+    c.share = max(kLeastSteps, (int)__builtin_fminf(part, 1e9f) + 1);
+  }
   return c;
 }
 
@@ -969,16 +1011,19 @@ struct Place {
 
 __device__ __forceinline__ Place place_of(const ChunkParams& P, const Request& group, int t) {
   const int lane = threadIdx.x & 63;
-  int b = group.g0;  // and as many on as have ended at or below t
+  Place at{group.g1 - 1, 0, 0};
+  bool found = false;
   for (int i = group.g0; i < group.g1; i += 64) {
-    const int end = P.starts[min(i + lane, group.g1 - 1) + 1];
-    const int n = min(count_upto(end, t), group.g1 - i);
-    if (b == i) b = i + n;
-    if (!__builtin_amdgcn_ballot_w64(b == i + 64)) break;
+    const int b = min(i + lane, group.g1 - 1);
+    const int end = P.starts[b + 1], full = max(P.lengths[b], 0);
+    const int n = count_upto(end, t), from = min(n, 63);
+    const int pos = __shfl(full, from, 64) - (min(__shfl(end, from, 64), P.tokens) - t);
+    const int len = min(__shfl(full, from, 64), P.max_pages * BC_PAGE_SIZE);
+    if (!found && n < 64) at = Place{min(i + n, group.g1 - 1), pos, len};
+    found = found || n < 64;
+    if (!__builtin_amdgcn_ballot_w64(!found)) break;
   }
-  b = min(b, group.g1 - 1);
-  const int pos = max(P.lengths[b], 0) - (min(P.starts[b + 1], P.tokens) - t);
-  return Place{b, pos, clamp_len(P, b)};
+  return at;
 }
 
 // This lane's row of the wave's 32: its place, what it sees, and its Q.
@@ -1147,12 +1192,19 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     }
   };
   if (tid < 4) s_bad[tid] = 0;
-  if (!C.first && !(FORKS && is_group(rq))) {
+  const bool by_rows = C.first || (FORKS && is_group(rq));  // what is seen depends on the rows
+  const bool ahead = FORKS && is_group(rq) && !C.first && C.window == 0;  // but not where it starts
+  if (!by_rows) {
     mine = rows_seen(C, rq, row0, min(row0 + 32, rq.rows));
     wg = rows_seen(C, rq, tile0, min(tile0 + kManyRows, rq.rows));
     range();
     load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
   } else {
+    if (ahead) {
+      wg.any_lo = 0;
+      wg.any_hi = rq.len - 1;
+      range();
+    }
     load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
     mine = wave_seen(R, row0 + lr < rq.rows);
     if (lane == 0) s_seen[wave] = mine;
@@ -1169,7 +1221,7 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     wg.any_hi = __builtin_amdgcn_readfirstlane(wg.any_hi);
     wg.all_lo = __builtin_amdgcn_readfirstlane(wg.all_lo);
     wg.all_hi = __builtin_amdgcn_readfirstlane(wg.all_hi);
-    range();
+    if (!ahead) range();
   }
 
   const int lrow = tid / CPR, lcol = 8 * (tid % CPR ^ swz<D>(lrow));
@@ -1845,7 +1897,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
   pin_plan<FORKS>(P);
   const Asked head = asked_of<FORKS>(P.c, lane, FORKS || P.part_acc != nullptr);
   Cutting cut{};
-  if (FORKS || P.part_acc) cut = cut_batch<FORKS>(P, head, lane);
+  if (FORKS || P.part_acc) cut = cut_batch<FORKS, FORKS || FP8>(P, head, lane);
   const bool counts = !FORKS && blockIdx.x == 0 && P.part_acc;
   // The narrow requests first: theirs is memory's time, the others' the
   // matrix units', so they run beside each other.
@@ -1984,22 +2036,31 @@ __global__ __launch_bounds__(256) void fork_join_kernel(TileParams P, int apart)
   for (long long x = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); x < total; x += step) {
     const long long pair = x / apart;
     const int sub = (int)(x - pair * apart), t = (int)(pair / C.hkv), kvh = (int)(pair - (long long)t * C.hkv);
-    const int b = request_of(C, t, lane);
-    if (b < 0) continue;
+    // The request of token t, the first of its rows, and its group, of loads in one
+    // round for up to 64 of either.
+    const Group head = groups_from(C, 0);
+    int b = 0, own0 = 0;
+    for (int i = 0; i < C.batch; i += 64) {
+      const int from = C.starts[min(i + lane, C.batch - 1)], to = C.starts[min(i + lane, C.batch - 1) + 1];
+      const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < C.batch && to <= t));
+      b += n;
+      if (n < 64) {
+        own0 = __builtin_amdgcn_readlane(from, n);
+        break;
+      }
+    }
+    if (b >= C.batch || own0 > t) continue;
     int shared;
-    const int g = __builtin_amdgcn_readfirstlane(group_of(C, b, lane, shared));
+    const int g = __builtin_amdgcn_readfirstlane(group_of(C, head, b, shared));
     shared = __builtin_amdgcn_readfirstlane(shared);
-    // Of the entry whose new tokens are `from` .. `to` - 1: the first of this
-    // token's rows in it, and its record there.  The rows of a token may lie in
-    // two tiles.
     auto start_of = [&](int from) { return min(max(from, 0), C.tokens); };
-    const Group group = shared > 0 ? group_at(C, g) : Group{};
-    const int own0 = start_of(C.starts[b]);
-    const int all0 = shared > 0 ? start_of(C.starts[group.g0]) : 0;
+    own0 = start_of(own0);
+    const int all0 = shared > 0 ? start_of(C.starts[group_at(C, g).g0]) : 0;
     for (int r = sub; r < C.group; r += apart) {
       int parts[2] = {}, first[2] = {}, stride[2] = {};
       auto look = [&](int i, int entry, int from) {
-        const int row = max(t - from, 0) * C.group + r, tile = row / kManyRows;
+        if (t < from) return;
+        const int row = (t - from) * C.group + r, tile = row / kManyRows;
         const int4 rec = P.records[record_of(P, entry, from, tile)];
         // Where starts decrease, a record may be another's or no one's.
         const long long last = rec.y + (long long)max(rec.x - 1, 0) * rec.z + row - tile * kManyRows;
@@ -2016,7 +2077,7 @@ __global__ __launch_bounds__(256) void fork_join_kernel(TileParams P, int apart)
         continue;
       float m = kNegInf, l = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
       for (int p = grp; p < parts[0] + parts[1]; p += GW) {
         const bool own = p < parts[0];
         const int at = own ? first[0] + p * stride[0] : first[1] + (p - parts[0]) * stride[1];
