@@ -311,10 +311,8 @@ __device__ __forceinline__ const TileParams& reread(Args args) {
   return *(const TileParams*)(Args)at;
 }
 
-template <bool FORKS>
 __device__ __forceinline__ void pin_plan(const TileParams& P) {
   const ChunkParams& C = P.c;
-  if constexpr (FORKS) asm volatile("" ::"s"(C.groups), "s"(C.shared), "s"(C.group_count));
   asm volatile("" ::"s"(C.starts), "s"(C.lengths), "s"(C.prefix), "s"(C.first), "s"(C.tokens),
                "s"(C.batch), "s"(C.group), "s"(C.hkv), "s"(C.hkv_mul), "s"(C.max_pages),
                "s"(C.causal), "s"(C.window), "s"(P.part_acc), "s"(P.target), "s"(P.waves),
@@ -388,149 +386,60 @@ __device__ __forceinline__ int lanes_upto(int x) {
   return x;
 }
 
-// Of 64 rising numbers, one per lane, how many are at most `x`.
-__device__ __forceinline__ int count_upto(int number, int x) {
-  int n = 0;
-#pragma unroll
-  for (int step = 32; step; step >>= 1) n += __shfl(number, n + step - 1, 64) <= x ? step : 0;
-  return n + (__shfl(number, n, 64) <= x ? 1 : 0);
-}
-
-// Group g: its members and the tokens they share, none of fewer than two members.
-struct Group {
-  int g0, g1, shared;
-};
-
-__device__ __forceinline__ Group group_at(const ChunkParams& P, int g) {
-  const int from = P.groups[g], to = P.groups[g + 1], tokens = P.shared[g];  // in one round
-  Group x;
-  x.g0 = min(max(from, 0), P.batch);
-  x.g1 = min(max(to, 0), P.batch);
-  x.shared = x.g1 - x.g0 > 1 ? min(max(tokens, 0), P.max_pages * BC_PAGE_SIZE) : 0;
-  return x;
-}
-
-// Of the 64 groups that the lanes hold, that of request b, a lane's own; -1, and 0
-// tokens, where it has none.  All lanes of the wave take part.
-__device__ __forceinline__ int group_in(const Group& x, int b, int& shared) {
-  const int n = count_upto(x.g0, b) - 1, from = max(n, 0);
-  const int end = __shfl(x.g1, from, 64), tokens = __shfl(x.shared, from, 64);
-  shared = n >= 0 && b < end ? tokens : 0;
-  return n;
-}
-
-// The groups i .. i + 63, a lane each; behind the last, groups of no request.
-__device__ __forceinline__ Group groups_from(const ChunkParams& P, int i) {
-  const int lane = threadIdx.x & 63;
-  const Group x = group_at(P, min(i + lane, P.group_count - 1));
-  return i + lane < P.group_count ? x : Group{0x7fffffff, 0, 0};
-}
-
-// The group of request b, a lane's own, of the first 64 (`head`) or those behind.
-__device__ __forceinline__ int group_of(const ChunkParams& P, const Group& head, int b, int& shared) {
-  int at = group_in(head, b, shared);
-  for (int i = 64; i < P.group_count; i += 64) {
-    int tokens;
-    const int n = group_in(groups_from(P, i), b, tokens);
-    if (n >= 0) {
-      at = i + n;
-      shared = tokens;
-    }
-  }
-  return at;
-}
-
-// An entry per lane: its rows and its work, as tiles of 128 rows by steps of
+// A request per lane: its rows and its work, as tiles of 128 rows by steps of
 // 64 tokens, or, with few rows, as tiles of 32 tokens (one at least, so that
 // rows which see nothing are written).
 struct Asked {
   int start, n, len, full, rows;
   int tiles, steps;        // of the wide form
   int first_tile, narrow;  // of the narrow form
-  int floor, g0, g1;       // with groups
 };
 
-__device__ __forceinline__ int wide_steps(const ChunkParams& P, int span) {
-  if (P.causal && P.window > 0) span = min(span, min(P.window, 1 << 29) + kManyRows + kStep);
+struct AskedEntry : Asked {
+  int floor, g0, g1;  // see Request
+};
+
+__device__ __forceinline__ int wide_steps(const ChunkParams& P, int span, int tile_rows) {
+  if (P.causal && P.window > 0) span = min(span, min(P.window, 1 << 29) + tile_rows + kStep);
   return max(1, (span + kStep - 1) / kStep);
 }
 
-template <bool FORKS>
-__device__ __forceinline__ int entries_of(const ChunkParams& P) {
-  return FORKS ? P.batch + P.group_count : P.batch;
+// The work of a request whose start, n, len, full and rows are known, from token
+// `floor` on, in tiles of TILE_ROWS rows.  With `tiles` the narrow form's tiles are those that the
+// rows' documents reach.
+template <int TILE_ROWS>
+__device__ __forceinline__ void ask_work(const ChunkParams& P, Asked& a, int floor, bool tiles) {
+  int tiles_of = 0, steps = 0, first_tile = 0, narrow = 0;
+  if (a.rows > kFewRows) {
+    tiles_of = (a.rows + TILE_ROWS - 1) / TILE_ROWS;
+    steps = wide_steps(P, max(a.len - floor, 0), TILE_ROWS);
+  } else if (a.rows > 0) {
+    int lo = P.window > 0 ? (int)max(0ll, (long long)a.full - a.n - P.window + 1) : 0;
+    if (P.first && tiles) {
+      int least = 0x7fffffff;
+      for (int i = 0; i < a.n; i += 4)  // four loads at a time
+#pragma unroll
+        for (int x = 0; x < 4; ++x) least = min(least, P.first[a.start + min(i + x, a.n - 1)]);
+      lo = max(lo, least);
+    }
+    first_tile = min(max(lo, floor), max(a.len - 1, 0)) / 32;
+    narrow = max(1, (a.len + 31) / 32 - first_tile);
+  }
+  a.tiles = tiles_of;
+  a.steps = steps;
+  a.first_tile = first_tile;
+  a.narrow = narrow;
 }
 
-// With `tiles` the narrow form's tiles are those that the rows' documents reach.
-template <bool FORKS>
 __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b, bool tiles) {
   Asked a{};
-  int start = 0, end = 0;
-  Group head{};
-  if constexpr (FORKS) {
-    // All that does not depend on each other is loaded in one round.
-    const int i = min(b, P.batch - 1);
-    const int s0 = P.starts[i], s1 = P.starts[i + 1], full = P.lengths[i];
-    head = groups_from(P, 0);
-    start = min(max(s0, 0), P.tokens);
-    end = min(max(s1, 0), P.tokens);
-    a.full = max(full, 0);
-    group_of(P, head, b, a.floor);
-    if (b >= P.batch) a.floor = 0;
-  } else if (b < P.batch) {
-    start = min(max(P.starts[b], 0), P.tokens);
-    end = min(max(P.starts[b + 1], 0), P.tokens);
-    a.full = max(P.lengths[b], 0);
-  }
   if (b < P.batch) {
-    a.start = start;
-    a.n = max(end - start, 0);
+    a.start = min(max(P.starts[b], 0), P.tokens);
+    a.n = max(min(max(P.starts[b + 1], 0), P.tokens) - a.start, 0);
+    a.full = max(P.lengths[b], 0);
     a.len = min(a.full, P.max_pages * BC_PAGE_SIZE);
     a.rows = a.n * P.group;
-    if (a.rows > kFewRows) {
-      a.tiles = (a.rows + kManyRows - 1) / kManyRows;
-      a.steps = wide_steps(P, FORKS ? max(a.len - a.floor, 0) : a.len);
-    } else if (a.rows > 0) {
-      int lo = P.window > 0 ? (int)max(0ll, (long long)a.full - a.n - P.window + 1) : 0;
-      if (P.first && tiles) {
-        int least = 0x7fffffff;
-        for (int i = 0; i < a.n; i += 4)  // four loads at a time
-#pragma unroll
-          for (int x = 0; x < 4; ++x) least = min(least, P.first[a.start + min(i + x, a.n - 1)]);
-        lo = max(lo, least);
-      }
-      if constexpr (FORKS) lo = max(lo, a.floor);
-      a.first_tile = min(lo, max(a.len - 1, 0)) / 32;
-      a.narrow = max(1, (a.len + 31) / 32 - a.first_tile);
-    }
-  }
-  if constexpr (FORKS) {
-    // A group's entry: its members from the lane that holds it, and, where the lanes
-    // hold all requests, the ends of its rows from theirs.
-    const int g = b - P.batch;
-    Group x{__shfl(head.g0, max(g, 0), 64), __shfl(head.g1, max(g, 0), 64), __shfl(head.shared, max(g, 0), 64)};
-    if (g >= 64 && g < P.group_count) x = group_at(P, g);
-    int from = __shfl(start, x.g0, 64), to = __shfl(end, x.g1 - 1, 64);
-    const bool is = g >= 0 && g < P.group_count && x.shared > 0;
-    if (is && (P.batch > 64 || b >= 64)) {
-      from = min(max(P.starts[x.g0], 0), P.tokens);
-      to = min(max(P.starts[x.g1], 0), P.tokens);
-    }
-    if (is) {
-      a.g0 = x.g0;
-      a.g1 = x.g1;
-      a.start = from;
-      a.n = max(to - from, 0);
-      a.len = x.shared;
-      a.rows = a.n * P.group;
-      // What the members' rows see of it under a window, or of documents, takes a
-      // look at each of them: the wide form does.
-      if (a.rows > kFewRows || (a.rows > 0 && (P.window > 0 || P.first))) {
-        a.tiles = (a.rows + kManyRows - 1) / kManyRows;
-        a.steps = wide_steps(P, a.len);
-      } else if (a.rows > 0) {
-        a.narrow = (a.len + 31) / 32;
-      }
-    }
+    ask_work<kManyRows>(P, a, 0, tiles);
   }
   return a;
 }
@@ -548,13 +457,13 @@ struct Cutting {
 
 // `ROUND`: the shares fill what the narrow requests' workgroups leave of a round;
 // else both are cut to the same time, if each had a part of the card to itself.
-template <bool FORKS, bool ROUND>
+template <bool ROUND>
 __device__ __forceinline__ Cutting cut_batch(const TileParams& P, const Asked& head, int lane) {
   const ChunkParams& C = P.c;
   float work = (float)head.tiles * (float)head.steps;
   int narrow = head.narrow;
-  for (int b = 64 + lane; b - lane < entries_of<FORKS>(C); b += 64) {
-    const Asked x = asked_of<FORKS>(C, b, true);
+  for (int b = 64 + lane; b - lane < C.batch; b += 64) {
+    const Asked x = asked_of(C, b, true);
     work += (float)x.tiles * (float)x.steps;
     narrow += x.narrow;
   }
@@ -587,8 +496,8 @@ struct Item {
 };
 
 // Entry b0 + at of the batch, of which lane `at` holds what is asked.
-template <bool FORKS>
-__device__ __forceinline__ Request request_at(const ChunkParams& C, const Asked& a, int b0, int at) {
+template <bool FORKS, typename A>
+__device__ __forceinline__ Request request_at(const ChunkParams& C, const A& a, int b0, int at) {
   Request r{b0 + at, __builtin_amdgcn_readlane(a.start, at), __builtin_amdgcn_readlane(a.len, at),
             __builtin_amdgcn_readlane(a.full - a.n, at), __builtin_amdgcn_readlane(a.rows, at)};
   if constexpr (FORKS) {
@@ -609,16 +518,15 @@ __device__ __forceinline__ Request request_at(const ChunkParams& C, const Asked&
 // counted are those whose writer, the first part's workgroup, is among the
 // first `launched` items and has place for its parts.  Both bounds rise from
 // one record to the next, so these are the first ones.
-template <bool FORKS>
 __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int share, long long idx,
                                           int lane, bool all, int launched) {
   const ChunkParams& C = P.c;
-  const bool split = FORKS || P.part_acc != nullptr;
+  const bool split = P.part_acc != nullptr;
   Item it{};
   long long before = 0;
   int slots = 0, cut = 0, records = 0, narrow = 0;
-  for (int b0 = 0; b0 < entries_of<FORKS>(C); b0 += 64) {
-    if (b0 > 0) a = asked_of<FORKS>(C, b0 + lane, split);
+  for (int b0 = 0; b0 < C.batch; b0 += 64) {
+    if (b0 > 0) a = asked_of(C, b0 + lane, split);
     const int parts = split && a.steps > share ? (a.steps + share - 1) / share : 1;
     const int tiles = split ? a.tiles : a.tiles + (a.narrow > 0);
     const int mine = tiles * parts;
@@ -629,7 +537,7 @@ __device__ __forceinline__ Item plan_item(const TileParams& P, Asked a, int shar
       const int local = (int)(idx - before);
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > local));
       it.found = true;
-      it.r = request_at<FORKS>(C, a, b0, at);
+      it.r = request_at<false>(C, a, b0, at);
       it.parts = __builtin_amdgcn_readlane(parts, at);
       const int in = local - __builtin_amdgcn_readlane(upto - mine, at);
       const int nth = it.parts == 1 ? in : in / it.parts;
@@ -1003,6 +911,14 @@ __device__ __forceinline__ void values16(const u32x4& w, float power, u32x4& lo,
              values2<T, true>(w[3], power)};
 }
 
+// Of 64 rising numbers, one per lane, how many are at most `x`.
+__device__ __forceinline__ int count_upto(int number, int x) {
+  int n = 0;
+#pragma unroll
+  for (int step = 32; step; step >>= 1) n += __shfl(number, n + step - 1, 64) <= x ? step : 0;
+  return n + (__shfl(number, n, 64) <= x ? 1 : 0);
+}
+
 // The member of a group that row t, a lane's own, belongs to, the row's place in
 // it, and its length.  All lanes of the wave take part.
 struct Place {
@@ -1129,26 +1045,6 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
   P.records[2 + 2 * i] = make_int4(first, stride, 0, 0);
 }
 
-// With groups: the record of tile `tile` of an entry whose rows start at `start`.
-// No two entries have one in common, since the rows of the ones before end there.
-__device__ __forceinline__ int record_of(const TileParams& P, int entry, int start, int tile) {
-  const int from = entry < P.c.batch ? entry : P.own_records + entry - P.c.batch;
-  return from + start * P.c.group / kManyRows + tile;
-}
-
-// The partial row of an entry's first row, where a tile is in one piece.
-__device__ __forceinline__ int single_row(const TileParams& P, const Request& rq) {
-  const int rows = P.c.tokens * P.c.group;
-  return P.single_rows + (is_group(rq) ? rows : 0) + rq.start * P.c.group;
-}
-
-// Part p of the tile's rows are the partial rows first + p * stride ...; parts 0:
-// there are none.
-__device__ __forceinline__ void put_fork_record(const TileParams& P, const Request& rq, int tile, int parts,
-                                                int first, int stride) {
-  P.records[record_of(P, rq.entry, rq.start, tile)] = make_int4(parts, first, stride, 0);
-}
-
 // The wide form: 128 rows per workgroup, 32 per wave, each 64-token step's K
 // and V shared through two LDS buffers, which loads straight into LDS fill one
 // step ahead; one barrier a step, two workgroups per CU (three at D = 64).
@@ -1161,7 +1057,7 @@ __device__ __forceinline__ void put_fork_record(const TileParams& P, const Reque
 //    over 2048, sixteen of them: 180 us, 670 TFLOP/s).
 //  - A full round of workgroups takes 8.6 us, launch included, and 2.1 per step
 //    (2048 new tokens over 2048 to 32768, none masked: 75.8 to 1082 us).
-template <typename T, int D, Form FORM, bool FP8, bool FORKS>
+template <typename T, int D, Form FORM, bool FP8>
 __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const Item& it, int kvh,
                                           uint16_t* s_kv, Seen* s_seen, int* s_bad) {
   const ChunkParams& C = A.c;
@@ -1192,20 +1088,13 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     }
   };
   if (tid < 4) s_bad[tid] = 0;
-  const bool by_rows = C.first || (FORKS && is_group(rq));  // what is seen depends on the rows
-  const bool ahead = FORKS && is_group(rq) && !C.first && C.window == 0;  // but not where it starts
-  if (!by_rows) {
+  if (!C.first) {
     mine = rows_seen(C, rq, row0, min(row0 + 32, rq.rows));
     wg = rows_seen(C, rq, tile0, min(tile0 + kManyRows, rq.rows));
     range();
-    load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
+    load_rows<T, D, FORM, false>(C, rq, row0 + lr, kvh, g, R, qB);
   } else {
-    if (ahead) {
-      wg.any_lo = 0;
-      wg.any_hi = rq.len - 1;
-      range();
-    }
-    load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
+    load_rows<T, D, FORM, false>(C, rq, row0 + lr, kvh, g, R, qB);
     mine = wave_seen(R, row0 + lr < rq.rows);
     if (lane == 0) s_seen[wave] = mine;
     __syncthreads();
@@ -1221,7 +1110,7 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     wg.any_hi = __builtin_amdgcn_readfirstlane(wg.any_hi);
     wg.all_lo = __builtin_amdgcn_readfirstlane(wg.all_lo);
     wg.all_hi = __builtin_amdgcn_readfirstlane(wg.all_hi);
-    if (!ahead) range();
+    range();
   }
 
   const int lrow = tid / CPR, lcol = 8 * (tid % CPR ^ swz<D>(lrow));
@@ -1387,9 +1276,8 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   const TileParams& P = reread(args);
   R.l += shfl_xor_f(R.l, 32);
   const int r = row0 + lr;
-  if (it.parts > 1 || (FORKS && joined(rq))) {
-    const int first = it.parts > 1 ? P.narrow_rows + (it.slot + it.part) * P.part_rows : single_row(P, rq) + tile0;
-    const size_t at = partial_row(P, first + wave * 32 + lr, kvh);
+  if (it.parts > 1) {
+    const size_t at = partial_row(P, P.narrow_rows + (it.slot + it.part) * P.part_rows + wave * 32 + lr, kvh);
     if (r < rq.rows) {
       if (g == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * at) = make_float2(R.m, R.l);
 #pragma unroll
@@ -1633,6 +1521,27 @@ struct Stream8 {
 template <typename T, int D, Form FORM, bool FP8>
 using StreamOf = typename std::conditional<FP8, Stream8<T, D, FORM>, Stream<T, D, FORM>>::type;
 
+// With groups: the record of tile `tile`, of tile_rows rows, of an entry whose new
+// tokens start at `start`.  No two entries have one in common, since the rows of the
+// ones before end there.
+__device__ __forceinline__ int record_of(const TileParams& P, int entry, int start, int tile) {
+  const int from = entry < P.c.batch ? entry : P.own_records + entry - P.c.batch;
+  return from + start * P.c.group / P.part_rows + tile;
+}
+
+// The partial row of an entry's first row, where a tile is in one piece.
+__device__ __forceinline__ int single_row(const TileParams& P, const Request& rq) {
+  const int rows = P.c.tokens * P.c.group;
+  return P.single_rows + (is_group(rq) ? rows : 0) + rq.start * P.c.group;
+}
+
+// Part p of the tile's rows are the partial rows first + p * stride ...; parts 0:
+// there are none.
+__device__ __forceinline__ void put_fork_record(const TileParams& P, const Request& rq, int tile, int parts,
+                                                int first, int stride) {
+  P.records[record_of(P, rq.entry, rq.start, tile)] = make_int4(parts, first, stride, 0);
+}
+
 // The narrow form over a batch: the tiles of all requests with few rows, one
 // after another, in ranges of equal length, a range per wave.  HBM-bound: 64
 // single tokens over 128-4096 tokens (32/8 heads, D = 128, 585 MB) 96 us, 6.5
@@ -1643,13 +1552,15 @@ using StreamOf = typename std::conditional<FP8, Stream8<T, D, FORM>, Stream<T, D
 // range leaves a partial.  Range r's partial of a request whose predecessors
 // have n rows starts at partial row 32 r + n: a range's next request is
 // further by the rows of the last one, a request's next range by 32.
-template <typename T, int D, Form FORM, bool FP8, bool FORKS>
-__device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cutting& cut,
+// `ask(b0)` is what is asked of the requests (with groups: entries) b0 .. b0 + 63,
+// `a` of the first, and `batch` how many there are; W waves per workgroup.
+template <typename T, int D, Form FORM, bool FP8, bool FORKS, int W, typename A, typename F>
+__device__ __forceinline__ void flat_body(const TileParams& P, A a, int batch, F ask, const Cutting& cut,
                                           uint16_t* s_kv) {
   const ChunkParams& C = P.c;
   const int lane = threadIdx.x & 63, g = lane >> 5, lr = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned task = 4 * blockIdx.x + wave;
+  const unsigned task = W * blockIdx.x + wave;
   const int range = task / (unsigned)C.hkv, kvh = task - (unsigned)range * C.hkv;
   if ((long long)range * cut.run >= cut.narrow) return;
   const int lo = range * cut.run, hi = min(lo + cut.run, cut.narrow);
@@ -1675,8 +1586,8 @@ __device__ __forceinline__ void flat_body(const TileParams& P, Asked a, const Cu
       rows_before += __builtin_amdgcn_readlane(rows_upto, 63);
       nth += __builtin_popcountll(some);
       b0 += 64;
-      if (b0 >= entries_of<FORKS>(C) || before >= hi) return false;
-      a = asked_of<FORKS>(C, b0 + lane, true);
+      if (b0 >= batch || before >= hi) return false;
+      a = ask(b0);
       look();
     }
     const int at = __builtin_ctzll(left);
@@ -1874,18 +1785,18 @@ __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request&
 }
 
 // Zeros for the rows of no request, by the workgroups that have no item.
-template <int D>
+template <int D, int THREADS>
 __device__ __forceinline__ void clear_rows(const ChunkParams& C, long long at, long long of) {
   const int head = min(max(C.starts[0], 0), C.tokens);
   const int tail = min(max(C.starts[C.batch], 0), C.tokens);
   const long long row = (long long)C.hq * (D / 8), gap = (long long)(tail - head) * row;
   const long long total = (long long)C.tokens * row - gap;
   u32x4* const out = reinterpret_cast<u32x4*>(C.out);
-  for (long long x = at * 256 + threadIdx.x; x < total; x += of * 256)
+  for (long long x = at * THREADS + threadIdx.x; x < total; x += of * THREADS)
     out[x < head * row ? x : x + gap] = u32x4{0, 0, 0, 0};
 }
 
-template <typename T, int D, Form FORM, bool FP8, bool FORKS>
+template <typename T, int D, Form FORM, bool FP8>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TileParams) {
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[2 * 2 * kStep * D];
   __shared__ float2 s_ml[4 * 32];
@@ -1894,11 +1805,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
   const int lane = threadIdx.x & 63;
   const Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
   const TileParams& P = reread(args);
-  pin_plan<FORKS>(P);
-  const Asked head = asked_of<FORKS>(P.c, lane, FORKS || P.part_acc != nullptr);
+  pin_plan(P);
+  const Asked head = asked_of(P.c, lane, P.part_acc != nullptr);
   Cutting cut{};
-  if (FORKS || P.part_acc) cut = cut_batch<FORKS, FORKS || FP8>(P, head, lane);
-  const bool counts = !FORKS && blockIdx.x == 0 && P.part_acc;
+  if (P.part_acc) cut = cut_batch<FP8>(P, head, lane);
+  const bool counts = blockIdx.x == 0 && P.part_acc;
   // The narrow requests first: theirs is memory's time, the others' the
   // matrix units', so they run beside each other.
   const bool flat = (int)blockIdx.x < cut.groups;
@@ -1908,38 +1819,31 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
   Item it{};
   if (!flat || counts) {
     const int launched = counts ? (int)(gridDim.x - cut.groups + P.c.hkv - 1) / P.c.hkv : 0;
-    it = plan_item<FORKS>(P, head, cut.share, flat ? -1ll : (long long)at, lane, counts, launched);
+    it = plan_item(P, head, cut.share, flat ? -1ll : (long long)at, lane, counts, launched);
   }
   if (counts && threadIdx.x == 0) P.records[0] = make_int4(it.records, it.narrow_records, 0, 0);
   if (flat) {
     const TileParams& A = reread(args);
     pin_rows<FP8>(A);
-    flat_body<T, D, FORM, FP8, FORKS>(A, head, cut, s_kv);
+    auto ask = [&](int b0) { return asked_of(A.c, b0 + lane, true); };
+    flat_body<T, D, FORM, FP8, false, 4>(A, head, A.c.batch, ask, cut, s_kv);
     return;
   }
   if (!it.found) {
     const long long items = it.items * P.c.hkv + cut.groups;
-    clear_rows<D>(P.c, blockIdx.x - items, gridDim.x - items);
+    clear_rows<D, 256>(P.c, blockIdx.x - items, gridDim.x - items);
     return;
   }
-  if constexpr (FORKS) {
-    if (it.part == 0 && kvh == 0 && threadIdx.x == 0)
-      put_fork_record(P, it.r, it.tile, it.parts,
-                      it.parts > 1 ? P.narrow_rows + it.slot * P.part_rows
-                                   : single_row(P, it.r) + it.tile * kManyRows,
-                      P.part_rows);
-  } else {
-    if (it.parts > 1 && it.part == 0 && kvh == 0 && threadIdx.x == 0)
-      put_record(P, it.record, it.r.start, it.tile * kManyRows,
-                 min(it.r.rows - it.tile * kManyRows, kManyRows), it.parts,
-                 P.narrow_rows + it.slot * P.part_rows, P.part_rows);
-  }
+  if (it.parts > 1 && it.part == 0 && kvh == 0 && threadIdx.x == 0)
+    put_record(P, it.record, it.r.start, it.tile * kManyRows,
+               min(it.r.rows - it.tile * kManyRows, kManyRows), it.parts,
+               P.narrow_rows + it.slot * P.part_rows, P.part_rows);
   const TileParams& A = reread(args);
   pin_rows<FP8>(A);
-  if (!FORKS && it.r.rows <= kFewRows)
+  if (it.r.rows <= kFewRows)
     narrow_body<T, D, FORM, FP8>(A.c, it.r, kvh, s_kv, s_ml);
   else
-    wide_body<T, D, FORM, FP8, FORKS>(A, args, it, kvh, s_kv, s_seen, s_bad);
+    wide_body<T, D, FORM, FP8>(A, args, it, kvh, s_kv, s_seen, s_bad);
 }
 
 // One part's state joined to another's.
@@ -2023,81 +1927,6 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(TileParams P, int apart
   }
 }
 
-// The join with groups: `apart` waves share the rows of a new token and KV head; of
-// a wave, each group of D / 4 lanes takes the parts of the request's own tokens and
-// then of its group's in turn.  Rows that their entry has written as output are
-// left.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void fork_join_kernel(TileParams P, int apart) {
-  constexpr int LPR = D / 4, GW = 64 / LPR;
-  const ChunkParams& C = P.c;
-  const int lane = threadIdx.x & 63, grp = lane / LPR, c = lane % LPR;
-  const long long total = (long long)C.tokens * C.hkv * apart, step = 4ll * gridDim.x;
-  for (long long x = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); x < total; x += step) {
-    const long long pair = x / apart;
-    const int sub = (int)(x - pair * apart), t = (int)(pair / C.hkv), kvh = (int)(pair - (long long)t * C.hkv);
-    // The request of token t, the first of its rows, and its group, of loads in one
-    // round for up to 64 of either.
-    const Group head = groups_from(C, 0);
-    int b = 0, own0 = 0;
-    for (int i = 0; i < C.batch; i += 64) {
-      const int from = C.starts[min(i + lane, C.batch - 1)], to = C.starts[min(i + lane, C.batch - 1) + 1];
-      const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < C.batch && to <= t));
-      b += n;
-      if (n < 64) {
-        own0 = __builtin_amdgcn_readlane(from, n);
-        break;
-      }
-    }
-    if (b >= C.batch || own0 > t) continue;
-    int shared;
-    const int g = __builtin_amdgcn_readfirstlane(group_of(C, head, b, shared));
-    shared = __builtin_amdgcn_readfirstlane(shared);
-    auto start_of = [&](int from) { return min(max(from, 0), C.tokens); };
-    own0 = start_of(own0);
-    const int all0 = shared > 0 ? start_of(C.starts[group_at(C, g).g0]) : 0;
-    for (int r = sub; r < C.group; r += apart) {
-      int parts[2] = {}, first[2] = {}, stride[2] = {};
-      auto look = [&](int i, int entry, int from) {
-        if (t < from) return;
-        const int row = (t - from) * C.group + r, tile = row / kManyRows;
-        const int4 rec = P.records[record_of(P, entry, from, tile)];
-        // Where starts decrease, a record may be another's or no one's.
-        const long long last = rec.y + (long long)max(rec.x - 1, 0) * rec.z + row - tile * kManyRows;
-        const bool sane = rec.x > 0 && rec.x <= 2 * (P.waves + P.most_parts) && rec.y >= 0 && rec.z > 0 &&
-                          last < P.total_rows;
-        parts[i] = sane ? rec.x : 0;
-        first[i] = rec.y + row - tile * kManyRows;
-        stride[i] = rec.z;
-      };
-      look(0, b, own0);
-      if (shared > 0)
-        look(1, C.batch + g, all0);
-      else if (parts[0] < 2)
-        continue;
-      float m = kNegInf, l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int p = grp; p < parts[0] + parts[1]; p += GW) {
-        const bool own = p < parts[0];
-        const int at = own ? first[0] + p * stride[0] : first[1] + (p - parts[0]) * stride[1];
-        const size_t row = partial_row(P, at, kvh);
-        const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * row);
-        join(m, l, acc, ml.x, ml.y, *reinterpret_cast<const float4*>(P.part_acc + row * D + 4 * c));
-      }
-#pragma unroll
-      for (int s = LPR; s < 64; s <<= 1)
-        join(m, l, acc, shfl_xor_f(m, s), shfl_xor_f(l, s),
-             make_float4(shfl_xor_f(acc.x, s), shfl_xor_f(acc.y, s), shfl_xor_f(acc.z, s),
-                         shfl_xor_f(acc.w, s)));
-      const float inv = one_over(l);
-      if (grp == 0)
-        *reinterpret_cast<uint2*>(C.out + ((size_t)t * C.hq + kvh * C.group + r) * D + 4 * c) =
-            make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-    }
-  }
-}
-
 // How a call with a workspace cuts its work; bytes 0: it does not.
 struct Cut {
   int target, waves, most_parts, part_rows, narrow_rows;
@@ -2155,11 +1984,11 @@ hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned
     P.narrow_rows = cut.narrow_rows;
   }
   if (C.cap > 0.f)
-    chunk_tile_kernel<T, D, Form::kCap, FP8, false><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kCap, FP8><<<dim3(grid), 256, 0, st>>>(P);
   else if (C.slopes)
-    chunk_tile_kernel<T, D, Form::kBias, FP8, false><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kBias, FP8><<<dim3(grid), 256, 0, st>>>(P);
   else
-    chunk_tile_kernel<T, D, Form::kPlain, FP8, false><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kPlain, FP8><<<dim3(grid), 256, 0, st>>>(P);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !ws) return err;
   // Enough workgroups for the rows of a record and KV head, on average, but not
@@ -2184,14 +2013,14 @@ hipError_t launch_tiles(const ChunkParams& P, int dim, int dtype, const Cut& cut
                    : launch_tiles<__bf16, 128, FP8>(P, cut, ws, (unsigned)grid, st);
 }
 
-// Workgroups of the tile kernel with a workspace, at most, of a batch whose entries
-// of more than 32 rows have `rows` rows in all.  Cut by shares, n tiles have less
-// than target / Hkv + n parts.  A workgroup without work still walks the batch to
-// see that, some 2 us, so none is launched beyond these.
-inline long long split_grid(const bc_shape& s, const Cut& cut, long long rows, long long entries) {
+// Workgroups of W waves of the tile kernel with a workspace, at most, of a batch
+// whose entries of more than 32 rows have `rows` rows in all.  Cut by shares, n
+// tiles have less than target / Hkv + n parts.  A workgroup without work still walks
+// the batch to see that, some 2 us, so none is launched beyond these.
+inline long long split_grid(const bc_shape& s, const Cut& cut, long long rows, long long entries, int W) {
   const long long wide = rows / (kFewRows + 1) < entries ? rows / (kFewRows + 1) : entries;
-  const long long items = wide > 0 ? rows / kManyRows + wide + cut.target / s.kv_heads + 1 : 0;
-  return items * s.kv_heads + ((long long)cut.waves * s.kv_heads + 3) / 4 + 1;
+  const long long items = wide > 0 ? rows / (32 * W) + wide + cut.target / s.kv_heads + 1 : 0;
+  return items * s.kv_heads + ((long long)cut.waves * s.kv_heads + W - 1) / W + 1;
 }
 
 // Workgroups of the tile kernel, at most.
