@@ -15,16 +15,20 @@
 
 namespace {
 
-// Waves per workgroup, each with 32 rows of a tile, and the steps that LDS holds.
-//  - D = 128: 256 rows, one workgroup per CU.  A group of up to 256 rows reads each
-//    page once; what is read once comes from HBM, some 2 us away under load, which
-//    three steps on their way cover.
-//  - D = 64: 128 rows, three workgroups per CU, as in the chunk attention: the softmax
-//    of three waves per SIMD is the bound there, not memory.
-template <int D>
-struct Form2 {
-  static constexpr int W = D == 128 ? 8 : 4;
-  static constexpr int kBuffers = D == 128 ? 4 : 3;
+// W waves per workgroup, each with 32 rows of a tile, and the steps of K and V that
+// LDS holds: those on their way, the one at hand, and, where half the waves lag by
+// half a step, the one before it.
+//  - D = 128, W = 8: one workgroup per CU, for groups of more than 128 rows, which so
+//    read each page once per 256.  What is read once comes from HBM, some 2 us away
+//    under load.
+//  - D = 128, W = 4: two per CU.  D = 64: three, since the softmax of three waves per
+//    SIMD is the bound there, not memory.
+template <int D, int W>
+struct Plan {
+  static constexpr bool kLag = W == 8;
+  static constexpr int kBuffers = kLag ? 4 : D == 64 ? 3 : 2;
+  static constexpr int kAhead = kLag ? 2 : kBuffers - 1;
+  static constexpr int kPerCu = kLag ? 1 : D == 64 ? 3 : 2;
 };
 
 // ---------------------------------------------------------------------------
@@ -147,9 +151,13 @@ struct Entries {
   }
 };
 
-// How the batch is cut, see Cutting: a step of the wide form takes its workgroup
-// about as long as a tile of the narrow one takes each of its waves.  What the
-// narrow entries leave of a round of workgroups is filled with shares.
+// How the batch is cut, see Cutting: a tile of the narrow form takes each of its
+// waves about kTileTime times as long as a step of the wide one takes its
+// workgroup.  What the narrow entries leave of a round of workgroups is filled with
+// shares.
+constexpr float kTileTime = 1.8f;
+constexpr int kLeastTiles = 2;  // fewest per wave
+
 template <int W>
 __device__ __forceinline__ Cutting cut_entries(const TileParams& P, const Entries<W>& all) {
   const ChunkParams& C = P.c;
@@ -164,9 +172,9 @@ __device__ __forceinline__ Cutting cut_entries(const TileParams& P, const Entrie
   Cutting c;
   work = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, wave_sum(work))));
   c.narrow = lanes_sum(narrow);
-  const float run = ((float)c.narrow + W * work) / (float)P.waves;
+  const float run = ((float)c.narrow + W / kTileTime * work) / (float)P.waves;
   c.run = max(min((int)__builtin_fminf(run, 1e9f) + 1, c.narrow), (c.narrow + P.waves - 1) / P.waves);
-  c.run = max(c.run, kLeastRun);
+  c.run = max(c.run, kLeastTiles);
   c.groups = ((c.narrow + c.run - 1) / c.run * C.hkv + W - 1) / W;
   // n tiles have less than work / share + n parts: one more than a round holds
   // would take the time of a second round.
@@ -218,14 +226,15 @@ __device__ __forceinline__ Item plan_entry(const TileParams& P, const Entries<W>
 
 // The wide form, with more rows per workgroup and more steps on their way than
 // wide_body has: 32 W rows, and kBuffers steps of K and V in LDS, of which one is
-// worked on while the others are filled.  One barrier a step, before which each wave
+// worked on while others are filled.  One barrier a step, before which each wave
 // waits for its own loads of the next step only.
-template <typename T, int D, Form FORM>
+template <typename T, int D, Form FORM, int W>
 __device__ __forceinline__ void deep_body(const TileParams& A, Args args, const Item& it, int kvh,
                                           uint16_t* s_kv, int* s_ids, Seen* s_seen, int* s_bad) {
   const ChunkParams& C = A.c;
   const Request& rq = it.r;
-  constexpr int W = Form2<D>::W, BUFFERS = Form2<D>::kBuffers, THREADS = 64 * W;
+  typedef Plan<D, W> L;
+  constexpr int BUFFERS = L::kBuffers, AHEAD = L::kAhead, THREADS = 64 * W;
   constexpr int KS = D / 16, CPR = D / 8;
   constexpr int NX = kStep * CPR / THREADS;   // chunks per thread and step, of K and of V each
   constexpr int HALF = kStep * D;             // halves of a step's K, then as many of V
@@ -277,7 +286,7 @@ __device__ __forceinline__ void deep_body(const TileParams& A, Args args, const 
   };
   auto issue_first = [&] {
 #pragma unroll
-    for (int u = 0; u < BUFFERS - 1; ++u) issue(u);
+    for (int u = 0; u < AHEAD; ++u) issue(u);
   };
   // Where the rows' places do not matter to what is read, the first steps go out
   // ahead of them: a group's rows see all that it shares.
@@ -325,11 +334,10 @@ __device__ __forceinline__ void deep_body(const TileParams& A, Args args, const 
     }
     return bad;
   };
-  // Until the loads of step t are there, of which `behind` steps' may be on their way.
+  // Until the loads of a step are there, of which those of `behind` more steps may
+  // be on their way.
   auto wait_step = [&](int behind) {
-    if (BUFFERS > 3 && behind >= 2)
-      wait_to<4 * NX>();
-    else if (behind >= 1)
+    if (AHEAD > 1 && behind > 0)
       wait_to<2 * NX>();
     else
       wait_loads();
@@ -337,21 +345,22 @@ __device__ __forceinline__ void deep_body(const TileParams& A, Args args, const 
 
   const Offsets<D> o = read_offsets<D>(lane);
   const float scale2 = scale2_of(C, FORM);
+  f32x16 sc[2];
+  // Of the step at hand: its buffer, and what was taken out of it.
+  int buf = 0;
   bool bad = false;
   wait_rows(qB);
   if (t0 < tend) {
-    wait_step(min(tend - 1 - t0, BUFFERS - 2));
+    wait_step(min(tend - 1 - t0, AHEAD - 1));
     if (!is_whole(t0)) bad = inspect(t0, 0);
     bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));
   }
-  int buf = 0, to = BUFFERS - 1;  // the step's at hand, and the one that is filled next
-#pragma unroll 1
-  for (int t = t0; t < tend; ++t) {
+  auto scores = [&](int t, Edges& e) {
     const uint16_t* const kt = s_kv + buf * (2 * HALF);
-    const int u = t + BUFFERS - 1, at = (u - t0) % 16;
+    const int u = t + AHEAD, at = (u - t0) % 16;
+    const int to = buf + AHEAD < BUFFERS ? buf + AHEAD : buf + AHEAD - BUFFERS;
     const bool next = u < tend;
     if (next && at == 0) take(u);
-    f32x16 sc[2];
     u32x4 kf[2][KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -368,30 +377,57 @@ __device__ __forceinline__ void deep_body(const TileParams& A, Args args, const 
         if (next) issue_chunk(s / 2, at, to);
       }
     }
-    Edges e{t * kStep < mine.all_lo, t * kStep + kStep - 1 > mine.all_hi, (pages & 15u) != 15u, 0};
+    e = Edges{t * kStep < mine.all_lo, t * kStep + kStep - 1 > mine.all_hi, (pages & 15u) != 15u, 0};
     if (e.pages) e.valid = tokens_of<4>(rq.len - t * kStep, pages & 15u);
+    if (next) pages |= ((unsigned)(pg.in_pool >> (4 * at)) & 15u) << (4 * AHEAD);
+  };
+  auto product = [&](int t, const Edges& e, int of, bool untidy) {
     finish_scores<D, FORM, 2>(C, sc, R, t * kStep, g, e);
     constexpr bool kAhead = D == 128 && FORM != Form::kCap;  // as in wide_body
     if (kAhead) __builtin_amdgcn_s_setprio(2);
-    weigh<T, D, 2>(sc, R, kt + HALF, o, scale2);
+    weigh<T, D, 2>(sc, R, s_kv + of * (2 * HALF) + HALF, o, scale2);
     if (kAhead) __builtin_amdgcn_s_setprio(0);
-    if (bad) add_untidy<T, D, false>(C, rq, kvh, R, t * kStep, kStep, g);
-    if (next) pages |= ((unsigned)(pg.in_pool >> (4 * at)) & 15u) << (4 * (BUFFERS - 1));
+    if (untidy) add_untidy<T, D, false>(C, rq, kvh, R, t * kStep, kStep, g);
+  };
+  auto end_step = [&](int t) {
     pages >>= 4;
     buf = buf + 1 < BUFFERS ? buf + 1 : 0;
-    to = to + 1 < BUFFERS ? to + 1 : 0;
     // Step s of the part sets flag s % 4 before the barrier that ends the step
     // before it; the flag is read behind that barrier and cleared behind the
     // next, two barriers before it is set again.
     const int s = t - t0;
     const bool look = t + 1 < tend && !is_whole(t + 1);
     if (t + 1 < tend) {
-      wait_step(min(tend - 2 - t, BUFFERS - 2));
+      wait_step(min(tend - 2 - t, AHEAD - 1));
       if (look && inspect(t + 1, buf)) s_bad[(s + 1) & 3] = 1;
     }
     __syncthreads();
     if (bad && tid == 0) s_bad[s & 3] = 0;
     bad = look && __builtin_amdgcn_readfirstlane(s_bad[(s + 1) & 3]);
+  };
+  if (!L::kLag || wave < W / 2) {
+#pragma unroll 1
+    for (int t = t0; t < tend; ++t) {
+      Edges e;
+      scores(t, e);
+      product(t, e, buf, bad);
+      end_step(t);
+    }
+  } else if (t0 < tend) {
+    // The other half of a SIMD's waves: a step's product behind the barrier that ends
+    // the step, so that it runs beside the scores of the first half, and the reverse.
+    Edges e;
+    scores(t0, e);
+    bool untidy = bad;
+    end_step(t0);
+#pragma unroll 1
+    for (int t = t0 + 1; t < tend; ++t) {
+      product(t - 1, e, buf > 0 ? buf - 1 : BUFFERS - 1, untidy);
+      scores(t, e);
+      untidy = bad;
+      end_step(t);
+    }
+    product(tend - 1, e, buf > 0 ? buf - 1 : BUFFERS - 1, untidy);
   }
 
   const TileParams& P = reread(args);
@@ -425,10 +461,9 @@ __device__ __forceinline__ void deep_body(const TileParams& A, Args args, const 
   }
 }
 
-template <typename T, int D, Form FORM>
-__global__ __launch_bounds__(64 * Form2<D>::W, D == 64 ? 3 : 2) void fork_tile_kernel(TileParams) {
-  constexpr int W = Form2<D>::W;
-  constexpr int kWide = Form2<D>::kBuffers * 2 * kStep * D, kFlat = W * 64 * D;
+template <typename T, int D, Form FORM, int W>
+__global__ __launch_bounds__(64 * W, D == 64 ? 3 : 2) void fork_tile_kernel(TileParams) {
+  constexpr int kWide = Plan<D, W>::kBuffers * 2 * kStep * D, kFlat = W * 64 * D;
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[kWide > kFlat ? kWide : kFlat];
   __shared__ int s_ids[64 * W];
   __shared__ Seen s_seen[W];
@@ -462,7 +497,7 @@ __global__ __launch_bounds__(64 * Form2<D>::W, D == 64 ? 3 : 2) void fork_tile_k
                     P.part_rows);
   const TileParams& A = reread(args);
   pin_rows<false>(A);
-  deep_body<T, D, FORM>(A, args, it, kvh, s_kv, s_ids, s_seen, s_bad);
+  deep_body<T, D, FORM, W>(A, args, it, kvh, s_kv, s_ids, s_seen, s_bad);
 }
 
 // The join with groups: `apart` waves share the rows of a new token and KV head; of
@@ -547,7 +582,11 @@ struct ForkCut : Cut {
   int single_rows, total_rows, own_records;
 };
 
-int waves_of(const bc_shape& s) { return s.dim == 128 ? Form2<128>::W : Form2<64>::W; }
+// Waves per workgroup, see Plan.
+int waves_of(const bc_shape& s, int tokens, int groups) {
+  const long long rows = (long long)tokens * (s.query_heads / s.kv_heads);
+  return s.dim == 128 && rows > 128ll * groups ? 8 : 4;
+}
 
 // How a call cuts its work; bytes 0: every request reads its own pages.
 ForkCut fork_cut(const bc_shape& s, int tokens, int groups) {
@@ -557,8 +596,9 @@ ForkCut fork_cut(const bc_shape& s, int tokens, int groups) {
       (s.batch + (long long)groups) * (s.max_pages + 1ll) > 1 << 28 ||
       (long long)s.batch * s.query_heads > 1 << 26)
     return c;
-  const int W = waves_of(s);
-  c.target = (s.dim == 128 ? 1 : 3) * bch::device_cus();  // workgroups in a round
+  const int W = waves_of(s, tokens, groups);
+  c.target = (W == 8 ? Plan<128, 8>::kPerCu : s.dim == 128 ? Plan<128, 4>::kPerCu : Plan<64, 4>::kPerCu) *
+             bch::device_cus();  // workgroups in a round
   c.waves = W * c.target / s.kv_heads > 1 ? W * c.target / s.kv_heads : 1;
   const long long own = rows < 32ll * s.batch ? rows : 32ll * s.batch;
   const long long of_groups = rows < 32ll * groups ? rows : 32ll * groups;
@@ -579,9 +619,8 @@ ForkCut fork_cut(const bc_shape& s, int tokens, int groups) {
   return c;
 }
 
-template <typename T, int D>
+template <typename T, int D, int W>
 hipError_t launch_forks(const ChunkParams& C, const ForkCut& cut, void* ws, unsigned grid, hipStream_t st) {
-  constexpr int THREADS = 64 * Form2<D>::W;
   char* const at = static_cast<char*>(ws);
   TileParams P{};
   P.c = C;
@@ -597,11 +636,11 @@ hipError_t launch_forks(const ChunkParams& C, const ForkCut& cut, void* ws, unsi
   P.total_rows = cut.total_rows;
   P.own_records = cut.own_records;
   if (C.cap > 0.f)
-    fork_tile_kernel<T, D, Form::kCap><<<dim3(grid), THREADS, 0, st>>>(P);
+    fork_tile_kernel<T, D, Form::kCap, W><<<dim3(grid), 64 * W, 0, st>>>(P);
   else if (C.slopes)
-    fork_tile_kernel<T, D, Form::kBias><<<dim3(grid), THREADS, 0, st>>>(P);
+    fork_tile_kernel<T, D, Form::kBias, W><<<dim3(grid), 64 * W, 0, st>>>(P);
   else
-    fork_tile_kernel<T, D, Form::kPlain><<<dim3(grid), THREADS, 0, st>>>(P);
+    fork_tile_kernel<T, D, Form::kPlain, W><<<dim3(grid), 64 * W, 0, st>>>(P);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   // A round of waves, eight workgroups per CU, with the rows of a token and KV head
@@ -612,6 +651,14 @@ hipError_t launch_forks(const ChunkParams& C, const ForkCut& cut, void* ws, unsi
   const long long join = (pairs * apart + 3) / 4;
   fork_join_kernel<T, D><<<dim3((unsigned)(join < most ? join : most)), 256, 0, st>>>(P, (int)apart);
   return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_forks(const ChunkParams& C, int dim, int W, const ForkCut& cut, void* ws, unsigned grid,
+                        hipStream_t st) {
+  return dim == 64 ? launch_forks<T, 64, 4>(C, cut, ws, grid, st)
+         : W == 4  ? launch_forks<T, 128, 4>(C, cut, ws, grid, st)
+                   : launch_forks<T, 128, 8>(C, cut, ws, grid, st);
 }
 
 }  // namespace
@@ -634,9 +681,9 @@ extern "C" int bc_shared_chunk_attention(bc_shape s, bc_chunk_inputs in, const i
   // under a window, or with documents, a group of few rows is of the wide form.
   const long long rows = (long long)in.tokens * (s.query_heads / s.kv_heads);
   const long long few = in.window > 0 || in.first ? (long long)(kFewRows + 1) * group_count : 0;
-  const long long grid =
-      split_grid(s, cut, 2 * rows + few, (long long)s.batch + group_count, waves_of(s));
-  const long long far = 1 << 26, most = kMostGroups * (long long)kThreads / (64 * waves_of(s));
+  const int W = waves_of(s, in.tokens, group_count);
+  const long long grid = split_grid(s, cut, 2 * rows + few, (long long)s.batch + group_count, W);
+  const long long far = 1 << 26, most = kMostGroups * (long long)kThreads / (64 * W);
   if (!use || !aligned16(in.q) || !aligned16(in.k) || !aligned16(in.v) || !aligned16(in.output) ||
       stride_bits(in) % 8 != 0 || in.k_strides.slot >= far || in.v_strides.slot >= far || grid > most)
     return bc_chunk_attention(s, in, nullptr, 0, stream);
@@ -646,9 +693,6 @@ extern "C" int bc_shared_chunk_attention(bc_shape s, bc_chunk_inputs in, const i
   P.shared = shared;
   P.group_count = group_count;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (in.dtype == BC_FLOAT16)
-    return s.dim == 64 ? launch_forks<_Float16, 64>(P, cut, workspace, (unsigned)grid, st)
-                       : launch_forks<_Float16, 128>(P, cut, workspace, (unsigned)grid, st);
-  return s.dim == 64 ? launch_forks<__bf16, 64>(P, cut, workspace, (unsigned)grid, st)
-                     : launch_forks<__bf16, 128>(P, cut, workspace, (unsigned)grid, st);
+  return in.dtype == BC_FLOAT16 ? launch_forks<_Float16>(P, s.dim, W, cut, workspace, (unsigned)grid, st)
+                                : launch_forks<__bf16>(P, s.dim, W, cut, workspace, (unsigned)grid, st);
 }
