@@ -501,11 +501,14 @@ __device__ __forceinline__ Request request_at(const ChunkParams& C, const A& a, 
   Request r{b0 + at, __builtin_amdgcn_readlane(a.start, at), __builtin_amdgcn_readlane(a.len, at),
             __builtin_amdgcn_readlane(a.full - a.n, at), __builtin_amdgcn_readlane(a.rows, at)};
   if constexpr (FORKS) {
-    r.entry = r.b;
     r.floor = __builtin_amdgcn_readlane(a.floor, at);
     r.g0 = __builtin_amdgcn_readlane(a.g0, at);
     r.g1 = __builtin_amdgcn_readlane(a.g1, at);
-    if (is_group(r)) r.b = r.g0;
+    r.entry = r.b;
+    if (is_group(r)) {  // those come behind the requests, from a full 64 on
+      r.entry += C.batch - (C.batch + 63) / 64 * 64;
+      r.b = r.g0;
+    }
   }
   r.prefix = prefix_of(C, r.b);
   return r;
@@ -942,16 +945,24 @@ __device__ __forceinline__ Place place_of(const ChunkParams& P, const Request& g
   return at;
 }
 
-// This lane's row of the wave's 32: its place, what it sees, and its Q.
-template <typename T, int D, Form FORM, bool FORKS>
-__device__ __forceinline__ void load_rows(const ChunkParams& C, const Request& it, int r, int kvh,
-                                          int g, Rows<D>& R, u32x4 (&qB)[D / 16]) {
+// Q of this lane's row of the wave's 32.
+template <int D>
+__device__ __forceinline__ void load_q(const ChunkParams& C, const Request& it, int r, int kvh, int g,
+                                       u32x4 (&qB)[D / 16]) {
   const bool real = r < it.rows;
   const int i = real ? by_group(C, r) : 0, h = kvh * C.group + (real ? r - i * C.group : 0);
   const int t = it.start + i;
   const uint16_t* const q = C.q + t * C.qt + h * C.qh + 8 * g;
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) qB[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
+}
+
+// The row's place and what it sees.
+template <int D, Form FORM, bool FORKS>
+__device__ __forceinline__ void start_rows(const ChunkParams& C, const Request& it, int r, int kvh, Rows<D>& R) {
+  const bool real = r < it.rows;
+  const int i = real ? by_group(C, r) : 0, h = kvh * C.group + (real ? r - i * C.group : 0);
+  const int t = it.start + i;
   R.pos = it.pos0 + i;
   int2 seen;
   if (FORKS && is_group(it)) {
@@ -975,6 +986,14 @@ __device__ __forceinline__ void load_rows(const ChunkParams& C, const Request& i
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int j = 0; j < 16; ++j) R.acc[dt][j] = 0.f;
+}
+
+// Both.
+template <typename T, int D, Form FORM, bool FORKS>
+__device__ __forceinline__ void load_rows(const ChunkParams& C, const Request& it, int r, int kvh,
+                                          int g, Rows<D>& R, u32x4 (&qB)[D / 16]) {
+  load_q<D>(C, it, r, kvh, g, qB);
+  start_rows<D, FORM, FORKS>(C, it, r, kvh, R);
 }
 
 // Bounds on what rows see: any of them the tokens any_lo .. any_hi at most, all
@@ -1611,10 +1630,20 @@ __device__ __forceinline__ void flat_body(const TileParams& P, A a, int batch, F
   int pages = st.in_pool(0);
   st.issue_k(0);
   st.issue_v(0);
+  // With groups a request's own part is short for a wave: Q comes a request ahead.
+  constexpr bool kAhead = FORKS;
+  u32x4 q_next[D / 16];
+  if constexpr (kAhead) load_q<D>(C, p.rq, lr, kvh, g, q_next);
   for (;;) {  // over the requests
     Rows<D> R;
     u32x4 qB[D / 16];
-    load_rows<T, D, FORM, FORKS>(C, p.rq, lr, kvh, g, R, qB);
+    if constexpr (kAhead) {
+      start_rows<D, FORM, FORKS>(C, p.rq, lr, kvh, R);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) qB[s] = q_next[s];
+    } else {
+      load_rows<T, D, FORM, FORKS>(C, p.rq, lr, kvh, g, R, qB);
+    }
     const Seen mine = C.first || (FORKS && is_group(p.rq)) ? wave_seen(R, lr < p.rq.rows)
                                                            : rows_seen(C, p.rq, 0, p.rq.rows);
     const int tend = p.first_tile + min(hi, p.x0 + p.tiles) - p.x0;
@@ -1624,6 +1653,9 @@ __device__ __forceinline__ void flat_body(const TileParams& P, A a, int batch, F
     const bool more = next_part(n);
     const int ids_more = more ? st.ids(n.rq.b, first_of(n), 1) : 0;
     wait_rows(qB);
+    if constexpr (kAhead) {
+      if (more) load_q<D>(C, n.rq, lr, kvh, g, q_next);
+    }
     for (;; ++t) {
       f32x16 sc[1];
       const bool same = t + 1 < tend, next = same || more;

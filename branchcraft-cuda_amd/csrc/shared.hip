@@ -29,10 +29,19 @@ struct Plan {
   static constexpr int kBuffers = kLag ? 4 : D == 64 ? 3 : 2;
   static constexpr int kAhead = kLag ? 2 : kBuffers - 1;
   static constexpr int kPerCu = kLag ? 1 : D == 64 ? 3 : 2;
+  static constexpr bool kRounds = kPerCu == 1;
 };
 
 // ---------------------------------------------------------------------------
 // The plan
+
+// threadIdx.x, found anew: what is computed from it belongs to the item at hand, and
+// does not take registers through the others.
+__device__ __forceinline__ int own_thread() {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
 
 // Group g: its members and the tokens they share, none of fewer than two members.
 struct Group {
@@ -78,76 +87,77 @@ __device__ __forceinline__ int group_of(const ChunkParams& P, const Group& head,
   return at;
 }
 
-// What an entry's work is found from, loaded before any of it is used.
-struct Loaded {
-  int start, end, full;
-};
-
-__device__ __forceinline__ Loaded load_entry(const ChunkParams& P, int b) {
-  const int i = min(b, P.batch - 1);
-  return {P.starts[i], P.starts[i + 1], P.lengths[i]};
-}
-
-template <int W>
-__device__ __forceinline__ AskedEntry entry_of(const ChunkParams& P, const Group& head, Loaded x, int b) {
-  const int start = min(max(x.start, 0), P.tokens), end = min(max(x.end, 0), P.tokens);
-  AskedEntry a{};
-  int floor;
-  group_of(P, head, b, floor);
-  if (b < P.batch) {
-    a.floor = floor;
-    a.start = start;
-    a.n = max(end - start, 0);
-    a.full = max(x.full, 0);
-    a.len = min(a.full, P.max_pages * BC_PAGE_SIZE);
-    a.rows = a.n * P.group;
-    ask_work<32 * W>(P, a, floor, true);
-  }
-  // A group's entry: its members from the lane that holds it, and, where the lanes
-  // hold all requests, the ends of its rows from theirs.
-  const int g = b - P.batch;
-  Group m{__shfl(head.g0, max(g, 0), 64), __shfl(head.g1, max(g, 0), 64), __shfl(head.shared, max(g, 0), 64)};
-  int from = __shfl(start, m.g0, 64), to = __shfl(end, m.g1 - 1, 64);
-  if (g >= 64 && g < P.group_count) m = group_at(P, g);
-  if (g >= 0 && g < P.group_count && m.shared > 0) {
-    if (P.batch > 64 || b >= 64) {
-      from = min(max(P.starts[m.g0], 0), P.tokens);
-      to = min(max(P.starts[m.g1], 0), P.tokens);
-    }
-    a.g0 = m.g0;
-    a.g1 = m.g1;
-    a.start = from;
-    a.n = max(to - from, 0);
-    a.len = m.shared;
-    a.rows = a.n * P.group;
-    // What the members' rows see of it under a window, or of documents, takes a
-    // look at each of them: the wide form does.
-    const bool wide = a.rows > kFewRows || (a.rows > 0 && (P.window > 0 || P.first));
-    a.tiles = wide ? (a.rows + 32 * W - 1) / (32 * W) : 0;
-    a.steps = wide ? wide_steps(P, a.len, 32 * W) : 0;
-    a.narrow = !wide && a.rows > 0 ? (a.len + 31) / 32 : 0;
-  }
-  return a;
-}
-
-// The entries of a batch, 64 at a time, one per lane; the first 128 stay.
+// The entries of a batch in blocks of 64, one per lane: the requests' blocks, then
+// the groups'.  The first two of the requests and the first of the groups stay, and
+// all that these do not depend on each other for is loaded in one round.
 template <int W>
 struct Entries {
-  const ChunkParams& C;
-  int lane, count;
-  Group head;
-  AskedEntry a0, a1;
-  __device__ __forceinline__ explicit Entries(const ChunkParams& c)
-      : C(c), lane(threadIdx.x & 63), count(c.batch + c.group_count), a1{} {
-    const Loaded x0 = load_entry(C, lane), x1 = load_entry(C, 64 + lane);
+  int lane, own_blocks, blocks;
+  Group head;  // a lane's of the first 64 groups
+  AskedEntry own0, own1, groups0;
+
+  __device__ __forceinline__ explicit Entries(const ChunkParams& C) : lane(own_thread() & 63), own1{} {
+    own_blocks = (C.batch + 63) / 64;
+    blocks = own_blocks + (C.group_count + 63) / 64;
+    const int3 x0 = load(C, lane), x1 = load(C, 64 + lane);
     head = groups_from(C, 0);
-    a0 = entry_of<W>(C, head, x0, lane);
-    if (count > 64) a1 = entry_of<W>(C, head, x1, 64 + lane);
+    own0 = request(C, x0, lane);
+    if (own_blocks > 1) own1 = request(C, x1, 64 + lane);
+    groups0 = group(C, head, lane);
   }
-  __device__ __forceinline__ AskedEntry at(const ChunkParams& c, int b0) const {
-    if (b0 == 0) return a0;
-    if (b0 == 64) return a1;
-    return entry_of<W>(c, head, load_entry(c, b0 + lane), b0 + lane);
+  __device__ __forceinline__ AskedEntry at(const ChunkParams& C, int block) const {
+    if (block == own_blocks) return groups0;
+    if (block == 0) return own0;
+    if (block == 1 && own_blocks > 1) return own1;
+    if (block < own_blocks) return request(C, load(C, 64 * block + lane), 64 * block + lane);
+    const int g = 64 * (block - own_blocks);
+    return group(C, groups_from(C, g), g + lane);
+  }
+
+ private:
+  static __device__ __forceinline__ int3 load(const ChunkParams& C, int b) {
+    const int i = min(b, C.batch - 1);
+    return make_int3(C.starts[i], C.starts[i + 1], C.lengths[i]);
+  }
+  __device__ __forceinline__ AskedEntry request(const ChunkParams& C, int3 x, int b) const {
+    AskedEntry a{};
+    int floor;
+    group_of(C, head, b, floor);
+    if (b < C.batch) {
+      a.floor = floor;
+      a.start = min(max(x.x, 0), C.tokens);
+      a.n = max(min(max(x.y, 0), C.tokens) - a.start, 0);
+      a.full = max(x.z, 0);
+      a.len = min(a.full, C.max_pages * BC_PAGE_SIZE);
+      a.rows = a.n * C.group;
+      ask_work<32 * W>(C, a, floor, true);
+    }
+    return a;
+  }
+  __device__ __forceinline__ AskedEntry group(const ChunkParams& C, const Group& m, int g) const {
+    AskedEntry a{};
+    // Where the lanes hold all requests, the ends of its rows are theirs.
+    int from = __shfl(own0.start, m.g0, 64), to = __shfl(own0.start + own0.n, m.g1 - 1, 64);
+    const bool is = g < C.group_count && m.shared > 0;
+    if (is && own_blocks > 1) {
+      from = min(max(C.starts[m.g0], 0), C.tokens);
+      to = min(max(C.starts[m.g1], 0), C.tokens);
+    }
+    if (is) {
+      a.g0 = m.g0;
+      a.g1 = m.g1;
+      a.start = from;
+      a.n = max(to - from, 0);
+      a.len = m.shared;
+      a.rows = a.n * C.group;
+      // What the members' rows see of it under a window, or of documents, takes a
+      // look at each of them: the wide form does.
+      const bool wide = a.rows > kFewRows || (a.rows > 0 && (C.window > 0 || C.first));
+      a.tiles = wide ? (a.rows + 32 * W - 1) / (32 * W) : 0;
+      a.steps = wide ? wide_steps(C, a.len, 32 * W) : 0;
+      a.narrow = !wide && a.rows > 0 ? (a.len + 31) / 32 : 0;
+    }
+    return a;
   }
 };
 
@@ -163,8 +173,8 @@ __device__ __forceinline__ Cutting cut_entries(const TileParams& P, const Entrie
   const ChunkParams& C = P.c;
   float work = 0.f;
   int narrow = 0, tiles = 0;
-  for (int b0 = 0; b0 < all.count; b0 += 64) {
-    const AskedEntry x = all.at(C, b0);
+  for (int block = 0; block < all.blocks; ++block) {
+    const AskedEntry x = all.at(C, block);
     work += (float)x.tiles * (float)x.steps;
     narrow += x.narrow;
     tiles += x.tiles;
@@ -188,12 +198,12 @@ __device__ __forceinline__ Cutting cut_entries(const TileParams& P, const Entrie
 template <int W>
 __device__ __forceinline__ Item plan_entry(const TileParams& P, const Entries<W>& all, int share, long long idx) {
   const ChunkParams& C = P.c;
-  const int lane = threadIdx.x & 63;
+  const int lane = own_thread() & 63;
   Item it{};
   long long before = 0;
   int slots = 0;
-  for (int b0 = 0; b0 < all.count; b0 += 64) {
-    const AskedEntry a = all.at(C, b0);
+  for (int block = 0; block < all.blocks; ++block) {
+    const AskedEntry a = all.at(C, block);
     const int parts = a.steps > share ? (a.steps + share - 1) / share : 1;
     const int mine = a.tiles * parts, cut_parts = parts > 1 ? mine : 0;
     const int upto = lanes_upto(mine);
@@ -202,7 +212,7 @@ __device__ __forceinline__ Item plan_entry(const TileParams& P, const Entries<W>
       const int local = (int)(idx - before);
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > local));
       it.found = true;
-      it.r = request_at<true>(C, a, b0, at);
+      it.r = request_at<true>(C, a, 64 * block, at);
       it.parts = __builtin_amdgcn_readlane(parts, at);
       const int in = local - __builtin_amdgcn_readlane(upto - mine, at);
       const int nth = it.parts == 1 ? in : in / it.parts;
@@ -239,7 +249,7 @@ __device__ __forceinline__ void deep_body(const TileParams& A, Args args, const 
   constexpr int NX = kStep * CPR / THREADS;   // chunks per thread and step, of K and of V each
   constexpr int HALF = kStep * D;             // halves of a step's K, then as many of V
   constexpr int WINDOW = THREADS / 4;         // steps whose page ids LDS holds
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = own_thread(), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, lr = lane & 31;
   const int tile0 = it.tile * (32 * W), row0 = tile0 + wave * 32;
@@ -469,35 +479,44 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 3 : 2) void fork_tile_kernel(Tile
   __shared__ Seen s_seen[W];
   __shared__ int s_bad[4];
   const Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
-  const TileParams& P = reread(args);
-  asm volatile("" ::"s"(P.c.groups), "s"(P.c.shared), "s"(P.c.group_count));
-  pin_plan(P);
-  const Entries<W> all(P.c);
-  const Cutting cut = cut_entries<W>(P, all);
-  // The narrow entries first, as in chunk_tile_kernel.
-  if ((int)blockIdx.x < cut.groups) {
+  // Where a workgroup fills a CU, a round of them is launched, and each takes its
+  // share of what is more: those without work, which see that in 4 us, would start
+  // behind the others' end.  It finds its next item anew, so that the plan's registers
+  // do not live through an item.
+  for (int round = 0;; ++round) {
+    const TileParams& P = reread(args);
+    asm volatile("" ::"s"(P.c.groups), "s"(P.c.shared), "s"(P.c.group_count));
+    pin_plan(P);
+    const Entries<W> all(P.c);
+    const Cutting cut = cut_entries<W>(P, all);
+    // The narrow entries first, as in chunk_tile_kernel.
+    if ((int)blockIdx.x < cut.groups) {
+      const TileParams& A = reread(args);
+      pin_rows<false>(A);
+      auto ask = [&](int b0) { return all.at(A.c, b0 / 64); };
+      flat_body<T, D, FORM, false, true, W>(A, all.own0, 64 * all.blocks, ask, cut, s_kv);
+      return;
+    }
+    const int wide = gridDim.x - cut.groups;
+    const long long idx = blockIdx.x - cut.groups + (long long)round * wide, at = idx / P.c.hkv;
+    const int kvh = (int)(idx - at * P.c.hkv);
+    const Item it = plan_entry<W>(P, all, cut.share, at);
+    if (!it.found) {
+      const long long items = Plan<D, W>::kRounds ? 0 : it.items * P.c.hkv;
+      clear_rows<D, 64 * W>(P.c, blockIdx.x - cut.groups - items, wide - items);
+      return;
+    }
+    if (it.part == 0 && kvh == 0 && threadIdx.x == 0)
+      put_fork_record(P, it.r, it.tile, it.parts,
+                      it.parts > 1 ? P.narrow_rows + it.slot * P.part_rows
+                                   : single_row(P, it.r) + it.tile * P.part_rows,
+                      P.part_rows);
     const TileParams& A = reread(args);
     pin_rows<false>(A);
-    auto ask = [&](int b0) { return all.at(A.c, b0); };
-    flat_body<T, D, FORM, false, true, W>(A, all.a0, all.count, ask, cut, s_kv);
-    return;
+    deep_body<T, D, FORM, W>(A, args, it, kvh, s_kv, s_ids, s_seen, s_bad);
+    if (!Plan<D, W>::kRounds) return;
+    __syncthreads();
   }
-  const int in = blockIdx.x - cut.groups, at = divide(in, P.c.hkv, P.c.hkv_mul);
-  const int kvh = in - at * P.c.hkv;
-  const Item it = plan_entry<W>(P, all, cut.share, at);
-  if (!it.found) {
-    const long long items = it.items * P.c.hkv + cut.groups;
-    clear_rows<D, 64 * W>(P.c, blockIdx.x - items, gridDim.x - items);
-    return;
-  }
-  if (it.part == 0 && kvh == 0 && threadIdx.x == 0)
-    put_fork_record(P, it.r, it.tile, it.parts,
-                    it.parts > 1 ? P.narrow_rows + it.slot * P.part_rows
-                                 : single_row(P, it.r) + it.tile * P.part_rows,
-                    P.part_rows);
-  const TileParams& A = reread(args);
-  pin_rows<false>(A);
-  deep_body<T, D, FORM, W>(A, args, it, kvh, s_kv, s_ids, s_seen, s_bad);
 }
 
 // The join with groups: `apart` waves share the rows of a new token and KV head; of
@@ -682,10 +701,10 @@ extern "C" int bc_shared_chunk_attention(bc_shape s, bc_chunk_inputs in, const i
   const long long rows = (long long)in.tokens * (s.query_heads / s.kv_heads);
   const long long few = in.window > 0 || in.first ? (long long)(kFewRows + 1) * group_count : 0;
   const int W = waves_of(s, in.tokens, group_count);
-  const long long grid = split_grid(s, cut, 2 * rows + few, (long long)s.batch + group_count, W);
-  const long long far = 1 << 26, most = kMostGroups * (long long)kThreads / (64 * W);
+  const long long bound = split_grid(s, cut, 2 * rows + few, (long long)s.batch + group_count, W);
+  const long long grid = W == 8 && bound > cut.target ? cut.target : bound, far = 1 << 26;
   if (!use || !aligned16(in.q) || !aligned16(in.k) || !aligned16(in.v) || !aligned16(in.output) ||
-      stride_bits(in) % 8 != 0 || in.k_strides.slot >= far || in.v_strides.slot >= far || grid > most)
+      stride_bits(in) % 8 != 0 || in.k_strides.slot >= far || in.v_strides.slot >= far || grid > kMostGroups)
     return bc_chunk_attention(s, in, nullptr, 0, stream);
   if (!in.q || !in.output) return BC_ERROR_INVALID_VALUE;
   ChunkParams P = chunk_params(s, in);
