@@ -399,20 +399,19 @@ struct AskedEntry : Asked {
   int floor, g0, g1;  // see Request
 };
 
-__device__ __forceinline__ int wide_steps(const ChunkParams& P, int span, int tile_rows) {
-  if (P.causal && P.window > 0) span = min(span, min(P.window, 1 << 29) + tile_rows + kStep);
+__device__ __forceinline__ int wide_steps(const ChunkParams& P, int span) {
+  if (P.causal && P.window > 0) span = min(span, min(P.window, 1 << 29) + kManyRows + kStep);
   return max(1, (span + kStep - 1) / kStep);
 }
 
 // The work of a request whose start, n, len, full and rows are known, from token
-// `floor` on, in tiles of TILE_ROWS rows.  With `tiles` the narrow form's tiles are those that the
-// rows' documents reach.
-template <int TILE_ROWS>
+// `floor` on.  With `tiles` the narrow form's tiles are those that the rows'
+// documents reach.
 __device__ __forceinline__ void ask_work(const ChunkParams& P, Asked& a, int floor, bool tiles) {
   int tiles_of = 0, steps = 0, first_tile = 0, narrow = 0;
   if (a.rows > kFewRows) {
-    tiles_of = (a.rows + TILE_ROWS - 1) / TILE_ROWS;
-    steps = wide_steps(P, max(a.len - floor, 0), TILE_ROWS);
+    tiles_of = (a.rows + kManyRows - 1) / kManyRows;
+    steps = wide_steps(P, max(a.len - floor, 0));
   } else if (a.rows > 0) {
     int lo = P.window > 0 ? (int)max(0ll, (long long)a.full - a.n - P.window + 1) : 0;
     if (P.first && tiles) {
@@ -439,7 +438,7 @@ __device__ __forceinline__ Asked asked_of(const ChunkParams& P, int b, bool tile
     a.full = max(P.lengths[b], 0);
     a.len = min(a.full, P.max_pages * BC_PAGE_SIZE);
     a.rows = a.n * P.group;
-    ask_work<kManyRows>(P, a, 0, tiles);
+    ask_work(P, a, 0, tiles);
   }
   return a;
 }
@@ -1064,6 +1063,27 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
   P.records[2 + 2 * i] = make_int4(first, stride, 0, 0);
 }
 
+// With groups: the record of tile `tile` of an entry whose new tokens start at
+// `start`.  No two entries have one in common, since the rows of the
+// ones before end there.
+__device__ __forceinline__ int record_of(const TileParams& P, int entry, int start, int tile) {
+  const int from = entry < P.c.batch ? entry : P.own_records + entry - P.c.batch;
+  return from + start * P.c.group / kManyRows + tile;
+}
+
+// The partial row of an entry's first row, where a tile is in one piece.
+__device__ __forceinline__ int single_row(const TileParams& P, const Request& rq) {
+  const int rows = P.c.tokens * P.c.group;
+  return P.single_rows + (is_group(rq) ? rows : 0) + rq.start * P.c.group;
+}
+
+// Part p of the tile's rows are the partial rows first + p * stride ...; parts 0:
+// there are none.
+__device__ __forceinline__ void put_fork_record(const TileParams& P, const Request& rq, int tile, int parts,
+                                                int first, int stride) {
+  P.records[record_of(P, rq.entry, rq.start, tile)] = make_int4(parts, first, stride, 0);
+}
+
 // The wide form: 128 rows per workgroup, 32 per wave, each 64-token step's K
 // and V shared through two LDS buffers, which loads straight into LDS fill one
 // step ahead; one barrier a step, two workgroups per CU (three at D = 64).
@@ -1076,7 +1096,7 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
 //    over 2048, sixteen of them: 180 us, 670 TFLOP/s).
 //  - A full round of workgroups takes 8.6 us, launch included, and 2.1 per step
 //    (2048 new tokens over 2048 to 32768, none masked: 75.8 to 1082 us).
-template <typename T, int D, Form FORM, bool FP8>
+template <typename T, int D, Form FORM, bool FP8, bool FORKS>
 __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const Item& it, int kvh,
                                           uint16_t* s_kv, Seen* s_seen, int* s_bad) {
   const ChunkParams& C = A.c;
@@ -1106,32 +1126,6 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
       ids_next = load_ids(t0 + 16);
     }
   };
-  if (tid < 4) s_bad[tid] = 0;
-  if (!C.first) {
-    mine = rows_seen(C, rq, row0, min(row0 + 32, rq.rows));
-    wg = rows_seen(C, rq, tile0, min(tile0 + kManyRows, rq.rows));
-    range();
-    load_rows<T, D, FORM, false>(C, rq, row0 + lr, kvh, g, R, qB);
-  } else {
-    load_rows<T, D, FORM, false>(C, rq, row0 + lr, kvh, g, R, qB);
-    mine = wave_seen(R, row0 + lr < rq.rows);
-    if (lane == 0) s_seen[wave] = mine;
-    __syncthreads();
-    wg = s_seen[0];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      wg.any_lo = min(wg.any_lo, s_seen[w].any_lo);
-      wg.any_hi = max(wg.any_hi, s_seen[w].any_hi);
-      wg.all_lo = max(wg.all_lo, s_seen[w].all_lo);
-      wg.all_hi = min(wg.all_hi, s_seen[w].all_hi);
-    }
-    wg.any_lo = __builtin_amdgcn_readfirstlane(wg.any_lo);
-    wg.any_hi = __builtin_amdgcn_readfirstlane(wg.any_hi);
-    wg.all_lo = __builtin_amdgcn_readfirstlane(wg.all_lo);
-    wg.all_hi = __builtin_amdgcn_readfirstlane(wg.all_hi);
-    range();
-  }
-
   const int lrow = tid / CPR, lcol = 8 * (tid % CPR ^ swz<D>(lrow));
   const unsigned koff = (unsigned)(((lrow % BC_PAGE_SIZE) * C.ks + lcol) * 2);
   const unsigned voff = (unsigned)(((lrow % BC_PAGE_SIZE) * C.vs + lcol) * 2);
@@ -1181,6 +1175,51 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     const unsigned dst = lds0 + buf * (4 * HALF) + x * 4096;
     load2_to_lds(Pages<FP8>::at(pg.k, from), Pages<FP8>::at(pg.v, from), koff, voff, dst, dst + 2 * HALF);
   };
+  if (tid < 4) s_bad[tid] = 0;
+  auto first_step = [&] {  // its loads
+    pg.take(C, kvh, ids);
+#pragma unroll
+    for (int x = 0; x < (FP8 ? NX8 : NX); ++x)
+      if constexpr (FP8)
+        fetch(x, 0);
+      else
+        issue_chunk(x, 0, 0);
+  };
+  // What a group's rows see depends on their requests, but without a window or
+  // documents it is read from its start to its end: its first step goes out ahead of
+  // the look at them.
+  const bool group = FORKS && is_group(rq), ahead = group && !C.first && C.window == 0;
+  if (!C.first && !group) {
+    mine = rows_seen(C, rq, row0, min(row0 + 32, rq.rows));
+    wg = rows_seen(C, rq, tile0, min(tile0 + kManyRows, rq.rows));
+    range();
+    load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
+  } else {
+    if (ahead) {
+      wg.any_lo = 0;
+      wg.any_hi = rq.len - 1;
+      range();
+      if (t0 < tend) first_step();
+    }
+    load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
+    mine = wave_seen(R, row0 + lr < rq.rows);
+    if (lane == 0) s_seen[wave] = mine;
+    __syncthreads();
+    wg = s_seen[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      wg.any_lo = min(wg.any_lo, s_seen[w].any_lo);
+      wg.any_hi = max(wg.any_hi, s_seen[w].any_hi);
+      wg.all_lo = max(wg.all_lo, s_seen[w].all_lo);
+      wg.all_hi = min(wg.all_hi, s_seen[w].all_hi);
+    }
+    wg.any_lo = __builtin_amdgcn_readfirstlane(wg.any_lo);
+    wg.any_hi = __builtin_amdgcn_readfirstlane(wg.any_hi);
+    wg.all_lo = __builtin_amdgcn_readfirstlane(wg.all_lo);
+    wg.all_hi = __builtin_amdgcn_readfirstlane(wg.all_hi);
+    if (!ahead) range();
+  }
+
   // Steps whole_lo .. whole_hi - 1 are seen whole by every row, given their pages.
   const int whole_lo = wg.all_lo / kStep + (wg.all_lo % kStep != 0);
   const int whole_hi = (min(wg.all_hi, rq.len - 1) + 1) / kStep;
@@ -1201,13 +1240,7 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   bool bad = false;
   int pages = 15;  // of the step at hand, a bit each: in the pool
   if (t0 < tend) {
-    pg.take(C, kvh, ids);
-#pragma unroll
-    for (int x = 0; x < (FP8 ? NX8 : NX); ++x)
-      if constexpr (FP8)
-        fetch(x, 0);
-      else
-        issue_chunk(x, 0, 0);
+    if (!ahead) first_step();
     pages = (int)pg.in_pool & 15;
     const bool whole = pages == 15 && t0 >= whole_lo && t0 < whole_hi;
     if constexpr (FP8) {
@@ -1295,8 +1328,10 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   const TileParams& P = reread(args);
   R.l += shfl_xor_f(R.l, 32);
   const int r = row0 + lr;
-  if (it.parts > 1) {
-    const size_t at = partial_row(P, P.narrow_rows + (it.slot + it.part) * P.part_rows + wave * 32 + lr, kvh);
+  if (it.parts > 1 || (FORKS && joined(rq))) {
+    const int first = FORKS && it.parts == 1 ? single_row(P, rq) + tile0
+                                             : P.narrow_rows + (it.slot + it.part) * P.part_rows;
+    const size_t at = partial_row(P, first + wave * 32 + lr, kvh);
     if (r < rq.rows) {
       if (g == 0) *reinterpret_cast<float2*>(P.part_ml + 2 * at) = make_float2(R.m, R.l);
 #pragma unroll
@@ -1540,27 +1575,6 @@ struct Stream8 {
 template <typename T, int D, Form FORM, bool FP8>
 using StreamOf = typename std::conditional<FP8, Stream8<T, D, FORM>, Stream<T, D, FORM>>::type;
 
-// With groups: the record of tile `tile`, of tile_rows rows, of an entry whose new
-// tokens start at `start`.  No two entries have one in common, since the rows of the
-// ones before end there.
-__device__ __forceinline__ int record_of(const TileParams& P, int entry, int start, int tile) {
-  const int from = entry < P.c.batch ? entry : P.own_records + entry - P.c.batch;
-  return from + start * P.c.group / P.part_rows + tile;
-}
-
-// The partial row of an entry's first row, where a tile is in one piece.
-__device__ __forceinline__ int single_row(const TileParams& P, const Request& rq) {
-  const int rows = P.c.tokens * P.c.group;
-  return P.single_rows + (is_group(rq) ? rows : 0) + rq.start * P.c.group;
-}
-
-// Part p of the tile's rows are the partial rows first + p * stride ...; parts 0:
-// there are none.
-__device__ __forceinline__ void put_fork_record(const TileParams& P, const Request& rq, int tile, int parts,
-                                                int first, int stride) {
-  P.records[record_of(P, rq.entry, rq.start, tile)] = make_int4(parts, first, stride, 0);
-}
-
 // The narrow form over a batch: the tiles of all requests with few rows, one
 // after another, in ranges of equal length, a range per wave.  HBM-bound: 64
 // single tokens over 128-4096 tokens (32/8 heads, D = 128, 585 MB) 96 us, 6.5
@@ -1572,14 +1586,14 @@ __device__ __forceinline__ void put_fork_record(const TileParams& P, const Reque
 // have n rows starts at partial row 32 r + n: a range's next request is
 // further by the rows of the last one, a request's next range by 32.
 // `ask(b0)` is what is asked of the requests (with groups: entries) b0 .. b0 + 63,
-// `a` of the first, and `batch` how many there are; W waves per workgroup.
-template <typename T, int D, Form FORM, bool FP8, bool FORKS, int W, typename A, typename F>
+// `a` of the first, and `batch` how many there are.
+template <typename T, int D, Form FORM, bool FP8, bool FORKS, typename A, typename F>
 __device__ __forceinline__ void flat_body(const TileParams& P, A a, int batch, F ask, const Cutting& cut,
                                           uint16_t* s_kv) {
   const ChunkParams& C = P.c;
   const int lane = threadIdx.x & 63, g = lane >> 5, lr = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned task = W * blockIdx.x + wave;
+  const unsigned task = 4 * blockIdx.x + wave;
   const int range = task / (unsigned)C.hkv, kvh = task - (unsigned)range * C.hkv;
   if ((long long)range * cut.run >= cut.narrow) return;
   const int lo = range * cut.run, hi = min(lo + cut.run, cut.narrow);
@@ -1631,7 +1645,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, A a, int batch, F
   st.issue_k(0);
   st.issue_v(0);
   // With groups a request's own part is short for a wave: Q comes a request ahead.
-  constexpr bool kAhead = FORKS;
+  constexpr bool kAhead = FORKS && FORM != Form::kCap;
   u32x4 q_next[D / 16];
   if constexpr (kAhead) load_q<D>(C, p.rq, lr, kvh, g, q_next);
   for (;;) {  // over the requests
@@ -1817,14 +1831,14 @@ __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request&
 }
 
 // Zeros for the rows of no request, by the workgroups that have no item.
-template <int D, int THREADS>
+template <int D>
 __device__ __forceinline__ void clear_rows(const ChunkParams& C, long long at, long long of) {
   const int head = min(max(C.starts[0], 0), C.tokens);
   const int tail = min(max(C.starts[C.batch], 0), C.tokens);
   const long long row = (long long)C.hq * (D / 8), gap = (long long)(tail - head) * row;
   const long long total = (long long)C.tokens * row - gap;
   u32x4* const out = reinterpret_cast<u32x4*>(C.out);
-  for (long long x = at * THREADS + threadIdx.x; x < total; x += of * THREADS)
+  for (long long x = at * 256 + threadIdx.x; x < total; x += of * 256)
     out[x < head * row ? x : x + gap] = u32x4{0, 0, 0, 0};
 }
 
@@ -1858,12 +1872,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
     const TileParams& A = reread(args);
     pin_rows<FP8>(A);
     auto ask = [&](int b0) { return asked_of(A.c, b0 + lane, true); };
-    flat_body<T, D, FORM, FP8, false, 4>(A, head, A.c.batch, ask, cut, s_kv);
+    flat_body<T, D, FORM, FP8, false>(A, head, A.c.batch, ask, cut, s_kv);
     return;
   }
   if (!it.found) {
     const long long items = it.items * P.c.hkv + cut.groups;
-    clear_rows<D, 256>(P.c, blockIdx.x - items, gridDim.x - items);
+    clear_rows<D>(P.c, blockIdx.x - items, gridDim.x - items);
     return;
   }
   if (it.parts > 1 && it.part == 0 && kvh == 0 && threadIdx.x == 0)
@@ -1875,7 +1889,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TilePa
   if (it.r.rows <= kFewRows)
     narrow_body<T, D, FORM, FP8>(A.c, it.r, kvh, s_kv, s_ml);
   else
-    wide_body<T, D, FORM, FP8>(A, args, it, kvh, s_kv, s_seen, s_bad);
+    wide_body<T, D, FORM, FP8, false>(A, args, it, kvh, s_kv, s_seen, s_bad);
 }
 
 // One part's state joined to another's.
@@ -2045,14 +2059,14 @@ hipError_t launch_tiles(const ChunkParams& P, int dim, int dtype, const Cut& cut
                    : launch_tiles<__bf16, 128, FP8>(P, cut, ws, (unsigned)grid, st);
 }
 
-// Workgroups of W waves of the tile kernel with a workspace, at most, of a batch
-// whose entries of more than 32 rows have `rows` rows in all.  Cut by shares, n
-// tiles have less than target / Hkv + n parts.  A workgroup without work still walks
-// the batch to see that, some 2 us, so none is launched beyond these.
-inline long long split_grid(const bc_shape& s, const Cut& cut, long long rows, long long entries, int W) {
+// Workgroups of the tile kernel with a workspace, at most, of a batch whose entries
+// of more than 32 rows have `rows` rows in all.  Cut by shares, n tiles have less
+// than target / Hkv + n parts.  A workgroup without work still walks the batch to
+// see that, some 2 us, so none is launched beyond these.
+inline long long split_grid(const bc_shape& s, const Cut& cut, long long rows, long long entries) {
   const long long wide = rows / (kFewRows + 1) < entries ? rows / (kFewRows + 1) : entries;
-  const long long items = wide > 0 ? rows / (32 * W) + wide + cut.target / s.kv_heads + 1 : 0;
-  return items * s.kv_heads + ((long long)cut.waves * s.kv_heads + W - 1) / W + 1;
+  const long long items = wide > 0 ? rows / kManyRows + wide + cut.target / s.kv_heads + 1 : 0;
+  return items * s.kv_heads + ((long long)cut.waves * s.kv_heads + 3) / 4 + 1;
 }
 
 // Workgroups of the tile kernel, at most.

@@ -276,7 +276,7 @@ extern "C" int bc_fp8_chunk_attention(bc_shape s, bc_chunk_inputs in, const uint
   const Cut cut = cut_of(s, in.tokens, true);
   const bool use = cut.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= cut.bytes;
   const long long rows = (long long)in.tokens * P.group;
-  const long long grid = use ? split_grid(s, cut, rows, s.batch, 4) : tile_grid(s, in.tokens, cut, false);
+  const long long grid = use ? split_grid(s, cut, rows, s.batch) : tile_grid(s, in.tokens, cut, false);
   const long long far = 1 << 27;  // bytes: offsets inside a page are 32-bit
   const bool tiled = aligned16(in.q) && aligned16(in.output) &&
                      (in.q_strides.token | in.q_strides.head) % 8 == 0 && in.k_strides.slot < far &&

@@ -68,4 +68,23 @@ def forks(groups, hq, hkv, d, dtype, *, seed=0, spread=1.0, lone_ends=0):
     shared = torch.tensor([s for s, _ in groups], dtype=torch.int32)
     if lone_ends:
         bounds, shared = bounds[1:-1], shared[1:-1]
-    return fix, bounds, shared
+    return widen(fix), bounds, shared
+
+
+def pays(fix, window=0):
+    """Whether the op reads shared pages once: by what the requests may see, each its
+    own, in a table of this width, and by their rows."""
+    batch, table = fix["pages"].shape[0], fix["pages"].shape[1] * C.PAGE
+    rows = fix["q"].shape[0] * (fix["q"].shape[1] // fix["k"].shape[2])
+    seen = min(window or table, table)
+    size = batch * seen * fix["k"].shape[2] * fix["k"].shape[3] * 4 / 1e6
+    return batch > 1 and table > 1024 and rows <= 80 * batch and size >= (400 if seen < table else 100)
+
+
+def widen(fix):
+    """The same batch in a table wide enough for that, with or without a window
+    (windows have no more tokens than the table then): columns of no page."""
+    batch, old = fix["pages"].shape
+    width = int(110e6 / (batch * C.PAGE * fix["k"].shape[2] * fix["k"].shape[3] * 4)) + 65
+    fix["pages"] = torch.cat((fix["pages"], torch.full((batch, max(width - old, 0)), -1, dtype=torch.int32)), 1)
+    return fix

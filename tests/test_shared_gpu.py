@@ -25,16 +25,14 @@ def attend(fix, groups, shared, **options):
     return out
 
 
-def tolerance(tol):
-    """A row's two parts are joined in 32 bits: exponentials and sums of a few
-    roundings more, of which C.reference's bound counts 16 per score."""
-    return tol
-
-
 def both(fix, groups, shared, what="", **options):
+    """A row's two parts are joined in 32 bits: exponentials and sums of a few
+    roundings more, of which C.reference's bound counts 16 per score.  Without a
+    window every case is one that reads shared pages once."""
+    assert F.pays(fix) or not len(shared)
     want, tol = C.reference(**fix, **options)
     got = attend(fix, groups, shared, **options)
-    C.check(got, want, tolerance(tol), what)
+    C.check(got, want, tol, what)
     return got
 
 
@@ -43,9 +41,9 @@ GROUPS = [
     [(16, [(1, 1), (1, 1)])],
     [(160, [(1, 1)] * 8)],
     [(2048, [(5, 1), (64, 1), (1, 1), (17, 1)])],
-    [(1000, [(30, 2), (40, 3)]), (64, [(3, 1), (80, 70)]), (0, [(20, 1), (30, 1)])],
-    [(130, [(9, 9), (200, 150), (5, 0), (31, 5)]), (333, [(40, 1)])],
-    [(48, [(20, 20)] * 40)],
+    [(1000, [(30, 2), (40, 3)]), (64, [(3, 1), (80, 40)]), (0, [(20, 1), (30, 1)])],
+    [(130, [(9, 9), (200, 90), (5, 0), (31, 5)]), (333, [(40, 1)] + [(7, 1)] * 5)],
+    [(48, [(11, 11)] * 40)],
     [(700, [(3, 1)] * 70), (32, [(8, 3)] * 3)],
     [(17, [(2, 1), (2, 2), (1, 0)]), (15, [(1, 1), (600, 1)])],
 ]
@@ -75,6 +73,33 @@ def test_long_prefixes(form, members, new):
     both(fix, groups, shared, form, **K.options_of(form, fix))
 
 
+@pytest.mark.parametrize("form", ["window", "window bias", "window full", "cap window", "window first"])
+def test_windows(form):
+    """With enough requests and heads that a window's tokens pay for it."""
+    fix, groups, shared = F.forks([(500, [(1 + i, 1) for i in range(40)]), (300, [(200 + 9 * i, 2) for i in range(24)])],
+                                  32, 32, 128, F16, seed=7)
+    options = dict(window=400)
+    assert F.pays(fix, 400)
+    if form == "window bias":
+        options["slopes"] = torch.rand(32, generator=torch.Generator().manual_seed(3)) - 0.25
+    if form == "window full":
+        options["causal"] = False
+    if form == "cap window":
+        options["cap"] = 5.0
+    if form == "window first":
+        options.update(K.options_of("first", fix))
+    both(fix, groups, shared, form, **options)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_small_batches_read_their_own_pages(new):
+    fix, groups, shared = F.forks([(64, [(new, new)] * 3)], 4, 2, 64, F16, seed=5)
+    fix["pages"] = fix["pages"][:, :6].contiguous()
+    assert not F.pays(fix)
+    want, tol = C.reference(**fix)
+    C.check(attend(fix, groups, shared), want, tol)
+
+
 def test_requests_outside_the_groups():
     fix, groups, shared = F.forks([(0, [(90, 3), (5, 1)]), (200, [(3, 1)] * 5), (100, [(4, 2)] * 3), (0, [(33, 33)])],
                                   4, 2, 64, F16, seed=5, lone_ends=1)
@@ -82,6 +107,8 @@ def test_requests_outside_the_groups():
     both(fix, groups, shared)
     none = torch.zeros(0, dtype=torch.int32)
     both(fix, groups[:1], none)
+    for bounds in ([2, 3, 7, 10], [2, 7, 7, 10], [3, 6, 7, 10]):  # of one and of no request
+        both(fix, torch.tensor(bounds, dtype=torch.int32), torch.tensor([64, 96, 96], dtype=torch.int32))
 
 
 def test_sharp_scores():
@@ -118,18 +145,22 @@ def test_pages_outside_the_pool_are_not_seen():
     both(fix, groups, shared)
 
 
+@pytest.mark.parametrize("members", [3, 40])
 @pytest.mark.parametrize("bad", [(2.0, float("inf")), (float("nan"), 1.0)])
-def test_what_a_row_does_not_see_may_hold_anything(bad):
-    """A token of the prefix that a window hides from some members and not from
+def test_what_a_row_does_not_see_may_hold_anything(bad, members):
+    """A token of the prefix that documents hide from some members and not from
     others."""
-    fix, groups, shared = F.forks([(200, [(5, 1), (60, 1), (5, 5)])], 4, 2, 64, BF16, seed=8)
-    at = 190  # seen by the first and the last with a window of 40, not by the second
-    page = int(fix["pages"][0, at // 16])
-    fix["k"][page, at % 16, 0, 3], fix["v"][page, at % 16, 0, 3] = bad
-    got = attend(fix, groups, shared, window=40).cpu()
-    fix["k"][page, at % 16, 0, 3] = fix["v"][page, at % 16, 0, 3] = 0
-    want, tol = C.reference(**fix, window=40)
-    C.check(got[1], want[1], tol[1])
+    fix, groups, shared = F.forks([(200, [(5, 1), (60, 1), (5, 5)] + [(1, 1)] * (members - 3))], 4, 2, 64, BF16, seed=8)
+    assert F.pays(fix)
+    page = int(fix["pages"][0, 190 // 16])
+    fix["k"][page, 190 % 16, 0, 3], fix["v"][page, 190 % 16, 0, 3] = bad
+    rows = fix["q"].shape[0]
+    first = torch.zeros(rows, dtype=torch.int32)
+    first[1], first[7:] = 191, 195
+    got = attend(fix, groups, shared, first=first).cpu()
+    fix["k"][page, 190 % 16, 0, 3] = fix["v"][page, 190 % 16, 0, 3] = 0
+    want, tol = C.reference(**fix, first=first)
+    hidden = [1, *range(7, rows)]
+    C.check(got[hidden], want[hidden], tol[hidden])
     C.check(got[:, 2:], want[:, 2:], tol[:, 2:])  # the other KV head's
-    seen = got[[0, 2, 3, 4, 5, 6], :2, 3]
-    assert not bool(seen.isfinite().any())
+    assert not bool(got[[0, 2, 3, 4, 5, 6], :2, 3].isfinite().any())
