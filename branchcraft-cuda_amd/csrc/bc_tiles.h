@@ -2059,6 +2059,13 @@ hipError_t launch_tiles(const ChunkParams& P, int dim, int dtype, const Cut& cut
                    : launch_tiles<__bf16, 128, FP8>(P, cut, ws, (unsigned)grid, st);
 }
 
+// Whether a window is as short as tables that are not cut, see cut_of (32 requests of
+// 8 new tokens, window 1024, 24/8 heads, bias: 26 us, cut 40).
+inline bool short_window(const bc_shape& s, const bc_chunk_inputs& in) {
+  const bool few = (long long)in.tokens * (s.query_heads / s.kv_heads) <= (long long)kFewRows * s.batch;
+  return in.causal && in.window > 0 && in.window <= (few ? 1024 : 512);
+}
+
 // Workgroups of the tile kernel with a workspace, at most, of a batch whose entries
 // of more than 32 rows have `rows` rows in all.  Cut by shares, n tiles have less
 // than target / Hkv + n parts.  A workgroup without work still walks the batch to

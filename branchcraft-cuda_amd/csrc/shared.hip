@@ -433,7 +433,7 @@ extern "C" int bc_shared_chunk_attention(bc_shape s, bc_chunk_inputs in, const i
   const long long far = 1 << 26;
   if (!use || !aligned16(in.q) || !aligned16(in.k) || !aligned16(in.v) || !aligned16(in.output) ||
       stride_bits(in) % 8 != 0 || in.k_strides.slot >= far || in.v_strides.slot >= far || grid > kMostGroups)
-    return bc_chunk_attention(s, in, workspace, workspace_bytes, stream);
+    return bc_chunk_attention(s, in, short_window(s, in) ? nullptr : workspace, workspace_bytes, stream);
   if (!in.q || !in.output) return BC_ERROR_INVALID_VALUE;
   ChunkParams P = chunk_params(s, in);
   P.groups = groups;
