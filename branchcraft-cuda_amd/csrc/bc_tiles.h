@@ -891,26 +891,33 @@ struct Pages {
   }
 };
 
-// Sixteen codes of a page, `off` bytes from its wave-uniform address.
+// Sixteen codes of a page, `off` bytes from its wave-uniform address; STREAM: of what
+// a call reads once (64 single tokens over 128-4096 tokens 59 us, 67 without).
+template <bool STREAM>
 __device__ __forceinline__ u32x4 load_codes(const void* page, unsigned off) {
   typedef const __attribute__((address_space(1))) char* Bytes;
-  return __builtin_nontemporal_load((const __attribute__((address_space(1))) u32x4*)((Bytes)page + off));
+  typedef const __attribute__((address_space(1))) u32x4* Codes;
+  const Codes at = (Codes)((Bytes)page + off);
+  return STREAM ? __builtin_nontemporal_load(at) : *at;
 }
 
-// Sixteen codes of row `row` of a tile into LDS, as the 16-byte chunks 2 c and
-// 2 c + 1 of its values.
-template <typename T, int D>
-__device__ __forceinline__ void put_values(const u32x4& lo, const u32x4& hi, uint16_t* tile, int row, int c) {
-  *reinterpret_cast<u32x4*>(tile + row * D + ((2 * c) ^ swz<D>(row)) * 8) = lo;
-  *reinterpret_cast<u32x4*>(tile + row * D + ((2 * c + 1) ^ swz<D>(row)) * 8) = hi;
-}
-
+// Sixteen codes as values, the first eight and the others.
 template <typename T>
 __device__ __forceinline__ void values16(const u32x4& w, float power, u32x4& lo, u32x4& hi) {
   lo = u32x4{values2<T, false>(w[0], power), values2<T, true>(w[0], power), values2<T, false>(w[1], power),
              values2<T, true>(w[1], power)};
   hi = u32x4{values2<T, false>(w[2], power), values2<T, true>(w[2], power), values2<T, false>(w[3], power),
              values2<T, true>(w[3], power)};
+}
+
+// Their 16-byte chunks 2 c and 2 c + 1 of row `row` of a tile into LDS.  A write takes
+// two turns, since eight lanes have either the even or the odd chunks; an order that
+// gives each bank to one lane costs a select per word and is no faster (1096 us for
+// 2048 new tokens of 32768, with it 1132; 64 single tokens 59.5 and 59.8).
+template <int D>
+__device__ __forceinline__ void put_values(const u32x4& lo, const u32x4& hi, uint16_t* tile, int row, int c) {
+  *reinterpret_cast<u32x4*>(tile + row * D + ((2 * c) ^ swz<D>(row)) * 8) = lo;
+  *reinterpret_cast<u32x4*>(tile + row * D + ((2 * c + 1) ^ swz<D>(row)) * 8) = hi;
 }
 
 // Of 64 rising numbers, one per lane, how many are at most `x`.
@@ -1136,15 +1143,15 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   // loaded where loads into LDS would be issued, and converted into LDS behind the
   // step's product.
   constexpr int CPR8 = D / 16, NX8 = kStep * CPR8 / 256;  // of 16 codes
-  const int crow = tid / CPR8, ccol = tid % CPR8;
+  const int crow = wave * (64 / CPR8) + lane / CPR8, ccol = lane % CPR8;
   const unsigned kcode = (unsigned)((crow % BC_PAGE_SIZE) * C.ks + ccol * 16);
   const unsigned vcode = (unsigned)((crow % BC_PAGE_SIZE) * C.vs + ccol * 16);
   u32x4 kc[NX8], vc[NX8];
   uint32_t kx[NX8], vx[NX8];
   auto fetch = [&](int x, int at) {
     const int from = 4 * at + (CPR8 == 8 ? 2 * x + (wave >> 1) : wave);
-    kc[x] = load_codes(Pages<FP8>::at(pg.k, from), kcode);
-    vc[x] = load_codes(Pages<FP8>::at(pg.v, from), vcode);
+    kc[x] = load_codes<false>(Pages<FP8>::at(pg.k, from), kcode);
+    vc[x] = load_codes<false>(Pages<FP8>::at(pg.v, from), vcode);
     const int page = __builtin_amdgcn_readlane(pg.id, from);
     const size_t scales = scale_at<D>(C, page, kvh, 0);
     const unsigned off = (crow % BC_PAGE_SIZE) * (D / kFp8Block) + ccol / 2;
@@ -1160,13 +1167,13 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
       const int row = crow + 256 / CPR8 * x;
       u32x4 lo, hi;
       values16<T>(kc[x], power_of(kx[x]), lo, hi);
-      put_values<T, D>(lo, hi, k, row, ccol);
+      put_values<D>(lo, hi, k, row, ccol);
       values16<T>(vc[x], power_of(vx[x]), lo, hi);
       if (!whole) {
         bad |= tidy_value<T>(lo, (ok >> row) & 1u);
         bad |= tidy_value<T>(hi, (ok >> row) & 1u);
       }
-      put_values<T, D>(lo, hi, k + HALF, row, ccol);
+      put_values<D>(lo, hi, k + HALF, row, ccol);
     }
     return bad;
   };
@@ -1512,11 +1519,11 @@ struct Stream8 {
     const uint8_t* const scales = lane < 32 ? C.k_scale : C.v_scale;
     powers_next = *reinterpret_cast<const Powers*>(scales + scale_at<D>(C, page, kvh, lane & 15));
 #pragma unroll
-    for (int i = 0; i < NL; ++i) k[i] = load_codes(Pages<true>::at(pg.k, 2 * at + i / NP), koff[i % NP]);
+    for (int i = 0; i < NL; ++i) k[i] = load_codes<true>(Pages<true>::at(pg.k, 2 * at + i / NP), koff[i % NP]);
   }
   __device__ __forceinline__ void issue_v(int at) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i) v[i] = load_codes(Pages<true>::at(pg.v, 2 * at + i / NP), voff[i % NP]);
+    for (int i = 0; i < NL; ++i) v[i] = load_codes<true>(Pages<true>::at(pg.v, 2 * at + i / NP), voff[i % NP]);
   }
   __device__ __forceinline__ int in_pool(int at) const { return (int)(pg.in_pool >> (2 * at)) & 3; }
 
@@ -1533,7 +1540,7 @@ struct Stream8 {
       const int row = i * RPL + lane / CPR;
       u32x4 lo, hi;
       values16<T>(k[i], power(row), lo, hi);
-      put_values<T, D>(lo, hi, kt, row, lane % CPR);
+      put_values<D>(lo, hi, kt, row, lane % CPR);
     }
     if (next) issue_k(at);
     wave_lds_sync();
@@ -1561,7 +1568,7 @@ struct Stream8 {
         bad |= tidy_value<T>(lo, (e.valid >> row) & 1u);
         bad |= tidy_value<T>(hi, (e.valid >> row) & 1u);
       }
-      put_values<T, D>(lo, hi, vt, row, lane % CPR);
+      put_values<D>(lo, hi, vt, row, lane % CPR);
     }
     if (next) issue_v(at);
     bad = __builtin_amdgcn_ballot_w64(bad) != 0;

@@ -137,9 +137,10 @@ __global__ __launch_bounds__(kThreads) void read_fp8_kernel(Fp8Params P) {
     }
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv)
-    *reinterpret_cast<uint4*>(P.out[kv] + (size_t)x * kPiece) =
-        make_uint4(values2<T, false>(codes[kv].x, power[kv]), values2<T, true>(codes[kv].x, power[kv]),
-                   values2<T, false>(codes[kv].y, power[kv]), values2<T, true>(codes[kv].y, power[kv]));
+    __builtin_nontemporal_store(
+        u32x4{values2<T, false>(codes[kv].x, power[kv]), values2<T, true>(codes[kv].x, power[kv]),
+              values2<T, false>(codes[kv].y, power[kv]), values2<T, true>(codes[kv].y, power[kv])},
+        reinterpret_cast<u32x4*>(P.out[kv] + (size_t)x * kPiece));
 }
 
 // Codes go by eight and 16 bytes, powers by two and four.
