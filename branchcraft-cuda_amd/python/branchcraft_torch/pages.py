@@ -188,6 +188,27 @@ class PageOwner:
             self.release(fresh)
         self.lengths[plan.request] = length
 
+    def shared_prefixes(self, requests: list[int]) -> tuple[list[int], list[int]]:
+        """Requests next to each other in the list that begin with the same pages:
+        ``(bounds, tokens)``, group g being ``requests[bounds[g]:bounds[g + 1]]``, whose
+        first ``tokens[g]`` tokens lie in pages of all of them.  A request joins the
+        group before it unless that would cost it half of what it shares."""
+        bounds, tokens = [], []
+        for i, request in enumerate(requests):
+            pages, length = self.pages[request], self.lengths[request]
+            if bounds:
+                first = self.pages[requests[bounds[-1]]]
+                most = min(tokens[-1], length)
+                same = most // PAGE_SIZE  # whole pages; most often all of them
+                if pages[:same] != first[:same]:
+                    same = next(n for n in range(same) if pages[n] != first[n])
+                if same and (2 * same * PAGE_SIZE > tokens[-1] or i == bounds[-1] + 1):
+                    tokens[-1] = same * PAGE_SIZE
+                    continue
+            bounds.append(i)
+            tokens.append(length)
+        return bounds + [len(requests)], tokens
+
     def check_invariants(self) -> None:
         """Refcounts equal live references; the free list holds exactly the
         unreferenced pages, once each."""

@@ -12,7 +12,10 @@ a shared partial page and the accepted-path copy -- runs as the
 every accepted node) and one for their index lists, and leaves the same pages and page tables
 as committing them one by one in the same order.  ``extend`` appends ordinary new
 tokens to several requests and attends to them: a chunk of a prompt, a turn, a
-decode step.
+decode step; with ``share``, pages that forks have in common are read once.
+
+``Fp8Cache`` is the same for ordinary tokens in 8 bits: half the pool, half the bytes
+of every step.
 """
 
 from __future__ import annotations
@@ -20,11 +23,12 @@ from __future__ import annotations
 import torch
 from torch.autograd.forward_ad import unpack_dual
 
-from . import (append_kv_, build_tables, chunk_attention, commit_path_, commit_paths_,
-               copy_pages_, int_tensor, tree_verify, write_prefix_)
+from . import (append_fp8_kv_, append_kv_, build_tables, chunk_attention, commit_path_,
+               commit_paths_, copy_pages_, fp8_chunk_attention, int_tensor, read_fp8_kv,
+               shared_chunk_attention, tree_verify, write_prefix_)
 from .pages import CommitPlan, PageOwner, Snapshot
 
-__all__ = ["PagedTreeCache", "Snapshot", "CommitPlan"]
+__all__ = ["PagedTreeCache", "Fp8Cache", "Snapshot", "CommitPlan"]
 
 
 class PagedTreeCache:
@@ -36,6 +40,26 @@ class PagedTreeCache:
         self.k = torch.zeros((physical_pages, 16, kv_heads, head_dim),
                              device=device, dtype=torch.float16)
         self.v = torch.zeros_like(self.k)
+
+    @property
+    def dtype(self) -> torch.dtype:
+        """The type of the rows that enter the cache, and of queries and outputs."""
+        return self.k.dtype
+
+    # What extend does on the device, by the pool's form.
+    def _pools(self) -> tuple[torch.Tensor, ...]:
+        return self.k, self.v
+
+    def _clone(self, old: torch.Tensor, fresh: torch.Tensor) -> None:
+        copy_pages_(self.k, self.v, old, fresh)
+
+    def _append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        append_kv_(self.k, self.v, k, v, slots)
+
+    def _attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+                starts: torch.Tensor, groups: tuple[torch.Tensor, ...], **options) -> torch.Tensor:
+        op = shared_chunk_attention if groups else chunk_attention
+        return op(q, self.k, self.v, table, lengths, starts, *groups, **options)
 
     # The reference exposes these as attributes.
     @property
@@ -177,7 +201,7 @@ class PagedTreeCache:
         return plans
 
     def extend(self, requests: list[int], counts: list[int], q: torch.Tensor,
-               k: torch.Tensor, v: torch.Tensor, **options) -> torch.Tensor:
+               k: torch.Tensor, v: torch.Tensor, *, share: bool = False, **options) -> torch.Tensor:
         """Append ``counts[i]`` new tokens to request ``requests[i]`` and attend.
 
         ``k`` and ``v`` [tokens, KV heads, dim] hold the new tokens' rows,
@@ -187,7 +211,11 @@ class PagedTreeCache:
         are planned as consecutive commits would take them: shared partial
         pages are cloned first.  A pool without room for all of it raises
         before anything changes, and so does a stream under capture; a call that
-        fails later leaves pages and lengths as before it.  A count may be zero."""
+        fails later leaves pages and lengths as before it.  A count may be zero.
+
+        ``share``: pages that requests next to each other in the list begin with in
+        common (forks of one prompt) are read once for all of them; the result is the
+        same up to rounding."""
         if len(requests) != len(counts) or len(set(requests)) != len(requests) or not requests:
             raise ValueError("requests must be distinct and match counts")
         total = sum(counts)
@@ -199,14 +227,14 @@ class PagedTreeCache:
         if (q.ndim != 3 or q.shape[0] != total or q.shape[2] != shape[2] or q.shape[1] < 1
                 or q.shape[1] % shape[1] or q.shape[1] > 4096):
             raise ValueError("q must have one row of query heads per new token")
-        if any(x.dtype != self.k.dtype or x.device != self.k.device for x in (q, k, v)):
+        if any(x.dtype != self.dtype or x.device != self.k.device for x in (q, k, v)):
             raise ValueError("q, k and v must have the cache's type and device")
         if not self.k.is_cuda:
             raise ValueError("extend needs a cache on the GPU")
         if any(x.requires_grad and torch.is_grad_enabled() or unpack_dual(x).tangent is not None
-               for x in (self.k, self.v, q, k, v)):
+               for x in (*self._pools(), q, k, v)):
             raise ValueError("extend is not differentiable: detach q, k and v, or use no_grad")
-        plain = {*map(type, (self.k, self.v, q, k, v))} <= {torch.Tensor, torch.nn.Parameter}
+        plain = {*map(type, (*self._pools(), q, k, v))} <= {torch.Tensor, torch.nn.Parameter}
         if plain and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("extend cannot be captured: its pages are planned on the host, "
                                "once per call; capture build_tables, append_kv_ and chunk_attention")
@@ -218,7 +246,7 @@ class PagedTreeCache:
         def store(x: torch.Tensor) -> int:
             return x.untyped_storage().data_ptr() if plain else x.untyped_storage()._cdata
 
-        pools = store(self.k), store(self.v)
+        pools = [store(x) for x in self._pools()]
         q, k, v = (x.clone() if store(x) in pools else x for x in (q, k, v))
         if options:  # refused here, before any page is taken
             empty, first = options, options.get("first")
@@ -229,7 +257,7 @@ class PagedTreeCache:
                 options["first"] = first = first.contiguous()
                 empty = options | {"first": first[:0]}
             none = self._upload([-1] * len(requests), [0] * len(requests), [0] * (len(requests) + 1))
-            chunk_attention(q[:0], self.k, self.v, none[0].unsqueeze(1), *none[1:], **empty)
+            self._attend(q[:0], none[0].unsqueeze(1), *none[1:], (), **empty)
         owner = self.owner
         # Requests that share a partial last page: all but the last to write
         # it take a clone.
@@ -253,15 +281,16 @@ class PagedTreeCache:
             clones = [plan.cow for plan in plans if plan.cow is not None]
             lists = [owner.pages[request] for request in requests]
             lengths = [owner.lengths[request] for request in requests]
-            old, fresh, ids, length, count = self._upload(
+            groups = owner.shared_prefixes(requests) if share else ()
+            old, fresh, ids, length, count, *groups = self._upload(
                 [old for old, _ in clones], [fresh for _, fresh in clones],
-                [page for pages in lists for page in pages], lengths, counts)
+                [page for pages in lists for page in pages], lengths, counts, *groups)
             if clones:
-                copy_pages_(self.k, self.v, old, fresh)
+                self._clone(old, fresh)
             width = max(1, *(len(pages) for pages in lists))
             table, starts, slots, _ = build_tables(ids, length, count, width, total)
-            append_kv_(self.k, self.v, k, v, slots)
-            return chunk_attention(q, self.k, self.v, table, length, starts, **options)
+            self._append(k, v, slots)
+            return self._attend(q, table, length, starts, tuple(groups), **options)
         except BaseException:
             # An allocation that failed, say.  Rows written so far lie behind
             # every holder's length, or in pages that are free again.
@@ -288,3 +317,91 @@ class PagedTreeCache:
         if cows:
             copy_pages_(self.k, self.v, old, fresh)
         commit_paths_(self.k, self.v, draft_k, draft_v, *table)
+
+
+class Fp8Cache(PagedTreeCache):
+    """Requests of ordinary tokens over a pool of 8 bits (see ``append_fp8_kv_``), with
+    rows, queries and outputs of ``dtype``: ``new``, ``fork``, ``checkpoint``,
+    ``rollback``, ``accept`` and ``extend`` as above, and ``read``.  Trees of draft
+    tokens are verified over a 16-bit pool: ``PagedTreeCache.new`` takes what ``read``
+    gives."""
+
+    def __init__(self, physical_pages: int, kv_heads: int, head_dim: int,
+                 dtype: torch.dtype = torch.bfloat16, device: str = "cuda"):
+        if head_dim not in (64, 128) or physical_pages < 1 or kv_heads < 1:
+            raise ValueError("head_dim must be 64/128; physical_pages and kv_heads must be positive")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("dtype must be FP16 or BF16")
+        self.owner = PageOwner(physical_pages)
+        self._dtype = dtype
+
+        def zeros(*shape: int, type: torch.dtype) -> torch.Tensor:
+            return torch.zeros(shape, device=device, dtype=torch.uint8).view(type)
+
+        self.k, self.v = (zeros(physical_pages, 16, kv_heads, head_dim, type=torch.float8_e4m3fn)
+                          for _ in range(2))
+        self.scale_k, self.scale_v = (zeros(physical_pages, kv_heads, 16, head_dim // 32,
+                                            type=torch.float8_e8m0fnu) for _ in range(2))
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self._dtype
+
+    def _pools(self) -> tuple[torch.Tensor, ...]:
+        return self.k, self.scale_k, self.v, self.scale_v
+
+    def _clone(self, old: torch.Tensor, fresh: torch.Tensor) -> None:
+        for x in self._pools():
+            pool = x.view(torch.uint8)
+            pool.index_copy_(0, fresh.long(), pool.index_select(0, old.long()))
+
+    def _append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        append_fp8_kv_(*self._pools(), k, v, slots)
+
+    def _attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+                starts: torch.Tensor, groups: tuple[torch.Tensor, ...], **options) -> torch.Tensor:
+        return fp8_chunk_attention(q, *self._pools(), table, lengths, starts, **options)
+
+    def _slots(self, request: int) -> torch.Tensor:
+        """The slots of all of a request's tokens."""
+        pages, tokens = self.owner.pages[request], self.owner.lengths[request]
+        ids, length = self._upload(pages, [tokens])
+        return build_tables(ids, length, length, max(1, len(pages)), tokens)[2]
+
+    def new(self, prefix_k: torch.Tensor, prefix_v: torch.Tensor) -> int:
+        """Create one request from [tokens, KV heads, head dim] tensors of the cache's type."""
+        if prefix_k.shape != prefix_v.shape or prefix_k.ndim != 3:
+            raise ValueError("prefix K/V shapes must match [tokens, heads, dim]")
+        if any(x.dtype != self.dtype or x.device != self.k.device for x in (prefix_k, prefix_v)):
+            raise ValueError("prefix must have the cache's type and device")
+        if tuple(prefix_k.shape[1:]) != tuple(self.k.shape[2:]):
+            raise ValueError("prefix head shape differs from cache")
+        if any(x.requires_grad and torch.is_grad_enabled() or unpack_dual(x).tangent is not None
+               for x in (prefix_k, prefix_v)):
+            raise ValueError("the cache is not differentiable: detach the prefix, or use no_grad")
+        rows = [x if x.stride(-1) == 1 else x.contiguous() for x in (prefix_k, prefix_v)]
+        request = self.owner.new(prefix_k.shape[0])
+        try:
+            self._append(*rows, self._slots(request))
+        except BaseException:  # the pages are free again, in the order they had
+            for page in reversed(self.owner.pages.pop(request)):
+                self.owner.release(page)
+            del self.owner.lengths[request]
+            raise
+        return request
+
+    def read(self, request: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """All of a request's K and V rows in the cache's type, [tokens, KV heads, head dim]."""
+        return read_fp8_kv(*self._pools(), self._slots(request), self.dtype)
+
+    def extend(self, requests: list[int], counts: list[int], q: torch.Tensor,
+               k: torch.Tensor, v: torch.Tensor, *, share: bool = False, **options) -> torch.Tensor:
+        """As ``PagedTreeCache.extend``, but every request reads its own pages."""
+        if share:
+            raise ValueError("share needs a 16-bit pool")
+        return super().extend(requests, counts, q, k, v, **options)
+
+    def verify(self, *_, **__):
+        raise NotImplementedError("trees are verified over a 16-bit pool: PagedTreeCache")
+
+    commit = commit_many = verify
