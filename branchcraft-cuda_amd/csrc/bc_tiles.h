@@ -41,12 +41,53 @@ struct ChunkParams {
   unsigned group_mul;        // ceil(2^32 / group), or 0: see divide
   unsigned hkv_mul;          // the same of hkv
   float scale, cap;
-  const uint8_t* k_scale;    // of an 8-bit cache, whose k, v and their strides are in bytes
+};
+
+struct TileParams {
+  ChunkParams c;
+  float* part_acc;  // [partial row][Hkv][D]; null: nothing is split
+  float* part_ml;   // [partial row][Hkv][2]: maximum and sum
+  int4* records;    // two counts, then two int4 per split tile and narrow request
+  int target;       // workgroups that a batch's work is cut for
+  int waves;        // ranges of the narrow requests' tiles, at most, per KV head
+  int most_parts;   // parts of split tiles, at most, per KV head
+  int part_rows;    // rows of such a part
+  int narrow_rows;  // partial rows of the narrow requests; the others' follow
+};
+
+// What the kernels of an 8-bit cache and of groups take on top.  Theirs alone have it
+// among their arguments: 48 bytes more there put those that the grid's size follows on
+// into another line, and a call of one token over 512 took 8.2 us in place of 7.9.
+struct MoreParams {
+  TileParams t;
+  const uint8_t* k_scale;  // of an 8-bit cache, whose k, v and their strides are in bytes
   const uint8_t* v_scale;
-  const int32_t* groups;     // of requests that begin with the same pages
+  const int32_t* groups;   // of requests that begin with the same pages
   const int32_t* shared;
   int group_count;
+  // With groups, see the entries below: records are one int4 each, of every entry's
+  // tiles (the groups' from own_records on), and behind the parts lie the partial
+  // rows of tiles in one piece, first those of the requests, then the groups'.
+  int single_rows;         // where these begin
+  int total_rows;          // all partial rows
+  int own_records;
 };
+
+template <bool FP8>
+using Taken = std::conditional_t<FP8, MoreParams, TileParams>;
+
+template <bool FP8>
+const Taken<FP8>& taken(const MoreParams& M) {
+  if constexpr (FP8)
+    return M;
+  else
+    return M.t;
+}
+
+// Of a kernel that takes them; its ChunkParams begin them.
+__device__ __forceinline__ const MoreParams& more(const ChunkParams& C) {
+  return reinterpret_cast<const MoreParams&>(C);
+}
 
 __device__ __forceinline__ float to_float(_Float16 x) { return (float)x; }
 __device__ __forceinline__ float to_float(__bf16 x) { return (float)x; }
@@ -166,7 +207,7 @@ __device__ __forceinline__ void attend_row(const ChunkParams& P, int t, int h, i
       if (ok) {
         const long long k = id * P.kp + (j & 15) * P.ks + kvh * P.kh;
         float dot = 0.f;
-        for (int d = 0; d < D; ++d) dot += load_elem<T>(q + d) * value(P.k, P.k_scale, k, id, j & 15, d);
+        for (int d = 0; d < D; ++d) dot += load_elem<T>(q + d) * value(P.k, more(P).k_scale, k, id, j & 15, d);
         s = dot * P.scale;
         if (P.cap > 0.f) s = P.cap * tanh_of(s / P.cap);
         s = s * kLog2e - slope * fabsf((float)(pos - j));
@@ -184,7 +225,7 @@ __device__ __forceinline__ void attend_row(const ChunkParams& P, int t, int h, i
         const float w = __shfl(p, from, 64);
         const long long v = page * P.vp + slot * P.vs + kvh * P.vh;
 #pragma unroll
-        for (int r = 0; r < R; ++r) acc[r] += w * value(P.v, P.v_scale, v, page, slot, 64 * r + lane);
+        for (int r = 0; r < R; ++r) acc[r] += w * value(P.v, more(P).v_scale, v, page, slot, 64 * r + lane);
       }
     }
   }
@@ -195,7 +236,8 @@ __device__ __forceinline__ void attend_row(const ChunkParams& P, int t, int h, i
 }
 
 template <typename T, int D, bool FP8>
-__global__ __launch_bounds__(kThreads) void chunk_rows_kernel(ChunkParams P) {
+__global__ __launch_bounds__(kThreads) void chunk_rows_kernel(Taken<FP8> A) {
+  const ChunkParams& P = reinterpret_cast<const ChunkParams&>(A);  // begins both
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.y * (kThreads / 64) + wave;
@@ -205,19 +247,20 @@ __global__ __launch_bounds__(kThreads) void chunk_rows_kernel(ChunkParams P) {
 }
 
 template <bool FP8>
-hipError_t launch_rows(const ChunkParams& P, int dim, int dtype, hipStream_t st) {
+hipError_t launch_rows(const MoreParams& M, int dim, int dtype, hipStream_t st) {
+  const ChunkParams& P = M.t.c;
   const dim3 grid(P.tokens < kMostGroups ? P.tokens : kMostGroups,
                   (P.hq + kThreads / 64 - 1) / (kThreads / 64));
   if (dtype == BC_FLOAT16) {
     if (dim == 64)
-      chunk_rows_kernel<_Float16, 64, FP8><<<grid, kThreads, 0, st>>>(P);
+      chunk_rows_kernel<_Float16, 64, FP8><<<grid, kThreads, 0, st>>>(taken<FP8>(M));
     else
-      chunk_rows_kernel<_Float16, 128, FP8><<<grid, kThreads, 0, st>>>(P);
+      chunk_rows_kernel<_Float16, 128, FP8><<<grid, kThreads, 0, st>>>(taken<FP8>(M));
   } else {
     if (dim == 64)
-      chunk_rows_kernel<__bf16, 64, FP8><<<grid, kThreads, 0, st>>>(P);
+      chunk_rows_kernel<__bf16, 64, FP8><<<grid, kThreads, 0, st>>>(taken<FP8>(M));
     else
-      chunk_rows_kernel<__bf16, 128, FP8><<<grid, kThreads, 0, st>>>(P);
+      chunk_rows_kernel<__bf16, 128, FP8><<<grid, kThreads, 0, st>>>(taken<FP8>(M));
   }
   return hipGetLastError();
 }
@@ -281,24 +324,6 @@ constexpr int kManyRows = 128;  // rows per workgroup of the wide form
 constexpr int kLeastSteps = 4;  // fewest steps per part of a split tile of rows
 constexpr int kLeastRun = 4;    // fewest 32-token tiles per wave of the narrow form
 
-struct TileParams {
-  ChunkParams c;
-  float* part_acc;  // [partial row][Hkv][D]; null: nothing is split
-  float* part_ml;   // [partial row][Hkv][2]: maximum and sum
-  int4* records;    // two counts, then two int4 per split tile and narrow request
-  int target;       // workgroups that a batch's work is cut for
-  int waves;        // ranges of the narrow requests' tiles, at most, per KV head
-  int most_parts;   // parts of split tiles, at most, per KV head
-  int part_rows;    // rows of such a part
-  int narrow_rows;  // partial rows of the narrow requests; the others' follow
-  // With groups, see the entries below: records are one int4 each, of every entry's
-  // tiles (the groups' from own_records on), and behind the parts lie the partial
-  // rows of tiles in one piece, first those of the requests, then the groups'.
-  int single_rows;  // where these begin
-  int total_rows;   // all partial rows
-  int own_records;
-};
-
 // The kernel's arguments, read anew: each phase of the tile kernel loads the
 // fields that it needs in one round at its start, and none lives through
 // another phase.  Read through the argument itself they were loaded in five
@@ -323,7 +348,7 @@ __device__ __forceinline__ void pin_plan(const TileParams& P) {
 template <bool FP8>
 __device__ __forceinline__ void pin_rows(const TileParams& P) {
   const ChunkParams& C = P.c;
-  if constexpr (FP8) asm volatile("" ::"s"(C.k_scale), "s"(C.v_scale), "s"(C.hkv));
+  if constexpr (FP8) asm volatile("" ::"s"(more(C).k_scale), "s"(more(C).v_scale), "s"(C.hkv));
   asm volatile("" ::"s"(C.q), "s"(C.k), "s"(C.v), "s"(C.pages), "s"(C.slopes), "s"(C.first),
                "s"(C.qt), "s"(C.qh), "s"(C.kp), "s"(C.ks), "s"(C.kh), "s"(C.vp), "s"(C.vs),
                "s"(C.vh), "s"(C.group), "s"(C.group_mul), "s"(C.max_pages), "s"(C.phys_pages),
@@ -831,7 +856,7 @@ __device__ __forceinline__ void add_untidy(const ChunkParams& C, const Request& 
     const long long at = p * C.vp + (j & 15) * C.vs + kvh * C.vh + 4 * g;
     const uint16_t* const v = C.v + (FP8 ? 0 : at);
     const uint8_t* const codes = reinterpret_cast<const uint8_t*>(C.v) + (FP8 ? at : 0);
-    const uint8_t* const scales = FP8 ? C.v_scale + scale_at<D>(C, p, kvh, j & 15) : nullptr;
+    const uint8_t* const scales = FP8 ? more(C).v_scale + scale_at<D>(C, p, kvh, j & 15) : nullptr;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -951,25 +976,35 @@ __device__ __forceinline__ Place place_of(const ChunkParams& P, const Request& g
   return at;
 }
 
-// Q of this lane's row of the wave's 32.
-template <int D>
-__device__ __forceinline__ void load_q(const ChunkParams& C, const Request& it, int r, int kvh, int g,
-                                       u32x4 (&qB)[D / 16]) {
+// This lane's row of the wave's 32: its token, counted from the request's first new
+// one, and its head.
+struct RowAt {
+  bool real;
+  int i, h;
+};
+
+__device__ __forceinline__ RowAt row_at(const ChunkParams& C, const Request& it, int r, int kvh) {
   const bool real = r < it.rows;
   const int i = real ? by_group(C, r) : 0, h = kvh * C.group + (real ? r - i * C.group : 0);
-  const int t = it.start + i;
-  const uint16_t* const q = C.q + t * C.qt + h * C.qh + 8 * g;
+  return {real, i, h};
+}
+
+// Its Q.
+template <int D>
+__device__ __forceinline__ void load_q(const ChunkParams& C, const Request& it, const RowAt& row, int g,
+                                       u32x4 (&qB)[D / 16]) {
+  const int t = it.start + row.i;
+  const uint16_t* const q = C.q + t * C.qt + row.h * C.qh + 8 * g;
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) qB[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
 }
 
-// The row's place and what it sees.
+// Its place and what it sees.
 template <int D, Form FORM, bool FORKS>
-__device__ __forceinline__ void start_rows(const ChunkParams& C, const Request& it, int r, int kvh, Rows<D>& R) {
-  const bool real = r < it.rows;
-  const int i = real ? by_group(C, r) : 0, h = kvh * C.group + (real ? r - i * C.group : 0);
-  const int t = it.start + i;
-  R.pos = it.pos0 + i;
+__device__ __forceinline__ void start_rows(const ChunkParams& C, const Request& it, const RowAt& row,
+                                           Rows<D>& R) {
+  const int t = it.start + row.i;
+  R.pos = it.pos0 + row.i;
   int2 seen;
   if (FORKS && is_group(it)) {
     const Place at = place_of(C, it, t);
@@ -979,11 +1014,11 @@ __device__ __forceinline__ void start_rows(const ChunkParams& C, const Request& 
     seen = row_range(C, it.b, t, R.pos, it.len);
     if constexpr (FORKS) seen.x = max(seen.x, it.floor);
   }
-  R.lo = real ? seen.x : 0;
-  R.hi = real ? seen.y : -1;
+  R.lo = row.real ? seen.x : 0;
+  R.hi = row.real ? seen.y : -1;
   R.slope = 0.f;
   if (FORM != Form::kPlain && C.slopes) {
-    const float slope = C.slopes[h];
+    const float slope = C.slopes[row.h];
     R.slope = FORM == Form::kCap ? slope / (2.f * C.cap) : slope / C.scale;
   }
   R.m = kNegInf;
@@ -994,12 +1029,13 @@ __device__ __forceinline__ void start_rows(const ChunkParams& C, const Request& 
     for (int j = 0; j < 16; ++j) R.acc[dt][j] = 0.f;
 }
 
-// Both.
+// All three.
 template <typename T, int D, Form FORM, bool FORKS>
 __device__ __forceinline__ void load_rows(const ChunkParams& C, const Request& it, int r, int kvh,
                                           int g, Rows<D>& R, u32x4 (&qB)[D / 16]) {
-  load_q<D>(C, it, r, kvh, g, qB);
-  start_rows<D, FORM, FORKS>(C, it, r, kvh, R);
+  const RowAt row = row_at(C, it, r, kvh);
+  load_q<D>(C, it, row, g, qB);
+  start_rows<D, FORM, FORKS>(C, it, row, R);
 }
 
 // Bounds on what rows see: any of them the tokens any_lo .. any_hi at most, all
@@ -1009,6 +1045,7 @@ struct Seen {
 };
 
 // Of rows r0 .. r1 - 1 of a request, from their places alone (no `first`).
+template <bool FORKS>
 __device__ __forceinline__ Seen rows_seen(const ChunkParams& C, const Request& rq, int r0, int r1) {
   if (r0 >= r1) return {0x7fffffff, -1, 0, 0x7fffffff};
   const int pa = rq.pos0 + by_group(C, r0), pb = rq.pos0 + by_group(C, r1 - 1), end = rq.len - 1;
@@ -1022,8 +1059,10 @@ __device__ __forceinline__ Seen rows_seen(const ChunkParams& C, const Request& r
     s.all_lo = max(0, max(pb, 0) - C.window + 1);
   }
   if (pa < 0) s.all_hi = -1;  // rows before the request see nothing
-  s.any_lo = max(s.any_lo, rq.floor);
-  s.all_lo = max(s.all_lo, rq.floor);
+  if constexpr (FORKS) {
+    s.any_lo = max(s.any_lo, rq.floor);
+    s.all_lo = max(s.all_lo, rq.floor);
+  }
   return s;
 }
 
@@ -1074,14 +1113,14 @@ __device__ __forceinline__ void put_record(const TileParams& P, int i, int start
 // `start`.  No two entries have one in common, since the rows of the
 // ones before end there.
 __device__ __forceinline__ int record_of(const TileParams& P, int entry, int start, int tile) {
-  const int from = entry < P.c.batch ? entry : P.own_records + entry - P.c.batch;
+  const int from = entry < P.c.batch ? entry : more(P.c).own_records + entry - P.c.batch;
   return from + start * P.c.group / kManyRows + tile;
 }
 
 // The partial row of an entry's first row, where a tile is in one piece.
 __device__ __forceinline__ int single_row(const TileParams& P, const Request& rq) {
   const int rows = P.c.tokens * P.c.group;
-  return P.single_rows + (is_group(rq) ? rows : 0) + rq.start * P.c.group;
+  return more(P.c).single_rows + (is_group(rq) ? rows : 0) + rq.start * P.c.group;
 }
 
 // Part p of the tile's rows are the partial rows first + p * stride ...; parts 0:
@@ -1133,6 +1172,45 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
       ids_next = load_ids(t0 + 16);
     }
   };
+  if (tid < 4) s_bad[tid] = 0;
+  // What a group's rows see depends on their requests, but without a window or
+  // documents it is read from its start to its end: its first step goes out ahead of
+  // the look at them.
+  const bool group = FORKS && is_group(rq), ahead = group && !C.first && C.window == 0;
+  auto rows = [&](auto early) {
+    if (!C.first && !group) {
+      mine = rows_seen<FORKS>(C, rq, row0, min(row0 + 32, rq.rows));
+      wg = rows_seen<FORKS>(C, rq, tile0, min(tile0 + kManyRows, rq.rows));
+      range();
+      load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
+    } else {
+      if (ahead) {
+        wg.any_lo = 0;
+        wg.any_hi = rq.len - 1;
+        range();
+        if (t0 < tend) early();
+      }
+      load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
+      mine = wave_seen(R, row0 + lr < rq.rows);
+      if (lane == 0) s_seen[wave] = mine;
+      __syncthreads();
+      wg = s_seen[0];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        wg.any_lo = min(wg.any_lo, s_seen[w].any_lo);
+        wg.any_hi = max(wg.any_hi, s_seen[w].any_hi);
+        wg.all_lo = max(wg.all_lo, s_seen[w].all_lo);
+        wg.all_hi = min(wg.all_hi, s_seen[w].all_hi);
+      }
+      wg.any_lo = __builtin_amdgcn_readfirstlane(wg.any_lo);
+      wg.any_hi = __builtin_amdgcn_readfirstlane(wg.any_hi);
+      wg.all_lo = __builtin_amdgcn_readfirstlane(wg.all_lo);
+      wg.all_hi = __builtin_amdgcn_readfirstlane(wg.all_hi);
+      if (!ahead) range();
+    }
+  };
+  if constexpr (!FORKS) rows([] {});
+
   const int lrow = tid / CPR, lcol = 8 * (tid % CPR ^ swz<D>(lrow));
   const unsigned koff = (unsigned)(((lrow % BC_PAGE_SIZE) * C.ks + lcol) * 2);
   const unsigned voff = (unsigned)(((lrow % BC_PAGE_SIZE) * C.vs + lcol) * 2);
@@ -1155,8 +1233,8 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     const int page = __builtin_amdgcn_readlane(pg.id, from);
     const size_t scales = scale_at<D>(C, page, kvh, 0);
     const unsigned off = (crow % BC_PAGE_SIZE) * (D / kFp8Block) + ccol / 2;
-    kx[x] = C.k_scale[scales + off];
-    vx[x] = C.v_scale[scales + off];
+    kx[x] = more(C).k_scale[scales + off];
+    vx[x] = more(C).v_scale[scales + off];
   };
   // ... and what inspect() does; `whole`: nothing.
   auto put = [&](int buf, bool whole, unsigned long long ok) {
@@ -1182,7 +1260,6 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     const unsigned dst = lds0 + buf * (4 * HALF) + x * 4096;
     load2_to_lds(Pages<FP8>::at(pg.k, from), Pages<FP8>::at(pg.v, from), koff, voff, dst, dst + 2 * HALF);
   };
-  if (tid < 4) s_bad[tid] = 0;
   auto first_step = [&] {  // its loads
     pg.take(C, kvh, ids);
 #pragma unroll
@@ -1192,41 +1269,7 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
       else
         issue_chunk(x, 0, 0);
   };
-  // What a group's rows see depends on their requests, but without a window or
-  // documents it is read from its start to its end: its first step goes out ahead of
-  // the look at them.
-  const bool group = FORKS && is_group(rq), ahead = group && !C.first && C.window == 0;
-  if (!C.first && !group) {
-    mine = rows_seen(C, rq, row0, min(row0 + 32, rq.rows));
-    wg = rows_seen(C, rq, tile0, min(tile0 + kManyRows, rq.rows));
-    range();
-    load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
-  } else {
-    if (ahead) {
-      wg.any_lo = 0;
-      wg.any_hi = rq.len - 1;
-      range();
-      if (t0 < tend) first_step();
-    }
-    load_rows<T, D, FORM, FORKS>(C, rq, row0 + lr, kvh, g, R, qB);
-    mine = wave_seen(R, row0 + lr < rq.rows);
-    if (lane == 0) s_seen[wave] = mine;
-    __syncthreads();
-    wg = s_seen[0];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      wg.any_lo = min(wg.any_lo, s_seen[w].any_lo);
-      wg.any_hi = max(wg.any_hi, s_seen[w].any_hi);
-      wg.all_lo = max(wg.all_lo, s_seen[w].all_lo);
-      wg.all_hi = min(wg.all_hi, s_seen[w].all_hi);
-    }
-    wg.any_lo = __builtin_amdgcn_readfirstlane(wg.any_lo);
-    wg.any_hi = __builtin_amdgcn_readfirstlane(wg.any_hi);
-    wg.all_lo = __builtin_amdgcn_readfirstlane(wg.all_lo);
-    wg.all_hi = __builtin_amdgcn_readfirstlane(wg.all_hi);
-    if (!ahead) range();
-  }
-
+  if constexpr (FORKS) rows(first_step);
   // Steps whole_lo .. whole_hi - 1 are seen whole by every row, given their pages.
   const int whole_lo = wg.all_lo / kStep + (wg.all_lo % kStep != 0);
   const int whole_hi = (min(wg.all_hi, rq.len - 1) + 1) / kStep;
@@ -1516,7 +1559,7 @@ struct Stream8 {
   }
   __device__ __forceinline__ void issue_k(int at) {
     const int page = __shfl(pg.id, 2 * at + ((lane >> 4) & 1), 64);
-    const uint8_t* const scales = lane < 32 ? C.k_scale : C.v_scale;
+    const uint8_t* const scales = lane < 32 ? more(C).k_scale : more(C).v_scale;
     powers_next = *reinterpret_cast<const Powers*>(scales + scale_at<D>(C, page, kvh, lane & 15));
 #pragma unroll
     for (int i = 0; i < NL; ++i) k[i] = load_codes<true>(Pages<true>::at(pg.k, 2 * at + i / NP), koff[i % NP]);
@@ -1654,19 +1697,19 @@ __device__ __forceinline__ void flat_body(const TileParams& P, A a, int batch, F
   // With groups a request's own part is short for a wave: Q comes a request ahead.
   constexpr bool kAhead = FORKS && FORM != Form::kCap;
   u32x4 q_next[D / 16];
-  if constexpr (kAhead) load_q<D>(C, p.rq, lr, kvh, g, q_next);
+  if constexpr (kAhead) load_q<D>(C, p.rq, row_at(C, p.rq, lr, kvh), g, q_next);
   for (;;) {  // over the requests
     Rows<D> R;
     u32x4 qB[D / 16];
     if constexpr (kAhead) {
-      start_rows<D, FORM, FORKS>(C, p.rq, lr, kvh, R);
+      start_rows<D, FORM, FORKS>(C, p.rq, row_at(C, p.rq, lr, kvh), R);
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) qB[s] = q_next[s];
     } else {
       load_rows<T, D, FORM, FORKS>(C, p.rq, lr, kvh, g, R, qB);
     }
     const Seen mine = C.first || (FORKS && is_group(p.rq)) ? wave_seen(R, lr < p.rq.rows)
-                                                           : rows_seen(C, p.rq, 0, p.rq.rows);
+                                                           : rows_seen<FORKS>(C, p.rq, 0, p.rq.rows);
     const int tend = p.first_tile + min(hi, p.x0 + p.tiles) - p.x0;
     // The next request's first pages, so that its first tile follows this
     // one's last as any tile follows another.
@@ -1675,7 +1718,7 @@ __device__ __forceinline__ void flat_body(const TileParams& P, A a, int batch, F
     const int ids_more = more ? st.ids(n.rq.b, first_of(n), 1) : 0;
     wait_rows(qB);
     if constexpr (kAhead) {
-      if (more) load_q<D>(C, n.rq, lr, kvh, g, q_next);
+      if (more) load_q<D>(C, n.rq, row_at(C, n.rq, lr, kvh), g, q_next);
     }
     for (;; ++t) {
       f32x16 sc[1];
@@ -1760,7 +1803,7 @@ __device__ __forceinline__ void narrow_body(const ChunkParams& C, const Request&
   Rows<D> R;
   u32x4 qB[D / 16];
   load_rows<T, D, FORM, false>(C, rq, lr, kvh, g, R, qB);
-  const Seen mine = C.first ? wave_seen(R, lr < rq.rows) : rows_seen(C, rq, 0, rq.rows);
+  const Seen mine = C.first ? wave_seen(R, lr < rq.rows) : rows_seen<false>(C, rq, 0, rq.rows);
   StreamOf<T, D, FORM, FP8> st(C, kvh, s_kv + wave * (2 * TILE));
   int t = mine.any_hi < mine.any_lo ? 1 : mine.any_lo / 32 + wave;
   const int tend = mine.any_hi < mine.any_lo ? 0 : mine.any_hi / 32 + 1;
@@ -1850,7 +1893,7 @@ __device__ __forceinline__ void clear_rows(const ChunkParams& C, long long at, l
 }
 
 template <typename T, int D, Form FORM, bool FP8>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(TileParams) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(Taken<FP8>) {
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[2 * 2 * kStep * D];
   __shared__ float2 s_ml[4 * 32];
   __shared__ Seen s_seen[4];
@@ -2021,10 +2064,9 @@ inline Cut cut_of(const bc_shape& s, int tokens, bool fp8) {
 }
 
 template <typename T, int D, bool FP8>
-hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned grid,
-                        hipStream_t st) {
-  TileParams P{};
-  P.c = C;
+hipError_t launch_tiles(MoreParams M, const Cut& cut, void* ws, unsigned grid, hipStream_t st) {
+  TileParams& P = M.t;
+  const ChunkParams& C = P.c;
   P.target = cut.target;
   if (ws) {
     char* const at = static_cast<char*>(ws);
@@ -2037,11 +2079,11 @@ hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned
     P.narrow_rows = cut.narrow_rows;
   }
   if (C.cap > 0.f)
-    chunk_tile_kernel<T, D, Form::kCap, FP8><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kCap, FP8><<<dim3(grid), 256, 0, st>>>(taken<FP8>(M));
   else if (C.slopes)
-    chunk_tile_kernel<T, D, Form::kBias, FP8><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kBias, FP8><<<dim3(grid), 256, 0, st>>>(taken<FP8>(M));
   else
-    chunk_tile_kernel<T, D, Form::kPlain, FP8><<<dim3(grid), 256, 0, st>>>(P);
+    chunk_tile_kernel<T, D, Form::kPlain, FP8><<<dim3(grid), 256, 0, st>>>(taken<FP8>(M));
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || !ws) return err;
   // Enough workgroups for the rows of a record and KV head, on average, but not
@@ -2057,13 +2099,13 @@ hipError_t launch_tiles(const ChunkParams& C, const Cut& cut, void* ws, unsigned
 }
 
 template <bool FP8>
-hipError_t launch_tiles(const ChunkParams& P, int dim, int dtype, const Cut& cut, void* ws, long long grid,
+hipError_t launch_tiles(const MoreParams& M, int dim, int dtype, const Cut& cut, void* ws, long long grid,
                         hipStream_t st) {
   if (dtype == BC_FLOAT16)
-    return dim == 64 ? launch_tiles<_Float16, 64, FP8>(P, cut, ws, (unsigned)grid, st)
-                     : launch_tiles<_Float16, 128, FP8>(P, cut, ws, (unsigned)grid, st);
-  return dim == 64 ? launch_tiles<__bf16, 64, FP8>(P, cut, ws, (unsigned)grid, st)
-                   : launch_tiles<__bf16, 128, FP8>(P, cut, ws, (unsigned)grid, st);
+    return dim == 64 ? launch_tiles<_Float16, 64, FP8>(M, cut, ws, (unsigned)grid, st)
+                     : launch_tiles<_Float16, 128, FP8>(M, cut, ws, (unsigned)grid, st);
+  return dim == 64 ? launch_tiles<__bf16, 64, FP8>(M, cut, ws, (unsigned)grid, st)
+                   : launch_tiles<__bf16, 128, FP8>(M, cut, ws, (unsigned)grid, st);
 }
 
 // Whether a window is as short as tables that are not cut, see cut_of (32 requests of
@@ -2154,12 +2196,7 @@ inline ChunkParams chunk_params(const bc_shape& s, const bc_chunk_inputs& in) {
                      group_mul,
                      hkv_mul,
                      in.scale,
-                     in.cap,
-                     nullptr,
-                     nullptr,
-                     nullptr,
-                     nullptr,
-                     0};
+                     in.cap};
 }
 
 }  // namespace

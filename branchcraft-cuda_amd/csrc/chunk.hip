@@ -209,11 +209,12 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
   if (!chunk_shape_ok(s, in.tokens) || !chunk_inputs_ok(in)) return BC_ERROR_INVALID_VALUE;
   if (in.tokens == 0) return BC_SUCCESS;
   if (!in.q || !in.output) return BC_ERROR_INVALID_VALUE;
-  const ChunkParams P = chunk_params(s, in);
+  MoreParams M{};
+  M.t.c = chunk_params(s, in);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   // Tiles of rows take 16-byte loads, 32-bit offsets inside a page and 31 bits
   // of rows and workgroups; anything else goes row by row.
-  const long long rows = (long long)in.tokens * P.group;
+  const long long rows = (long long)in.tokens * M.t.c.group;
   const Cut cut = cut_of(s, in.tokens, false);
   const bool use = cut.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= cut.bytes;
   const long long grid = tile_grid(s, in.tokens, cut, use);
@@ -222,6 +223,6 @@ extern "C" int bc_chunk_attention(bc_shape s, bc_chunk_inputs in, void* workspac
                      stride_bits(in) % 8 == 0 && in.k_strides.slot < far && in.v_strides.slot < far &&
                      rows <= 1 << 30 && grid <= kMostGroups;
   void* const ws = use ? workspace : nullptr;
-  if (tiled) return launch_tiles<false>(P, s.dim, in.dtype, cut, ws, grid, st);
-  return launch_rows<false>(P, s.dim, in.dtype, st);
+  if (tiled) return launch_tiles<false>(M, s.dim, in.dtype, cut, ws, grid, st);
+  return launch_rows<false>(M, s.dim, in.dtype, st);
 }

@@ -269,15 +269,16 @@ extern "C" int bc_fp8_chunk_attention(bc_shape s, bc_chunk_inputs in, const uint
     return BC_ERROR_INVALID_VALUE;
   if (in.tokens == 0) return BC_SUCCESS;
   if (!in.q || !in.output) return BC_ERROR_INVALID_VALUE;
-  ChunkParams P = chunk_params(s, in);
-  P.k_scale = k_scale;
-  P.v_scale = v_scale;
+  MoreParams M{};
+  M.t.c = chunk_params(s, in);
+  M.k_scale = k_scale;
+  M.v_scale = v_scale;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   // As in bc_chunk_attention.
   const Cut cut = cut_of(s, in.tokens, true);
   const bool use = cut.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= cut.bytes &&
                    !short_window(s, in);
-  const long long rows = (long long)in.tokens * P.group;
+  const long long rows = (long long)in.tokens * M.t.c.group;
   const long long grid = use ? split_grid(s, cut, rows, s.batch) : tile_grid(s, in.tokens, cut, false);
   const long long far = 1 << 27;  // bytes: offsets inside a page are 32-bit
   const bool tiled = aligned16(in.q) && aligned16(in.output) &&
@@ -285,6 +286,6 @@ extern "C" int bc_fp8_chunk_attention(bc_shape s, bc_chunk_inputs in, const uint
                      in.v_strides.slot < far && rows <= 1 << 30 &&
                      grid <= kMostGroups;
   void* const ws = use ? workspace : nullptr;
-  if (tiled) return launch_tiles<true>(P, s.dim, in.dtype, cut, ws, grid, st);
-  return launch_rows<true>(P, s.dim, in.dtype, st);
+  if (tiled) return launch_tiles<true>(M, s.dim, in.dtype, cut, ws, grid, st);
+  return launch_rows<true>(M, s.dim, in.dtype, st);
 }

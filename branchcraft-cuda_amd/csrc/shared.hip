@@ -24,7 +24,7 @@ struct Group {
 };
 
 __device__ __forceinline__ Group group_at(const ChunkParams& P, int g) {
-  const int from = P.groups[g], to = P.groups[g + 1], tokens = P.shared[g];  // in one round
+  const int from = more(P).groups[g], to = more(P).groups[g + 1], tokens = more(P).shared[g];  // in one round
   Group x;
   x.g0 = min(max(from, 0), P.batch);
   x.g1 = min(max(to, 0), P.batch);
@@ -35,8 +35,8 @@ __device__ __forceinline__ Group group_at(const ChunkParams& P, int g) {
 // The groups i .. i + 63, a lane each; behind the last, groups of no request.
 __device__ __forceinline__ Group groups_from(const ChunkParams& P, int i) {
   const int lane = threadIdx.x & 63;
-  const Group x = group_at(P, min(i + lane, P.group_count - 1));
-  return i + lane < P.group_count ? x : Group{0x7fffffff, 0, 0};
+  const Group x = group_at(P, min(i + lane, more(P).group_count - 1));
+  return i + lane < more(P).group_count ? x : Group{0x7fffffff, 0, 0};
 }
 
 // Of the 64 groups that the lanes hold, that of request b, a lane's own; -1, and 0
@@ -51,7 +51,7 @@ __device__ __forceinline__ int group_in(const Group& x, int b, int& shared) {
 // The group of request b, a lane's own, of the first 64 (`head`) or those behind.
 __device__ __forceinline__ int group_of(const ChunkParams& P, const Group& head, int b, int& shared) {
   int at = group_in(head, b, shared);
-  for (int i = 64; i < P.group_count; i += 64) {
+  for (int i = 64; i < more(P).group_count; i += 64) {
     int tokens;
     const int n = group_in(groups_from(P, i), b, tokens);
     if (n >= 0) {
@@ -72,7 +72,7 @@ struct Entries {
 
   __device__ __forceinline__ explicit Entries(const ChunkParams& C) : lane(threadIdx.x & 63), own1{} {
     own_blocks = (C.batch + 63) / 64;
-    blocks = own_blocks + (C.group_count + 63) / 64;
+    blocks = own_blocks + (more(C).group_count + 63) / 64;
     const int3 x0 = load(C, lane), x1 = load(C, 64 + lane);
     head = groups_from(C, 0);
     own0 = request(C, x0, lane);
@@ -112,7 +112,7 @@ struct Entries {
     AskedEntry a{};
     // Where the lanes hold all requests, the ends of its rows are theirs.
     int from = __shfl(own0.start, m.g0, 64), to = __shfl(own0.start + own0.n, m.g1 - 1, 64);
-    const bool is = g < C.group_count && m.shared > 0;
+    const bool is = g < more(C).group_count && m.shared > 0;
     if (is && own_blocks > 1) {
       from = min(max(C.starts[m.g0], 0), C.tokens);
       to = min(max(C.starts[m.g1], 0), C.tokens);
@@ -207,13 +207,13 @@ __device__ __forceinline__ Item plan_entry(const TileParams& P, const Entries& a
 // The kernels
 
 template <typename T, int D, Form FORM>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void fork_tile_kernel(TileParams) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void fork_tile_kernel(MoreParams) {
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[2 * 2 * kStep * D];
   __shared__ Seen s_seen[4];
   __shared__ int s_bad[4];
   const Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
   const TileParams& P = reread(args);
-  asm volatile("" ::"s"(P.c.groups), "s"(P.c.shared), "s"(P.c.group_count));
+  asm volatile("" ::"s"(more(P.c).groups), "s"(more(P.c).shared), "s"(more(P.c).group_count));
   pin_plan(P);
   const Entries all(P.c);
   const Cutting cut = cut_entries(P, all);
@@ -249,8 +249,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void fork_tile_kernel(TilePar
 // then of its group's in turn.  Rows that their entry has written as output are
 // left.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void fork_join_kernel(TileParams P, int apart) {
+__global__ __launch_bounds__(256) void fork_join_kernel(MoreParams M, int apart) {
   constexpr int LPR = D / 4, GW = 64 / LPR;
+  const TileParams& P = M.t;
   const ChunkParams& C = P.c;
   const int lane = threadIdx.x & 63, grp = lane / LPR, c = lane % LPR;
   const long long total = (long long)C.tokens * C.hkv * apart, step = 4ll * gridDim.x;
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(256) void fork_join_kernel(TileParams P, int apart)
         // Where starts decrease, a record may be another's or no one's.
         const long long last = rec.y + (long long)max(rec.x - 1, 0) * rec.z + row - tile * kManyRows;
         const bool sane = rec.x > 0 && rec.x <= 2 * (P.waves + P.most_parts) && rec.y >= 0 && rec.z > 0 &&
-                          last < P.total_rows;
+                          last < M.total_rows;
         parts[i] = sane ? rec.x : 0;
         first[i] = rec.y + row - tile * kManyRows;
         stride[i] = rec.z;
@@ -375,10 +376,10 @@ ForkCut fork_cut(const bc_shape& s, int tokens, int groups) {
 }
 
 template <typename T, int D>
-hipError_t launch_forks(const ChunkParams& C, const ForkCut& cut, void* ws, unsigned grid, hipStream_t st) {
+hipError_t launch_forks(MoreParams M, const ForkCut& cut, void* ws, unsigned grid, hipStream_t st) {
   char* const at = static_cast<char*>(ws);
-  TileParams P{};
-  P.c = C;
+  TileParams& P = M.t;
+  const ChunkParams& C = P.c;
   P.target = cut.target;
   P.part_acc = reinterpret_cast<float*>(at);
   P.part_ml = reinterpret_cast<float*>(at + cut.acc_bytes);
@@ -387,15 +388,15 @@ hipError_t launch_forks(const ChunkParams& C, const ForkCut& cut, void* ws, unsi
   P.most_parts = cut.most_parts;
   P.part_rows = cut.part_rows;
   P.narrow_rows = cut.narrow_rows;
-  P.single_rows = cut.single_rows;
-  P.total_rows = cut.total_rows;
-  P.own_records = cut.own_records;
+  M.single_rows = cut.single_rows;
+  M.total_rows = cut.total_rows;
+  M.own_records = cut.own_records;
   if (C.cap > 0.f)
-    fork_tile_kernel<T, D, Form::kCap><<<dim3(grid), 256, 0, st>>>(P);
+    fork_tile_kernel<T, D, Form::kCap><<<dim3(grid), 256, 0, st>>>(M);
   else if (C.slopes)
-    fork_tile_kernel<T, D, Form::kBias><<<dim3(grid), 256, 0, st>>>(P);
+    fork_tile_kernel<T, D, Form::kBias><<<dim3(grid), 256, 0, st>>>(M);
   else
-    fork_tile_kernel<T, D, Form::kPlain><<<dim3(grid), 256, 0, st>>>(P);
+    fork_tile_kernel<T, D, Form::kPlain><<<dim3(grid), 256, 0, st>>>(M);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   // A round of waves, eight workgroups per CU, with the rows of a token and KV head
@@ -404,7 +405,7 @@ hipError_t launch_forks(const ChunkParams& C, const ForkCut& cut, void* ws, unsi
   long long apart = 4 * most / pairs;
   apart = apart < 1 ? 1 : apart < C.group ? apart : C.group;
   const long long join = (pairs * apart + 3) / 4;
-  fork_join_kernel<T, D><<<dim3((unsigned)(join < most ? join : most)), 256, 0, st>>>(P, (int)apart);
+  fork_join_kernel<T, D><<<dim3((unsigned)(join < most ? join : most)), 256, 0, st>>>(M, (int)apart);
   return hipGetLastError();
 }
 
@@ -435,14 +436,15 @@ extern "C" int bc_shared_chunk_attention(bc_shape s, bc_chunk_inputs in, const i
       stride_bits(in) % 8 != 0 || in.k_strides.slot >= far || in.v_strides.slot >= far || grid > kMostGroups)
     return bc_chunk_attention(s, in, short_window(s, in) ? nullptr : workspace, workspace_bytes, stream);
   if (!in.q || !in.output) return BC_ERROR_INVALID_VALUE;
-  ChunkParams P = chunk_params(s, in);
-  P.groups = groups;
-  P.shared = shared;
-  P.group_count = group_count;
+  MoreParams M{};
+  M.t.c = chunk_params(s, in);
+  M.groups = groups;
+  M.shared = shared;
+  M.group_count = group_count;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (in.dtype == BC_FLOAT16)
-    return s.dim == 64 ? launch_forks<_Float16, 64>(P, cut, workspace, (unsigned)grid, st)
-                       : launch_forks<_Float16, 128>(P, cut, workspace, (unsigned)grid, st);
-  return s.dim == 64 ? launch_forks<__bf16, 64>(P, cut, workspace, (unsigned)grid, st)
-                     : launch_forks<__bf16, 128>(P, cut, workspace, (unsigned)grid, st);
+    return s.dim == 64 ? launch_forks<_Float16, 64>(M, cut, workspace, (unsigned)grid, st)
+                       : launch_forks<_Float16, 128>(M, cut, workspace, (unsigned)grid, st);
+  return s.dim == 64 ? launch_forks<__bf16, 64>(M, cut, workspace, (unsigned)grid, st)
+                     : launch_forks<__bf16, 128>(M, cut, workspace, (unsigned)grid, st);
 }
