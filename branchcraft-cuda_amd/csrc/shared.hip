@@ -48,16 +48,32 @@ __device__ __forceinline__ int group_in(const Group& x, int b, int& shared) {
   return n;
 }
 
-// The group of request b, a lane's own, of the first 64 (`head`) or those behind.
+// The group of request b, a lane's own, with b rising over the lanes: of the first 64
+// (`head`), or of those from the last that begins at or before the first lane's
+// request on, found in 64 steps at a time.  Looked through from the first on they
+// were 32 rounds of loads for 2048 groups, of every block of requests.
 __device__ __forceinline__ int group_of(const ChunkParams& P, const Group& head, int b, int& shared) {
   int at = group_in(head, b, shared);
-  for (int i = 64; i < more(P).group_count; i += 64) {
+  const int count = more(P).group_count;
+  if (count <= 64) return at;
+  const int lane = threadIdx.x & 63, first = __builtin_amdgcn_readfirstlane(b);
+  int from = 0;
+  for (int n = count; n > 64;) {
+    const int step = (n + 63) / 64, i = lane * step;
+    const bool upto = i < n && more(P).groups[from + min(i, n - 1)] <= first;
+    const int skipped = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(upto)) - 1, 0) * step;
+    from += skipped;
+    n = min(step, n - skipped);
+  }
+  for (int i = from; i < count; i += 64) {
+    const Group x = groups_from(P, i);
     int tokens;
-    const int n = group_in(groups_from(P, i), b, tokens);
+    const int n = group_in(x, b, tokens);
     if (n >= 0) {
       at = i + n;
       shared = tokens;
     }
+    if (__builtin_amdgcn_readlane(x.g0, 63) > __builtin_amdgcn_readlane(b, 63)) break;
   }
   return at;
 }
@@ -334,6 +350,9 @@ struct ForkCut : Cut {
 //    25.5 and 27.3, 277 MB (32 requests) 24 and 40, 8.9 GB (64, 32768) 82 and 774.
 //  - Tables of up to 1024 tokens, which are not cut there: 64 requests, 512 tokens 31
 //    and 16; past them, 1024 and up to 64 more, 22 and 35.
+//  - Many requests of little each: every workgroup walks the batch, some 5 us per 64
+//    requests.  Groups of 4: 504 requests of 0.5 MB 105 and 72, of 1 MB 110 and 107,
+//    120 of 2.1 MB 34 and 47; of 8: 1024 of 2.1 MB 355 and 503.
 //  - Under a window what is shared is less: 1024 tokens, 268 MB 50 and 47, 537 MB 38
 //    and 51.
 //  - Requests of many rows fill tiles by themselves: 8 of 64 rows over 8192 shared
@@ -342,7 +361,8 @@ bool sharing_pays(const bc_shape& s, int tokens, int window) {
   const long long table = (long long)s.max_pages * BC_PAGE_SIZE, rows = (long long)tokens * (s.query_heads / s.kv_heads);
   const long long seen = window > 0 && window < table ? window : table;
   const double mb = (double)s.batch * (double)seen * s.kv_heads * s.dim * 4 / 1e6;
-  return s.batch > 1 && table > 1024 && rows <= 80ll * s.batch && mb >= (seen < table ? 400 : 100);
+  return s.batch > 1 && table > 1024 && rows <= 80ll * s.batch && mb >= (seen < table ? 400 : 100) &&
+         mb >= 1.2 * s.batch;
 }
 
 // How a call cuts its work; bytes 0: every request reads its own pages.

@@ -78,13 +78,15 @@ def pays(fix, window=0):
     rows = fix["q"].shape[0] * (fix["q"].shape[1] // fix["k"].shape[2])
     seen = min(window or table, table)
     size = batch * seen * fix["k"].shape[2] * fix["k"].shape[3] * 4 / 1e6
-    return batch > 1 and table > 1024 and rows <= 80 * batch and size >= (400 if seen < table else 100)
+    return (batch > 1 and table > 1024 and rows <= 80 * batch and size >= (400 if seen < table else 100)
+            and size >= 1.2 * batch)
 
 
 def widen(fix):
     """The same batch in a table wide enough for that, with or without a window
     (windows have no more tokens than the table then): columns of no page."""
     batch, old = fix["pages"].shape
-    width = int(110e6 / (batch * C.PAGE * fix["k"].shape[2] * fix["k"].shape[3] * 4)) + 65
+    each = max(110e6 / batch, 1.3e6)  # bytes of K and V per request
+    width = int(each / (C.PAGE * fix["k"].shape[2] * fix["k"].shape[3] * 4)) + 65
     fix["pages"] = torch.cat((fix["pages"], torch.full((batch, max(width - old, 0)), -1, dtype=torch.int32)), 1)
     return fix

@@ -23,6 +23,21 @@ def test_more_requests_and_groups_than_a_wave_has_lanes(shape):
     both(fix, bounds, shared)
 
 
+@pytest.mark.parametrize("sizes", ["pairs", "after a large one", "with empty ones"])
+def test_groups_beyond_the_first_64_of_requests_in_blocks(sizes):
+    """A request's group is found among up to thousands: pairs, one group over several
+    blocks of 64 requests before them, and groups of none between them."""
+    pairs = [(16 + g % 4 * 16, [(1 + g % 3, 1), (2, 1)]) for g in range(150)]
+    if sizes == "after a large one":
+        pairs = pairs[:70] + [(64, [(2, 1)] * 150)] + pairs[70:]
+    fix, bounds, shared = F.forks(pairs, 2, 1, 64, F16, seed=12, lone_ends=1)
+    if sizes == "with empty ones":  # three of no request before every eighth
+        at = [i for i in range(len(shared)) for _ in range(4 if i % 8 == 7 else 1)]
+        bounds, shared = torch.cat((bounds[at], bounds[-1:])), shared[at]
+        assert len(shared) > 192 and (bounds[1:] >= bounds[:-1]).all()
+    both(fix, bounds, shared)
+
+
 @pytest.mark.parametrize("hq,hkv", [(73, 73), (129, 1), (146, 73)])
 def test_many_kv_heads_and_wide_groups(hq, hkv):
     fix, bounds, shared = F.forks([(160, [(3, 1)] * 9), (40, [(20, 1)] * 2)], hq, hkv, 64, BF16, seed=4)
