@@ -248,7 +248,8 @@ def shared_chunk_attention(q, k, v, pages, lengths, starts, groups, shared, *, s
     """``chunk_attention`` for requests that begin alike, such as forks: requests
     ``groups[g] .. groups[g+1] - 1`` have their first ``shared[g]`` tokens in pages
     of the same contents, which are read once for all of them (those of the first
-    one).  ``groups`` (rising) and ``shared`` are int32 tensors on the GPU; requests
+    one) where the sizes of the call say that this pays; elsewhere each request's are.
+    ``groups`` (not decreasing) and ``shared`` are int32 tensors on the GPU; requests
     outside all groups share nothing.  The results are ``chunk_attention``'s up to
     rounding."""
     return _shared_chunk_attention(q, k, v, pages, lengths, starts, groups, shared, scale, causal, window,

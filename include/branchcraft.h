@@ -468,8 +468,8 @@ size_t bc_chunk_attention_workspace_size(bc_shape shape, int tokens);
 /* K and V of a paged cache in 8 bits.  Codes, e4m3 [P, 16, Hkv, D], in any order
  * of pages, slots and heads (strides in bytes, multiples of 16; 16-byte aligned);
  * scales, a byte for every 32 values of a head, contiguous [P, Hkv, 16, D / 32]
- * and 4-byte aligned, so that those of a page and head lie side by side: byte x is 2^(x - 127).  A
- * value is its code times its block's scale.  A pool of zeros holds zeros.  Scale
+ * and 4-byte aligned, so that those of a page and head lie side by side: byte x is
+ * 2^(x - 127).  A value is its code times its block's scale.  A pool of zeros holds zeros.  Scale
  * bytes of 255 are never written; values read under one are not specified. */
 typedef struct bc_fp8_pool {
   uint8_t* k;
@@ -517,21 +517,25 @@ size_t bc_fp8_chunk_attention_workspace_size(bc_shape shape, int tokens);
 /* ---- requests that begin with the same pages ---- */
 
 /* bc_chunk_attention for forks: the requests groups[g] .. groups[g+1] - 1 have
- * their first shared[g] tokens in common, in pages of the same contents, of which
- * those in the first one's row of `pages` are read, once for all of them.
- * groups [group_count + 1] must rise, within [0, batch]; requests outside them
- * share nothing, and neither does a group of one.  shared [group_count] need not
- * be whole pages; at most the table's row counts.  Rows see what they see in
- * bc_chunk_attention, and the results differ from its by rounding alone.  Without
- * a workspace, and in the cases that go row by row there, every request's own row
- * of `pages` is read instead.  Also rejects: group_count < 0 or over batch, null
- * groups, null shared with groups. */
+ * their first shared[g] tokens in common, in pages of the same contents.
+ * groups [group_count + 1] must not decrease, within [0, batch]; requests outside
+ * them share nothing, and neither does a group of one.  shared [group_count] need
+ * not be whole pages; at most the table's row counts.  Rows see what they see in
+ * bc_chunk_attention, and the results differ from its by rounding alone.
+ *
+ * Where that pays, by shapes and window alone, the shared pages are read once for
+ * all of a group, those in the first one's row of `pages`: tables longer than 1024
+ * tokens, up to 80 rows (new tokens times group) a request, and 100 MB of K and V
+ * in the tables (400 within a window shorter than them), 1.2 MB a request.
+ * Elsewhere, without a workspace, and in the cases that go row by row there, every
+ * request's own row of `pages` is read, so each has to hold all of its pages.
+ * Also rejects: group_count < 0 or over batch, null groups, null shared with
+ * groups. */
 int bc_shared_chunk_attention(bc_shape shape, bc_chunk_inputs in, const int32_t* groups,
                               const int32_t* shared, int group_count, void* workspace,
                               size_t workspace_bytes, bc_stream_t stream);
 
-/* Bytes of workspace with which it reads shared pages once; 0 where it never
- * does. */
+/* Bytes of workspace for either way, as bc_chunk_attention_workspace_size. */
 size_t bc_shared_chunk_attention_workspace_size(bc_shape shape, int tokens, int group_count);
 
 /* Library version string, for logs. */
