@@ -281,11 +281,13 @@ __global__ __launch_bounds__(256) void fork_join_kernel(MoreParams M, int apart)
     // The request of token t, the first of its rows, and its group, of loads in one
     // round for up to 64 of either.
     const Group head = groups_from(C, 0);
-    int b = 0, own0 = 0;
+    int b = 0, own0 = 0, block = 0, from = 0;
     for (int i = 0; i < C.batch; i += 64) {
-      const int from = C.starts[min(i + lane, C.batch - 1)], to = C.starts[min(i + lane, C.batch - 1) + 1];
+      from = C.starts[min(i + lane, C.batch - 1)];
+      const int to = C.starts[min(i + lane, C.batch - 1) + 1];
       const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < C.batch && to <= t));
       b += n;
+      block = i;
       if (n < 64) {
         own0 = __builtin_amdgcn_readlane(from, n);
         break;
@@ -297,45 +299,53 @@ __global__ __launch_bounds__(256) void fork_join_kernel(MoreParams M, int apart)
     shared = __builtin_amdgcn_readfirstlane(shared);
     auto start_of = [&](int from) { return min(max(from, 0), C.tokens); };
     own0 = start_of(own0);
-    const int all0 = shared > 0 ? start_of(C.starts[group_at(C, g).g0]) : 0;
-    for (int r = sub; r < C.group; r += apart) {
-      int parts[2] = {}, first[2] = {}, stride[2] = {};
-      auto look = [&](int i, int entry, int from) {
-        if (t < from) return;
-        const int row = (t - from) * C.group + r, tile = row / kManyRows;
-        const int4 rec = P.records[record_of(P, entry, from, tile)];
+    int all0 = 0;
+    if (shared > 0) {  // from what the lanes have, where they have it
+      const int g0 = M.group_count <= 64 ? __builtin_amdgcn_readlane(head.g0, g & 63) : group_at(C, g).g0;
+      all0 = start_of(g0 >= block ? __builtin_amdgcn_readlane(from, (g0 - block) & 63) : C.starts[g0]);
+    }
+    // The records of up to 32 rows in one round: a lane each, of the request's entry
+    // and, in the upper half of the wave, of the group's.
+    for (int r0 = sub; r0 < C.group; r0 += 32 * apart) {
+      const bool of_group = lane >= 32;
+      const int mine = r0 + (lane & 31) * apart, start = of_group ? all0 : own0;
+      int parts = 0, first = 0, stride = 0;
+      if (mine < C.group && t >= start && (!of_group || shared > 0)) {
+        const int row = (t - start) * C.group + mine, tile = row / kManyRows;
+        const int4 rec = P.records[record_of(P, of_group ? C.batch + g : b, start, tile)];
         // Where starts decrease, a record may be another's or no one's.
         const long long last = rec.y + (long long)max(rec.x - 1, 0) * rec.z + row - tile * kManyRows;
         const bool sane = rec.x > 0 && rec.x <= 2 * (P.waves + P.most_parts) && rec.y >= 0 && rec.z > 0 &&
                           last < M.total_rows;
-        parts[i] = sane ? rec.x : 0;
-        first[i] = rec.y + row - tile * kManyRows;
-        stride[i] = rec.z;
-      };
-      look(0, b, own0);
-      if (shared > 0)
-        look(1, C.batch + g, all0);
-      else if (parts[0] < 2)
-        continue;
-      float m = kNegInf, l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int p = grp; p < parts[0] + parts[1]; p += GW) {
-        const bool own = p < parts[0];
-        const int at = own ? first[0] + p * stride[0] : first[1] + (p - parts[0]) * stride[1];
-        const size_t row = partial_row(P, at, kvh);
-        const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * row);
-        join(m, l, acc, ml.x, ml.y, *reinterpret_cast<const float4*>(P.part_acc + row * D + 4 * c));
+        parts = sane ? rec.x : 0;
+        first = rec.y + row - tile * kManyRows;
+        stride = rec.z;
       }
+      for (int i = 0; i < 32 && r0 + i * apart < C.group; ++i) {
+        const int r = r0 + i * apart;
+        const int own_parts = __builtin_amdgcn_readlane(parts, i), all_parts = __builtin_amdgcn_readlane(parts, 32 + i);
+        const int own_first = __builtin_amdgcn_readlane(first, i), all_first = __builtin_amdgcn_readlane(first, 32 + i);
+        const int own_stride = __builtin_amdgcn_readlane(stride, i), all_stride = __builtin_amdgcn_readlane(stride, 32 + i);
+        if (shared <= 0 && own_parts < 2) continue;
+        float m = kNegInf, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int p = grp; p < own_parts + all_parts; p += GW) {
+          const int at = p < own_parts ? own_first + p * own_stride : all_first + (p - own_parts) * all_stride;
+          const size_t row = partial_row(P, at, kvh);
+          const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * row);
+          join(m, l, acc, ml.x, ml.y, *reinterpret_cast<const float4*>(P.part_acc + row * D + 4 * c));
+        }
 #pragma unroll
-      for (int s = LPR; s < 64; s <<= 1)
-        join(m, l, acc, shfl_xor_f(m, s), shfl_xor_f(l, s),
-             make_float4(shfl_xor_f(acc.x, s), shfl_xor_f(acc.y, s), shfl_xor_f(acc.z, s),
-                         shfl_xor_f(acc.w, s)));
-      const float inv = one_over(l);
-      if (grp == 0)
-        *reinterpret_cast<uint2*>(C.out + ((size_t)t * C.hq + kvh * C.group + r) * D + 4 * c) =
-            make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+        for (int s = LPR; s < 64; s <<= 1)
+          join(m, l, acc, shfl_xor_f(m, s), shfl_xor_f(l, s),
+               make_float4(shfl_xor_f(acc.x, s), shfl_xor_f(acc.y, s), shfl_xor_f(acc.z, s),
+                           shfl_xor_f(acc.w, s)));
+        const float inv = one_over(l);
+        if (grp == 0)
+          *reinterpret_cast<uint2*>(C.out + ((size_t)t * C.hq + kvh * C.group + r) * D + 4 * c) =
+              make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+      }
     }
   }
 }
