@@ -589,12 +589,13 @@ uint8_t* bytes_of(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr
 
 // The checks of both calls on an 8-bit cache's rows, and the cache.
 bc_fp8_pool fp8_pool(const char* op, const at::Tensor& cache_k, const at::Tensor& scale_k,
-                     const at::Tensor& cache_v, const at::Tensor& scale_v, const at::Tensor& slots) {
+                     const at::Tensor& cache_v, const at::Tensor& scale_v, const at::Tensor& slots,
+                     const char* slots_name = "slots") {
   check_codes(cache_k, "cache_k");
   check_codes(cache_v, "cache_v");
   check_scales(scale_k, "scale_k", cache_k);
   check_scales(scale_v, "scale_v", cache_v);
-  check_dev_contig(slots, "slots", at::kInt);
+  check_dev_contig(slots, slots_name, at::kInt);
   TORCH_CHECK(cache_k.size(0) > 0 && cache_k.size(1) == BC_PAGE_SIZE && cache_k.size(2) > 0 &&
                   cache_v.sizes() == cache_k.sizes() && slots.dim() == 1,
               op, " shape mismatch");
@@ -658,6 +659,45 @@ void append_fp8_kv_autograd(at::Tensor& cache_k, at::Tensor& scale_k, at::Tensor
                             const at::Tensor& slots) {
   refuse_tracked("append_fp8_kv_", {&cache_k, &scale_k, &cache_v, &scale_v, &k, &v});
   append_fp8_kv_versions(cache_k, scale_k, cache_v, scale_v, k, v, slots);
+}
+
+// Pages of an 8-bit cache (see bc_copy_fp8_pages).
+void copy_fp8_pages_hip(at::Tensor& cache_k, at::Tensor& scale_k, at::Tensor& cache_v,
+                        at::Tensor& scale_v, const at::Tensor& src_pages, const at::Tensor& dst_pages) {
+  const bc_fp8_pool pool = fp8_pool("copy_fp8_pages_", cache_k, scale_k, cache_v, scale_v, src_pages,
+                                    "src_pages");
+  check_dev_contig(dst_pages, "dst_pages", at::kInt);
+  TORCH_CHECK(dst_pages.sizes() == src_pages.sizes(), "copy_fp8_pages_ shape mismatch");
+  TORCH_CHECK(dst_pages.device() == src_pages.device(), "all tensors must share a device");
+  const at::Tensor* const written[] = {&cache_k, &scale_k, &cache_v, &scale_v};
+  for (int i = 0; i < 4; ++i) {
+    at::assert_no_internal_overlap(*written[i]);
+    for (int j = 0; j < i; ++j) at::assert_no_overlap(*written[i], *written[j]);
+  }
+  if (src_pages.size(0) == 0) return;
+  const c10::DeviceGuard guard(cache_k.device());
+  check_launch(bc_copy_fp8_pages(pool_shape(cache_k), pool, src_pages.data_ptr<int>(),
+                                 dst_pages.data_ptr<int>(), int(src_pages.size(0)), current_stream()),
+               "copy_fp8_pages_");
+}
+
+void copy_fp8_pages_versions(at::Tensor& cache_k, at::Tensor& scale_k, at::Tensor& cache_v,
+                             at::Tensor& scale_v, const at::Tensor& src_pages,
+                             const at::Tensor& dst_pages) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("branchcraft::copy_fp8_pages_", "")
+                             .typed<decltype(copy_fp8_pages_hip)>();
+  for (at::Tensor* x : {&cache_k, &scale_k, &cache_v, &scale_v})
+    x->unsafeGetTensorImpl()->bump_version();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  op.call(cache_k, scale_k, cache_v, scale_v, src_pages, dst_pages);
+}
+
+void copy_fp8_pages_autograd(at::Tensor& cache_k, at::Tensor& scale_k, at::Tensor& cache_v,
+                             at::Tensor& scale_v, const at::Tensor& src_pages,
+                             const at::Tensor& dst_pages) {
+  refuse_tracked("copy_fp8_pages_", {&cache_k, &scale_k, &cache_v, &scale_v});
+  copy_fp8_pages_versions(cache_k, scale_k, cache_v, scale_v, src_pages, dst_pages);
 }
 
 // Rows of an 8-bit cache in 16 bits (see bc_read_fp8_kv).
@@ -929,6 +969,7 @@ TORCH_LIBRARY(branchcraft, m) {
   m.def("append_kv_(Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor k, Tensor v, Tensor slots) -> ()");
   m.def("chunk_attention(Tensor q, Tensor k, Tensor v, Tensor pages, Tensor lengths, Tensor starts, float? scale=None, bool causal=True, int window=0, float cap=0., Tensor? slopes=None, Tensor? prefix=None, Tensor? first=None) -> Tensor");
   m.def("append_fp8_kv_(Tensor(a!) cache_k, Tensor(b!) scale_k, Tensor(c!) cache_v, Tensor(d!) scale_v, Tensor k, Tensor v, Tensor slots) -> ()");
+  m.def("copy_fp8_pages_(Tensor(a!) cache_k, Tensor(b!) scale_k, Tensor(c!) cache_v, Tensor(d!) scale_v, Tensor src_pages, Tensor dst_pages) -> ()");
   m.def("read_fp8_kv(Tensor cache_k, Tensor scale_k, Tensor cache_v, Tensor scale_v, Tensor slots, ScalarType dtype) -> (Tensor, Tensor)");
   m.def("fp8_chunk_attention(Tensor q, Tensor k, Tensor scale_k, Tensor v, Tensor scale_v, Tensor pages, Tensor lengths, Tensor starts, float? scale=None, bool causal=True, int window=0, float cap=0., Tensor? slopes=None, Tensor? prefix=None, Tensor? first=None) -> Tensor");
   m.def("shared_chunk_attention(Tensor q, Tensor k, Tensor v, Tensor pages, Tensor lengths, Tensor starts, Tensor groups, Tensor shared, float? scale=None, bool causal=True, int window=0, float cap=0., Tensor? slopes=None, Tensor? prefix=None, Tensor? first=None) -> Tensor");
@@ -947,6 +988,7 @@ TORCH_LIBRARY_IMPL(branchcraft, CUDA, m) {
   m.impl("append_kv_", append_kv_hip);
   m.impl("chunk_attention", chunk_attention_hip);
   m.impl("append_fp8_kv_", append_fp8_kv_hip);
+  m.impl("copy_fp8_pages_", copy_fp8_pages_hip);
   m.impl("read_fp8_kv", read_fp8_kv_hip);
   m.impl("fp8_chunk_attention", fp8_chunk_attention_hip);
   m.impl("shared_chunk_attention", shared_chunk_attention_hip);
@@ -956,6 +998,7 @@ TORCH_LIBRARY_IMPL(branchcraft, ADInplaceOrView, m) {
   m.impl("write_prefix_", write_prefix_versions);
   m.impl("append_kv_", append_kv_versions);
   m.impl("append_fp8_kv_", append_fp8_kv_versions);
+  m.impl("copy_fp8_pages_", copy_fp8_pages_versions);
 }
 
 TORCH_LIBRARY_IMPL(branchcraft, Autograd, m) {
@@ -963,6 +1006,7 @@ TORCH_LIBRARY_IMPL(branchcraft, Autograd, m) {
   m.impl("append_kv_", append_kv_autograd);
   m.impl("chunk_attention", chunk_attention_autograd);
   m.impl("append_fp8_kv_", append_fp8_kv_autograd);
+  m.impl("copy_fp8_pages_", copy_fp8_pages_autograd);
   m.impl("read_fp8_kv", read_fp8_kv_autograd);
   m.impl("fp8_chunk_attention", fp8_chunk_attention_autograd);
   m.impl("shared_chunk_attention", shared_chunk_attention_autograd);

@@ -36,7 +36,7 @@ EXPORTED = (
     "bc_packed_decode_ws", "bc_packed_decode_noalloc", "bc_version",
     "bc_build_tables", "bc_append_kv", "bc_chunk_attention",
     "bc_chunk_attention_workspace_size",
-    "bc_append_fp8_kv", "bc_read_fp8_kv", "bc_fp8_chunk_attention",
+    "bc_append_fp8_kv", "bc_read_fp8_kv", "bc_copy_fp8_pages", "bc_fp8_chunk_attention",
     "bc_fp8_chunk_attention_workspace_size", "bc_shared_chunk_attention",
     "bc_shared_chunk_attention_workspace_size",
 )
@@ -153,6 +153,8 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
     lib.bc_read_fp8_kv.argtypes = [Shape, Fp8Pool, c_void_p, c_int, c_int, c_void_p, c_void_p,
                                    c_void_p]
     lib.bc_read_fp8_kv.restype = c_int
+    lib.bc_copy_fp8_pages.argtypes = [Shape, Fp8Pool, c_void_p, c_void_p, c_int, c_void_p]
+    lib.bc_copy_fp8_pages.restype = c_int
     lib.bc_fp8_chunk_attention.argtypes = [Shape, ChunkInputs, c_void_p, c_void_p, c_void_p,
                                            c_size_t, c_void_p]
     lib.bc_fp8_chunk_attention.restype = c_int

@@ -6,8 +6,8 @@ with the reference's schemas (bindings/torch_ops.cpp:144-148 of
 Haaziq386/branchcraft-cuda) plus ``paged_decode`` (the reference's C++
 ``branchcraft::decode``), ``copy_pages_``, ``commit_paths_`` and the chunk ops
 (``build_tables``, ``append_kv_``, ``chunk_attention``), an 8-bit cache
-(``append_fp8_kv_``, ``read_fp8_kv``, ``fp8_chunk_attention``) and attention for
-forks (``shared_chunk_attention``).  There is no CPU or Python fallback: a missing
+(``append_fp8_kv_``, ``copy_fp8_pages_``, ``read_fp8_kv``, ``fp8_chunk_attention``)
+and attention for forks (``shared_chunk_attention``).  There is no CPU or Python fallback: a missing
 extension raises ImportError, and the ops have only a GPU implementation.
 
 FakeTensor implementations follow python/branchcraft_torch/__init__.py:18-31
@@ -88,6 +88,11 @@ def _fake_chunk_attention(q, k, v, pages, lengths, starts, scale=None, causal=Tr
 
 @torch.library.register_fake("branchcraft::append_fp8_kv_")
 def _fake_append_fp8_kv(cache_k, scale_k, cache_v, scale_v, k, v, slots):
+    return None
+
+
+@torch.library.register_fake("branchcraft::copy_fp8_pages_")
+def _fake_copy_fp8_pages(cache_k, scale_k, cache_v, scale_v, src_pages, dst_pages):
     return None
 
 
@@ -227,6 +232,13 @@ def append_fp8_kv_(cache_k, scale_k, cache_v, scale_v, k, v, slots):
     return _append_fp8_kv(cache_k, scale_k, cache_v, scale_v, k, v, slots)
 
 
+def copy_fp8_pages_(cache_k, scale_k, cache_v, scale_v, src_pages, dst_pages):
+    """Copy whole pages of an 8-bit cache, codes and scales, as ``copy_pages_`` copies
+    those of a 16-bit one: every pair at once, so destinations must be distinct and
+    none may also be a source."""
+    return torch.ops.branchcraft.copy_fp8_pages_(cache_k, scale_k, cache_v, scale_v, src_pages, dst_pages)
+
+
 def read_fp8_kv(cache_k, scale_k, cache_v, scale_v, slots, dtype):
     """Rows of an 8-bit cache in FP16 or BF16, ``(k, v)``, each [len(slots), KV heads,
     dim]; zeros for slots of -1 and outside the pool.  What was written from a type
@@ -258,6 +270,6 @@ def shared_chunk_attention(q, k, v, pages, lengths, starts, groups, shared, *, s
 
 __all__ = ["tree_verify", "packed_decode_out", "paged_decode",
            "commit_path_", "copy_pages_", "commit_paths_", "write_prefix_", "int_tensor",
-           "build_tables", "append_kv_", "chunk_attention", "append_fp8_kv_", "read_fp8_kv",
+           "build_tables", "append_kv_", "chunk_attention", "append_fp8_kv_", "copy_fp8_pages_", "read_fp8_kv",
            "fp8_chunk_attention", "shared_chunk_attention",
            "LIBRARY_PATH"]

@@ -24,8 +24,8 @@ import torch
 from torch.autograd.forward_ad import unpack_dual
 
 from . import (append_fp8_kv_, append_kv_, build_tables, chunk_attention, commit_path_,
-               commit_paths_, copy_pages_, fp8_chunk_attention, int_tensor, read_fp8_kv,
-               shared_chunk_attention, tree_verify, write_prefix_)
+               commit_paths_, copy_fp8_pages_, copy_pages_, fp8_chunk_attention, int_tensor,
+               read_fp8_kv, shared_chunk_attention, tree_verify, write_prefix_)
 from .pages import CommitPlan, PageOwner, Snapshot
 
 __all__ = ["PagedTreeCache", "Fp8Cache", "Snapshot", "CommitPlan"]
@@ -351,9 +351,7 @@ class Fp8Cache(PagedTreeCache):
         return self.k, self.scale_k, self.v, self.scale_v
 
     def _clone(self, old: torch.Tensor, fresh: torch.Tensor) -> None:
-        for x in self._pools():
-            pool = x.view(torch.uint8)
-            pool.index_copy_(0, fresh.long(), pool.index_select(0, old.long()))
+        copy_fp8_pages_(*self._pools(), old, fresh)
 
     def _append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         append_fp8_kv_(*self._pools(), k, v, slots)

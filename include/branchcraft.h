@@ -502,6 +502,11 @@ int bc_append_fp8_kv(bc_shape shape, const bc_half* k, const bc_half* v,
 int bc_read_fp8_kv(bc_shape shape, bc_fp8_pool pool, const int32_t* slots, int tokens,
                    int dtype, bc_half* k, bc_half* v, bc_stream_t stream);
 
+/* Whole pages, codes and scales, as bc_copy_pages; rejects what bc_append_fp8_kv
+ * rejects of the pool. */
+int bc_copy_fp8_pages(bc_shape shape, bc_fp8_pool pool, const int32_t* src_pages,
+                      const int32_t* dst_pages, int count, bc_stream_t stream);
+
 /* bc_chunk_attention over a cache of 8 bits: in.k and in.v are the codes and
  * in.k_strides and in.v_strides their strides in bytes (see bc_fp8_pool; the same
  * alignment is asked for), q, the output and the arithmetic are of in.dtype, to

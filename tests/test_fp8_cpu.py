@@ -45,6 +45,13 @@ def test_rows_are_refused():
         assert lib.bc_read_fp8_kv(*args) == INVALID, (at, x)
     good[3] = 0
     assert lib.bc_read_fp8_kv(*good) == 0
+    good = [_shape(), _pool(), FAKE, FAKE, 3, None]
+    bad = [(0, _shape(**x)) for x in BAD_POOL_SHAPES] + [(1, _pool(**x)) for x in BAD_POOLS]
+    for at, x in bad + [(2, None), (3, None), (4, -1)]:
+        args = list(good)
+        args[at] = x
+        assert lib.bc_copy_fp8_pages(*args) == INVALID, (at, x)
+    assert lib.bc_copy_fp8_pages(*good[:2], None, None, 0, None) == 0
 
 
 @pytest.mark.parametrize("bad", BAD_SHAPES, ids=str)
@@ -108,6 +115,8 @@ def test_fake_tensors_and_versions():
         before = [x._version for x in pool]
         bt.append_fp8_kv_(*pool, *rows, slots)
         assert [x._version - b for x, b in zip(pool, before)] == [1] * 4 and rows[0]._version == 0
+        bt.copy_fp8_pages_(*pool, slots, slots)
+        assert [x._version - b for x, b in zip(pool, before)] == [2] * 4
         for x in bt.read_fp8_kv(*pool, slots, torch.float16):
             assert x.shape == (7, 2, 64) and x.dtype == torch.float16
         out = bt.fp8_chunk_attention(q, *pool, *ints, cap=3.0, window=4)

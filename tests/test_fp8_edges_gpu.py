@@ -278,6 +278,10 @@ def test_row_refusals():
                  (pool[0].half(), *pool[1:], slots, F16), (pool[0], pool[1][:-1], *pool[2:], slots, F16)]:
         with pytest.raises((RuntimeError, NotImplementedError)):
             bt.read_fp8_kv(*args)
+    for args in [(*pool, slots, slots[:2]), (*pool, slots.long(), slots), (*pool, slots, slots.cpu()), (*pool, slots[None], slots[None]),
+                 (pool[0], pool[1], pool[0], pool[3], slots, slots), (pool[0].half(), *pool[1:], slots, slots)]:
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            bt.copy_fp8_pages_(*args)
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])

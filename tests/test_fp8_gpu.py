@@ -49,6 +49,31 @@ def rows(n, hkv, d, dtype, seed=0):
     return x
 
 
+@pytest.mark.parametrize("hkv,d", [(1, 64), (8, 128), (3, 64), (73, 128)])
+@pytest.mark.parametrize("form", ["plain", "packed pool", "heads pool"])
+@pytest.mark.parametrize("count", [0, 1, 10])
+def test_pages_are_copied(count, form, hkv, d):
+    """Bit for bit; pairs with a page outside the pool, or of one page, do nothing."""
+    import branchcraft_torch as bt
+    ck, sk, cv, sv = empty_pool(20, hkv, d)
+    if form == "packed pool":
+        whole = torch.stack((ck.view(torch.uint8), cv.view(torch.uint8)), 1).view(F.E4M3)
+        ck, cv = whole[:, 0], whole[:, 1]
+    elif form == "heads pool":
+        ck, cv = (x.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(F.E4M3) for x in (ck, cv))
+    src = torch.tensor([3, 0, 19, 3, -1, 20, 4, 8, 2**31 - 1, 5][:count], dtype=torch.int32)
+    dst = torch.tensor([7, 18, 1, 2, 9, 10, 20, 8, 11, -2**31][:count], dtype=torch.int32)
+    want = [raw(x).cpu().clone() for x in (ck, sk, cv, sv)]
+    for a, b in zip(src.tolist(), dst.tolist()):
+        if 0 <= a < 20 and 0 <= b < 20:
+            for x in want:
+                x[b] = x[a]
+    bt.copy_fp8_pages_(ck, sk, cv, sv, src.cuda(), dst.cuda())
+    torch.cuda.synchronize()
+    for x, y in zip((ck, sk, cv, sv), want):
+        assert torch.equal(raw(x).cpu(), y)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
 @pytest.mark.parametrize("tokens,hkv,d", [(1, 8, 128), (3, 1, 64), (17, 3, 64), (300, 8, 128), (70, 40, 128)])
 @pytest.mark.parametrize("form", ["plain", "fused", "heads_first", "unaligned", "expanded", "packed pool",
