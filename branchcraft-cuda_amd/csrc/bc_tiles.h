@@ -1309,6 +1309,11 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   // the compiler's wait, inside the loop, also covers the loads that each step
   // has just issued.
   wait_rows(qB);
+  // Products start from the bias where registers allow that.  Over an 8-bit cache at D
+  // = 128 some 30 would be spilled, in every step: there it is added behind them, one
+  // more instruction a score (2048 new tokens of 16384 612 us, 834 with spills; of 16
+  // bits 535; 4 x 1024 of 4096 312, 429; 280).
+  constexpr bool kStarts = FORM == Form::kBias && !(FP8 && D == 128);
   // One step, its K and V in buffer `buf`; the next one's loads go out between
   // the score products.
   auto step = [&](auto which, int t) {
@@ -1329,12 +1334,11 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
 #pragma unroll
       for (int i = 0; i < 2; ++i) kf[i][s] = lds16(kt + i * 32 * D + o.k[s]);
     const f32x16 zero = {};
-    if (FORM == Form::kBias) start_scores<D, 2>(C, sc, R, t * kStep, g);
+    if (kStarts) start_scores<D, 2>(C, sc, R, t * kStep, g);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        sc[i] = Num<T>::mfma(kf[i][s], qB[s], FORM != Form::kBias && s == 0 ? zero : sc[i]);
+      for (int i = 0; i < 2; ++i) sc[i] = Num<T>::mfma(kf[i][s], qB[s], !kStarts && s == 0 ? zero : sc[i]);
       if (!FP8 && s % 2 == 1 && s / 2 < NX) {
         if (next) issue_chunk(s / 2, at, buf ^ 1);
       }
@@ -1347,6 +1351,12 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
     }
     Edges e{t * kStep < mine.all_lo, t * kStep + kStep - 1 > mine.all_hi, pages != 15, 0};
     if (e.pages) e.valid = tokens_of<4>(rq.len - t * kStep, pages);
+    if (FORM == Form::kBias && !kStarts) {
+      f32x16 bias[2];
+      start_scores<D, 2>(C, bias, R, t * kStep, g);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sc[i] += bias[i];
+    }
     finish_scores<D, FORM, 2>(C, sc, R, t * kStep, g, e);
     // The softmax and its product ahead of other waves' score products, so that
     // the two of a SIMD do not fall into step: 4096 of 4096 tokens (D = 128) 167
@@ -1899,8 +1909,13 @@ __device__ __forceinline__ void clear_rows(const ChunkParams& C, long long at, l
     out[x < head * row ? x : x + gap] = u32x4{0, 0, 0, 0};
 }
 
+// Workgroups per CU: three at D = 64 (see wide_body), but two for the biased and capped
+// forms of an 8-bit cache, which spill with the registers of three: 64 single tokens
+// over 2048, bias 39 us and cap 41 (three: 42, 46), 24 mixed requests with a cap 95
+// (103), against 4 x 1024 new tokens of 4096 199 and 247 (188, 234).
 template <typename T, int D, Form FORM, bool FP8>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void chunk_tile_kernel(Taken<FP8>) {
+__global__ __launch_bounds__(256, D == 64 && !(FP8 && FORM != Form::kPlain) ? 3 : 2) void chunk_tile_kernel(
+    Taken<FP8>) {
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[2 * 2 * kStep * D];
   __shared__ float2 s_ml[4 * 32];
   __shared__ Seen s_seen[4];
