@@ -1309,11 +1309,12 @@ __device__ __forceinline__ void wide_body(const TileParams& A, Args args, const 
   // the compiler's wait, inside the loop, also covers the loads that each step
   // has just issued.
   wait_rows(qB);
-  // Products start from the bias where registers allow that.  Over an 8-bit cache at D
-  // = 128 some 30 would be spilled, in every step: there it is added behind them, one
-  // more instruction a score (2048 new tokens of 16384 612 us, 834 with spills; of 16
-  // bits 535; 4 x 1024 of 4096 312, 429; 280).
-  constexpr bool kStarts = FORM == Form::kBias && !(FP8 && D == 128);
+  // Products start from the bias where registers allow that.  Over an 8-bit cache, and
+  // with groups, at D = 128 some would be spilled, in every step: there it is added
+  // behind them, one more instruction a score (8 bits, 2048 new tokens of 16384 612 us,
+  // 834 with spills, of 16 bits 535; 4 x 1024 of 4096 312, 429, 280; 64 single tokens
+  // over a shared 16384 64, 69).
+  constexpr bool kStarts = FORM == Form::kBias && !((FP8 || FORKS) && D == 128);
   // One step, its K and V in buffer `buf`; the next one's loads go out between
   // the score products.
   auto step = [&](auto which, int t) {
