@@ -44,6 +44,52 @@ class CommitPlan:
     new_length: int = 0
 
 
+def _neighbours(common: list[int], count: int) -> list[tuple[int, int]]:
+    """A list of ``count`` requests, of which i and i + 1 have ``common[i]`` pages in
+    common, as groups ``(members, pages in common)`` with the largest sum of
+    (members - 1) * pages.
+
+    ``saved[n]`` is that sum of the first n.  A last group from j on with p pages gives
+    saved[j] + (n - 1 - j) * p.  The starts j of equal p lie on the stack together, p
+    rising; the best of them for a p that only falls is found on the upper hull of their
+    points (j, saved[j]), from its front on."""
+    saved, last = [0], [(0, 0)]  # of the best last group: where it starts, and its pages
+    stack: list[tuple[int, list[int]]] = []
+
+    def join(front: list[int], more: list[int]) -> list[int]:
+        for j in more:
+            while len(front) > 1:
+                h, i = front[-2:]
+                if (saved[i] - saved[h]) * (j - h) > (saved[j] - saved[h]) * (i - h):
+                    break
+                front.pop()
+            front.append(j)
+        return front
+
+    for n in range(1, count + 1):
+        if n > 1:
+            pages, starts = common[n - 2], [n - 2]
+            while stack and stack[-1][0] >= pages:
+                starts = join(stack.pop()[1], starts)
+            if pages:  # else the stack is empty
+                stack.append((pages, starts))
+        best, of = saved[n - 1], (n - 1, 0)
+        for pages, starts in stack:
+            while len(starts) > 1 and saved[starts[1]] - saved[starts[0]] >= (starts[1] - starts[0]) * pages:
+                del starts[0]
+            value = saved[starts[0]] + (n - 1 - starts[0]) * pages
+            if value > best:
+                best, of = value, (starts[0], pages)
+        saved.append(best)
+        last.append(of)
+    groups, n = [], count
+    while n:
+        start, pages = last[n]
+        groups.append((n - start, pages))
+        n = start
+    return groups[::-1]
+
+
 class PageOwner:
     def __init__(self, physical_pages: int):
         if physical_pages < 1:
@@ -191,23 +237,30 @@ class PageOwner:
     def shared_prefixes(self, requests: list[int]) -> tuple[list[int], list[int]]:
         """Requests next to each other in the list that begin with the same pages:
         ``(bounds, tokens)``, group g being ``requests[bounds[g]:bounds[g + 1]]``, whose
-        first ``tokens[g]`` tokens lie in pages of all of them.  A request joins the
-        group before it unless that would cost it half of what it shares."""
-        bounds, tokens = [], []
-        for i, request in enumerate(requests):
-            pages, length = self.pages[request], self.lengths[request]
-            if bounds:
-                first = self.pages[requests[bounds[-1]]]
-                most = min(tokens[-1], length)
-                same = most // PAGE_SIZE  # whole pages; most often all of them
-                if pages[:same] != first[:same]:
-                    same = next(n for n in range(same) if pages[n] != first[n])
-                if same and (2 * same * PAGE_SIZE > tokens[-1] or i == bounds[-1] + 1):
-                    tokens[-1] = same * PAGE_SIZE
-                    continue
-            bounds.append(i)
-            tokens.append(length)
-        return bounds + [len(requests)], tokens
+        first ``tokens[g]`` tokens lie in pages of all of them (a group of one: all that
+        it has).  The list is cut where most tokens are then read once for several
+        requests instead of for each."""
+        common = [self._common_pages(a, b) for a, b in zip(requests, requests[1:])]
+        bounds, tokens = [0], []
+        for members, pages in _neighbours(common, len(requests)):
+            tokens.append(pages * PAGE_SIZE if members > 1 else self.lengths[requests[bounds[-1]]])
+            bounds.append(bounds[-1] + members)
+        return bounds, tokens
+
+    def _common_pages(self, a: int, b: int) -> int:
+        """Whole pages that two requests begin with."""
+        x, y = self.pages[a], self.pages[b]
+        end = min(self.lengths[a], self.lengths[b]) // PAGE_SIZE
+        if x[:end] == y[:end]:  # most often
+            return end
+        start = 0  # the first difference lies in start .. end - 1
+        while end - start > 1:
+            middle = (start + end) // 2
+            if x[start:middle] == y[start:middle]:
+                start = middle
+            else:
+                end = middle
+        return start
 
     def check_invariants(self) -> None:
         """Refcounts equal live references; the free list holds exactly the
