@@ -215,7 +215,7 @@ class PagedTreeCache:
 
         ``share``: pages that requests next to each other in the list begin with in
         common (forks of one prompt) are read once for all of them; the result is the
-        same up to rounding."""
+        same up to rounding, and where no two share a page to the bit."""
         if len(requests) != len(counts) or len(set(requests)) != len(requests) or not requests:
             raise ValueError("requests must be distinct and match counts")
         total = sum(counts)
@@ -282,6 +282,8 @@ class PagedTreeCache:
             lists = [owner.pages[request] for request in requests]
             lengths = [owner.lengths[request] for request in requests]
             groups = owner.shared_prefixes(requests) if share else ()
+            if groups and len(groups[1]) == len(requests):  # no two share a page
+                groups = ()
             old, fresh, ids, length, count, *groups = self._upload(
                 [old for old, _ in clones], [fresh for _, fresh in clones],
                 [page for pages in lists for page in pages], lengths, counts, *groups)

@@ -105,3 +105,25 @@ def test_no_other_groups_read_fewer_tokens(seed):
 def test_prefixes_of_no_request():
     from branchcraft_torch.pages import PageOwner
     assert PageOwner(4).shared_prefixes([]) == ([0], [])
+
+
+@pytest.mark.parametrize("forks", [0, 1])
+def test_extend_without_common_pages_is_the_plain_call(forks, monkeypatch):
+    """Also where pages are shared by requests that the call does not name next to each
+    other, and by one request of the call alone."""
+    from branchcraft_torch import transaction
+    seen = []
+    for name in ("chunk_attention", "shared_chunk_attention"):
+        real = getattr(transaction, name)
+        monkeypatch.setattr(transaction, name, lambda *a, _real=real, _name=name, **k: (seen.append(_name), _real(*a, **k))[1])
+    with FakeTensorMode():
+        def fill(n, heads=2):
+            return torch.zeros(n, heads, 64, device="cuda", dtype=torch.float16)
+
+        cache = transaction.PagedTreeCache(40, 2, 64)
+        a, b, c = (cache.new(fill(n), fill(n)) for n in (50, 70, 15))
+        d, e = cache.fork(a), cache.fork(c)  # of c no whole page is shared
+        requests = [a, d, b, c, e] if forks else [a, b, d, c, e]
+        cache.extend(requests, [1] * 5, fill(5, 4), fill(5), fill(5), share=True)
+        cache.extend([a], [2], fill(2, 4), fill(2), fill(2), share=True)
+    assert seen == ["shared_chunk_attention" if forks else "chunk_attention", "chunk_attention"]
