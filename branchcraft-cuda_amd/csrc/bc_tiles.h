@@ -7,6 +7,7 @@
 
 #include "bc_device.h"
 #include "bc_host.h"
+#include "bc_rules.h"
 
 using namespace bcd;
 
@@ -319,7 +320,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 constexpr int kStep = 64;       // tokens per step of a tile of rows
-constexpr int kFewRows = 32;    // rows of a request that take the narrow form
+using bch::kFewRows;
 constexpr int kManyRows = 128;  // rows per workgroup of the wide form
 constexpr int kLeastSteps = 4;  // fewest steps per part of a split tile of rows
 constexpr int kLeastRun = 4;    // fewest 32-token tiles per wave of the narrow form
@@ -2129,13 +2130,6 @@ hipError_t launch_tiles(const MoreParams& M, int dim, int dtype, const Cut& cut,
                      : launch_tiles<_Float16, 128, FP8>(M, cut, ws, (unsigned)grid, st);
   return dim == 64 ? launch_tiles<__bf16, 64, FP8>(M, cut, ws, (unsigned)grid, st)
                    : launch_tiles<__bf16, 128, FP8>(M, cut, ws, (unsigned)grid, st);
-}
-
-// Whether a window is as short as tables that are not cut, see cut_of (32 requests of
-// 8 new tokens, window 1024, 24/8 heads, bias: 26 us, cut 40).
-inline bool short_window(const bc_shape& s, const bc_chunk_inputs& in) {
-  const bool few = (long long)in.tokens * (s.query_heads / s.kv_heads) <= (long long)kFewRows * s.batch;
-  return in.causal && in.window > 0 && in.window <= (few ? 1024 : 512);
 }
 
 // Workgroups of the tile kernel with a workspace, at most, of a batch whose entries

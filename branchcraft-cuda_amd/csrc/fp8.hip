@@ -326,10 +326,10 @@ extern "C" int bc_fp8_chunk_attention(bc_shape s, bc_chunk_inputs in, const uint
   M.k_scale = k_scale;
   M.v_scale = v_scale;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  // As in bc_chunk_attention.
+  // As in bc_chunk_attention, which cuts tables also under a short window.
   const Cut cut = cut_of(s, in.tokens, true);
   const bool use = cut.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= cut.bytes &&
-                   !short_window(s, in);
+                   !bch::short_window(s, in);
   const long long rows = (long long)in.tokens * M.t.c.group;
   const long long grid = use ? split_grid(s, cut, rows, s.batch) : tile_grid(s, in.tokens, cut, false);
   const long long far = 1 << 27;  // bytes: offsets inside a page are 32-bit

@@ -357,33 +357,11 @@ struct ForkCut : Cut {
   int single_rows, total_rows, own_records;
 };
 
-// Whether reading shared pages once can pay for the entries' own starts and the
-// join, by what the host knows: the K and V that the requests may see, each its own,
-// and their rows.  Measured, 32/8 heads, D = 128, single tokens, with and without:
-//  - 69 MB (8 requests, 2048 shared tokens) 22.0 and 21.3 us, 136 MB (4096 tokens)
-//    25.5 and 27.3, 277 MB (32 requests) 24 and 40, 8.9 GB (64, 32768) 82 and 774.
-//  - Tables of up to 1024 tokens, which are not cut there: 64 requests, 512 tokens 31
-//    and 16; past them, 1024 and up to 64 more, 22 and 35.
-//  - Many requests of little each: every workgroup walks the batch, some 5 us per 64
-//    requests.  Groups of 4: 504 requests of 0.5 MB 105 and 72, of 1 MB 110 and 107,
-//    120 of 2.1 MB 34 and 47; of 8: 1024 of 2.1 MB 355 and 503.
-//  - Under a window what is shared is less: 1024 tokens, 268 MB 50 and 47, 537 MB 38
-//    and 51.
-//  - Requests of many rows fill tiles by themselves: 8 of 64 rows over 8192 shared
-//    tokens 46 and 51 us, of 96 rows 58 and 55.
-bool sharing_pays(const bc_shape& s, int tokens, int window) {
-  const long long table = (long long)s.max_pages * BC_PAGE_SIZE, rows = (long long)tokens * (s.query_heads / s.kv_heads);
-  const long long seen = window > 0 && window < table ? window : table;
-  const double mb = (double)s.batch * (double)seen * s.kv_heads * s.dim * 4 / 1e6;
-  return s.batch > 1 && table > 1024 && rows <= 80ll * s.batch && mb >= (seen < table ? 400 : 100) &&
-         mb >= 1.2 * s.batch;
-}
-
 // How a call cuts its work; bytes 0: every request reads its own pages.
 ForkCut fork_cut(const bc_shape& s, int tokens, int groups) {
   ForkCut c{};
   const long long rows = (long long)tokens * (s.query_heads / s.kv_heads);
-  if (groups < 1 || rows < 1 || !sharing_pays(s, tokens, 0) || rows > 1 << 28 ||
+  if (groups < 1 || rows < 1 || !bch::sharing_pays(s, tokens, 0) || rows > 1 << 28 ||
       (s.batch + (long long)groups) * (s.max_pages + 1ll) > 1 << 28 ||
       (long long)s.batch * s.query_heads > 1 << 26)
     return c;
@@ -458,7 +436,7 @@ extern "C" int bc_shared_chunk_attention(bc_shape s, bc_chunk_inputs in, const i
       (group_count > 0 && !shared) || group_count > s.batch)
     return BC_ERROR_INVALID_VALUE;
   const ForkCut cut = fork_cut(s, in.tokens, group_count);
-  const bool use = cut.bytes > 0 && sharing_pays(s, in.tokens, in.window) && workspace && aligned16(workspace) &&
+  const bool use = cut.bytes > 0 && bch::sharing_pays(s, in.tokens, in.window) && workspace && aligned16(workspace) &&
                    workspace_bytes >= cut.bytes;
   // As in bc_chunk_attention.  Rows count twice, as a request's and as a group's;
   // under a window, or with documents, a group of few rows is of the wide form.
@@ -468,7 +446,7 @@ extern "C" int bc_shared_chunk_attention(bc_shape s, bc_chunk_inputs in, const i
   const long long far = 1 << 26;
   if (!use || !aligned16(in.q) || !aligned16(in.k) || !aligned16(in.v) || !aligned16(in.output) ||
       stride_bits(in) % 8 != 0 || in.k_strides.slot >= far || in.v_strides.slot >= far || grid > kMostGroups)
-    return bc_chunk_attention(s, in, short_window(s, in) ? nullptr : workspace, workspace_bytes, stream);
+    return bc_chunk_attention(s, in, bch::short_window(s, in) ? nullptr : workspace, workspace_bytes, stream);
   if (!in.q || !in.output) return BC_ERROR_INVALID_VALUE;
   MoreParams M{};
   M.t.c = chunk_params(s, in);

@@ -22,6 +22,7 @@
 #include <tuple>
 #include <vector>
 
+#include "bc_rules.h"
 #include "branchcraft.h"
 
 namespace {
@@ -860,7 +861,9 @@ at::Tensor fp8_chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, con
   return chunk_call(q, k, v, true, pages, lengths, starts,
                     {scale, causal, window, cap, slopes, prefix, first},
                     [&](const bc_shape& shape, const bc_chunk_inputs& in) {
-                      const size_t bytes = bc_fp8_chunk_attention_workspace_size(shape, in.tokens);
+                      const size_t bytes = bch::short_window(shape, in)
+                                               ? 0
+                                               : bc_fp8_chunk_attention_workspace_size(shape, in.tokens);
                       const at::Tensor ws = workspace_of(q, bytes);
                       check_launch(bc_fp8_chunk_attention(shape, in, bytes_of(scale_k), bytes_of(scale_v),
                                                           bytes ? ws.data_ptr() : nullptr, bytes,
@@ -890,8 +893,11 @@ at::Tensor shared_chunk_attention_hip(const at::Tensor& q, const at::Tensor& k, 
   return chunk_call(q, k, v, false, pages, lengths, starts,
                     {scale, causal, window, cap, slopes, prefix, first},
                     [&](const bc_shape& shape, const bc_chunk_inputs& in) {
+                      const bool once = count > 0 && bch::sharing_pays(shape, in.tokens, in.window);
                       const size_t bytes =
-                          bc_shared_chunk_attention_workspace_size(shape, in.tokens, count);
+                          !once && bch::short_window(shape, in)
+                              ? 0
+                              : bc_shared_chunk_attention_workspace_size(shape, in.tokens, count);
                       const at::Tensor ws = workspace_of(q, bytes);
                       check_launch(bc_shared_chunk_attention(shape, in, groups.data_ptr<int>(),
                                                              shared.data_ptr<int>(), count,

@@ -516,7 +516,9 @@ int bc_fp8_chunk_attention(bc_shape shape, bc_chunk_inputs in, const uint8_t* k_
                            const uint8_t* v_scale, void* workspace, size_t workspace_bytes,
                            bc_stream_t stream);
 
-/* Bytes of workspace for it, as bc_chunk_attention_workspace_size. */
+/* Bytes of workspace for it, as bc_chunk_attention_workspace_size, and 17 MB more at
+ * D = 128.  Not used within a causal window of up to 512 tokens (1024 where the rows
+ * are at most 32 * batch). */
 size_t bc_fp8_chunk_attention_workspace_size(bc_shape shape, int tokens);
 
 /* ---- requests that begin with the same pages ---- */
@@ -540,7 +542,10 @@ int bc_shared_chunk_attention(bc_shape shape, bc_chunk_inputs in, const int32_t*
                               const int32_t* shared, int group_count, void* workspace,
                               size_t workspace_bytes, bc_stream_t stream);
 
-/* Bytes of workspace for either way, as bc_chunk_attention_workspace_size. */
+/* Bytes of workspace for either way: where these sizes let shared pages be read once,
+ * 80 to 105 MB and, at D = 128, up to 2 KB for each new token and query head; else
+ * bc_chunk_attention_workspace_size's.  Not used where every request reads its own
+ * pages within a window as short as above. */
 size_t bc_shared_chunk_attention_workspace_size(bc_shape shape, int tokens, int group_count);
 
 /* Library version string, for logs. */
