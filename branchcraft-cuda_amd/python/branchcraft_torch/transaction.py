@@ -31,6 +31,31 @@ from .pages import CommitPlan, PageOwner, Snapshot
 __all__ = ["PagedTreeCache", "Fp8Cache", "Snapshot", "CommitPlan"]
 
 
+LEAST_SHARED = 256  # tokens
+
+
+def _worth_reading_once(bounds: list[int], tokens: list[int], lengths: list[int],
+                        window: int) -> tuple[list[int], list[int]] | tuple[()]:
+    """The groups of ``PageOwner.shared_prefixes`` as the attention is told of them:
+    those that share few tokens as sharing none, and () where they spare too little.
+
+    Every group starts with a round trip of its own and every row is joined, whatever is
+    shared (attention of single tokens, 32/8 heads, D = 128, shared and plain, us): 64
+    requests of 2048 tokens in pairs that share 16 tokens 121 and 66, 64 tokens 88 and
+    66, 256 70 and 66, 1024 65 and 66; all 64 together 256 tokens 67 and 62, 1024 48 and
+    54.  Over 155 batches of forks at five head layouts the calls that these two rules
+    choose took 83 % of the plain ones' time (geometric mean) and 6 % (3 us) more at most."""
+    saved, once = 0, []
+    for a, b, n in zip(bounds, bounds[1:], tokens):
+        # What each member sees of it, within a window that ends with the request.
+        seen = [max(n - max(x - window, 0), 0) if window else n for x in lengths[a:b]]
+        worth = b - a > 1 and max(seen) >= LEAST_SHARED
+        once.append(n if worth else 0)
+        saved += sum(seen) - max(seen) if worth else 0
+    read = sum(min(x, window) if window else x for x in lengths)
+    return (bounds, once) if saved and 4 * saved >= read else ()
+
+
 class PagedTreeCache:
     def __init__(self, physical_pages: int, kv_heads: int, head_dim: int,
                  device: str = "cuda"):
@@ -214,8 +239,9 @@ class PagedTreeCache:
         fails later leaves pages and lengths as before it.  A count may be zero.
 
         ``share``: pages that requests next to each other in the list begin with in
-        common (forks of one prompt) are read once for all of them; the result is the
-        same up to rounding, and where no two share a page to the bit."""
+        common (forks of one prompt) are read once for all of them, where that spares a
+        quarter of what is read; the result is the same up to rounding, and elsewhere to
+        the bit."""
         if len(requests) != len(counts) or len(set(requests)) != len(requests) or not requests:
             raise ValueError("requests must be distinct and match counts")
         total = sum(counts)
@@ -281,9 +307,10 @@ class PagedTreeCache:
             clones = [plan.cow for plan in plans if plan.cow is not None]
             lists = [owner.pages[request] for request in requests]
             lengths = [owner.lengths[request] for request in requests]
-            groups = owner.shared_prefixes(requests) if share else ()
-            if groups and len(groups[1]) == len(requests):  # no two share a page
-                groups = ()
+            groups = ()
+            if share:
+                groups = _worth_reading_once(*owner.shared_prefixes(requests), lengths,
+                                             options.get("window", 0))
             old, fresh, ids, length, count, *groups = self._upload(
                 [old for old, _ in clones], [fresh for _, fresh in clones],
                 [page for pages in lists for page in pages], lengths, counts, *groups)

@@ -107,23 +107,57 @@ def test_prefixes_of_no_request():
     assert PageOwner(4).shared_prefixes([]) == ([0], [])
 
 
-@pytest.mark.parametrize("forks", [0, 1])
-def test_extend_without_common_pages_is_the_plain_call(forks, monkeypatch):
-    """Also where pages are shared by requests that the call does not name next to each
-    other, and by one request of the call alone."""
+# (Tokens in common, own tokens, members) of families behind one system prompt, the
+# window, and the groups and tokens that extend tells the attention of.
+BATCHES = {
+    "nothing in common": (0, [(0, 700, 1)] * 5, 0, None),
+    "a system prompt": (64, [(0, 700, 1)] * 5, 0, None),
+    "few tokens of many": (0, [(320, 5000, 2)] * 3, 0, None),
+    "little of much": (0, [(2048, 9, 4)] + [(0, 7000, 1)] * 4, 0, None),
+    "forks": (0, [(1024, 30, 3)], 0, ([0, 3], [1024])),
+    "forks beside others": (32, [(0, 700, 1), (2048, 30, 8), (0, 300, 2)], 0, ([0, 1, 9, 11], [0, 2080, 0])),
+    "forks behind a window": (0, [(1024, 900, 6)], 1000, None),
+    "forks in a window": (0, [(1024, 300, 6)], 1000, ([0, 6], [1024])),
+    "one fork in a window": (0, [(1024, 300, 1), (0, 20, 6)], 1000, None),
+}
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+def test_extend_shares_where_that_spares_enough(batch, monkeypatch):
+    """Elsewhere it is the plain call."""
     from branchcraft_torch import transaction
-    seen = []
+    calls = []
+
+    def attention(name, real):
+        def call(*args, **options):
+            if args[0].shape[0]:  # not the check of the options
+                calls.append(name)
+            return real(*args, **options)
+        return call
+
     for name in ("chunk_attention", "shared_chunk_attention"):
-        real = getattr(transaction, name)
-        monkeypatch.setattr(transaction, name, lambda *a, _real=real, _name=name, **k: (seen.append(_name), _real(*a, **k))[1])
+        monkeypatch.setattr(transaction, name, attention(name, getattr(transaction, name)))
+    uploads = []
+    upload = transaction.PagedTreeCache._upload
+    monkeypatch.setattr(transaction.PagedTreeCache, "_upload",
+                        lambda self, *lists: (uploads.append(lists), upload(self, *lists))[1])
+    system, families, window, want = BATCHES[batch]
     with FakeTensorMode():
-        def fill(n, heads=2):
+        def fill(n, heads=1):
             return torch.zeros(n, heads, 64, device="cuda", dtype=torch.float16)
 
-        cache = transaction.PagedTreeCache(40, 2, 64)
-        a, b, c = (cache.new(fill(n), fill(n)) for n in (50, 70, 15))
-        d, e = cache.fork(a), cache.fork(c)  # of c no whole page is shared
-        requests = [a, d, b, c, e] if forks else [a, b, d, c, e]
-        cache.extend(requests, [1] * 5, fill(5, 4), fill(5), fill(5), share=True)
-        cache.extend([a], [2], fill(2, 4), fill(2), fill(2), share=True)
-    assert seen == ["shared_chunk_attention" if forks else "chunk_attention", "chunk_attention"]
+        cache = transaction.PagedTreeCache(4000, 1, 64)
+        root = cache.new(fill(system), fill(system))
+        requests = []
+        for common, own, members in families:
+            first = cache.fork(root)
+            if common:
+                cache.owner.plan_commit(first, common)
+            family = [first] + [cache.fork(first) for _ in range(members - 1)]
+            for x in family:
+                cache.owner.plan_commit(x, own - 1)
+            requests += family
+        n = len(requests)
+        cache.extend(requests, [1] * n, fill(n, 2), fill(n), fill(n), share=True, **(dict(window=window) if window else {}))
+    assert calls == ["chunk_attention" if want is None else "shared_chunk_attention"]
+    assert uploads[-1][5:] == (() if want is None else want)
