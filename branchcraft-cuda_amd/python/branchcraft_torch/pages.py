@@ -44,6 +44,27 @@ class CommitPlan:
     new_length: int = 0
 
 
+def _same_pages(x: list[int], y: list[int], end: int, guess: int) -> int:
+    """How many of their first ``end`` pages two tables begin with in common; ``guess``,
+    what the ones before have, is most often it."""
+    if not end or x[0] != y[0]:
+        return 0
+    at = min(max(guess, 1), end)
+    if x[:at] == y[:at]:
+        if at == end or x[at] != y[at]:
+            return at
+        low, high = at, end + 1
+    else:
+        low, high = 1, at
+    while high - low > 1:  # the same up to low, and not up to high
+        middle = (low + high) // 2
+        if x[low:middle] == y[low:middle]:
+            low = middle
+        else:
+            high = middle
+    return low
+
+
 def _neighbours(common: list[int], count: int) -> list[tuple[int, int]]:
     """A list of ``count`` requests, of which i and i + 1 have ``common[i]`` pages in
     common, as groups ``(members, pages in common)`` with the largest sum of
@@ -53,6 +74,8 @@ def _neighbours(common: list[int], count: int) -> list[tuple[int, int]]:
     saved[j] + (n - 1 - j) * p.  The starts j of equal p lie on the stack together, p
     rising; the best of them for a p that only falls is found on the upper hull of their
     points (j, saved[j]), from its front on."""
+    if not any(common):
+        return [(1, 0)] * count
     saved, last = [0], [(0, 0)]  # of the best last group: where it starts, and its pages
     stack: list[tuple[int, list[int]]] = []
 
@@ -240,27 +263,15 @@ class PageOwner:
         first ``tokens[g]`` tokens lie in pages of all of them (a group of one: all that
         it has).  The list is cut where most tokens are then read once for several
         requests instead of for each."""
-        common = [self._common_pages(a, b) for a, b in zip(requests, requests[1:])]
+        common: list[int] = []
+        for a, b in zip(requests, requests[1:]):
+            end = min(self.lengths[a], self.lengths[b]) // PAGE_SIZE
+            common.append(_same_pages(self.pages[a], self.pages[b], end, common[-1] if common else end))
         bounds, tokens = [0], []
         for members, pages in _neighbours(common, len(requests)):
             tokens.append(pages * PAGE_SIZE if members > 1 else self.lengths[requests[bounds[-1]]])
             bounds.append(bounds[-1] + members)
         return bounds, tokens
-
-    def _common_pages(self, a: int, b: int) -> int:
-        """Whole pages that two requests begin with."""
-        x, y = self.pages[a], self.pages[b]
-        end = min(self.lengths[a], self.lengths[b]) // PAGE_SIZE
-        if x[:end] == y[:end]:  # most often
-            return end
-        start = 0  # the first difference lies in start .. end - 1
-        while end - start > 1:
-            middle = (start + end) // 2
-            if x[start:middle] == y[start:middle]:
-                start = middle
-            else:
-                end = middle
-        return start
 
     def check_invariants(self) -> None:
         """Refcounts equal live references; the free list holds exactly the

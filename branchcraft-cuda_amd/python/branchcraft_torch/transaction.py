@@ -44,7 +44,7 @@ def _worth_reading_once(bounds: list[int], tokens: list[int], lengths: list[int]
     requests of 2048 tokens in pairs that share 16 tokens 121 and 66, 64 tokens 88 and
     66, 256 70 and 66, 1024 65 and 66; all 64 together 256 tokens 67 and 62, 1024 48 and
     54.  Over 155 batches of forks at five head layouts the calls that these two rules
-    choose took 83 % of the plain ones' time (geometric mean) and 6 % (3 us) more at most."""
+    choose took 79 % of the plain ones' time (geometric mean) and 6 % (3 us) more at most."""
     saved, once = 0, []
     for a, b, n in zip(bounds, bounds[1:], tokens):
         # What each member sees of it, within a window that ends with the request.

@@ -161,3 +161,13 @@ def test_extend_shares_where_that_spares_enough(batch, monkeypatch):
         cache.extend(requests, [1] * n, fill(n, 2), fill(n), fill(n), share=True, **(dict(window=window) if window else {}))
     assert calls == ["chunk_attention" if want is None else "shared_chunk_attention"]
     assert uploads[-1][5:] == (() if want is None else want)
+
+
+@pytest.mark.parametrize("same", [0, 1, 2, 5, 8, 9])
+def test_common_pages_whatever_is_guessed(same):
+    from branchcraft_torch.pages import _same_pages
+    x = list(range(9))
+    y = x[:same] + [100 + i for i in range(9 - same)]
+    for end in range(10):
+        for guess in range(12):
+            assert _same_pages(x, y, end, guess) == min(same, end)
