@@ -1914,7 +1914,10 @@ __device__ __forceinline__ void clear_rows(const ChunkParams& C, long long at, l
 // Workgroups per CU: three at D = 64 (see wide_body), but two for the biased and capped
 // forms of an 8-bit cache, which spill with the registers of three: 64 single tokens
 // over 2048, bias 39 us and cap 41 (three: 42, 46), 24 mixed requests with a cap 95
-// (103), against 4 x 1024 new tokens of 4096 199 and 247 (188, 234).
+// (103), against 4 x 1024 new tokens of 4096 199 and 247 (188, 234).  At D = 128 the
+// 8-bit forms have 256 registers and keep more in memory: the capped one 30, four of
+// them loaded and one stored in every tile of the narrow body, the biased one three,
+// the plain one two.  Of the 16-bit forms the capped one at D = 64 keeps one.
 template <typename T, int D, Form FORM, bool FP8>
 __global__ __launch_bounds__(256, D == 64 && !(FP8 && FORM != Form::kPlain) ? 3 : 2) void chunk_tile_kernel(
     Taken<FP8>) {

@@ -225,7 +225,8 @@ __device__ __forceinline__ Item plan_entry(const TileParams& P, const Entries& a
 // 64 single tokens over a shared 32768 and 16 to 1024 of their own (32/8 heads, D =
 // 128, 263 MB): 71 us, 3.7 TB/s, and the join 9; HBM would take 41.  The group's two
 // tiles of rows per KV head run over the same pages, once from L2, beside the
-// requests' own parts; matrix units 28 %, vector units 34 % of the cycles.
+// requests' own parts; matrix units 28 %, vector units 34 % of the cycles.  The biased
+// and capped forms at D = 64 keep five registers in memory, outside their loops.
 template <typename T, int D, Form FORM>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void fork_tile_kernel(MoreParams) {
   __shared__ __attribute__((aligned(256))) uint16_t s_kv[2 * 2 * kStep * D];

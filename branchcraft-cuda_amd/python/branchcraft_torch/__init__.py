@@ -263,7 +263,8 @@ def shared_chunk_attention(q, k, v, pages, lengths, starts, groups, shared, *, s
     one) where the sizes of the call say that this pays; elsewhere each request's are.
     ``groups`` (not decreasing) and ``shared`` are int32 tensors on the GPU; requests
     outside all groups share nothing.  The results are ``chunk_attention``'s up to
-    rounding."""
+    rounding.  What is shared is not looked at for that choice: groups of less than some
+    256 tokens cost more than they spare (``PagedTreeCache.extend`` leaves them out)."""
     return _shared_chunk_attention(q, k, v, pages, lengths, starts, groups, shared, scale, causal, window,
                                    cap, slopes, prefix, first)
 

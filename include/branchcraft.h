@@ -535,7 +535,13 @@ size_t bc_fp8_chunk_attention_workspace_size(bc_shape shape, int tokens);
  * tokens, up to 80 rows (new tokens times group) a request, and 100 MB of K and V
  * in the tables (400 within a window shorter than them), 1.2 MB a request.
  * Elsewhere, without a workspace, and in the cases that go row by row there, every
- * request's own row of `pages` is read, so each has to hold all of its pages.
+ * request's own row of `pages` is read, so each has to hold all of its pages; within a
+ * window as short as below such a call is faster than bc_chunk_attention, which keeps
+ * to its split and to the bits that it gives.
+ * What is shared is not known on the host: a group starts with a round trip of its own
+ * and all rows are joined, whatever it spares.  64 requests of 2048 tokens (32/8 heads,
+ * D = 128) in pairs take 121 us with 16 tokens shared, 65 with 1024, and 66 apart, so
+ * groups of less than some 256 tokens are better left out, and such calls apart.
  * Also rejects: group_count < 0 or over batch, null groups, null shared with
  * groups. */
 int bc_shared_chunk_attention(bc_shape shape, bc_chunk_inputs in, const int32_t* groups,
