@@ -34,10 +34,11 @@ __all__ = ["PagedTreeCache", "Fp8Cache", "Snapshot", "CommitPlan"]
 LEAST_SHARED = 256  # tokens
 
 
-def _worth_reading_once(bounds: list[int], tokens: list[int], lengths: list[int],
+def _worth_reading_once(bounds: list[int], tokens: list[int], lengths: list[int], counts: list[int],
                         window: int) -> tuple[list[int], list[int]] | tuple[()]:
     """The groups of ``PageOwner.shared_prefixes`` as the attention is told of them:
-    those that share few tokens as sharing none, and () where they spare too little.
+    those that share few tokens as sharing none, and () where they spare too little of
+    what the requests with new tokens read.
 
     Every group starts with a round trip of its own and every row is joined, whatever is
     shared (attention of single tokens, 32/8 heads, D = 128, shared and plain, us): 64
@@ -48,11 +49,12 @@ def _worth_reading_once(bounds: list[int], tokens: list[int], lengths: list[int]
     saved, once = 0, []
     for a, b, n in zip(bounds, bounds[1:], tokens):
         # What each member sees of it, within a window that ends with the request.
-        seen = [max(n - max(x - window, 0), 0) if window else n for x in lengths[a:b]]
-        worth = b - a > 1 and max(seen) >= LEAST_SHARED
+        seen = [max(n - max(x - window, 0), 0) if window else n
+                for x, new in zip(lengths[a:b], counts[a:b]) if new]
+        worth = len(seen) > 1 and max(seen) >= LEAST_SHARED
         once.append(n if worth else 0)
         saved += sum(seen) - max(seen) if worth else 0
-    read = sum(min(x, window) if window else x for x in lengths)
+    read = sum(min(x, window) if window else x for x, new in zip(lengths, counts) if new)
     return (bounds, once) if saved and 4 * saved >= read else ()
 
 
@@ -309,7 +311,7 @@ class PagedTreeCache:
             lengths = [owner.lengths[request] for request in requests]
             groups = ()
             if share:
-                groups = _worth_reading_once(*owner.shared_prefixes(requests), lengths,
+                groups = _worth_reading_once(*owner.shared_prefixes(requests), lengths, counts,
                                              options.get("window", 0))
             old, fresh, ids, length, count, *groups = self._upload(
                 [old for old, _ in clones], [fresh for _, fresh in clones],

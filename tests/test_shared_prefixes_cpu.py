@@ -171,3 +171,22 @@ def test_common_pages_whatever_is_guessed(same):
     for end in range(10):
         for guess in range(12):
             assert _same_pages(x, y, end, guess) == min(same, end)
+
+
+@pytest.mark.parametrize("counts,shares", [([1, 0, 0, 0], False), ([0, 0, 0, 1], False), ([1, 0, 0, 2], True),
+                                           ([0, 3, 1, 0], True), ([0, 0, 0, 0], False)])
+def test_requests_without_new_tokens_read_nothing(counts, shares, monkeypatch):
+    from branchcraft_torch import transaction
+    calls = []
+    for name in ("chunk_attention", "shared_chunk_attention"):
+        real = getattr(transaction, name)
+        monkeypatch.setattr(transaction, name, lambda *a, _real=real, _name=name: (calls.append(_name), _real(*a))[1])
+    with FakeTensorMode():
+        def fill(n, heads=1):
+            return torch.zeros(n, heads, 64, device="cuda", dtype=torch.float16)
+
+        cache = transaction.PagedTreeCache(400, 1, 64)
+        a = cache.new(fill(2000), fill(2000))
+        n = sum(counts)
+        cache.extend([a] + [cache.fork(a) for _ in range(3)], counts, fill(n, 2), fill(n), fill(n), share=True)
+    assert calls == ["shared_chunk_attention" if shares else "chunk_attention"]

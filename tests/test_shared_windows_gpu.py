@@ -173,3 +173,46 @@ def test_the_two_references_agree():
     fix, _, _ = F.forks([(64, [(1 + i, 1 + i % 3) for i in range(5)])], 4, 2, 64, F16, seed=14)
     for x, y in zip(by_rows(fix), C.reference(**fix)):
         assert torch.allclose(x, y, rtol=1e-12, atol=1e-15)
+
+
+# ---------------------------------------------------------------------------
+# Whole calls
+
+
+@pytest.mark.parametrize("window", [0, 3000])
+def test_extend_over_forks_beside_others(window):
+    """A chat, forks of a document and forks of a short note, all behind one system
+    prompt; the note itself has no new tokens."""
+    from branchcraft_torch.transaction import PagedTreeCache
+    g = torch.Generator("cuda").manual_seed(8)
+    hq, hkv, d = 32, 16, 64
+
+    def rand(n, heads):
+        return torch.randn((n, heads, d), generator=g, device="cuda", dtype=F16)
+
+    cache = PagedTreeCache(1000, hkv, d)
+    root = cache.new(rand(32, hkv), rand(32, hkv))
+
+    def grow(x, n):
+        cache.extend([x], [n], rand(n, hq), rand(n, hkv), rand(n, hkv))
+        return x
+
+    chat, document, note = (grow(cache.fork(root), n) for n in (700, 3800, 150))
+    who = [chat, document] + [cache.fork(document) for _ in range(30)] + [note, cache.fork(note)]
+    for turn in range(2):
+        counts = [3] + [1, 2] * 15 + [1, 0] + [1]
+        total = sum(counts)
+        q, k, v = rand(total, hq), rand(total, hkv), rand(total, hkv)
+        got = cache.extend(who, counts, q, k, v, share=True, window=window)
+        lists = [cache.pages[x] for x in who]
+        table = torch.full((len(who), max(map(len, lists))), -1, dtype=torch.int32)
+        for i, pages in enumerate(lists):
+            table[i, :len(pages)] = torch.tensor(pages)
+        starts = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32)
+        fix = dict(q=q.cpu(), k=cache.k.cpu(), v=cache.v.cpu(), pages=table, starts=starts,
+                   lengths=torch.tensor([cache.lengths[x] for x in who], dtype=torch.int32))
+        assert F.pays(fix, window)
+        bounds, tokens = cache.owner.shared_prefixes(who)
+        assert bounds == [0, 1, 32, 34] and tokens[1] == 3832 // 16 * 16
+        want, tol = C.reference(**fix, window=window)
+        C.check(got, want, tol)
